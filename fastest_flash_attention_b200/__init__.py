@@ -16,7 +16,8 @@ from .block_sparse import (
 )
 
 __version__ = "1.0.0"
-from .kv_cache import PagedKVCache, ContinuousKVCache
+from .kv_cache import PagedKVCache, ContinuousKVCache, copy_pages, move_tokens
+from .rotary import apply_rotary, rotary_append, rotary_tables
 from .decode import paged_decode
 from .fa4 import FA4AttnFunc, fa4_attn_func, fa4_forward_dispatch
 from .modules import FastestFlashMHA, FastestFlashGQA, FastestFlashMLA, FastestFlashFA4, RotaryEmbedding
@@ -30,5 +31,6 @@ __all__ = [
     "FastestFlashGQA", "FastestFlashMLA", "FastestFlashFA4", "PagedKVCache", "ContinuousKVCache",
     "create_causal_block_mask", "create_sliding_window_block_mask", "create_local_block_mask",
     "auto_select_block_size", "check_triton_available", "paged_decode", "MLADecoder", "mla_decode",
+    "copy_pages", "move_tokens", "rotary_tables", "apply_rotary", "rotary_append",
     "ring_attention_forward", "ring_attention_backward", "ring_attention_func", "zigzag_shard", "zigzag_unshard",
 ]

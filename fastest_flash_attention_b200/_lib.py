@@ -7,6 +7,7 @@ library's last error string.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from pathlib import Path
@@ -120,6 +121,27 @@ SIGNATURES: dict[str, tuple] = {
         _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,  # dtype n_tokens Hkv D page_size num_pages
         _c_i64p, _c_void_p,  # new_strides stream
     ]),
+    "ffa_page_copy": (_c_int, [
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p,  # k_pages v_pages src dst
+        _c_int, _c_int, ctypes.c_int64, _c_u32p, _c_void_p,  # n num_pages page_bytes err stream
+    ]),
+    "ffa_token_move": (_c_int, [
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p,  # k_pages v_pages src_slots dst_slots
+        _c_int, _c_int, _c_int, _c_int, _c_int, _c_u32p, _c_void_p,  # n Hkv page_size num_pages row_bytes err stream
+    ]),
+    "ffa_rotary": (_c_int, [
+        _c_void_p, _c_i64p, _c_void_p, _c_i64p, _c_void_p, _c_i64p, _c_void_p, _c_i64p,  # q s qo s k s ko s
+        _c_void_p, _c_void_p, ctypes.c_int64, _c_void_p, _c_int, ctypes.c_int64,  # cos sin len pos pos64 pos_sb
+        _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,  # dtype B S Hq Hkv D rot il inverse
+        _c_u32p, _c_void_p,  # err stream
+    ]),
+    "ffa_rotary_append": (_c_int, [
+        _c_void_p, _c_i64p, _c_void_p, _c_i64p, _c_void_p, _c_i64p, _c_void_p, _c_i64p,  # q s qo s k s v s
+        _c_void_p, _c_void_p, ctypes.c_int64, _c_void_p, _c_int, _c_void_p,  # cos sin len pos pos64 slots
+        _c_void_p, _c_void_p,  # k_pages v_pages
+        _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,  # dtype n Hq Hkv D rot interleaved
+        _c_int, _c_int, _c_u32p, _c_void_p,  # page_size num_pages err stream
+    ]),
 }
 
 _LIB: ctypes.CDLL | None = None
@@ -170,6 +192,14 @@ def stream_of(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
+_HERE = contextlib.nullcontext()
+
+
+def device_of(t: torch.Tensor):
+    """Context in which t's device is current (nothing to switch, and nothing to pay, where it already is)."""
+    return _HERE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
 _ERR_WORDS: dict[int, torch.Tensor] = {}
 
 
@@ -188,6 +218,8 @@ _DATA_ERRORS = {
     0x1FF: "block mask keeps more key tiles than the forward kernel's tile list holds",
     0x3E0: "paged decode: a context length is negative or exceeds max_pages_per_req * page_size",
     0x3E1: "paged decode: a block-table entry is outside [0, num_pages)",
+    0x3E2: "page copy: a page id or token slot is outside the pool",
+    0x3E3: "rotary: a position is outside the cos / sin tables",
 }
 
 

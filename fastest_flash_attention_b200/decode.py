@@ -27,10 +27,12 @@ def default_chunks_per_split(ctx_max: int, R: int, Hkv: int, num_sms: int = 148)
     return max(16, min(128, math.ceil(chunks / splits)))
 
 
-def check_block_table(block_table: torch.Tensor, ctx_lens: torch.Tensor, num_pages: int, page_size: int) -> None:
+def check_block_table(block_table: torch.Tensor, ctx_lens: torch.Tensor, num_pages: int, page_size: int,
+                      sliding_window: Optional[int] = None, sink_tokens: int = 0) -> None:
     """Host-side validation of paging data (CPU tensors): every context length
     in [0, width * page_size] and every page id a request reads in
-    [0, num_pages).  Raises ValueError naming the first bad request.  The
+    [0, num_pages) (with a window, a request reads the pages of its last
+    sliding_window tokens and of its first sink_tokens).  Raises ValueError naming the first bad request.  The
     decode kernels repeat these checks on the device (reporting through the
     error word) for tables that never pass through the host."""
     bt = block_table.to("cpu", torch.int64)
@@ -44,6 +46,9 @@ def check_block_table(block_table: torch.Tensor, ctx_lens: torch.Tensor, num_pag
         raise ValueError(f"ctx_lens[{r}] = {int(lens[r])} is outside [0, {width * page_size}] "
                          f"({width} pages of {page_size} tokens)")
     used = (torch.arange(width)[None, :] * page_size) < lens[:, None]  # pages each request reads
+    if sliding_window:
+        first = torch.arange(width)[None, :] * page_size
+        used &= (first + page_size > lens[:, None] - sliding_window) | (first < sink_tokens)
     bad = used & ((bt < 0) | (bt >= num_pages))
     if bool(bad.any()):
         r, c = (int(x) for x in bad.nonzero()[0])

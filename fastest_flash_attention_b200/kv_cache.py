@@ -11,16 +11,21 @@ assignment is host bookkeeping; the K/V bytes are scattered on the device
 by ``ffa_paged_append`` in one launch per call instead of a per-token loop.
 Beyond the reference API, ``block_table()`` exports the tables as an int32
 tensor and ``decode()`` runs the sm_100a split-KV decode directly on the
-pool, with no gather.
+pool, with no gather.  For long conversations, sequences are forked (full
+pages shared, counted), trimmed (pages that left a sliding window freed) and
+compacted (first tokens and window moved to fresh pages); the bytes move in
+one launch of ``copy_pages`` / ``move_tokens``.
 """
 from __future__ import annotations
 
-from typing import List, Optional, Sequence, Tuple
+from typing import Dict, List, Optional, Sequence, Tuple, Union
 
+import numpy as np
 import torch
 
 from . import _lib
 from .decode import check_block_table
+from .utils import check_window
 
 
 class ContinuousKVCache:
@@ -74,6 +79,89 @@ class ContinuousKVCache:
         return self.k_cache[:batch_size, :, :max_len], self.v_cache[:batch_size, :, :max_len]
 
 
+Ids = Union[torch.Tensor, Sequence[int]]
+
+
+def _id_pair(src: Ids, dst: Ids, limit: int, device: torch.device, what: str) -> Tuple[torch.Tensor, torch.Tensor]:
+    """src and dst as int32 device tensors of one length.  Ids given on the
+    host are checked: each in [0, limit), destinations distinct and none of
+    them a source.  Ids on the device are taken as they are (the kernels skip
+    and report those outside the pool)."""
+    pair = []
+    for name, ids in (("src", src), ("dst", dst)):
+        t = ids if isinstance(ids, torch.Tensor) else torch.tensor(list(ids), dtype=torch.int64)
+        if t.dim() != 1 or t.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"{name} must be a 1-D int32 / int64 tensor or a list of {what}s")
+        pair.append(t)
+    if pair[0].numel() != pair[1].numel():
+        raise ValueError(f"{pair[0].numel()} source and {pair[1].numel()} destination {what}s")
+    if not (pair[0].is_cuda or pair[1].is_cuda):
+        s, d = (t.tolist() for t in pair)
+        bad = [x for x in s + d if not 0 <= x < limit]
+        if bad:
+            raise ValueError(f"{what} {bad[0]} is outside [0, {limit})")
+        if len(set(d)) < len(d) or not set(s).isdisjoint(d):
+            raise ValueError(f"destination {what}s must be distinct and none of them a source")
+    out = [t.to(device, torch.int32) for t in pair]
+    return tuple(t if t.is_contiguous() else t.contiguous() for t in out)
+
+
+def _check_pools(k_pages: torch.Tensor, v_pages: Optional[torch.Tensor]) -> None:
+    _lib.require_cuda(k_pages, v_pages)
+    if v_pages is not None and (v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype
+                                or v_pages.device != k_pages.device):
+        raise ValueError("k_pages and v_pages must have one shape, dtype and device")
+    if not k_pages.is_contiguous() or (v_pages is not None and not v_pages.is_contiguous()):
+        raise ValueError("page pools must be contiguous")
+
+
+def copy_pages(k_pages: torch.Tensor, v_pages: Optional[torch.Tensor], src: Ids, dst: Ids) -> None:
+    """Copy whole pages src[i] -> dst[i] inside the pools, in one launch.
+
+    Pools [P, ...] contiguous, any dtype; v_pages may be None (a latent cache
+    has one pool).  src, dst: page ids, int32 / int64 on the device (or on the
+    host, where they are checked); destinations are distinct and none of them
+    is a source.
+    """
+    _check_pools(k_pages, v_pages)
+    src, dst = _id_pair(src, dst, k_pages.shape[0], k_pages.device, "page id")
+    if k_pages.numel() == 0 or src.numel() == 0:
+        return
+    with _lib.device_of(k_pages):
+        st = _lib.load().ffa_page_copy(
+            k_pages.data_ptr(), v_pages.data_ptr() if v_pages is not None else None, src.data_ptr(), dst.data_ptr(),
+            src.numel(), k_pages.shape[0], k_pages.stride(0) * k_pages.element_size(),
+            _lib.err_word(k_pages.device).data_ptr(), _lib.stream_of(k_pages))
+    _lib.check(st, "ffa_page_copy")
+    if _lib.sync_check_enabled():
+        _lib.check_device_errors(k_pages.device)
+
+
+def move_tokens(k_pages: torch.Tensor, v_pages: Optional[torch.Tensor], src_slots: Ids, dst_slots: Ids) -> None:
+    """Copy single tokens' rows (every kv head) from slot src_slots[i] to slot
+    dst_slots[i] inside the pools, in one launch; slot = page * page_size +
+    offset.
+
+    Pools [P, Hkv, page_size, D], or [P, page_size, D] (a latent cache),
+    contiguous, any dtype; v_pages may be None.  Slots as copy_pages' page ids.
+    """
+    _check_pools(k_pages, v_pages)
+    if k_pages.dim() not in (3, 4):
+        raise ValueError(f"pools must be [P, Hkv, page_size, D] or [P, page_size, D], got {tuple(k_pages.shape)}")
+    P, page_size, D = k_pages.shape[0], k_pages.shape[-2], k_pages.shape[-1]
+    src_slots, dst_slots = _id_pair(src_slots, dst_slots, P * page_size, k_pages.device, "slot")
+    if k_pages.numel() == 0 or src_slots.numel() == 0:
+        return
+    with _lib.device_of(k_pages):
+        st = _lib.load().ffa_token_move(
+            k_pages.data_ptr(), v_pages.data_ptr() if v_pages is not None else None, src_slots.data_ptr(),
+            dst_slots.data_ptr(), src_slots.numel(), k_pages.shape[1] if k_pages.dim() == 4 else 1, page_size, P,
+            D * k_pages.element_size(), _lib.err_word(k_pages.device).data_ptr(), _lib.stream_of(k_pages))
+    _lib.check(st, "ffa_token_move")
+    if _lib.sync_check_enabled():
+        _lib.check_device_errors(k_pages.device)
+
+
 class PagedKVCache:
     """Paged KV cache (kv_cache.py:110-240) with device-side append and decode."""
 
@@ -87,6 +175,7 @@ class PagedKVCache:
         self.v_pages = torch.zeros(max_pages, num_heads, page_size, head_dim, dtype=dtype, device=device)
         self.free_pages: List[int] = list(range(max_pages))
         self.sequences: dict = {}
+        self._more_owners: Dict[int, int] = {}  # page -> sequences that share it beyond the first
 
     # ---- allocator (kv_cache.py:157-168) ----
     def allocate_page(self) -> int:
@@ -97,8 +186,23 @@ class PagedKVCache:
     def free_sequence(self, seq_id: int):
         if seq_id in self.sequences:
             for page_id in self.sequences[seq_id]["page_table"]:
-                self.free_pages.append(page_id)
+                self._release(page_id)
             del self.sequences[seq_id]
+
+    def _release(self, page_id: int) -> int:
+        """One owner less; a page without owners goes to the back of the free
+        list.  Returns the pages freed (an entry of -1 was freed before)."""
+        if page_id < 0:
+            return 0
+        others = self._more_owners.get(page_id, 0)
+        if others:
+            if others == 1:
+                del self._more_owners[page_id]
+            else:
+                self._more_owners[page_id] = others - 1
+            return 0
+        self.free_pages.append(page_id)
+        return 1
 
     def _assign_slots(self, seq_id: int, n: int) -> List[int]:
         """Slot (page * page_size + offset) of each appended token, allocating
@@ -146,10 +250,115 @@ class PagedKVCache:
             return None, None
         seq = self.sequences[seq_id]
         L = seq["len"]
+        if min(seq["page_table"]) < 0:
+            raise RuntimeError(f"PagedKVCache: pages of sequence {seq_id} left its window and were freed")
         idx = torch.tensor(seq["page_table"], dtype=torch.long, device=self.k_pages.device)
         k = self.k_pages[idx].permute(1, 0, 2, 3).reshape(self.num_heads, -1, self.head_dim)[:, :L]
         v = self.v_pages[idx].permute(1, 0, 2, 3).reshape(self.num_heads, -1, self.head_dim)[:, :L]
         return k.contiguous(), v.contiguous()
+
+    # ---- long conversations (no reference counterpart) ----
+    def position(self, seq_id: int) -> int:
+        """Position of the next token: the cached tokens and those that compact_sequences dropped."""
+        seq = self.sequences.get(seq_id)
+        return seq["len"] + seq.get("dropped", 0) if seq else 0
+
+    def fork_sequence(self, src_id: int, dst_id: int) -> None:
+        """New sequence dst_id with the same tokens as src_id."""
+        self.fork_sequences([(src_id, dst_id)])
+
+    def fork_sequences(self, pairs: Sequence[Tuple[int, int]]) -> None:
+        """New sequences with the tokens of existing ones, (source, new) for
+        each.  Full pages are never written again, so they are shared and
+        counted; a last page in part filled is copied, all of them in one
+        launch.  A failing call changes nothing."""
+        made = [d for _, d in pairs]
+        for s, d in pairs:
+            if s not in self.sequences:
+                raise KeyError(f"PagedKVCache: no sequence {s} to fork")
+            if d in self.sequences or made.count(d) > 1:
+                raise ValueError(f"PagedKVCache: sequence {d} exists already")
+        parts = sum(self.sequences[s]["len"] % self.page_size != 0 for s, _ in pairs)
+        if parts > len(self.free_pages):
+            raise RuntimeError("PagedKVCache: out of physical pages")
+        old, new = [], []
+        for s, d in pairs:
+            seq = self.sequences[s]
+            table = list(seq["page_table"])
+            if seq["len"] % self.page_size:
+                old.append(table.pop())
+                new.append(self.allocate_page())
+            for page in table:
+                if page >= 0:
+                    self._more_owners[page] = self._more_owners.get(page, 0) + 1
+            if seq["len"] % self.page_size:
+                table.append(new[-1])
+            self.sequences[d] = dict(seq, page_table=table)
+        if old and self.k_pages.is_cuda:
+            copy_pages(self.k_pages, self.v_pages, old, new)
+        elif old:  # host-side pool
+            self.k_pages[new] = self.k_pages[old]
+            self.v_pages[new] = self.v_pages[old]
+
+    def trim_sequence(self, seq_id: int, sliding_window: int, sink_tokens: int = 0) -> int:
+        """Free the pages whose tokens are all outside the last sliding_window
+        tokens and the first sink_tokens (their table entries become -1; the
+        windowed decode never reads them).  Returns the pages freed."""
+        check_window(sliding_window, sink_tokens)
+        seq = self.sequences[seq_id]
+        table, freed = seq["page_table"], 0
+        first = -(-sink_tokens // self.page_size)  # the first page without a sink token
+        for i in range(first, max(first, (seq["len"] - sliding_window) // self.page_size)):
+            freed += self._release(table[i])
+            table[i] = -1
+        return freed
+
+    def compact_sequences(self, seq_ids: Sequence[int], sliding_window: int, sink_tokens: int = 0) -> int:
+        """Drop every token outside the last sliding_window and the first
+        sink_tokens of each sequence and move the kept ones to fresh pages,
+        densely, in one launch.  The windowed decode gives the same result
+        before and after (rotated keys keep their positions; ``position()``
+        goes on counting the dropped tokens).  Returns the tokens dropped; a
+        failing call changes nothing."""
+        check_window(sliding_window, sink_tokens)
+        if len(set(seq_ids)) < len(seq_ids):
+            raise ValueError("PagedKVCache: a sequence is named twice")
+        ps, work = self.page_size, []
+        for s in seq_ids:
+            n = self.sequences[s]["len"]
+            start = max(n - sliding_window, 0)
+            sinks = min(sink_tokens, start)
+            if sinks < start:
+                work.append((s, np.r_[0:sinks, start:n]))
+        src, dst, dropped = [], [], 0
+        for s, kept in work:
+            seq = self.sequences[s]
+            old = np.asarray(seq["page_table"], dtype=np.int64)
+            src.append(old[kept // ps] * ps + kept % ps)
+            if src[-1].min() < 0:
+                raise RuntimeError(f"PagedKVCache: pages of sequence {s} in this window were freed")
+        if sum(-(-len(kept) // ps) for _, kept in work) > len(self.free_pages):
+            raise RuntimeError("PagedKVCache: out of physical pages")
+        for (s, kept), _ in zip(work, src):
+            seq = self.sequences[s]
+            fresh = [self.allocate_page() for _ in range(-(-len(kept) // ps))]
+            at = np.arange(len(kept))
+            dst.append(np.asarray(fresh, dtype=np.int64)[at // ps] * ps + at % ps)
+            seq["old_pages"], seq["page_table"] = seq["page_table"], fresh
+            dropped += seq["len"] - len(kept)
+            seq["dropped"] = seq.get("dropped", 0) + seq["len"] - len(kept)
+            seq["len"] = len(kept)
+        if work:
+            src_t, dst_t = (torch.from_numpy(np.concatenate(x)) for x in (src, dst))
+            if self.k_pages.is_cuda:
+                move_tokens(self.k_pages, self.v_pages, src_t.to(self.k_pages.device), dst_t)
+            else:  # host-side pool
+                for pool in (self.k_pages, self.v_pages):
+                    pool[dst_t // ps, :, dst_t % ps] = pool[src_t // ps, :, src_t % ps]
+        for s, _ in work:
+            for page in self.sequences[s].pop("old_pages"):
+                self._release(page)
+        return dropped
 
     @property
     def num_free_pages(self) -> int:
@@ -160,8 +369,10 @@ class PagedKVCache:
         return self.max_pages * self.page_size
 
     # ---- device views for the decode kernel ----
-    def block_table(self, seq_ids: Sequence[int], device=None) -> Tuple[torch.Tensor, torch.Tensor]:
-        """(block_table int32 [R, max_pages_of_batch], ctx_lens int32 [R]) on `device`."""
+    def block_table(self, seq_ids: Sequence[int], device=None, *, sliding_window: Optional[int] = None,
+                    sink_tokens: int = 0) -> Tuple[torch.Tensor, torch.Tensor]:
+        """(block_table int32 [R, max_pages_of_batch], ctx_lens int32 [R]) on
+        `device`.  With a window, pages outside it may have been freed."""
         device = device or self.k_pages.device
         tables = [self.sequences[s]["page_table"] for s in seq_ids]
         width = max(1, max(len(t) for t in tables))
@@ -170,15 +381,18 @@ class PagedKVCache:
             if t:
                 bt[i, :len(t)] = torch.tensor(t, dtype=torch.int32)
         lens = torch.tensor([self.sequences[s]["len"] for s in seq_ids], dtype=torch.int32)
-        check_block_table(bt, lens, self.max_pages, self.page_size)
+        check_block_table(bt, lens, self.max_pages, self.page_size, sliding_window, sink_tokens)
         return bt.to(device), lens.to(device)
 
     def decode(self, q: torch.Tensor, seq_ids: Sequence[int], *, scale: Optional[float] = None,
-               softcap: Optional[float] = None, return_lse: bool = False):
-        """One-token attention of q [R, Hq, D] over each sequence's cached K/V."""
+               softcap: Optional[float] = None, return_lse: bool = False, sliding_window: Optional[int] = None,
+               sink_tokens: int = 0):
+        """One-token attention of q [R, Hq, D] over each sequence's cached K/V
+        (with a window: over its last tokens and the first sink_tokens)."""
         from .decode import paged_decode
 
-        bt, lens = self.block_table(seq_ids, q.device)
+        bt, lens = self.block_table(seq_ids, q.device, sliding_window=sliding_window, sink_tokens=sink_tokens)
         max_ctx = max(self.sequences[s]["len"] for s in seq_ids)
         return paged_decode(q, self.k_pages, self.v_pages, bt, lens, scale=scale, softcap=softcap,
-                            return_lse=return_lse, max_ctx=max_ctx)
+                            return_lse=return_lse, max_ctx=max_ctx, sliding_window=sliding_window,
+                            sink_tokens=sink_tokens)

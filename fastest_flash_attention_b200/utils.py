@@ -68,3 +68,11 @@ def repeat_kv(kv: torch.Tensor, num_q_heads: int, num_kv_heads: int) -> torch.Te
     ratio = num_q_heads // num_kv_heads
     B, H_kv, S, D = kv.shape
     return kv[:, :, None, :, :].expand(B, H_kv, ratio, S, D).reshape(B, num_q_heads, S, D)
+
+
+def check_window(sliding_window, sink_tokens) -> None:
+    """Raise for a sliding window or a count of first tokens kept visible that means nothing."""
+    if sink_tokens < 0:
+        raise ValueError(f"sink_tokens must not be negative, got {sink_tokens}")
+    if sliding_window is not None and sliding_window <= 0:
+        raise ValueError(f"sliding_window must be positive, got {sliding_window}")

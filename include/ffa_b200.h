@@ -56,7 +56,8 @@ const char* ffa_last_error(void);
  * into a caller-provided uint32 in device memory (nullptr disables it), and
  * invalid data they find: 0x3E0 a decode context length outside
  * [0, max_pages_per_req * page_size], 0x3E1 a block-table page id outside
- * [0, num_pages), 0x1FF a block mask keeping more key tiles than the forward's
+ * [0, num_pages), 0x3E2 a page id or slot of a copy outside the pool, 0x3E3 a
+ * rotary position outside the tables, 0x1FF a block mask keeping more key tiles than the forward's
  * tile list holds (the offending loads are skipped; treat the call as failed).
  * ffa_read_error copies it to *out (synchronising `stream`). */
 int ffa_read_error(const uint32_t* dev_err, uint32_t* out, void* stream);
@@ -241,6 +242,58 @@ int ffa_mla_latent_append(const void* lat, int64_t lat_row_stride, const void* k
 int ffa_paged_append(const void* k_new, const void* v_new, void* k_pages, void* v_pages, const int* slots,
                      int dtype, int n_tokens, int Hkv, int D, int page_size, int num_pages,
                      const int64_t* new_strides, void* stream);
+
+/* ----------------------------------------------------------------------------
+ * Copies inside paged-KV pools (no counterpart in the reference, whose paged
+ * cache only appends and frees): the bytes of a forked sequence's last page,
+ * of a defragmentation, of a sequence compacted to its window.
+ *   ffa_page_copy   pages src[i] -> dst[i] of page_bytes each, in k_pages and
+ *                   (unless NULL) v_pages
+ *   ffa_token_move  token rows (all Hkv heads) of row_bytes each from slot
+ *                   src_slots[i] to dst_slots[i], slot = page * page_size +
+ *                   offset, pools [num_pages, Hkv, page_size, row_bytes]
+ * Destinations are distinct and none of them is a source.  An id outside the
+ * pool leaves its entry out and records 0x3E2 in *dev_err.  page_bytes and
+ * row_bytes are even; multiples of 16 take 16-byte copies.  One launch.
+ * ------------------------------------------------------------------------- */
+int ffa_page_copy(void* k_pages, void* v_pages, const int* src, const int* dst, int n, int num_pages,
+                  int64_t page_bytes, uint32_t* dev_err, void* stream);
+
+int ffa_token_move(void* k_pages, void* v_pages, const int* src_slots, const int* dst_slots, int n, int Hkv,
+                   int page_size, int num_pages, int row_bytes, uint32_t* dev_err, void* stream);
+
+/* ----------------------------------------------------------------------------
+ * Rotary positions.  The reference's rotary (modules/flash_mla.py:29-52) is a
+ * chain of torch operations inside its MLA module; these serve q and k of any
+ * attention.  For each pair (a, b) of a head's first `rot` values (even, <= D)
+ *   (a, b) -> (a cos - b sin, b cos + a sin);  the rest passes through,
+ * pairs (i, i + rot/2), or (2i, 2i+1) with interleaved != 0; inverse != 0
+ * turns by the negative angle (the gradient).
+ *   cos, sin: fp32 [table_len, rot/2] contiguous; pos: int32 (int64 with
+ *   pos64 != 0) token positions; one outside [0, table_len) passes its token
+ *   through and records 0x3E3 in *dev_err.
+ *   dtype F16, BF16 or F32 (fp32 arithmetic, rounded once).
+ *
+ * ffa_rotary: q [B, Hq, S, D] and k [B, Hkv, S, D] (Hkv = 0: none) with
+ *   strides {batch, head, token} for inputs and outputs (in place allowed);
+ *   pos [S], or [B, S] with pos_batch_stride elements between rows.
+ * ffa_rotary_append: one launch for n_tokens new tokens of a paged cache:
+ *   q [n_tokens, Hq, D] -> q_out (strides {token, head}); k turned and v as it
+ *   is ([n_tokens, Hkv, D]) into row slots[t] of the pools [num_pages, Hkv,
+ *   page_size, D]; a slot outside the pool writes no row.  pos [n_tokens].
+ * ------------------------------------------------------------------------- */
+int ffa_rotary(const void* q, const int64_t* q_strides, void* q_out, const int64_t* qo_strides, const void* k,
+               const int64_t* k_strides, void* k_out, const int64_t* ko_strides, const float* cos,
+               const float* sin, int64_t table_len, const void* pos, int pos64, int64_t pos_batch_stride,
+               int dtype, int B, int S, int Hq, int Hkv, int D, int rot, int interleaved, int inverse,
+               uint32_t* dev_err, void* stream);
+
+int ffa_rotary_append(const void* q, const int64_t* q_strides, void* q_out, const int64_t* qo_strides,
+                      const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                      const float* cos, const float* sin, int64_t table_len, const void* pos, int pos64,
+                      const int* slots, void* k_pages, void* v_pages, int dtype, int n_tokens, int Hq, int Hkv,
+                      int D, int rot, int interleaved, int page_size, int num_pages, uint32_t* dev_err,
+                      void* stream);
 
 /* ----------------------------------------------------------------------------
  * Log-sum-exp merge of a partial attention result into a running one, for
