@@ -121,6 +121,14 @@ SIGNATURES: dict[str, tuple] = {
         _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,  # dtype n_tokens Hkv D page_size num_pages
         _c_i64p, _c_void_p,  # new_strides stream
     ]),
+    "ffa_window_decode": (_c_int, [
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,  # q k_pages v_pages block_table ctx_lens
+        _c_void_p, _c_void_p,  # out lse
+        _c_int, _c_int, _c_int, _c_int, _c_int,  # dtype R Hq Hkv D
+        _c_int, _c_int, _c_int,  # num_pages page_size max_pages_per_req
+        _c_i64p, _c_i64p, _c_float, _c_float,  # q_strides o_strides scale softcap
+        _c_int, _c_int, _c_int, _c_u32p, _c_void_p,  # window sinks max_ctx err stream
+    ]),
     "ffa_page_copy": (_c_int, [
         _c_void_p, _c_void_p, _c_void_p, _c_void_p,  # k_pages v_pages src dst
         _c_int, _c_int, ctypes.c_int64, _c_u32p, _c_void_p,  # n num_pages page_bytes err stream
@@ -188,8 +196,17 @@ def i64arr(*vals: int):
     return (ctypes.c_int64 * len(vals))(*vals)
 
 
+_I64X3 = ctypes.c_int64 * 3
+
+
+def strides3(t: torch.Tensor):
+    """The first three strides of a 4-D tensor, for an entry point's {batch, head, token} argument."""
+    return _I64X3(*t.stride()[:3])
+
+
 def stream_of(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+    # the raw handle: building a Stream object costs over 2 us a call
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
 _HERE = contextlib.nullcontext()

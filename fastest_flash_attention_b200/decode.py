@@ -6,6 +6,10 @@ S_q = 1 (ops/attention_forward.py:23).  ``paged_decode`` computes the same
 attention directly from the page pool: a split-KV kernel reads every K/V
 byte of the context once per kv head (all query heads of a GQA group share
 the read) and a merge kernel combines the splits by LSE.
+
+With ``sliding_window`` a request attends its last tokens and, with
+``sink_tokens``, its first ones (no counterpart in the reference): one launch
+that reads those tokens' K/V alone, so pages outside may have been freed.
 """
 from __future__ import annotations
 
@@ -15,6 +19,7 @@ from typing import Optional
 import torch
 
 from . import _lib
+from .utils import check_window
 
 
 def default_chunks_per_split(ctx_max: int, R: int, Hkv: int, num_sms: int = 148) -> int:
@@ -57,13 +62,25 @@ def check_block_table(block_table: torch.Tensor, ctx_lens: torch.Tensor, num_pag
 
 def paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
                  ctx_lens: torch.Tensor, *, scale: Optional[float] = None, softcap: Optional[float] = None,
-                 return_lse: bool = False, chunks_per_split: Optional[int] = None, max_ctx: Optional[int] = None):
+                 return_lse: bool = False, chunks_per_split: Optional[int] = None, max_ctx: Optional[int] = None,
+                 sliding_window: Optional[int] = None, sink_tokens: int = 0):
     """Decode attention for R requests.
 
     q [R, Hq, D]; k_pages/v_pages [P, Hkv, page_size, D] (contiguous);
     block_table [R, max_pages] int32; ctx_lens [R] int32 (device tensors).
     Returns o [R, Hq, D] (q's dtype) and, if requested, lse [R, Hq] fp32.
+
+    sliding_window: a request sees the last sliding_window tokens of its
+    context (the query's own token is the last of them) and its first
+    sink_tokens; without a window it sees all of them.  The windowed call takes
+    any page size, any group of query heads and head dims up to 128 (multiples
+    of 8); block-table entries of pages outside the window may be anything,
+    and chunks_per_split does not apply to it.
     """
+    check_window(sliding_window or None, sink_tokens)
+    if sliding_window:
+        return _window_decode(q, k_pages, v_pages, block_table, ctx_lens, scale, softcap, return_lse, max_ctx,
+                              sliding_window, sink_tokens)
     _lib.require_cuda(q, k_pages, v_pages, block_table, ctx_lens)
     R, Hq, D = q.shape
     P, Hkv, page_size, Dk = k_pages.shape
@@ -97,6 +114,46 @@ def paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
             float(scale), float(softcap or 0.0), int(chunks_per_split), ws.data_ptr(), ws_bytes,
             _lib.err_word(q.device).data_ptr(), _lib.stream_of(q))
     _lib.check(st, "ffa_paged_decode")
+    if _lib.sync_check_enabled():
+        _lib.check_device_errors(q.device)
+    return (out, lse) if return_lse else out
+
+
+def _window_decode(q, k_pages, v_pages, block_table, ctx_lens, scale, softcap, return_lse, max_ctx, window, sinks):
+    _lib.require_cuda(q, k_pages, v_pages, block_table, ctx_lens)
+    if q.dim() != 3 or k_pages.dim() != 4:
+        raise ValueError(f"q must be [R, Hq, D] and the pools [P, Hkv, page_size, D], got {tuple(q.shape)} and "
+                         f"{tuple(k_pages.shape)}")
+    R, Hq, D = q.shape
+    P, Hkv, page_size, Dk = k_pages.shape
+    if Dk != D or v_pages.shape != k_pages.shape:
+        raise ValueError("q / page pool head dims disagree")
+    if Hq % Hkv:
+        raise ValueError(f"query heads ({Hq}) must be a multiple of key/value heads ({Hkv})")
+    if D % 8 or D > 128:
+        raise ValueError(f"windowed decode takes head dims up to 128 that are multiples of 8, got {D}")
+    if q.dtype not in _lib.DTYPE_CODE or k_pages.dtype != q.dtype or v_pages.dtype != q.dtype:
+        raise ValueError("paged_decode needs fp16/bf16 q and pages of the same dtype")
+    if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
+        raise ValueError("page pools must be contiguous")
+    if block_table.dim() != 2 or block_table.shape[0] != R or tuple(ctx_lens.shape) != (R,):
+        raise ValueError("block_table must be [R, max_pages] and ctx_lens [R]")
+    bt = block_table.to(torch.int32).contiguous()
+    lens = ctx_lens.to(torch.int32).contiguous()
+    if q.stride(2) != 1 or q.stride(0) % 2 or q.stride(1) % 2 or q.data_ptr() % 4:
+        q = q.contiguous()
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    big = 2 ** 31 - 1  # a window of any length: the kernel's is 32 bits, contexts fit it
+    out = torch.empty((R, Hq, D), dtype=q.dtype, device=q.device)
+    lse = torch.empty((R, Hq), dtype=torch.float32, device=q.device) if return_lse else None
+    with _lib.device_of(q):
+        st = _lib.load().ffa_window_decode(
+            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), bt.data_ptr(), lens.data_ptr(), out.data_ptr(),
+            lse.data_ptr() if return_lse else None, _lib.DTYPE_CODE[q.dtype], R, Hq, Hkv, D, P, page_size,
+            bt.shape[1], _lib.i64arr(q.stride(0), q.stride(1)), _lib.i64arr(Hq * D, D), scale, softcap or 0.0,
+            min(window, big), min(sinks, big), max_ctx or 0, _lib.err_word(q.device).data_ptr(), _lib.stream_of(q))
+    _lib.check(st, "ffa_window_decode")
     if _lib.sync_check_enabled():
         _lib.check_device_errors(q.device)
     return (out, lse) if return_lse else out

@@ -94,12 +94,12 @@ def _rotate(q: torch.Tensor, k: Optional[torch.Tensor], cos: torch.Tensor, sin: 
     B, Hq, S, D = q.shape
     q = _unit_last(q)
     qo = torch.empty_like(q)
-    qs, qd = _lib.i64arr(*q.stride()[:3]), _lib.i64arr(*qo.stride()[:3])
+    qs, qd = _lib.strides3(q), _lib.strides3(qo)
     if k is not None:
         k = _unit_last(k)
         ko = torch.empty_like(k)
         Hkv, kptr, koptr = k.shape[1], k.data_ptr(), ko.data_ptr()
-        ks, kd = _lib.i64arr(*k.stride()[:3]), _lib.i64arr(*ko.stride()[:3])
+        ks, kd = _lib.strides3(k), _lib.strides3(ko)
     else:
         ko, Hkv, kptr, koptr, ks, kd = None, 0, None, None, None, None
     with _lib.device_of(q):

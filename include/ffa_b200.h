@@ -179,6 +179,23 @@ int ffa_paged_decode(const void* q, const void* k_pages, const void* v_pages, co
                      size_t workspace_bytes, uint32_t* dev_err, void* stream);
 
 /* ----------------------------------------------------------------------------
+ * Paged decode over a sliding window and the first tokens (no counterpart in
+ * the reference).  As ffa_paged_decode, but request r attends the last
+ * `window` (> 0) of its ctx_lens[r] tokens and the first `sinks` of them, and
+ * only those tokens' table entries and K/V rows are read: pages outside both
+ * may have been freed.  Any page_size and group size, D a multiple of 8 up to
+ * 128.  max_ctx (0: not known) bounds the context lengths for the choice of
+ * the split.  A request that sees nothing (length 0) gets 0 and LSE -inf.
+ * One launch on `stream`, no workspace: a cluster of CTAs splits a request's
+ * tokens and joins them through distributed shared memory.
+ * ------------------------------------------------------------------------- */
+int ffa_window_decode(const void* q, const void* k_pages, const void* v_pages, const int* block_table,
+                      const int* ctx_lens, void* out, float* lse, int dtype, int R, int Hq, int Hkv, int D,
+                      int num_pages, int page_size, int max_pages_per_req, const int64_t* q_strides,
+                      const int64_t* o_strides, float scale, float softcap, int window, int sinks, int max_ctx,
+                      uint32_t* dev_err, void* stream);
+
+/* ----------------------------------------------------------------------------
  * MLA absorbed decode.  Replaces modules/flash_mla.py:116 FastestFlashMLA
  * forward for one new token per request (the reference re-runs the whole
  * prefix through up-projections; here W_UK is folded into the query and
