@@ -74,6 +74,22 @@ SIGNATURES: dict[str, tuple] = {
         _c_void_p, _c_int, _c_int, _c_int, _c_int,  # block_mask n_br n_bc bq bkv
         _c_void_p, _c_size_t, _c_u32p, _c_void_p,  # workspace bytes err stream
     ]),
+    "ffa_fwd_sink": (_c_int, [
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,  # q k v o lse
+        _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,  # dtype B Hq Hkv Sq Skv D Dv
+        _c_i64p, _c_i64p, _c_i64p, _c_i64p,  # strides
+        _c_float, _c_int, _c_int, _c_int, _c_int, _c_float,  # scale causal q_offset window sinks softcap
+        _c_u32p, _c_void_p,  # err stream
+    ]),
+    "ffa_bwd_sink_workspace_size": (_c_size_t, [_c_int] * 9),  # B Hq Hkv Sq Skv D Dv window sinks
+    "ffa_bwd_sink": (_c_int, [
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,  # dout q k v o lse
+        _c_void_p, _c_void_p, _c_void_p,  # dq dk dv
+        _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,  # dtype B Hq Hkv Sq Skv D Dv
+        _c_i64p, _c_i64p, _c_i64p, _c_i64p, _c_i64p, _c_i64p, _c_i64p, _c_i64p,  # strides q k v o do dq dk dv
+        _c_float, _c_int, _c_int, _c_int, _c_int, _c_float,  # scale causal q_offset window sinks softcap
+        _c_void_p, _c_size_t, _c_u32p, _c_void_p,  # workspace bytes err stream
+    ]),
     "ffa_bwd_noalloc": (_c_int, [
         _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,  # dout q k v o lse
         _c_void_p, _c_void_p, _c_void_p,  # dq dk dv

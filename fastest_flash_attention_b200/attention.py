@@ -75,15 +75,29 @@ def _tma_ready(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
 
 
 def _strides_bhs(t: torch.Tensor):
-    return _lib.i64arr(t.stride(0), t.stride(1), t.stride(2))
+    return _lib.strides3(t)
+
+
+def _sinks(window: Optional[int], sink: int, block_mask: Optional[torch.Tensor]) -> int:
+    """First keys kept visible outside the window, 0 where they change nothing."""
+    if sink < 0:
+        raise ValueError(f"sink_tokens must not be negative, got {sink}")
+    if not sink or not window or window < 0:
+        return 0
+    if block_mask is not None:
+        raise ValueError("sink_tokens with a sliding window take no block_mask")
+    return min(int(sink), 2 ** 31 - 1)
 
 
 def flash_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float, causal: bool = False,
               q_offset: int = 0, window: Optional[int] = None, softcap: Optional[float] = None,
               block_mask: Optional[torch.Tensor] = None, mask_block: Tuple[int, int] = (64, 64),
-              compute_dtype: Optional[torch.dtype] = None, want_lse: bool = True
+              compute_dtype: Optional[torch.dtype] = None, want_lse: bool = True, sink: int = 0
               ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """Run the sm_100a forward kernel on 4-D [B, H, S, D] tensors.
+
+    sink: keys [0, sink) stay visible outside the window (as far as causality
+    allows); without a window they are visible anyway.
 
     Returns (O in the kernel dtype with q's stride order, LSE [B, Hq, Sq] fp32).
     """
@@ -99,12 +113,13 @@ def flash_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float
     if kdims is None:
         raise ValueError(f"head dims (qk={D}, v={Dv}) not supported by the sm_100a forward kernel "
                          f"(supported: qk <= {MAX_HEAD_DIM}, v <= 128)")
+    sink = _sinks(window, sink, block_mask)
     dt = kernel_dtype(q, compute_dtype)
     if kdims != (D, Dv):
         o, lse = flash_fwd(_pad_last(q.to(dt), kdims[0]), _pad_last(k.to(dt), kdims[0]),
                            _pad_last(v.to(dt), kdims[1]), scale=scale, causal=causal, q_offset=q_offset,
                            window=window, softcap=softcap, block_mask=block_mask, mask_block=mask_block,
-                           compute_dtype=compute_dtype, want_lse=want_lse)
+                           compute_dtype=compute_dtype, want_lse=want_lse, sink=sink)
         return o[..., :Dv], lse
     q = _tma_ready(q, dt)
     k = _tma_ready(k, dt)
@@ -120,15 +135,18 @@ def flash_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float
         n_br, n_bc = bm.shape
         bm_ptr = bm.data_ptr()
     lib = _lib.load()
-    with torch.cuda.device(q.device):
-        st = lib.ffa_fwd(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr() if lse is not None else None,
-            _ATTN_DTYPE_CODE[dt], B, Hq, Hkv, Sq, Skv, D, Dv,
-            _strides_bhs(q), _strides_bhs(k), _strides_bhs(v), _strides_bhs(o),
-            float(scale), int(bool(causal)), int(q_offset), int(window or 0), float(softcap or 0.0),
-            bm_ptr, n_br, n_bc, int(mask_block[0]), int(mask_block[1]),
-            _lib.err_word(q.device).data_ptr(), _lib.stream_of(q))
-    _lib.check(st, "ffa_fwd")
+    operands = (q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr() if lse is not None else None,
+                _ATTN_DTYPE_CODE[dt], B, Hq, Hkv, Sq, Skv, D, Dv,
+                _strides_bhs(q), _strides_bhs(k), _strides_bhs(v), _strides_bhs(o),
+                float(scale), int(bool(causal)), int(q_offset), int(window or 0))
+    tail = (_lib.err_word(q.device).data_ptr(), _lib.stream_of(q))
+    with _lib.device_of(q):
+        if sink:
+            st = lib.ffa_fwd_sink(*operands, sink, float(softcap or 0.0), *tail)
+        else:
+            st = lib.ffa_fwd(*operands, float(softcap or 0.0), bm_ptr, n_br, n_bc, int(mask_block[0]),
+                             int(mask_block[1]), *tail)
+    _lib.check(st, "ffa_fwd_sink" if sink else "ffa_fwd")
     if block_mask is not None:
         bm.record_stream(torch.cuda.current_stream(q.device))
     if _lib.sync_check_enabled():
@@ -153,6 +171,7 @@ def fastest_flash_attn_forward(
     num_kv_heads: Optional[int] = None,
     kv_cache: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
     return_lse: bool = False,
+    sink_tokens: int = 0,
 ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """Forward attention (ops/attention_forward.py:23-167).
 
@@ -161,6 +180,10 @@ def fastest_flash_attn_forward(
     GQA/MQA (H_q a multiple of H_kv) is handled natively without repeating
     K/V; ``num_kv_heads`` is accepted for compatibility.  ``two_pass`` needs
     no second pass here: the kernel's LSE is already exact.
+
+    ``sink_tokens`` (not in the reference): the first keys, which stay visible
+    outside ``sliding_window`` as far as causality allows; they take no
+    ``block_mask``.
     """
     if config is not None:  # attention_forward.py:66-73
         causal = config.causal
@@ -170,6 +193,7 @@ def fastest_flash_attn_forward(
         compute_dtype = config.compute_dtype
         num_kv_heads = config.num_kv_heads
         return_lse = config.return_lse
+        sink_tokens = config.sink_tokens
 
     in_dtype = q.dtype
     q, k, v, squeezed = maybe_unsqueeze_head(q, k, v)
@@ -199,7 +223,7 @@ def fastest_flash_attn_forward(
 
     o, lse = flash_fwd(q, k, v, scale=scale, causal=causal, q_offset=q_offset, window=sliding_window,
                        softcap=softcap, block_mask=block_mask, mask_block=(bq, bkv),
-                       compute_dtype=compute_dtype, want_lse=return_lse)
+                       compute_dtype=compute_dtype, want_lse=return_lse, sink=sink_tokens)
     if o.dtype != in_dtype:
         o = o.to(in_dtype)
     if lse is not None:
@@ -215,12 +239,13 @@ def flash_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Ten
               lse: torch.Tensor, *, scale: float, causal: bool = False, q_offset: int = 0,
               window: Optional[int] = None, softcap: Optional[float] = None,
               block_mask: Optional[torch.Tensor] = None, mask_block: Tuple[int, int] = (64, 64),
-              compute_dtype: Optional[torch.dtype] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+              compute_dtype: Optional[torch.dtype] = None, sink: int = 0
+              ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Run the deterministic sm_100a backward on 4-D tensors.
 
     lse: [B, Hq, Sq] (or [B, Hq, Sq, 1]) natural-log LSE from the forward.
     block_mask / mask_block: the tile mask the forward was given (masked
-    pairs contribute nothing to any gradient).
+    pairs contribute nothing to any gradient); sink: its visible first keys.
     Returns (dq, dk, dv) in the kernel dtype; dk/dv have k's head count
     (GQA groups are summed inside the kernel).
     """
@@ -234,6 +259,7 @@ def flash_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Ten
                          f"(supported: qk <= {MAX_HEAD_DIM}, v <= 128)")
     if Hq % Hkv != 0:
         raise ValueError(f"query heads ({Hq}) must be a multiple of key/value heads ({Hkv})")
+    sink = _sinks(window, sink, block_mask)
     dt = kernel_dtype(q, compute_dtype)
     if kdims != (D, Dv):
         # zero columns: Delta, dP and the kept gradient columns are unchanged
@@ -241,7 +267,7 @@ def flash_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Ten
         dq, dk, dv = flash_bwd(_pad_last(dout.to(dt), kv), _pad_last(q.to(dt), kd), _pad_last(k.to(dt), kd),
                                _pad_last(v.to(dt), kv), _pad_last(o.to(dt), kv), lse, scale=scale, causal=causal,
                                q_offset=q_offset, window=window, softcap=softcap, block_mask=block_mask,
-                               mask_block=mask_block, compute_dtype=compute_dtype)
+                               mask_block=mask_block, compute_dtype=compute_dtype, sink=sink)
         return dq[..., :D], dk[..., :D], dv[..., :Dv]
     q, k, v, o, dout = (_tma_ready(t, dt) for t in (q, k, v, o, dout))
     if lse.dim() == 4:
@@ -251,20 +277,26 @@ def flash_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Ten
     dk = torch.empty_like(k)
     dv = torch.empty_like(v)
     lib = _lib.load()
-    ws_bytes = lib.ffa_bwd_workspace_size(B, Hq, Sq)
+    if sink:
+        ws_bytes = lib.ffa_bwd_sink_workspace_size(B, Hq, Hkv, Sq, Skv, D, Dv, window, sink)
+    else:
+        ws_bytes = lib.ffa_bwd_workspace_size(B, Hq, Sq)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
     common = (dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(),
               dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ATTN_DTYPE_CODE[dt], B, Hq, Hkv, Sq, Skv, D, v.shape[3],
               _strides_bhs(q), _strides_bhs(k), _strides_bhs(v), _strides_bhs(o), _strides_bhs(dout),
               _strides_bhs(dq), _strides_bhs(dk), _strides_bhs(dv),
-              float(scale), int(bool(causal)), int(q_offset), int(window or 0), float(softcap or 0.0))
+              float(scale), int(bool(causal)), int(q_offset), int(window or 0))
+    cap = float(softcap or 0.0)
     tail = (ws.data_ptr(), ws_bytes, _lib.err_word(q.device).data_ptr(), _lib.stream_of(q))
-    with torch.cuda.device(q.device):
-        if block_mask is None:
-            st = lib.ffa_bwd(*common, *tail)
+    with _lib.device_of(q):
+        if sink:
+            st = lib.ffa_bwd_sink(*common, sink, cap, *tail)
+        elif block_mask is None:
+            st = lib.ffa_bwd(*common, cap, *tail)
         else:
             bm = block_mask.to(device=q.device, dtype=torch.uint8).contiguous()
-            st = lib.ffa_bwd_masked(*common, bm.data_ptr(), bm.shape[0], bm.shape[1], int(mask_block[0]),
+            st = lib.ffa_bwd_masked(*common, cap, bm.data_ptr(), bm.shape[0], bm.shape[1], int(mask_block[0]),
                                     int(mask_block[1]), *tail)
             bm.record_stream(torch.cuda.current_stream(q.device))
     _lib.check(st, "ffa_bwd")
@@ -288,6 +320,7 @@ def fastest_flash_attn_backward(
     sliding_window: Optional[int] = None,
     q_offset: int = 0,
     block_mask: Optional[torch.Tensor] = None,
+    sink_tokens: int = 0,
 ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Backward (ops/attention_backward.py:19-76): (dq, dk, dv) from the
     forward's output and LSE, recomputing the attention tile by tile.
@@ -295,13 +328,13 @@ def fastest_flash_attn_backward(
     ``block_size`` sets the granularity of ``block_mask`` (as in the forward);
     the kernel's own tiles are fixed.  ``block_mask`` goes beyond the
     reference, whose backward ignores it: given the forward's mask, the
-    gradients are those of the masked forward.  Gradients come back in the
-    dtypes of q, k and v.
+    gradients are those of the masked forward; so are those of a forward with
+    ``sink_tokens``.  Gradients come back in the dtypes of q, k and v.
     """
     bs = block_size if block_size is not None else auto_select_block_size(q.shape[-2], k.shape[-2], q.shape[-1])
     dq, dk, dv = flash_bwd(grad_output, q, k, v, output, lse, scale=scale if scale is not None else
                            1.0 / math.sqrt(q.shape[-1]), causal=causal, q_offset=q_offset, window=sliding_window,
-                           softcap=softcap, block_mask=block_mask, mask_block=(bs, bs))
+                           softcap=softcap, block_mask=block_mask, mask_block=(bs, bs), sink=sink_tokens)
     return dq.to(q.dtype), dk.to(k.dtype), dv.to(v.dtype)
 
 
@@ -311,10 +344,12 @@ class FastestFlashAttnFunc(Function):
     Accepts GQA (fewer K/V heads than query heads) natively."""
 
     @staticmethod
-    def forward(ctx, q, k, v, scale, causal, block_size, softcap, sliding_window, two_pass, block_mask=None):
+    def forward(ctx, q, k, v, scale, causal, block_size, softcap, sliding_window, two_pass, block_mask=None,
+                sink_tokens=0):
         output, lse = fastest_flash_attn_forward(
             q, k, v, scale=scale, causal=causal, block_size=block_size, softcap=softcap,
-            sliding_window=sliding_window, two_pass=two_pass, block_mask=block_mask, return_lse=True)
+            sliding_window=sliding_window, two_pass=two_pass, block_mask=block_mask, return_lse=True,
+            sink_tokens=sink_tokens)
         ctx.save_for_backward(q, k, v, output, lse)
         ctx.block_mask = block_mask
         ctx.scale = scale
@@ -322,6 +357,7 @@ class FastestFlashAttnFunc(Function):
         ctx.block_size = block_size
         ctx.softcap = softcap
         ctx.sliding_window = sliding_window
+        ctx.sink_tokens = sink_tokens
         return output
 
     @staticmethod
@@ -332,10 +368,11 @@ class FastestFlashAttnFunc(Function):
             q, k, v, output, lse, grad_output = (t.unsqueeze(1) for t in (q, k, v, output, lse, grad_output))
         dq, dk, dv = fastest_flash_attn_backward(
             grad_output, q, k, v, output, lse, scale=ctx.scale, causal=ctx.causal, block_size=ctx.block_size,
-            softcap=ctx.softcap, sliding_window=ctx.sliding_window, block_mask=ctx.block_mask)
+            softcap=ctx.softcap, sliding_window=ctx.sliding_window, block_mask=ctx.block_mask,
+            sink_tokens=ctx.sink_tokens)
         if was_3d:
             dq, dk, dv = dq.squeeze(1), dk.squeeze(1), dv.squeeze(1)
-        return dq, dk, dv, None, None, None, None, None, None, None
+        return dq, dk, dv, None, None, None, None, None, None, None, None
 
 
 def fastest_flash_attn_func(
@@ -349,9 +386,11 @@ def fastest_flash_attn_func(
     sliding_window: Optional[int] = None,
     two_pass: bool = False,
     block_mask: Optional[torch.Tensor] = None,
+    sink_tokens: int = 0,
 ) -> torch.Tensor:
     """Differentiable attention (ops/attention_func.py:93-125).  The trailing
-    ``block_mask`` (tiles of ``block_size``) is an addition: the reference's
-    autograd path has no block mask."""
+    ``block_mask`` (tiles of ``block_size``) and ``sink_tokens`` (first keys
+    that stay visible outside the window) are additions: the reference's
+    autograd path has neither."""
     return FastestFlashAttnFunc.apply(q, k, v, scale, causal, block_size, softcap, sliding_window, two_pass,
-                                      block_mask)
+                                      block_mask, sink_tokens)

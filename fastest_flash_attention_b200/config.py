@@ -32,6 +32,7 @@ class AttentionConfig:
     max_seqlen_q: int = 0
     max_seqlen_kv: int = 0
     page_size: int = 64
+    sink_tokens: int = 0  # first keys that stay visible outside sliding_window (not in the reference)
 
     def resolve_block_sizes(self, S_q: int, S_kv: int, D: int) -> Tuple[int, int]:
         """(block_q, block_kv), auto-selecting either that is 0 (config.py:75-81)."""

@@ -68,6 +68,13 @@ struct BwdParams {
   float sc_poly[3];    // softcap_small2 coefficients for k = sc_pre
   int use_softcap;
   int causal, window;
+  // SINK kernels: keys [0, sink) stay visible outside the window.  The key
+  // tiles that hold them, [0, n_sink_tiles), see every later query: sink_parts
+  // CTAs share such a tile's queries and leave fp32 sums in sink_ws
+  // [B * Hkv, n_sink_tiles, sink_parts, 128, DV + D], which a last launch adds
+  // up in order.
+  int sink, n_sink_tiles, sink_parts;
+  float* sink_ws;
   // optional tile mask [n_br, n_bc] of (mask_bq x mask_bkv) blocks, the one
   // the forward was given: masked pairs get P = 0 (nullptr: none)
   const uint8_t* block_mask;
@@ -88,6 +95,7 @@ enum : uint32_t {
 };
 
 // 64-row query sub-tiles [i_lo, i_hi) that interact with 128-key tile j.
+template <bool SINK>
 __device__ __forceinline__ void q_range_for_key_tile(const BwdParams& p, int j, int& i_lo, int& i_hi) {
   const int n_q = (p.Sq + BWD_BS - 1) / BWD_BS;
   const int k_lo = j * BWD_BT, k_hi = min(k_lo + BWD_BT, p.Skv) - 1;
@@ -97,7 +105,7 @@ __device__ __forceinline__ void q_range_for_key_tile(const BwdParams& p, int j, 
     const int qmin = k_lo - p.q_offset;
     i_lo = qmin > 0 ? min(qmin / BWD_BS, n_q) : 0;
   }
-  if (p.window > 0) {  // need some q_abs <= k_hi + window - 1
+  if (p.window > 0 && !(SINK && j < p.n_sink_tiles)) {  // need some q_abs <= k_hi + window - 1
     const int qmax = k_hi + p.window - 1 - p.q_offset;
     i_hi = qmax < 0 ? 0 : min(n_q, qmax / BWD_BS + 1);
   }
@@ -571,7 +579,9 @@ struct DkdvCfg {
 // The dK/dV epilogue at D = DV = 128 stages 16 warp boxes of 4 KB in the stage smem.
 static_assert(DkdvCfg<128, 128>::NS * DkdvCfg<128, 128>::STAGE >= 16 * 32 * 128, "dK/dV store staging");
 
-template <typename T, int D, int DV, bool BM>
+// SINK: the CTAs of the sink tiles' query shares come first, (b, kv head) by
+// (b, kv head), then the other key tiles in the plain order.
+template <typename T, int D, int DV, bool BM, bool SINK>
 __global__ void __launch_bounds__(BWD_THREADS, 1)
     ffa_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                         const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDO,
@@ -599,17 +609,37 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
   // (b, kv head) pairs in groups of p.grp_kv whose Q / dO stay in L2 while
   // the group's key tiles stream them; within a group key tiles go in order
   // (under causal masking the first ones see the most queries).
-  const int g0 = (int)(blockIdx.x / ((unsigned)p.grp_kv * n_j)) * p.grp_kv;
-  const int gn = min(p.grp_kv, BHk - g0);
-  const int rem = (int)blockIdx.x - g0 * n_j;
-  const int j = rem / gn;
-  const int bhk = g0 + rem % gn;
+  int j, bhk, part = -1;  // part: this CTA's share of a sink tile's queries
+  if (SINK) {
+    const int shares = BHk * p.n_sink_tiles * p.sink_parts;
+    if ((int)blockIdx.x < shares) {
+      bhk = (int)blockIdx.x % BHk;
+      j = (int)blockIdx.x / BHk % p.n_sink_tiles;
+      part = (int)blockIdx.x / BHk / p.n_sink_tiles;
+    } else {
+      const int rem = (int)blockIdx.x - shares;
+      bhk = rem % BHk;
+      j = p.n_sink_tiles + rem / BHk;
+    }
+  } else {
+    const int g0 = (int)(blockIdx.x / ((unsigned)p.grp_kv * n_j)) * p.grp_kv;
+    const int gn = min(p.grp_kv, BHk - g0);
+    const int rem = (int)blockIdx.x - g0 * n_j;
+    j = rem / gn;
+    bhk = g0 + rem % gn;
+  }
   const int b = bhk / p.Hkv, hkv = bhk % p.Hkv;
   const int group = p.Hq / p.Hkv;
   int i_lo, i_hi;
-  q_range_for_key_tile(p, j, i_lo, i_hi);
+  q_range_for_key_tile<SINK>(p, j, i_lo, i_hi);
   const int n_i = i_hi - i_lo;
-  const int n = n_i * group;  // units: (query head of the group, 64-row query sub-tile), head-major
+  // units: (query head of the group, 64-row query sub-tile), head-major; this
+  // CTA's are [u_lo, u_lo + n)
+  int n = n_i * group, u_lo = 0;
+  if (SINK && part >= 0) {
+    u_lo = (int)((int64_t)n * part / p.sink_parts);
+    n = (int)((int64_t)n * (part + 1) / p.sink_parts) - u_lo;
+  }
   constexpr uint32_t FMT = DtypeFmt<T>::value;
 
   if (threadIdx.x == 0) bwd_init_bars(bars, NS, 2 * 4);
@@ -638,7 +668,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
       for (int u = 0; u < n; ++u) {
         const int s = u % NS, use = u / NS;
         if (use > 0 && !mbar_wait(&bars->st_empty[s], (use - 1) & 1, p.ec, abort_flag, SITE_BWD_EMPTY)) break;
-        const int g = u / n_i, i = i_lo + u % n_i;
+        const int g = (u_lo + u) / n_i, i = i_lo + (u_lo + u) % n_i;
         const int h = hkv * group + g;
         mbar_arrive_expect_tx(&bars->st_full[s], Cfg::STAGE + 2 * BWD_BS * 4);
         uint8_t* dst = sStage + s * Cfg::STAGE;
@@ -746,13 +776,15 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
     // Kept query columns of this key, in absolute query positions minus q_offset:
     // causal keeps q >= key - q_offset, the window keeps q <= key + window - 1 - q_offset.
     const int q_keep_lo = p.causal ? key - p.q_offset : -0x3fffffff;
-    const int q_keep_hi = key >= p.Skv ? -0x40000000 : (p.window > 0 ? key + p.window - 1 - p.q_offset : 0x3fffffff);
+    const int q_keep_hi = key >= p.Skv ? -0x40000000
+                          : (p.window > 0 && !(SINK && key < p.sink)) ? key + p.window - 1 - p.q_offset
+                                                                     : 0x3fffffff;
     for (int u = pair; u < n && ok; u += 2) {
       ok = __all_sync(0xffffffffu, mbar_wait(&bars->sp_full[pair], (u >> 1) & 1, p.ec, abort_flag, SITE_BWD_SP));
       if (!ok) break;
       tc_fence_after();
       const int s = u % NS;
-      const int q0 = (i_lo + u % n_i) * BWD_BS + 32 * half;
+      const int q0 = (i_lo + (u_lo + u) % n_i) * BWD_BS + 32 * half;
       const int keep_lo = q_keep_lo - q0, keep_hi = q_keep_hi - q0;
       uint32_t bm_bits = ~0u;
       if (BM && key < p.Skv) {  // queries are the block mask's rows here
@@ -779,7 +811,25 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
     const uint32_t tacc = tmem + lane_off + TM_ACC + pair * DV;
     const float mul = pair ? p.scale : 1.f;
     const int ncol = pair ? D : DV;
-    if (D == 128 && DV == 128 && (have || n == 0)) {
+    if (SINK && part >= 0) {
+      // fp32 sums of this share of the queries
+      float* dst = p.sink_ws + ((((int64_t)bhk * p.n_sink_tiles + j) * p.sink_parts + part) * BWD_BT + r) * (DV + D) +
+                   pair * DV;
+#pragma unroll 1
+      for (int c = half * (ncol / 2); c < (half + 1) * (ncol / 2); c += 32) {
+        uint32_t v[32];
+        if (have) {
+          tmem_ld32(tacc + c, v);
+          tmem_ld_wait32(v);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = 0u;
+        }
+#pragma unroll
+        for (int e = 0; e < 32; e += 4)
+          *reinterpret_cast<uint4*>(dst + c + e) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+      }
+    } else if (D == 128 && DV == 128 && (have || n == 0)) {
       // Each warp packs its 32 rows x 64 columns into the (now idle) stage
       // smem in the 128-byte-swizzled layout and hands them to one TMA store,
       // so the CTA leaves once the copy has read the smem instead of once
@@ -881,7 +931,8 @@ struct DqCfg {
   static constexpr int SMEM = BAR_OFF + 256 + 1024;
 };
 
-template <typename T, int D, int DV, bool BM>
+// SINK: the units that hold sinks and lie left of the window's first come first.
+template <typename T, int D, int DV, bool BM, bool SINK>
 __global__ void __launch_bounds__(BWD_THREADS, 1)
     ffa_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                       const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDO,
@@ -921,7 +972,10 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
   constexpr int R = UK / BWD_BS;
   j_lo = j_lo / R;
   j_hi = (j_hi + R - 1) / R;
+  const int n_sink = SINK ? min((p.sink + UK - 1) / UK, j_lo) : 0;
+  j_lo -= n_sink;  // unit u >= n_sink is key unit j_lo + u
   const int n = max(0, j_hi - j_lo);
+  auto unit_at = [&](int u) -> int { return SINK && u < n_sink ? u : j_lo + u; };
   constexpr uint32_t FMT = DtypeFmt<T>::value;
 
   if (threadIdx.x == 0) bwd_init_bars(bars, 8, Cfg::WIDE ? 4 * 4 : 2 * 4);
@@ -951,7 +1005,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
       // then K (or {K, V}) into slot u % NSK
       int issued_k = 0, issued_v = 0;
       for (int u = 0; u < n; ++u) {
-        const int jj = j_lo + u;
+        const int jj = unit_at(u);
         if (Cfg::SPLIT) {
           const int sv = 4 + u % NSV, usev = u / NSV;
           if (usev > 0 && !mbar_wait(&bars->st_empty[sv], (usev - 1) & 1, p.ec, abort_flag, SITE_BWD_EMPTY)) break;
@@ -1069,15 +1123,21 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
       ok = __all_sync(0xffffffffu, mbar_wait(&bars->sp_full[bb], (u >> 1) & 1, p.ec, abort_flag, SITE_BWD_SP));
       if (!ok) break;
       tc_fence_after();
-      const int c0 = (j_lo + u) * UK + colw;
-      const int keep_lo = k_keep_lo - c0, keep_hi = k_keep_hi - c0;
+      const int c0 = unit_at(u) * UK + colw;
+      int keep_lo = k_keep_lo - c0, keep_hi = k_keep_hi - c0;
       uint32_t bm_bits = ~0u;
+      if (SINK && c0 < p.sink) {
+        // the window's range or the sinks before it: one keep bit per column
+        bm_bits = range_bits32(keep_lo, keep_hi) | range_bits32(0, min(keep_hi, p.sink - 1 - c0));
+        keep_lo = 0, keep_hi = 31;
+      }
       if (BM) {  // keys are the block mask's columns here
         const uint8_t* mrow = p.block_mask + (size_t)(min(row, p.Sq - 1) / p.mask_bq) * p.n_bc;
         bm_bits = block_mask_bits32(c0, p.mask_bkv, p.n_bc, [&](int bc) { return mrow[bc] != 0; });
       }
-      const bool masked = !__all_sync(0xffffffffu, keep_lo <= 0 && keep_hi >= 31 && (!BM || bm_bits == ~0u));
-      ok = bwd_unit<T, false, false, BM>(p, tS, tDP, &bars->tmem_free[bb], nullptr, nullptr, row_nl2, row_dl,
+      const bool masked =
+          !__all_sync(0xffffffffu, keep_lo <= 0 && keep_hi >= 31 && (!(BM || SINK) || bm_bits == ~0u));
+      ok = bwd_unit<T, false, false, BM || SINK>(p, tS, tDP, &bars->tmem_free[bb], nullptr, nullptr, row_nl2, row_dl,
                                          keep_lo, keep_hi, bm_bits, masked, &bars->pt_free[bb],
                                      u >= 2 ? ((u - 2) >> 1) & 1 : -1, abort_flag, nullptr, sDSw + bb * Cfg::DS, r,
                                      chunk_half);
@@ -1110,6 +1170,46 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
   }
 }
 
+
+// Adds up the query shares of the sink tiles, in order: one thread for four
+// columns of a key row of dV (then dK, times the softmax scale).
+template <typename T, int D, int DV>
+__global__ void __launch_bounds__(256) ffa_bwd_sink_sum_kernel(const BwdParams p) {
+  constexpr int V4 = (D + DV) / 4;
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = t / V4;
+  const int c = (int)(t % V4) * 4;
+  const int64_t tile = row / BWD_BT;  // (b, kv head) * n_sink_tiles + j
+  if (tile >= (int64_t)p.B * p.Hkv * p.n_sink_tiles) return;
+  const int j = (int)(tile % p.n_sink_tiles), bhk = (int)(tile / p.n_sink_tiles);
+  const int r = (int)(row % BWD_BT), key = j * BWD_BT + r;
+  if (key >= p.Skv) return;
+  const float* src = p.sink_ws + (tile * p.sink_parts * BWD_BT + r) * (D + DV) + c;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = 0; i < p.sink_parts; ++i) {
+    const float4 x = *reinterpret_cast<const float4*>(src + (int64_t)i * BWD_BT * (D + DV));
+    a.x += x.x, a.y += x.y, a.z += x.z, a.w += x.w;
+  }
+  const int b = bhk / p.Hkv, hkv = bhk % p.Hkv;
+  const bool is_k = c >= DV;
+  const float mul = is_k ? p.scale : 1.f;
+  T* dst = is_k ? reinterpret_cast<T*>(p.dk) + b * p.dk_sb + hkv * p.dk_sh + (int64_t)key * p.dk_ss + (c - DV)
+                : reinterpret_cast<T*>(p.dv) + b * p.dv_sb + hkv * p.dv_sh + (int64_t)key * p.dv_ss + c;
+  *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(a.x * mul, a.y * mul), pack2<T>(a.z * mul, a.w * mul));
+}
+
+// Key tiles that hold sinks, and the CTAs that share each one's queries: about
+// as many units (64-row query sub-tiles) per CTA as the window gives another
+// key tile, so that no CTA runs much longer than the rest.
+static void bwd_sink_shape(int Sq, int Skv, int window, int sink, int& tiles, int& parts) {
+  const int keys = sink < Skv ? sink : Skv;
+  tiles = (keys + BWD_BT - 1) / BWD_BT;
+  const int64_t n_q = ((int64_t)Sq + BWD_BS - 1) / BWD_BS;
+  const int64_t usual = ((int64_t)window + BWD_BT + BWD_BS - 1) / BWD_BS + 1;
+  int64_t n = (n_q + usual - 1) / usual;
+  if (n > 64) n = 64;
+  parts = (int)(n < 1 ? 1 : n);
+}
 
 // CTA-order group sizes (see the kernels' block mapping): groups whose
 // streamed operands fit in about 48 MB of L2 together, so each streamed tile
@@ -1149,7 +1249,7 @@ static void bwd_head_groups(BwdParams& p, int D, int DV) {
   if ((long long)(p.Sq + BWD_BT - 1) / BWD_BT * BH < 10LL * sms) p.grp_q = BH;
 }
 
-template <typename T, int D, int DV, bool BM>
+template <typename T, int D, int DV, bool BM, bool SINK>
 static int launch_bwd(const CUtensorMap* maps, const BwdParams& p, const void* o, const void* dout,
                       const float* lse, float* lse2, float* delta, const int64_t* o_str, const int64_t* do_str,
                       cudaStream_t st) {
@@ -1181,16 +1281,22 @@ static int launch_bwd(const CUtensorMap* maps, const BwdParams& p, const void* o
   if (s) return s;
   // 2. dK / dV
   {
-    auto kern = ffa_bwd_dkdv_kernel<T, D, DV, BM>;
+    auto kern = ffa_bwd_dkdv_kernel<T, D, DV, BM, SINK>;
     static std::atomic<uint64_t> done{0};
     if ((s = smem_attr_once(kern, DkdvCfg<D, DV>::SMEM, done))) return s;
-    const int grid = (p.Skv + BWD_BT - 1) / BWD_BT * p.B * p.Hkv;
+    const int tiles = (p.Skv + BWD_BT - 1) / BWD_BT;
+    const int grid = (SINK ? tiles - p.n_sink_tiles + p.n_sink_tiles * p.sink_parts : tiles) * p.B * p.Hkv;
     kern<<<grid, BWD_THREADS, DkdvCfg<D, DV>::SMEM, st>>>(maps[0], maps[1], maps[2], maps[3], maps[4], maps[5], p);
     if ((s = launch_status())) return s;
+    if (SINK) {
+      const int64_t threads_sum = (int64_t)p.B * p.Hkv * p.n_sink_tiles * BWD_BT * ((D + DV) / 4);
+      ffa_bwd_sink_sum_kernel<T, D, DV><<<(unsigned)((threads_sum + 255) / 256), 256, 0, st>>>(p);
+      if ((s = launch_status())) return s;
+    }
   }
   // 3. dQ
   {
-    auto kern = ffa_bwd_dq_kernel<T, D, DV, BM>;
+    auto kern = ffa_bwd_dq_kernel<T, D, DV, BM, SINK>;
     static std::atomic<uint64_t> done{0};
     if ((s = smem_attr_once(kern, DqCfg<D, DV>::SMEM, done))) return s;
     const int grid = (p.Sq + BWD_BT - 1) / BWD_BT * p.B * p.Hq;
@@ -1207,15 +1313,24 @@ extern "C" size_t ffa_bwd_workspace_size(int B, int Hq, int Sq) {
   return 2 * (size_t)B * Hq * sq_pad * sizeof(float) + 256;
 }
 
-extern "C" int ffa_bwd_masked(const void* dout, const void* q, const void* k, const void* v, const void* o,
-                              const float* lse, void* dq, void* dk, void* dv, int dtype, int B, int Hq, int Hkv,
-                              int Sq, int Skv, int D, int Dv, const int64_t* q_strides, const int64_t* k_strides,
-                              const int64_t* v_strides, const int64_t* o_strides, const int64_t* do_strides,
-                              const int64_t* dq_strides, const int64_t* dk_strides, const int64_t* dv_strides,
-                              float scale, int causal, int q_offset, int window, float softcap,
-                              const uint8_t* block_mask, int n_br, int n_bc, int mask_bq, int mask_bkv,
-                              void* workspace, size_t workspace_bytes, uint32_t* dev_err, void* stream) {
-  using namespace ffa;
+extern "C" size_t ffa_bwd_sink_workspace_size(int B, int Hq, int Hkv, int Sq, int Skv, int D, int Dv, int window,
+                                              int sinks) {
+  int tiles = 0, parts = 0;
+  ffa::bwd_sink_shape(Sq, Skv, window, sinks, tiles, parts);
+  return ffa_bwd_workspace_size(B, Hq, Sq) + 16 +
+         (size_t)B * Hkv * tiles * parts * ffa::BWD_BT * ((size_t)D + Dv) * sizeof(float);
+}
+
+namespace ffa {
+
+static int bwd_impl(const void* dout, const void* q, const void* k, const void* v, const void* o, const float* lse,
+                    void* dq, void* dk, void* dv, int dtype, int B, int Hq, int Hkv, int Sq, int Skv, int D, int Dv,
+                    const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                    const int64_t* o_strides, const int64_t* do_strides, const int64_t* dq_strides,
+                    const int64_t* dk_strides, const int64_t* dv_strides, float scale, int causal, int q_offset,
+                    int window, int sink, float softcap, const uint8_t* block_mask, int n_br, int n_bc, int mask_bq,
+                    int mask_bkv, void* workspace, size_t workspace_bytes, uint32_t* dev_err, void* stream) {
+  if (sink > Skv) sink = Skv;
   if (!dout || !q || !k || !v || !o || !lse || !dq || !dk || !dv) return FFA_ERR_INVALID_ARG;
   if (block_mask && (n_br <= 0 || n_bc <= 0 || mask_bq <= 0 || mask_bkv <= 0 ||
                      (int64_t)n_br * mask_bq < Sq || (int64_t)n_bc * mask_bkv < Skv))
@@ -1226,11 +1341,13 @@ extern "C" int ffa_bwd_masked(const void* dout, const void* q, const void* k, co
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || Sq <= 0 || Skv <= 0 || Hq % Hkv != 0) return FFA_ERR_INVALID_ARG;
   if (!((D == 64 && Dv == 64) || (D == 128 && Dv == 128) || (D == 192 && Dv == 128))) return FFA_ERR_UNSUPPORTED;
   if (dtype != FFA_DTYPE_BF16 && dtype != FFA_DTYPE_F16 && dtype != FFA_DTYPE_F32) return FFA_ERR_UNSUPPORTED;
-  const size_t need = ffa_bwd_workspace_size(B, Hq, Sq);
+  const size_t stats = ffa_bwd_workspace_size(B, Hq, Sq);
+  const size_t need =
+      sink > 0 ? ffa_bwd_sink_workspace_size(B, Hq, Hkv, Sq, Skv, D, Dv, window, sink) : stats;
   if (!workspace || workspace_bytes < need) return FFA_ERR_WORKSPACE;
   if (dtype == FFA_DTYPE_F32)
     return f32_bwd(dout, q, k, v, o, lse, dq, dk, dv, B, Hq, Hkv, Sq, Skv, D, Dv, q_strides, k_strides, v_strides,
-                   o_strides, do_strides, dq_strides, dk_strides, dv_strides, scale, causal, q_offset, window,
+                   o_strides, do_strides, dq_strides, dk_strides, dv_strides, scale, causal, q_offset, window, sink,
                    softcap, block_mask, n_br, n_bc, mask_bq, mask_bkv,
                    reinterpret_cast<void*>((reinterpret_cast<uintptr_t>(workspace) + 127) & ~uintptr_t(127)), stream);
   const int64_t* outs[3] = {dq_strides, dk_strides, dv_strides};
@@ -1274,6 +1391,13 @@ extern "C" int ffa_bwd_masked(const void* dout, const void* q, const void* k, co
   softcap_poly_coeffs(p.sc_pre, p.sc_poly);
   p.causal = causal;
   p.window = window > 0 ? window : 0;
+  if (sink > 0) {
+    p.sink = sink;
+    bwd_sink_shape(Sq, Skv, window, sink, p.n_sink_tiles, p.sink_parts);
+    p.sink_ws = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(workspace) + stats + 15) & ~uintptr_t(15));
+    const int64_t ctas = ((int64_t)(Skv + BWD_BT - 1) / BWD_BT + (int64_t)p.n_sink_tiles * p.sink_parts) * B * Hkv;
+    if (ctas > 0x7fffffffLL) return FFA_ERR_UNSUPPORTED;
+  }
   p.block_mask = block_mask;
   p.n_br = n_br;
   p.n_bc = n_bc;
@@ -1306,23 +1430,36 @@ extern "C" int ffa_bwd_masked(const void* dout, const void* q, const void* k, co
                       64, 32);
   if (st) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  auto run = [&](auto bm) -> int {
-    constexpr bool BM = decltype(bm)::value;
-    if (dtype == FFA_DTYPE_BF16) {
-      if (D == 64)
-        return launch_bwd<__nv_bfloat16, 64, 64, BM>(maps, p, o, dout, lse, lse2, delta, o_strides, do_strides, s);
+  auto run = [&](auto bm, auto sk) -> int {
+    constexpr bool BM = decltype(bm)::value, SINK = decltype(sk)::value;
+    auto typed = [&](auto t) -> int {
+      using T = decltype(t);
+      if (D == 64) return launch_bwd<T, 64, 64, BM, SINK>(maps, p, o, dout, lse, lse2, delta, o_strides, do_strides, s);
       if (D == 128)
-        return launch_bwd<__nv_bfloat16, 128, 128, BM>(maps, p, o, dout, lse, lse2, delta, o_strides, do_strides, s);
-      return launch_bwd<__nv_bfloat16, 192, 128, BM>(maps, p, o, dout, lse, lse2, delta, o_strides, do_strides, s);
-    }
-    if (D == 64) return launch_bwd<__half, 64, 64, BM>(maps, p, o, dout, lse, lse2, delta, o_strides, do_strides, s);
-    if (D == 128)
-      return launch_bwd<__half, 128, 128, BM>(maps, p, o, dout, lse, lse2, delta, o_strides, do_strides, s);
-    return launch_bwd<__half, 192, 128, BM>(maps, p, o, dout, lse, lse2, delta, o_strides, do_strides, s);
+        return launch_bwd<T, 128, 128, BM, SINK>(maps, p, o, dout, lse, lse2, delta, o_strides, do_strides, s);
+      return launch_bwd<T, 192, 128, BM, SINK>(maps, p, o, dout, lse, lse2, delta, o_strides, do_strides, s);
+    };
+    return dtype == FFA_DTYPE_BF16 ? typed(__nv_bfloat16{}) : typed(__half{});
   };
-  // Block-mask support is compiled into its own kernels, so the unmasked
-  // kernels carry none of its per-unit work.
-  return block_mask ? run(std::true_type{}) : run(std::false_type{});
+  // Block-mask and sink support are compiled into their own kernels, so the
+  // plain kernels carry none of their per-unit work.
+  if (sink > 0) return run(std::false_type{}, std::true_type{});
+  return block_mask ? run(std::true_type{}, std::false_type{}) : run(std::false_type{}, std::false_type{});
+}
+
+}  // namespace ffa
+
+extern "C" int ffa_bwd_masked(const void* dout, const void* q, const void* k, const void* v, const void* o,
+                              const float* lse, void* dq, void* dk, void* dv, int dtype, int B, int Hq, int Hkv,
+                              int Sq, int Skv, int D, int Dv, const int64_t* q_strides, const int64_t* k_strides,
+                              const int64_t* v_strides, const int64_t* o_strides, const int64_t* do_strides,
+                              const int64_t* dq_strides, const int64_t* dk_strides, const int64_t* dv_strides,
+                              float scale, int causal, int q_offset, int window, float softcap,
+                              const uint8_t* block_mask, int n_br, int n_bc, int mask_bq, int mask_bkv,
+                              void* workspace, size_t workspace_bytes, uint32_t* dev_err, void* stream) {
+  return ffa::bwd_impl(dout, q, k, v, o, lse, dq, dk, dv, dtype, B, Hq, Hkv, Sq, Skv, D, Dv, q_strides, k_strides,
+                       v_strides, o_strides, do_strides, dq_strides, dk_strides, dv_strides, scale, causal, q_offset,
+                       window, 0, softcap, block_mask, n_br, n_bc, mask_bq, mask_bkv, workspace, workspace_bytes, dev_err, stream);
 }
 
 extern "C" int ffa_bwd(const void* dout, const void* q, const void* k, const void* v, const void* o,
@@ -1335,4 +1472,17 @@ extern "C" int ffa_bwd(const void* dout, const void* q, const void* k, const voi
   return ffa_bwd_masked(dout, q, k, v, o, lse, dq, dk, dv, dtype, B, Hq, Hkv, Sq, Skv, D, Dv, q_strides, k_strides,
                         v_strides, o_strides, do_strides, dq_strides, dk_strides, dv_strides, scale, causal, q_offset,
                         window, softcap, nullptr, 0, 0, 0, 0, workspace, workspace_bytes, dev_err, stream);
+}
+
+extern "C" int ffa_bwd_sink(const void* dout, const void* q, const void* k, const void* v, const void* o,
+                            const float* lse, void* dq, void* dk, void* dv, int dtype, int B, int Hq, int Hkv, int Sq,
+                            int Skv, int D, int Dv, const int64_t* q_strides, const int64_t* k_strides,
+                            const int64_t* v_strides, const int64_t* o_strides, const int64_t* do_strides,
+                            const int64_t* dq_strides, const int64_t* dk_strides, const int64_t* dv_strides,
+                            float scale, int causal, int q_offset, int window, int sinks, float softcap,
+                            void* workspace, size_t workspace_bytes, uint32_t* dev_err, void* stream) {
+  if (window <= 0 || sinks < 0) return FFA_ERR_INVALID_ARG;
+  return ffa::bwd_impl(dout, q, k, v, o, lse, dq, dk, dv, dtype, B, Hq, Hkv, Sq, Skv, D, Dv, q_strides, k_strides,
+                       v_strides, o_strides, do_strides, dq_strides, dk_strides, dv_strides, scale, causal, q_offset,
+                       window, sinks, softcap, nullptr, 0, 0, 0, 0, workspace, workspace_bytes, dev_err, stream);
 }

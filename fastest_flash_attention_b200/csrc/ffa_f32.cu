@@ -44,6 +44,7 @@ struct F32Params {
   float* delta;        // backward scratch [B, Hq, Sq]
   int64_t q_s[3], k_s[3], v_s[3], o_s[3], do_s[3], out_s[3], dq_s[3], dk_s[3], dv_s[3];
   int B, Hq, Hkv, Sq, Skv, q_offset, causal, window;
+  int sink;  // keys [0, sink) stay visible outside the window
   float scale, softcap;
   const uint8_t* bm;
   int n_br, n_bc, mbq, mbk;
@@ -53,7 +54,7 @@ struct F32Params {
 __device__ __forceinline__ bool f32_visible(const F32Params& p, int i, int j) {
   if (i >= p.Sq || j >= p.Skv) return false;
   if (p.causal && j > i + p.q_offset) return false;
-  if (p.window > 0 && j < i + p.q_offset - p.window + 1) return false;
+  if (p.window > 0 && j < i + p.q_offset - p.window + 1 && j >= p.sink) return false;
   if (p.bm && !p.bm[(size_t)(i / p.mbq) * p.n_bc + j / p.mbk]) return false;
   return true;
 }
@@ -71,8 +72,21 @@ __device__ __forceinline__ void f32_query_range(const F32Params& p, int j0, int 
   lo = 0;
   hi = p.Sq;
   if (p.causal) lo = max(lo, j0 - p.q_offset);
-  if (p.window > 0) hi = min(hi, j1 - p.q_offset + p.window);
+  if (p.window > 0 && j0 >= p.sink) hi = min(hi, j1 - p.q_offset + p.window);
 }
+
+// The 64-key tiles a query tile walks: those that hold sinks left of the
+// window's first tile, then the range's.  tile(it) for it in [0, n).
+struct F32Walk {
+  int first, n_sink, n;
+  __device__ __forceinline__ F32Walk(const F32Params& p, int klo, int khi) {
+    const int end = khi > 0 ? (khi + F_BN - 1) / F_BN : 0;
+    first = max(klo, 0) / F_BN;
+    n_sink = min((p.sink + F_BN - 1) / F_BN, min(first, end));
+    n = n_sink + max(end - first, 0);
+  }
+  __device__ __forceinline__ int tile(int it) const { return it < n_sink ? it : first + it - n_sink; }
+};
 
 // Copies rows [r0, r0 + 64) of a [*, W] fp32 matrix (row stride `rs` elements)
 // into smem rows of pitch W + 4; rows at or past `nrows` become zero.
@@ -219,25 +233,26 @@ __global__ void __launch_bounds__(F_THREADS) ffa_f32_fwd_kernel(const F32Params 
   }
   int klo, khi;
   f32_key_range(p, i0, i1, klo, khi);
-  const int kt0 = max(klo, 0) / F_BN;
-  if (kt0 * F_BN < khi) {
-    f32_load_tile_async<DQ>(sKV, kb, p.k_s[2], kt0 * F_BN, p.Skv);
-    f32_load_tile_async<DV>(sKV + 64 * (DQ + 4), vb, p.v_s[2], kt0 * F_BN, p.Skv);
+  const F32Walk walk(p, klo, khi);
+  if (walk.n > 0) {
+    f32_load_tile_async<DQ>(sKV, kb, p.k_s[2], walk.tile(0) * F_BN, p.Skv);
+    f32_load_tile_async<DV>(sKV + 64 * (DQ + 4), vb, p.v_s[2], walk.tile(0) * F_BN, p.Skv);
   }
   cp_async_commit();  // Q and the first K / V tile
-  for (int kt = kt0; kt * F_BN < khi; ++kt) {
-    const int j0 = kt * F_BN;
-    float* sK = sKV + ((kt - kt0) % NKV) * KV_STRIDE;
+  for (int it = 0; it < walk.n; ++it) {
+    const int j0 = walk.tile(it) * F_BN;
+    float* sK = sKV + (it % NKV) * KV_STRIDE;
     float* sV = sK + 64 * (DQ + 4);
     __syncthreads();  // the previous tile's reads (of sP and of the buffer refilled next) are done
-    if (NKV == 2 && (kt + 1) * F_BN < khi) {
-      float* nK = sKV + ((kt + 1 - kt0) % 2) * KV_STRIDE;
-      f32_load_tile_async<DQ>(nK, kb, p.k_s[2], j0 + F_BN, p.Skv);
-      f32_load_tile_async<DV>(nK + 64 * (DQ + 4), vb, p.v_s[2], j0 + F_BN, p.Skv);
+    if (NKV == 2 && it + 1 < walk.n) {
+      float* nK = sKV + ((it + 1) % 2) * KV_STRIDE;
+      const int j1 = walk.tile(it + 1) * F_BN;
+      f32_load_tile_async<DQ>(nK, kb, p.k_s[2], j1, p.Skv);
+      f32_load_tile_async<DV>(nK + 64 * (DQ + 4), vb, p.v_s[2], j1, p.Skv);
       cp_async_commit();
       cp_async_wait<1>();  // all but the tile just requested
     } else {
-      if (NKV == 1 && kt > kt0) {
+      if (NKV == 1 && it > 0) {
         f32_load_tile_async<DQ>(sK, kb, p.k_s[2], j0, p.Skv);
         f32_load_tile_async<DV>(sV, vb, p.v_s[2], j0, p.Skv);
         cp_async_commit();
@@ -432,8 +447,9 @@ __global__ void __launch_bounds__(F_THREADS) ffa_f32_dq_kernel(const F32Params p
     for (int c = 0; c < DQ / 64; ++c) adq[i][c] = make_float4(0.f, 0.f, 0.f, 0.f);
   int klo, khi;
   f32_key_range(p, i0, i1, klo, khi);
-  for (int kt = max(klo, 0) / F_BN; kt * F_BN < khi; ++kt) {
-    const int j0 = kt * F_BN;
+  const F32Walk walk(p, klo, khi);
+  for (int it = 0; it < walk.n; ++it) {
+    const int j0 = walk.tile(it) * F_BN;
     __syncthreads();
     f32_load_tile<DQ>(sK, kb, p.k_s[2], j0, p.Skv);
     f32_load_tile<DV>(sV, vb, p.v_s[2], j0, p.Skv);
@@ -511,8 +527,9 @@ int f32_bwd_launch(const F32Params& p, cudaStream_t s) {
 bool f32_dims_ok(int D, int Dv) { return (D == 64 && Dv == 64) || (D == 128 && Dv == 128) || (D == 192 && Dv == 128); }
 
 void f32_common(F32Params& p, int B, int Hq, int Hkv, int Sq, int Skv, float scale, int causal, int q_offset,
-                int window, float softcap, const uint8_t* block_mask, int n_br, int n_bc, int mask_bq,
+                int window, int sink, float softcap, const uint8_t* block_mask, int n_br, int n_bc, int mask_bq,
                 int mask_bkv) {
+  p.sink = window > 0 ? sink : 0;
   p.B = B;
   p.Hq = Hq;
   p.Hkv = Hkv;
@@ -535,7 +552,7 @@ void f32_common(F32Params& p, int B, int Hq, int Hkv, int Sq, int Skv, float sca
 // fp32 forward behind ffa_fwd (dtype FFA_DTYPE_F32); same argument checks.
 int f32_fwd(const void* q, const void* k, const void* v, void* o, float* lse, int B, int Hq, int Hkv, int Sq,
             int Skv, int D, int Dv, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
-            const int64_t* o_strides, float scale, int causal, int q_offset, int window, float softcap,
+            const int64_t* o_strides, float scale, int causal, int q_offset, int window, int sink, float softcap,
             const uint8_t* block_mask, int n_br, int n_bc, int mask_bq, int mask_bkv, void* stream) {
   if (!f32_dims_ok(D, Dv)) return FFA_ERR_UNSUPPORTED;
   if (!f32_strides_ok(q, q_strides) || !f32_strides_ok(k, k_strides) || !f32_strides_ok(v, v_strides) ||
@@ -552,8 +569,8 @@ int f32_fwd(const void* q, const void* k, const void* v, void* o, float* lse, in
   f32_copy_strides(p.k_s, k_strides);
   f32_copy_strides(p.v_s, v_strides);
   f32_copy_strides(p.out_s, o_strides);
-  f32_common(p, B, Hq, Hkv, Sq, Skv, scale, causal, q_offset, window, softcap, block_mask, n_br, n_bc, mask_bq,
-             mask_bkv);
+  f32_common(p, B, Hq, Hkv, Sq, Skv, scale, causal, q_offset, window, sink, softcap, block_mask, n_br, n_bc,
+             mask_bq, mask_bkv);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (D == 64) return f32_fwd_launch<64, 64>(p, s);
   if (D == 128) return f32_fwd_launch<128, 128>(p, s);
@@ -567,7 +584,7 @@ int f32_bwd(const void* dout, const void* q, const void* k, const void* v, const
             const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
             const int64_t* o_strides, const int64_t* do_strides, const int64_t* dq_strides,
             const int64_t* dk_strides, const int64_t* dv_strides, float scale, int causal, int q_offset,
-            int window, float softcap, const uint8_t* block_mask, int n_br, int n_bc, int mask_bq, int mask_bkv,
+            int window, int sink, float softcap, const uint8_t* block_mask, int n_br, int n_bc, int mask_bq, int mask_bkv,
             void* workspace, void* stream) {
   if (!f32_dims_ok(D, Dv)) return FFA_ERR_UNSUPPORTED;
   if (!f32_strides_ok(q, q_strides) || !f32_strides_ok(k, k_strides) || !f32_strides_ok(v, v_strides) ||
@@ -594,8 +611,8 @@ int f32_bwd(const void* dout, const void* q, const void* k, const void* v, const
   f32_copy_strides(p.dq_s, dq_strides);
   f32_copy_strides(p.dk_s, dk_strides);
   f32_copy_strides(p.dv_s, dv_strides);
-  f32_common(p, B, Hq, Hkv, Sq, Skv, scale, causal, q_offset, window, softcap, block_mask, n_br, n_bc, mask_bq,
-             mask_bkv);
+  f32_common(p, B, Hq, Hkv, Sq, Skv, scale, causal, q_offset, window, sink, softcap, block_mask, n_br, n_bc,
+             mask_bq, mask_bkv);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (D == 64) return f32_bwd_launch<64, 64>(p, s);
   if (D == 128) return f32_bwd_launch<128, 128>(p, s);

@@ -23,6 +23,7 @@
 #include "ffa_host.h"
 
 #include <cstdlib>
+#include <type_traits>
 
 namespace ffa {
 
@@ -109,6 +110,7 @@ struct FwdParams {
   float sc_poly[3];   // softcap_small2 coefficients for k = sc_pre
   int use_softcap;
   int causal, window;
+  int sink;  // SINK kernels: keys [0, sink) stay visible outside the window
   const uint8_t* block_mask;
   int n_br, n_bc, mask_bq, mask_bkv;
   ErrCtx ec;
@@ -127,6 +129,7 @@ struct FwdBars {
   int n_tiles;
   int j_lo;
   int use_list;
+  int n_sink;
 };
 
 enum : uint32_t {
@@ -140,7 +143,12 @@ enum : uint32_t {
 };
 
 
-template <typename T, int D, int DV, int NQT>
+// SINK: a sliding window with the first p.sink keys visible outside it (as far
+// as causality allows).  The walk takes the key tiles that hold sinks and lie
+// left of the window's first, then the window's; sinks inside the window's
+// tiles are kept by the same per-element mask.  A kernel of its own, so the
+// others carry none of it.
+template <typename T, int D, int DV, int NQT, bool SINK>
 __global__ void __launch_bounds__(FwdShape<NQT>::THREADS, FwdShape<NQT>::MIN_BLOCKS)
     ffa_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                    const __grid_constant__ CUtensorMap tmV, const FwdParams p) {
@@ -217,8 +225,10 @@ __global__ void __launch_bounds__(FwdShape<NQT>::THREADS, FwdShape<NQT>::MIN_BLO
     }
     if (p.block_mask == nullptr) {
       if (lane == 0) {
-        bars->j_lo = j_lo;
-        bars->n_tiles = max(0, j_hi - j_lo);
+        const int n_sink = SINK ? min((p.sink + FWD_BN - 1) / FWD_BN, j_lo) : 0;
+        bars->j_lo = j_lo - n_sink;  // tile_at's offset past the sink tiles
+        bars->n_sink = n_sink;
+        bars->n_tiles = max(0, j_hi - j_lo) + n_sink;
         bars->use_list = 0;
       }
     } else {
@@ -255,7 +265,11 @@ __global__ void __launch_bounds__(FwdShape<NQT>::THREADS, FwdShape<NQT>::MIN_BLO
   const int n = bars->n_tiles;
   const int j_lo = bars->j_lo;
   const bool use_list = bars->use_list != 0;
-  auto tile_at = [&](int it) -> int { return use_list ? (int)list[it] : j_lo + it; };
+  const int n_sink = SINK ? bars->n_sink : 0;
+  auto tile_at = [&](int it) -> int {
+    if (SINK) return it < n_sink ? it : j_lo + it;
+    return use_list ? (int)list[it] : j_lo + it;
+  };
   constexpr uint32_t FMT = DtypeFmt<T>::value;
 
   if (warp >= 4 * NQT) {
@@ -496,7 +510,8 @@ __global__ void __launch_bounds__(FwdShape<NQT>::THREADS, FwdShape<NQT>::MIN_BLO
       }
       const int c0 = j * FWD_BN;
       const bool need_mask = (p.causal && c0 + FWD_BN - 1 > a_lo) ||
-                             (p.window > 0 && c0 < a_hi - p.window + 1) || (c0 + FWD_BN > p.Skv) ||
+                             (p.window > 0 && c0 < a_hi - p.window + 1 && !(SINK && c0 + FWD_BN <= p.sink)) ||
+                             (c0 + FWD_BN > p.Skv) ||
                              (p.block_mask != nullptr);
       if (need_mask) {
         // Visible keys of this row form one range [lo_c, hi] (causal, window
@@ -507,12 +522,28 @@ __global__ void __launch_bounds__(FwdShape<NQT>::THREADS, FwdShape<NQT>::MIN_BLO
         const int lo_c = p.window > 0 ? max(arow - p.window + 1 - c0, 0) : 0;
         const uint32_t span = hi >= lo_c ? (uint32_t)(hi - lo_c) : 0xffffffffu;
         const uint32_t ninf = __float_as_uint(-INFINITY);
+        if (SINK && c0 < p.sink) {
+          // the window's range or the sinks before it, both up to `hi`: one
+          // keep bit for each column
+          const int n_keep = min(p.sink - c0, hi + 1);
+          uint32_t kb[4];
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const int a = max(lo_c - 32 * w, 0), e = min(hi - 32 * w, 31);
+            const int z = min(n_keep - 32 * w, 32);
+            kb[w] = e >= a ? ((2u << (e - a)) - 1u) << a : 0u;
+            if (z > 0) kb[w] |= z == 32 ? ~0u : (1u << z) - 1u;
+          }
+#pragma unroll
+          for (int c = 0; c < FWD_BN; ++c) s[c] = ((kb[c / 32] >> (c % 32)) & 1u) ? s[c] : ninf;
+        } else {
 #pragma unroll
         for (int c = 0; c < FWD_BN; ++c) {
           const bool keep = span != 0xffffffffu && (uint32_t)(c - lo_c) <= span;
           s[c] = keep ? s[c] : ninf;
         }
-        if (p.block_mask != nullptr) {
+        }
+        if (!SINK && p.block_mask != nullptr) {
           // Column keep-bits of this row from the block mask (a runtime loop
           // over the mask blocks the tile touches), applied with an unrolled
           // bit test so s[] stays in registers.
@@ -654,11 +685,11 @@ __global__ void __launch_bounds__(FwdShape<NQT>::THREADS, FwdShape<NQT>::MIN_BLO
   }
 }
 
-template <typename T, int D, int DV, int NQT>
+template <typename T, int D, int DV, int NQT, bool SINK>
 static int launch_fwd(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const FwdParams& p,
                       int grid, cudaStream_t stream) {
   using Cfg = FwdCfg<D, DV, NQT>;
-  auto kern = ffa_fwd_kernel<T, D, DV, NQT>;
+  auto kern = ffa_fwd_kernel<T, D, DV, NQT, SINK>;
   static std::atomic<uint64_t> attr_done{0};
   if (int st = smem_attr_once(kern, Cfg::SMEM, attr_done)) return st;
   kern<<<grid, FwdShape<NQT>::THREADS, Cfg::SMEM, stream>>>(mq, mk, mv, p);
@@ -720,14 +751,12 @@ static int fwd_query_tiles(int D, int Sq, int Skv, int causal, int window, bool 
   return (D == 64 && cols <= FWD_NQT1_MAX_COLS) ? 1 : 2;
 }
 
-}  // namespace ffa
-
-extern "C" int ffa_fwd(const void* q, const void* k, const void* v, void* o, float* lse, int dtype, int B,
-                       int Hq, int Hkv, int Sq, int Skv, int D, int Dv, const int64_t* q_strides,
-                       const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides, float scale,
-                       int causal, int q_offset, int window, float softcap, const uint8_t* block_mask, int n_br,
-                       int n_bc, int mask_bq, int mask_bkv, uint32_t* dev_err, void* stream) {
-  using namespace ffa;
+static int fwd_impl(const void* q, const void* k, const void* v, void* o, float* lse, int dtype, int B, int Hq,
+                    int Hkv, int Sq, int Skv, int D, int Dv, const int64_t* q_strides, const int64_t* k_strides,
+                    const int64_t* v_strides, const int64_t* o_strides, float scale, int causal, int q_offset,
+                    int window, int sink, float softcap, const uint8_t* block_mask, int n_br, int n_bc, int mask_bq,
+                    int mask_bkv, uint32_t* dev_err, void* stream) {
+  if (sink > Skv) sink = Skv;
   if (!q || !k || !v || !o || !q_strides || !k_strides || !v_strides || !o_strides) return FFA_ERR_INVALID_ARG;
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || Sq <= 0 || Skv < 0 || Hq % Hkv != 0) return FFA_ERR_INVALID_ARG;
   if (!((D == 64 && Dv == 64) || (D == 128 && Dv == 128) || (D == 192 && Dv == 128))) return FFA_ERR_UNSUPPORTED;
@@ -740,7 +769,7 @@ extern "C" int ffa_fwd(const void* q, const void* k, const void* v, void* o, flo
     return FFA_ERR_INVALID_ARG;
   if (dtype == FFA_DTYPE_F32)
     return f32_fwd(q, k, v, o, lse, B, Hq, Hkv, Sq, Skv, D, Dv, q_strides, k_strides, v_strides, o_strides, scale,
-                   causal, q_offset, window, softcap, block_mask, n_br, n_bc, mask_bq, mask_bkv, stream);
+                   causal, q_offset, window, sink, softcap, block_mask, n_br, n_bc, mask_bq, mask_bkv, stream);
   if (!aligned16(o) || (o_strides[2] % 8) || (o_strides[1] % 8) || (o_strides[0] % 8)) return FFA_ERR_INVALID_ARG;
 
   FwdParams p{};
@@ -765,6 +794,7 @@ extern "C" int ffa_fwd(const void* q, const void* k, const void* v, void* o, flo
   softcap_poly_coeffs(p.sc_pre, p.sc_poly);
   p.causal = causal;
   p.window = window > 0 ? window : 0;
+  p.sink = sink;
   p.block_mask = block_mask;
   p.n_br = n_br;
   p.n_bc = n_bc;
@@ -790,20 +820,43 @@ extern "C" int ffa_fwd(const void* q, const void* k, const void* v, void* o, flo
   const long long grid = (long long)p.n_qblk * B * Hq;
   if (grid > 0x7fffffffLL) return FFA_ERR_UNSUPPORTED;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == FFA_DTYPE_BF16) {
-    if (D == 64)
-      return nqt == 1 ? launch_fwd<__nv_bfloat16, 64, 64, 1>(mq, mk, mv, p, (int)grid, s)
-                      : launch_fwd<__nv_bfloat16, 64, 64, 2>(mq, mk, mv, p, (int)grid, s);
-    if (D == 128)
-      return nqt == 1 ? launch_fwd<__nv_bfloat16, 128, 128, 1>(mq, mk, mv, p, (int)grid, s)
-                      : launch_fwd<__nv_bfloat16, 128, 128, 2>(mq, mk, mv, p, (int)grid, s);
-    return launch_fwd<__nv_bfloat16, 192, 128, 2>(mq, mk, mv, p, (int)grid, s);
-  }
-  if (D == 64)
-    return nqt == 1 ? launch_fwd<__half, 64, 64, 1>(mq, mk, mv, p, (int)grid, s)
-                    : launch_fwd<__half, 64, 64, 2>(mq, mk, mv, p, (int)grid, s);
-  if (D == 128)
-    return nqt == 1 ? launch_fwd<__half, 128, 128, 1>(mq, mk, mv, p, (int)grid, s)
-                    : launch_fwd<__half, 128, 128, 2>(mq, mk, mv, p, (int)grid, s);
-  return launch_fwd<__half, 192, 128, 2>(mq, mk, mv, p, (int)grid, s);
+  // Sinks are compiled into their own kernels, so the others carry none of
+  // their per-tile work.
+  auto run = [&](auto sk) -> int {
+    constexpr bool SINK = decltype(sk)::value;
+    auto typed = [&](auto t) -> int {
+      using T = decltype(t);
+      if (D == 64)
+        return nqt == 1 ? launch_fwd<T, 64, 64, 1, SINK>(mq, mk, mv, p, (int)grid, s)
+                        : launch_fwd<T, 64, 64, 2, SINK>(mq, mk, mv, p, (int)grid, s);
+      if (D == 128)
+        return nqt == 1 ? launch_fwd<T, 128, 128, 1, SINK>(mq, mk, mv, p, (int)grid, s)
+                        : launch_fwd<T, 128, 128, 2, SINK>(mq, mk, mv, p, (int)grid, s);
+      return launch_fwd<T, 192, 128, 2, SINK>(mq, mk, mv, p, (int)grid, s);
+    };
+    return dtype == FFA_DTYPE_BF16 ? typed(__nv_bfloat16{}) : typed(__half{});
+  };
+  return sink > 0 ? run(std::true_type{}) : run(std::false_type{});
+}
+
+}  // namespace ffa
+
+extern "C" int ffa_fwd(const void* q, const void* k, const void* v, void* o, float* lse, int dtype, int B,
+                       int Hq, int Hkv, int Sq, int Skv, int D, int Dv, const int64_t* q_strides,
+                       const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides, float scale,
+                       int causal, int q_offset, int window, float softcap, const uint8_t* block_mask, int n_br,
+                       int n_bc, int mask_bq, int mask_bkv, uint32_t* dev_err, void* stream) {
+  return ffa::fwd_impl(q, k, v, o, lse, dtype, B, Hq, Hkv, Sq, Skv, D, Dv, q_strides, k_strides, v_strides, o_strides,
+                       scale, causal, q_offset, window, 0, softcap, block_mask, n_br, n_bc, mask_bq, mask_bkv, dev_err,
+                       stream);
+}
+
+extern "C" int ffa_fwd_sink(const void* q, const void* k, const void* v, void* o, float* lse, int dtype, int B,
+                            int Hq, int Hkv, int Sq, int Skv, int D, int Dv, const int64_t* q_strides,
+                            const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides,
+                            float scale, int causal, int q_offset, int window, int sinks, float softcap,
+                            uint32_t* dev_err, void* stream) {
+  if (window <= 0 || sinks < 0) return FFA_ERR_INVALID_ARG;
+  return ffa::fwd_impl(q, k, v, o, lse, dtype, B, Hq, Hkv, Sq, Skv, D, Dv, q_strides, k_strides, v_strides, o_strides,
+                       scale, causal, q_offset, window, sinks, softcap, nullptr, 0, 0, 0, 0, dev_err, stream);
 }

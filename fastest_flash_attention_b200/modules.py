@@ -40,6 +40,8 @@ def _merge(o: torch.Tensor, B: int, S: int) -> torch.Tensor:
 
 
 class _AttnBase(nn.Module):
+    sink_tokens = 0  # first keys kept visible outside sliding_window (an addition to the reference's modules)
+
     def _attend(self, q, k, v, use_causal, bs, kv_cache, return_lse, fa4: bool = False):
         if self.training and not return_lse and kv_cache is None:
             if fa4:
@@ -49,11 +51,14 @@ class _AttnBase(nn.Module):
                                     pingpong=self.pingpong, deterministic=self.deterministic)
             else:
                 out = fastest_flash_attn_func(q, k, v, scale=self.scale, causal=use_causal, block_size=bs or 64,
-                                              softcap=self.softcap, sliding_window=self.sliding_window)
+                                              softcap=self.softcap, sliding_window=self.sliding_window,
+                                              sink_tokens=self.sink_tokens)
             return out, None
-        fn = fa4_forward_dispatch if fa4 else fastest_flash_attn_forward
-        return fn(q, k, v, scale=self.scale, causal=use_causal, block_size=bs, softcap=self.softcap,
+        kw = dict(scale=self.scale, causal=use_causal, block_size=bs, softcap=self.softcap,
                   sliding_window=self.sliding_window, kv_cache=kv_cache, return_lse=return_lse)
+        if fa4:
+            return fa4_forward_dispatch(q, k, v, **kw)
+        return fastest_flash_attn_forward(q, k, v, sink_tokens=self.sink_tokens, **kw)
 
 
 class FastestFlashMHA(_AttnBase):
@@ -61,8 +66,9 @@ class FastestFlashMHA(_AttnBase):
 
     def __init__(self, hidden_size: int, num_heads: int, head_dim: Optional[int] = None, dropout: float = 0.0,
                  bias: bool = False, causal: bool = False, block_size: int = 0, softcap: Optional[float] = None,
-                 sliding_window: Optional[int] = None):
+                 sliding_window: Optional[int] = None, sink_tokens: int = 0):
         super().__init__()
+        self.sink_tokens = sink_tokens
         self.hidden_size = hidden_size
         self.num_heads = num_heads
         self.head_dim = head_dim or hidden_size // num_heads
@@ -105,8 +111,9 @@ class FastestFlashGQA(_AttnBase):
 
     def __init__(self, hidden_size: int, num_heads: int, num_kv_heads: int, head_dim: Optional[int] = None,
                  bias: bool = False, causal: bool = False, block_size: int = 0, softcap: Optional[float] = None,
-                 sliding_window: Optional[int] = None):
+                 sliding_window: Optional[int] = None, sink_tokens: int = 0):
         super().__init__()
+        self.sink_tokens = sink_tokens
         self.hidden_size = hidden_size
         self.num_heads = num_heads
         self.num_kv_heads = num_kv_heads

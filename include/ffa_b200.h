@@ -131,6 +131,32 @@ int ffa_bwd_masked(const void* dout, const void* q, const void* k, const void* v
                    int mask_bkv, void* workspace, size_t workspace_bytes, uint32_t* dev_err, void* stream);
 
 /* ----------------------------------------------------------------------------
+ * Sliding window with the first tokens kept visible ("sinks"; no counterpart
+ * in the reference): ffa_fwd / ffa_bwd with window > 0 where keys [0, sinks)
+ * are visible outside the window too, as far as causality allows:
+ *   j visible iff (j <= i + q_offset if causal) and
+ *                 (j >= i + q_offset - window + 1 or j < sinks).
+ * Same types, shapes, strides, softcap and determinism (no block mask).  The
+ * backward's workspace comes from ffa_bwd_sink_workspace_size: a sink sees
+ * every later query, so the queries of the key tiles that hold sinks are
+ * shared by several CTAs, whose fp32 sums one more launch adds up in order.
+ * ------------------------------------------------------------------------- */
+int ffa_fwd_sink(const void* q, const void* k, const void* v, void* o, float* lse, int dtype, int B, int Hq,
+                 int Hkv, int Sq, int Skv, int D, int Dv, const int64_t* q_strides, const int64_t* k_strides,
+                 const int64_t* v_strides, const int64_t* o_strides, float scale, int causal, int q_offset,
+                 int window, int sinks, float softcap, uint32_t* dev_err, void* stream);
+
+size_t ffa_bwd_sink_workspace_size(int B, int Hq, int Hkv, int Sq, int Skv, int D, int Dv, int window, int sinks);
+
+int ffa_bwd_sink(const void* dout, const void* q, const void* k, const void* v, const void* o, const float* lse,
+                 void* dq, void* dk, void* dv, int dtype, int B, int Hq, int Hkv, int Sq, int Skv, int D, int Dv,
+                 const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                 const int64_t* o_strides, const int64_t* do_strides, const int64_t* dq_strides,
+                 const int64_t* dk_strides, const int64_t* dv_strides, float scale, int causal, int q_offset,
+                 int window, int sinks, float softcap, void* workspace, size_t workspace_bytes, uint32_t* dev_err,
+                 void* stream);
+
+/* ----------------------------------------------------------------------------
  * Allocation-free backward.  No counterpart in the reference: this entry
  * point exists for callers that cannot allocate device memory (code handed
  * only its input/output buffers by a host framework, or hosts that forbid a
