@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import os
 from pathlib import Path
 
@@ -208,16 +209,16 @@ def check(status: int, fn: str) -> None:
         raise RuntimeError(f"{fn} failed: {STATUS_NAMES.get(status, status)}" + (f" ({msg})" if msg else ""))
 
 
+@functools.lru_cache(maxsize=4096)
 def i64arr(*vals: int):
+    """int64 array argument of an entry point (which only reads it, so equal
+    values share one; building one costs over half a microsecond)."""
     return (ctypes.c_int64 * len(vals))(*vals)
-
-
-_I64X3 = ctypes.c_int64 * 3
 
 
 def strides3(t: torch.Tensor):
     """The first three strides of a 4-D tensor, for an entry point's {batch, head, token} argument."""
-    return _I64X3(*t.stride()[:3])
+    return i64arr(*t.stride()[:3])
 
 
 def stream_of(t: torch.Tensor) -> int:

@@ -68,8 +68,8 @@ def _tma_ready(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     (unit stride in D, 16-byte aligned base and outer strides)."""
     if t.dtype != dtype:
         t = t.to(dtype)
-    if (t.stride(-1) != 1 or any(s % 8 for s in t.stride()[:-1]) or t.data_ptr() % 16
-            or any(s == 0 for s in t.stride()[:-1])):
+    sb, sh, ss, sd = t.stride()
+    if sd != 1 or (sb | sh | ss) % 8 or t.data_ptr() % 16 or not (sb and sh and ss):
         t = t.contiguous()
     return t
 
@@ -213,13 +213,14 @@ def fastest_flash_attn_forward(
     if scale is None:
         scale = 1.0 / math.sqrt(D)
 
-    if block_size is None:
-        if config is not None:
-            bq, bkv = config.resolve_block_sizes(S_q, S_kv, D)
-        else:
-            bq = bkv = auto_select_block_size(S_q, S_kv, D)
-    else:
+    if block_size is not None:
         bq = bkv = block_size
+    elif block_mask is None:  # the size only says what a block of the mask covers
+        bq = bkv = 64
+    elif config is not None:
+        bq, bkv = config.resolve_block_sizes(S_q, S_kv, D)
+    else:
+        bq = bkv = auto_select_block_size(S_q, S_kv, D)
 
     o, lse = flash_fwd(q, k, v, scale=scale, causal=causal, q_offset=q_offset, window=sliding_window,
                        softcap=softcap, block_mask=block_mask, mask_block=(bq, bkv),

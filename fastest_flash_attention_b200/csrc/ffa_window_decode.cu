@@ -19,11 +19,15 @@
 // the block with warp-level tensor-core MMAs, and keeps its own running
 // maximum and sum.  No warp waits for another before the join.
 //
-// HBM-bound: the K and V bytes of the visible tokens, read once per kv head.
+// HBM-bound: the K and V bytes of the visible tokens, read once per kv head;
+// 64 requests, window 4096 + 4, 32/8 heads, D 128: 165 us, 6.16 TB/s (0.94 of a
+// measured copy).  One request alone is bound by latencies (11 us: the launch,
+// the length, the table, the rows, each warp's few chunks, two cluster barriers).
 // P is rounded to the data's type for the P V product (the tensor core's
 // operand), the row sums add the unrounded values; statistics, O and the join
 // are fp32.
 #include <cooperative_groups.h>
+#include <math.h>
 
 #include "ffa_common.cuh"
 #include "ffa_host.h"
@@ -32,7 +36,14 @@ namespace ffa {
 
 namespace cg = cooperative_groups;
 
-constexpr int WD_CHUNK = 16;  // tokens per chunk (one K-step of P V)
+// Tokens per chunk: one running-maximum update, one K-step of P V.  32 tokens
+// took as long per token (a warp is bound by its instructions, about 30 a token)
+// and left fewer warps for the same shared memory: 192 us against 165 on 64
+// requests of a 4096-token window, 32/8 heads, D 128.
+constexpr int WD_CHUNK = 16;
+// Warps per CTA.  8 leave one CTA per SM: 199 us on the case above; 2 with
+// three chunks in flight each: 159 us there, but 14.2 us against 11.1 for one
+// request alone.
 constexpr int WD_WARPS = 4;
 constexpr int WD_THREADS = WD_WARPS * 32;
 
@@ -58,10 +69,12 @@ struct WdParams {
 
 template <int DP>
 struct WdCfg {
-  static constexpr int HALF = WD_CHUNK * 128;        // 16 rows x 64 elements
+  static constexpr int HALF = WD_CHUNK * 128;        // a chunk's rows x 64 elements
   static constexpr int KV_BYTES = WD_CHUNK * DP * 2; // one chunk of K (or V)
   static constexpr int STAGE = 2 * KV_BYTES;
-  static constexpr int STAGES = DP == 64 ? 4 : 2;    // chunks a warp has in flight
+  // chunks a warp has in flight: 64 KB of rings, three CTAs per SM (96 KB, two
+  // CTAs: 183 us on the case above)
+  static constexpr int STAGES = DP == 64 ? 4 : 2;
   static constexpr int RING = WD_WARPS * STAGES * STAGE;
   // the joins overlay the rings, idle by then: per warp, then per CTA,
   // 16 rows x (m, l, O[DP])
@@ -156,7 +169,7 @@ __global__ void __launch_bounds__(WD_THREADS) ffa_window_decode_kernel(const WdP
   const int64_t row_bytes = (int64_t)p.D * 2;
   const uint8_t* kcol = static_cast<const uint8_t*>(p.kp) + col * 16;
   const uint8_t* vcol = static_cast<const uint8_t*>(p.vp) + col * 16;
-  auto issue = [&](int i, int my_row) {  // chunk i of this warp; my_row: pool row of the chunk's row lane % 16
+  auto issue = [&](int i, int my_row) {  // chunk i of this warp; my_row: pool row of the chunk's row lane % WD_CHUNK
     const uint32_t d = dst0 + (i % S) * Cfg::STAGE;
 #pragma unroll
     for (int k = 0; k < WD_CHUNK / STEP; ++k) {
@@ -170,7 +183,7 @@ __global__ void __launch_bounds__(WD_THREADS) ffa_window_decode_kernel(const WdP
       }
     }
   };
-  auto vidx = [&](int i) { return (c0 + warp + i * WD_WARPS) * WD_CHUNK + (lane & 15); };
+  auto vidx = [&](int i) { return (c0 + warp + i * WD_WARPS) * WD_CHUNK + lane % WD_CHUNK; };
   // table entries run one chunk ahead of the copies that need them
   int pages[S + 1];
 #pragma unroll
@@ -208,28 +221,35 @@ __global__ void __launch_bounds__(WD_THREADS) ffa_window_decode_kernel(const WdP
     __syncwarp();
     const uint32_t kbase = smem_u32(ring + (i % S) * Cfg::STAGE);
     const uint32_t vbase = kbase + Cfg::KV_BYTES;
-    float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    constexpr int NT = WD_CHUNK / 8;  // n-tiles of 8 tokens
+    float x[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) x[nt][0] = x[nt][1] = x[nt][2] = x[nt][3] = 0.f;
 #pragma unroll
     for (int kk = 0; kk < DP / 16; ++kk) {
       const int hf = kk / 4, ch = 2 * (kk % 4) + (mi & 1);
-      const int tok = mr + 8 * (mi >> 1);
-      uint32_t b00, b01, b10, b11;
-      ldsm_x4(sw128(kbase + hf * Cfg::HALF, tok, ch), b00, b01, b10, b11);
-      mma16816<T>(sc[0], qa[kk], b00, b01);
-      mma16816<T>(sc[1], qa[kk], b10, b11);
-    }
-    const int v0 = (c0 + warp + i * WD_WARPS) * WD_CHUNK;
-    float x[2][4];
 #pragma unroll
-    for (int nt = 0; nt < 2; ++nt)
+      for (int nt = 0; nt < NT; nt += 2) {
+        const int tok = nt * 8 + mr + 8 * (mi >> 1);
+        uint32_t b00, b01, b10, b11;
+        ldsm_x4(sw128(kbase + hf * Cfg::HALF, tok, ch), b00, b01, b10, b11);
+        mma16816<T>(x[nt], qa[kk], b00, b01);
+        mma16816<T>(x[nt + 1], qa[kk], b10, b11);
+      }
+    }
+    const int left = rows.nv - (c0 + warp + i * WD_WARPS) * WD_CHUNK;  // tokens of this chunk
+    float mx_lo = -INFINITY, mx_hi = -INFINITY;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        float v = sc[nt][e];
-        v = p.use_softcap ? tanh_acc(v * p.sc_pre) * p.sc_post : v * p.scale_log2;
-        x[nt][e] = v0 + nt * 8 + 2 * t + (e & 1) < rows.nv ? v : -INFINITY;
+        const float v = x[nt][e];
+        const float y = p.use_softcap ? tanh_acc(v * p.sc_pre) * p.sc_post : v * p.scale_log2;
+        x[nt][e] = nt * 8 + 2 * t + (e & 1) < left ? y : -INFINITY;
       }
-    float mx_lo = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1]));
-    float mx_hi = fmaxf(fmaxf(x[0][2], x[0][3]), fmaxf(x[1][2], x[1][3]));
+      mx_lo = fmaxf(mx_lo, fmaxf(x[nt][0], x[nt][1]));
+      mx_hi = fmaxf(mx_hi, fmaxf(x[nt][2], x[nt][3]));
+    }
 #pragma unroll
     for (int off = 1; off < 4; off <<= 1) {
       mx_lo = fmaxf(mx_lo, __shfl_xor_sync(0xffffffffu, mx_lo, off));
@@ -254,26 +274,29 @@ __global__ void __launch_bounds__(WD_THREADS) ffa_window_decode_kernel(const WdP
       m_hi = mn_hi;
     }
     const float u_lo = (m_lo == -INFINITY) ? 0.f : m_lo, u_hi = (m_hi == -INFINITY) ? 0.f : m_hi;
-    float pr[2][4];
 #pragma unroll
-    for (int nt = 0; nt < 2; ++nt) {
-      pr[nt][0] = ex2(x[nt][0] - u_lo);
-      pr[nt][1] = ex2(x[nt][1] - u_lo);
-      pr[nt][2] = ex2(x[nt][2] - u_hi);
-      pr[nt][3] = ex2(x[nt][3] - u_hi);
-      l_lo += pr[nt][0] + pr[nt][1];
-      l_hi += pr[nt][2] + pr[nt][3];
-    }
-    const uint32_t pa[4] = {pack2<T>(pr[0][0], pr[0][1]), pack2<T>(pr[0][2], pr[0][3]),
-                            pack2<T>(pr[1][0], pr[1][1]), pack2<T>(pr[1][2], pr[1][3])};
+    for (int ks = 0; ks < NT / 2; ++ks) {  // 16 tokens: one K-step of P V
+      float(*pr)[4] = x + 2 * ks;
 #pragma unroll
-    for (int nt = 0; nt < DP / 8; nt += 2) {
-      const int hf = nt / 8, ch = (nt % 8) + (mi >> 1);
-      const int tok = mr + 8 * (mi & 1);
-      uint32_t b0, b1, b2, b3;
-      ldsm_x4_t(sw128(vbase + hf * Cfg::HALF, tok, ch), b0, b1, b2, b3);
-      mma16816<T>(o[nt], pa, b0, b1);
-      mma16816<T>(o[nt + 1], pa, b2, b3);
+      for (int nt = 0; nt < 2; ++nt) {
+        pr[nt][0] = ex2(pr[nt][0] - u_lo);
+        pr[nt][1] = ex2(pr[nt][1] - u_lo);
+        pr[nt][2] = ex2(pr[nt][2] - u_hi);
+        pr[nt][3] = ex2(pr[nt][3] - u_hi);
+        l_lo += pr[nt][0] + pr[nt][1];
+        l_hi += pr[nt][2] + pr[nt][3];
+      }
+      const uint32_t pa[4] = {pack2<T>(pr[0][0], pr[0][1]), pack2<T>(pr[0][2], pr[0][3]),
+                              pack2<T>(pr[1][0], pr[1][1]), pack2<T>(pr[1][2], pr[1][3])};
+#pragma unroll
+      for (int nt = 0; nt < DP / 8; nt += 2) {
+        const int hf = nt / 8, ch = (nt % 8) + (mi >> 1);
+        const int tok = 16 * ks + mr + 8 * (mi & 1);
+        uint32_t b0, b1, b2, b3;
+        ldsm_x4_t(sw128(vbase + hf * Cfg::HALF, tok, ch), b0, b1, b2, b3);
+        mma16816<T>(o[nt], pa, b0, b1);
+        mma16816<T>(o[nt + 1], pa, b2, b3);
+      }
     }
     __syncwarp();  // every lane has read the stage before it is refilled
     if (i + S < n) issue(i + S, rows.row(vidx(i + S), next_page));
@@ -359,13 +382,23 @@ __global__ void __launch_bounds__(WD_THREADS) ffa_window_decode_kernel(const WdP
   cluster.sync();  // no CTA leaves while another reads its shared memory
 }
 
-// CTAs per cluster: enough that the grid fills the SMs several times over (the
-// last wave's idle SMs cost little then), but no less than 64 tokens each (a
-// chunk per warp), and at most 16.
-static int wd_splits(int64_t pairs, int visible) {
-  int splits = 1;
-  while (splits < 16 && pairs * splits < 148 * 8 && visible >= 2 * splits * WD_WARPS * WD_CHUNK) splits *= 2;
-  return splits;
+// CTAs per cluster (a power of two up to 16, no less than a chunk per warp):
+// the count with the least waves x (tokens per CTA + what a CTA costs beside
+// them).  Three CTAs fit an SM; a CTA's start and join cost about as much as
+// 19200 / D tokens (5 us against 35 ns a token of K and V at D = 128 with every
+// SM streaming).  Measured at 1, 2, 4, 8, 16: the case above 201, 177, 165, 195,
+// 295 us (it takes 4); one request 64, 36, 21, 13.6, 11.1 (16); 5 requests of up
+// to 3000 tokens, window 1000, 20 heads of 64: 15.3, 11.5, 9.1, 15.0, 26 (4).
+static int wd_splits(int64_t pairs, int64_t visible, int D) {
+  int best = 1;
+  double least = 0;
+  for (int s = 1; s <= 16 && (s == 1 || visible >= (int64_t)s * WD_WARPS * WD_CHUNK); s *= 2) {
+    double waves = (double)(pairs * s) / (148 * 3);
+    if (waves < 3) waves = ceil(waves);
+    const double cost = waves * ((double)visible / s + 19200.0 / D);
+    if (s == 1 || cost < least) best = s, least = cost;
+  }
+  return best;
 }
 
 template <typename T, int DP>
@@ -452,7 +485,7 @@ extern "C" int ffa_window_decode(const void* q, const void* k_pages, const void*
   // the most tokens a request can see
   int64_t visible = max_ctx > 0 && max_ctx < p.max_ctx ? max_ctx : p.max_ctx;
   if (visible > (int64_t)window + sinks) visible = (int64_t)window + sinks;
-  p.splits = wd_splits(pairs, (int)visible);
+  p.splits = wd_splits(pairs, visible, D);
   const int64_t grid = pairs * p.splits;
   if (grid > 0x7fffffffLL) return FFA_ERR_UNSUPPORTED;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -119,6 +119,10 @@ def paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     return (out, lse) if return_lse else out
 
 
+def _int32(t: torch.Tensor) -> torch.Tensor:
+    return t if t.dtype is torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+
+
 def _window_decode(q, k_pages, v_pages, block_table, ctx_lens, scale, softcap, return_lse, max_ctx, window, sinks):
     _lib.require_cuda(q, k_pages, v_pages, block_table, ctx_lens)
     if q.dim() != 3 or k_pages.dim() != 4:
@@ -138,20 +142,21 @@ def _window_decode(q, k_pages, v_pages, block_table, ctx_lens, scale, softcap, r
         raise ValueError("page pools must be contiguous")
     if block_table.dim() != 2 or block_table.shape[0] != R or tuple(ctx_lens.shape) != (R,):
         raise ValueError("block_table must be [R, max_pages] and ctx_lens [R]")
-    bt = block_table.to(torch.int32).contiguous()
-    lens = ctx_lens.to(torch.int32).contiguous()
-    if q.stride(2) != 1 or q.stride(0) % 2 or q.stride(1) % 2 or q.data_ptr() % 4:
+    bt, lens = _int32(block_table), _int32(ctx_lens)
+    sr, sh, sd = q.stride()
+    if sd != 1 or (sr | sh) % 2 or q.data_ptr() % 4:
         q = q.contiguous()
+        sr, sh, _ = q.stride()
     if scale is None:
         scale = 1.0 / math.sqrt(D)
     big = 2 ** 31 - 1  # a window of any length: the kernel's is 32 bits, contexts fit it
-    out = torch.empty((R, Hq, D), dtype=q.dtype, device=q.device)
-    lse = torch.empty((R, Hq), dtype=torch.float32, device=q.device) if return_lse else None
+    out = q.new_empty((R, Hq, D))
+    lse = q.new_empty((R, Hq), dtype=torch.float32) if return_lse else None
     with _lib.device_of(q):
         st = _lib.load().ffa_window_decode(
             q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), bt.data_ptr(), lens.data_ptr(), out.data_ptr(),
             lse.data_ptr() if return_lse else None, _lib.DTYPE_CODE[q.dtype], R, Hq, Hkv, D, P, page_size,
-            bt.shape[1], _lib.i64arr(q.stride(0), q.stride(1)), _lib.i64arr(Hq * D, D), scale, softcap or 0.0,
+            bt.shape[1], _lib.i64arr(sr, sh), _lib.i64arr(Hq * D, D), scale, softcap or 0.0,
             min(window, big), min(sinks, big), max_ctx or 0, _lib.err_word(q.device).data_ptr(), _lib.stream_of(q))
     _lib.check(st, "ffa_window_decode")
     if _lib.sync_check_enabled():

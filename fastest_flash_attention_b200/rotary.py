@@ -203,7 +203,7 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.
     if slots.dtype != torch.int32 or tuple(slots.shape) != (T,):
         raise ValueError(f"slots must be int32 [T], got {slots.dtype} {tuple(slots.shape)}")
     q, k, v, positions, slots = (_unit_last(t) for t in (q, k, v, positions, slots))
-    out = torch.empty((T, Hq, D), dtype=dt, device=q.device)
+    out = q.new_empty((T, Hq, D))
     arr = _lib.i64arr
     with _lib.device_of(q):
         st = _lib.load().ffa_rotary_append(
