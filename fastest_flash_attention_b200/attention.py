@@ -74,8 +74,7 @@ def _tma_ready(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     return t
 
 
-def _strides_bhs(t: torch.Tensor):
-    return _lib.strides3(t)
+_strides_bhs = _lib.strides3
 
 
 def _sinks(window: Optional[int], sink: int, block_mask: Optional[torch.Tensor]) -> int:
@@ -128,7 +127,7 @@ def flash_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float
         o = torch.empty_like(q)  # keeps q's stride order when q is dense
     else:
         o = torch.empty((B, Sq, Hq, Dv), dtype=dt, device=q.device).transpose(1, 2)
-    lse = torch.empty((B, Hq, Sq), dtype=torch.float32, device=q.device) if want_lse else None
+    lse = q.new_empty((B, Hq, Sq), dtype=torch.float32) if want_lse else None
     bm_ptr, n_br, n_bc = None, 0, 0
     if block_mask is not None:
         bm = block_mask.to(device=q.device, dtype=torch.uint8).contiguous()
@@ -282,7 +281,7 @@ def flash_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Ten
         ws_bytes = lib.ffa_bwd_sink_workspace_size(B, Hq, Hkv, Sq, Skv, D, Dv, window, sink)
     else:
         ws_bytes = lib.ffa_bwd_workspace_size(B, Hq, Sq)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+    ws = q.new_empty(ws_bytes, dtype=torch.uint8)
     common = (dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(),
               dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ATTN_DTYPE_CODE[dt], B, Hq, Hkv, Sq, Skv, D, v.shape[3],
               _strides_bhs(q), _strides_bhs(k), _strides_bhs(v), _strides_bhs(o), _strides_bhs(dout),

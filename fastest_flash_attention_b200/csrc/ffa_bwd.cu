@@ -1198,19 +1198,6 @@ __global__ void __launch_bounds__(256) ffa_bwd_sink_sum_kernel(const BwdParams p
   *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(a.x * mul, a.y * mul), pack2<T>(a.z * mul, a.w * mul));
 }
 
-// Key tiles that hold sinks, and the CTAs that share each one's queries: about
-// as many units (64-row query sub-tiles) per CTA as the window gives another
-// key tile, so that no CTA runs much longer than the rest.
-static void bwd_sink_shape(int Sq, int Skv, int window, int sink, int& tiles, int& parts) {
-  const int keys = sink < Skv ? sink : Skv;
-  tiles = (keys + BWD_BT - 1) / BWD_BT;
-  const int64_t n_q = ((int64_t)Sq + BWD_BS - 1) / BWD_BS;
-  const int64_t usual = ((int64_t)window + BWD_BT + BWD_BS - 1) / BWD_BS + 1;
-  int64_t n = (n_q + usual - 1) / usual;
-  if (n > 64) n = 64;
-  parts = (int)(n < 1 ? 1 : n);
-}
-
 // CTA-order group sizes (see the kernels' block mapping): groups whose
 // streamed operands fit in about 48 MB of L2 together, so each streamed tile
 // is read from HBM once per group instead of once per CTA that reads it.
@@ -1315,10 +1302,14 @@ extern "C" size_t ffa_bwd_workspace_size(int B, int Hq, int Sq) {
 
 extern "C" size_t ffa_bwd_sink_workspace_size(int B, int Hq, int Hkv, int Sq, int Skv, int D, int Dv, int window,
                                               int sinks) {
-  int tiles = 0, parts = 0;
-  ffa::bwd_sink_shape(Sq, Skv, window, sinks, tiles, parts);
-  return ffa_bwd_workspace_size(B, Hq, Sq) + 16 +
-         (size_t)B * Hkv * tiles * parts * ffa::BWD_BT * ((size_t)D + Dv) * sizeof(float);
+  size_t rows = 0;  // fp32 sums: of the tensor-core kernels' 128-key tiles, or of the fp32 kernels' 64-key ones
+  for (int tile : {64, ffa::BWD_BT}) {
+    int tiles = 0, parts = 0;
+    ffa::bwd_sink_shape(tile, Sq, Skv, window, sinks, tiles, parts);
+    const size_t n = (size_t)tiles * parts * tile;
+    if (n > rows) rows = n;
+  }
+  return ffa_bwd_workspace_size(B, Hq, Sq) + 16 + (size_t)B * Hkv * rows * ((size_t)D + Dv) * sizeof(float);
 }
 
 namespace ffa {
@@ -1345,11 +1336,13 @@ static int bwd_impl(const void* dout, const void* q, const void* k, const void* 
   const size_t need =
       sink > 0 ? ffa_bwd_sink_workspace_size(B, Hq, Hkv, Sq, Skv, D, Dv, window, sink) : stats;
   if (!workspace || workspace_bytes < need) return FFA_ERR_WORKSPACE;
+  float* sink_ws = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(workspace) + stats + 15) & ~uintptr_t(15));
   if (dtype == FFA_DTYPE_F32)
     return f32_bwd(dout, q, k, v, o, lse, dq, dk, dv, B, Hq, Hkv, Sq, Skv, D, Dv, q_strides, k_strides, v_strides,
                    o_strides, do_strides, dq_strides, dk_strides, dv_strides, scale, causal, q_offset, window, sink,
                    softcap, block_mask, n_br, n_bc, mask_bq, mask_bkv,
-                   reinterpret_cast<void*>((reinterpret_cast<uintptr_t>(workspace) + 127) & ~uintptr_t(127)), stream);
+                   reinterpret_cast<void*>((reinterpret_cast<uintptr_t>(workspace) + 127) & ~uintptr_t(127)), sink_ws,
+                   stream);
   const int64_t* outs[3] = {dq_strides, dk_strides, dv_strides};
   for (auto* st : outs)
     if ((st[0] % 8) || (st[1] % 8) || (st[2] % 8)) return FFA_ERR_INVALID_ARG;
@@ -1393,8 +1386,8 @@ static int bwd_impl(const void* dout, const void* q, const void* k, const void* 
   p.window = window > 0 ? window : 0;
   if (sink > 0) {
     p.sink = sink;
-    bwd_sink_shape(Sq, Skv, window, sink, p.n_sink_tiles, p.sink_parts);
-    p.sink_ws = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(workspace) + stats + 15) & ~uintptr_t(15));
+    bwd_sink_shape(BWD_BT, Sq, Skv, window, sink, p.n_sink_tiles, p.sink_parts);
+    p.sink_ws = sink_ws;
     const int64_t ctas = ((int64_t)(Skv + BWD_BT - 1) / BWD_BT + (int64_t)p.n_sink_tiles * p.sink_parts) * B * Hkv;
     if (ctas > 0x7fffffffLL) return FFA_ERR_UNSUPPORTED;
   }

@@ -45,6 +45,11 @@ struct F32Params {
   int64_t q_s[3], k_s[3], v_s[3], o_s[3], do_s[3], out_s[3], dq_s[3], dk_s[3], dv_s[3];
   int B, Hq, Hkv, Sq, Skv, q_offset, causal, window;
   int sink;  // keys [0, sink) stay visible outside the window
+  // backward: the first sink_tiles key tiles hold sinks and see every later
+  // query; sink_parts CTAs share each one's queries and leave their sums in
+  // sink_ws [B * Hkv, sink_tiles, sink_parts, 64, DQ + DV] (0 tiles: no sharing)
+  int sink_tiles, sink_parts;
+  float* sink_ws;
   float scale, softcap;
   const uint8_t* bm;
   int n_br, n_bc, mbq, mbk;
@@ -332,7 +337,8 @@ __global__ void __launch_bounds__(256) ffa_f32_delta_kernel(const F32Params p) {
 }
 
 // dK / dV: one CTA per (64-key tile, kv head, batch); it walks the query
-// heads of the GQA group and their visible 64-query tiles in order.
+// heads of the GQA group and their visible 64-query tiles in order.  With
+// shared sink tiles, the CTAs of their shares come first.
 template <int DQ, int DV>
 __global__ void __launch_bounds__(F_THREADS) ffa_f32_dkdv_kernel(const F32Params p) {
   extern __shared__ float4 f32_smem4[];
@@ -344,7 +350,11 @@ __global__ void __launch_bounds__(F_THREADS) ffa_f32_dkdv_kernel(const F32Params
   float* sDST = sPT + 64 * 68;
   float* sLse = sDST + 64 * 68;
   float* sDelta = sLse + 64;
-  const int kt = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
+  const int hk = blockIdx.y, b = blockIdx.z;
+  const int shares = p.sink_tiles * p.sink_parts;
+  const bool shared = (int)blockIdx.x < shares;
+  const int kt = shared ? blockIdx.x % p.sink_tiles : blockIdx.x - shares + p.sink_tiles;
+  const int part = shared ? blockIdx.x / p.sink_tiles : 0, parts = shared ? p.sink_parts : 1;
   const int group = p.Hq / p.Hkv;
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
   const int j0 = kt * F_BN, j1 = min(j0 + F_BN, p.Skv) - 1;
@@ -360,45 +370,60 @@ __global__ void __launch_bounds__(F_THREADS) ffa_f32_dkdv_kernel(const F32Params
   }
   int qlo, qhi;
   f32_query_range(p, j0, j1, qlo, qhi);
-  for (int g = 0; g < group; ++g) {
-    const int h = hk * group + g;
+  // units: (query head of the group, 64-query tile), head-major
+  const int qt0 = max(qlo, 0) / F_BM;
+  const int n_qt = qhi > qt0 * F_BM ? (qhi + F_BM - 1) / F_BM - qt0 : 0;
+  const int64_t units = (int64_t)group * n_qt;
+  const int u1 = (int)(units * (part + 1) / parts);
+  for (int u = (int)(units * part / parts); u < u1; ++u) {
+    const int h = hk * group + u / n_qt;
     const float* qb = p.q + b * p.q_s[0] + h * p.q_s[1];
     const float* db = p.dout + b * p.do_s[0] + h * p.do_s[1];
     const int64_t rb = ((int64_t)b * p.Hq + h) * p.Sq;
-    for (int qt = max(qlo, 0) / F_BM; qt * F_BM < qhi; ++qt) {
-      const int i0 = qt * F_BM;
-      __syncthreads();
-      f32_load_tile<DQ>(sQ, qb, p.q_s[2], i0, p.Sq);
-      f32_load_tile<DV>(sDO, db, p.do_s[2], i0, p.Sq);
-      if (threadIdx.x < 64) {
-        const int qi = i0 + threadIdx.x;
-        sLse[threadIdx.x] = qi < p.Sq ? p.lse[rb + qi] : 0.f;
-        sDelta[threadIdx.x] = qi < p.Sq ? p.delta[rb + qi] : 0.f;
-      }
-      __syncthreads();
-      float s[4][4], dp[4][4];
-      f32_scores<DQ>(sK, sQ, ty, tx, s);   // S^T: rows = keys, columns = queries
-      f32_scores<DV>(sV, sDO, ty, tx, dp);  // dP^T
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int kj = j0 + 4 * ty + i;
-#pragma unroll
-        for (int jj = 0; jj < 4; ++jj) {
-          const int ql = tx + 16 * jj, qi = i0 + ql;
-          float th = 0.f;
-          const float x = f32_score(p, s[i][jj], &th);
-          const bool vis = f32_visible(p, qi, kj);
-          const float pr = vis ? expf(x - sLse[ql]) : 0.f;
-          float ds = pr * (dp[i][jj] - sDelta[ql]);
-          if (p.softcap > 0.f) ds *= 1.f - th * th;
-          sPT[(4 * ty + i) * 68 + ql] = pr;
-          sDST[(4 * ty + i) * 68 + ql] = ds;
-        }
-      }
-      __syncthreads();
-      f32_accumulate<DV>(sPT, sDO, ty, tx, adv);
-      f32_accumulate<DQ>(sDST, sQ, ty, tx, adk);
+    const int i0 = (qt0 + u % n_qt) * F_BM;
+    __syncthreads();
+    f32_load_tile<DQ>(sQ, qb, p.q_s[2], i0, p.Sq);
+    f32_load_tile<DV>(sDO, db, p.do_s[2], i0, p.Sq);
+    if (threadIdx.x < 64) {
+      const int qi = i0 + threadIdx.x;
+      sLse[threadIdx.x] = qi < p.Sq ? p.lse[rb + qi] : 0.f;
+      sDelta[threadIdx.x] = qi < p.Sq ? p.delta[rb + qi] : 0.f;
     }
+    __syncthreads();
+    float s[4][4], dp[4][4];
+    f32_scores<DQ>(sK, sQ, ty, tx, s);   // S^T: rows = keys, columns = queries
+    f32_scores<DV>(sV, sDO, ty, tx, dp);  // dP^T
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int kj = j0 + 4 * ty + i;
+#pragma unroll
+      for (int jj = 0; jj < 4; ++jj) {
+        const int ql = tx + 16 * jj, qi = i0 + ql;
+        float th = 0.f;
+        const float x = f32_score(p, s[i][jj], &th);
+        const bool vis = f32_visible(p, qi, kj);
+        const float pr = vis ? expf(x - sLse[ql]) : 0.f;
+        float ds = pr * (dp[i][jj] - sDelta[ql]);
+        if (p.softcap > 0.f) ds *= 1.f - th * th;
+        sPT[(4 * ty + i) * 68 + ql] = pr;
+        sDST[(4 * ty + i) * 68 + ql] = ds;
+      }
+    }
+    __syncthreads();
+    f32_accumulate<DV>(sPT, sDO, ty, tx, adv);
+    f32_accumulate<DQ>(sDST, sQ, ty, tx, adk);
+  }
+  if (shared) {
+    float* dst = p.sink_ws + ((((int64_t)b * p.Hkv + hk) * p.sink_tiles + kt) * p.sink_parts + part) * 64 * (DQ + DV);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float* row = dst + (4 * ty + i) * (DQ + DV) + 4 * tx;
+#pragma unroll
+      for (int c = 0; c < DV / 64; ++c) *reinterpret_cast<float4*>(row + 64 * c) = adv[i][c];
+#pragma unroll
+      for (int c = 0; c < DQ / 64; ++c) *reinterpret_cast<float4*>(row + DV + 64 * c) = adk[i][c];
+    }
+    return;
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -412,6 +437,31 @@ __global__ void __launch_bounds__(F_THREADS) ffa_f32_dkdv_kernel(const F32Params
           adk[i][c].x * p.scale, adk[i][c].y * p.scale, adk[i][c].z * p.scale, adk[i][c].w * p.scale);
 #pragma unroll
     for (int c = 0; c < DV / 64; ++c) *reinterpret_cast<float4*>(vrow + 4 * tx + 64 * c) = adv[i][c];
+  }
+}
+
+// Adds up the shares of the sink tiles in order: one thread for four columns of a key row.
+template <int DQ, int DV>
+__global__ void __launch_bounds__(F_THREADS) ffa_f32_sink_sum_kernel(const F32Params p) {
+  constexpr int V4 = (DQ + DV) / 4;
+  const int64_t t = (int64_t)blockIdx.x * F_THREADS + threadIdx.x;
+  const int64_t row = t / V4, tile = row / F_BN;
+  const int c = (int)(t % V4) * 4, r = (int)(row % F_BN);
+  if (tile >= (int64_t)p.B * p.Hkv * p.sink_tiles) return;
+  const int kj = (int)(tile % p.sink_tiles) * F_BN + r;
+  if (kj >= p.Skv) return;
+  const int hk = (int)(tile / p.sink_tiles % p.Hkv), b = (int)(tile / p.sink_tiles / p.Hkv);
+  const float* src = p.sink_ws + (tile * p.sink_parts * 64 + r) * (DQ + DV) + c;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = 0; i < p.sink_parts; ++i) {
+    const float4 x = *reinterpret_cast<const float4*>(src + (int64_t)i * 64 * (DQ + DV));
+    a.x += x.x, a.y += x.y, a.z += x.z, a.w += x.w;
+  }
+  if (c < DV) {
+    *reinterpret_cast<float4*>(p.dv + b * p.dv_s[0] + hk * p.dv_s[1] + (int64_t)kj * p.dv_s[2] + c) = a;
+  } else {
+    *reinterpret_cast<float4*>(p.dk + b * p.dk_s[0] + hk * p.dk_s[1] + (int64_t)kj * p.dk_s[2] + (c - DV)) =
+        make_float4(a.x * p.scale, a.y * p.scale, a.z * p.scale, a.w * p.scale);
   }
 }
 
@@ -517,9 +567,14 @@ int f32_bwd_launch(const F32Params& p, cudaStream_t s) {
   ffa_f32_delta_kernel<DV><<<(unsigned)((rows + 7) / 8), 256, 0, s>>>(p);
   if (int st = launch_status()) return st;
   static std::atomic<uint64_t> done_kv{0}, done_q{0};
-  int st = f32_launch(ffa_f32_dkdv_kernel<DQ, DV>, dim3((p.Skv + F_BN - 1) / F_BN, p.Hkv, p.B),
-                      F32Smem<DQ, DV>::DKDV, p, s, done_kv);
+  const int kv_ctas = (p.Skv + F_BN - 1) / F_BN - p.sink_tiles + p.sink_tiles * p.sink_parts;
+  int st = f32_launch(ffa_f32_dkdv_kernel<DQ, DV>, dim3(kv_ctas, p.Hkv, p.B), F32Smem<DQ, DV>::DKDV, p, s, done_kv);
   if (st) return st;
+  if (p.sink_tiles > 0) {
+    const int64_t sums = (int64_t)p.B * p.Hkv * p.sink_tiles * F_BN * ((DQ + DV) / 4);
+    ffa_f32_sink_sum_kernel<DQ, DV><<<(unsigned)((sums + F_THREADS - 1) / F_THREADS), F_THREADS, 0, s>>>(p);
+    if ((st = launch_status())) return st;
+  }
   return f32_launch(ffa_f32_dq_kernel<DQ, DV>, dim3((p.Sq + F_BM - 1) / F_BM, p.Hq, p.B), F32Smem<DQ, DV>::DQK, p,
                     s, done_q);
 }
@@ -585,7 +640,7 @@ int f32_bwd(const void* dout, const void* q, const void* k, const void* v, const
             const int64_t* o_strides, const int64_t* do_strides, const int64_t* dq_strides,
             const int64_t* dk_strides, const int64_t* dv_strides, float scale, int causal, int q_offset,
             int window, int sink, float softcap, const uint8_t* block_mask, int n_br, int n_bc, int mask_bq, int mask_bkv,
-            void* workspace, void* stream) {
+            void* workspace, float* sink_ws, void* stream) {
   if (!f32_dims_ok(D, Dv)) return FFA_ERR_UNSUPPORTED;
   if (!f32_strides_ok(q, q_strides) || !f32_strides_ok(k, k_strides) || !f32_strides_ok(v, v_strides) ||
       !f32_strides_ok(o, o_strides) || !f32_strides_ok(dout, do_strides) || !f32_strides_ok(dq, dq_strides) ||
@@ -603,6 +658,7 @@ int f32_bwd(const void* dout, const void* q, const void* k, const void* v, const
   p.dk = static_cast<float*>(dk);
   p.dv = static_cast<float*>(dv);
   p.delta = static_cast<float*>(workspace);
+  p.sink_ws = sink_ws;
   f32_copy_strides(p.q_s, q_strides);
   f32_copy_strides(p.k_s, k_strides);
   f32_copy_strides(p.v_s, v_strides);
@@ -613,6 +669,7 @@ int f32_bwd(const void* dout, const void* q, const void* k, const void* v, const
   f32_copy_strides(p.dv_s, dv_strides);
   f32_common(p, B, Hq, Hkv, Sq, Skv, scale, causal, q_offset, window, sink, softcap, block_mask, n_br, n_bc,
              mask_bq, mask_bkv);
+  if (p.sink > 0) bwd_sink_shape(F_BN, Sq, Skv, window, sink, p.sink_tiles, p.sink_parts);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (D == 64) return f32_bwd_launch<64, 64>(p, s);
   if (D == 128) return f32_bwd_launch<128, 128>(p, s);

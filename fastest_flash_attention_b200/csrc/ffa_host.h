@@ -64,6 +64,19 @@ int f32_bwd(const void* dout, const void* q, const void* k, const void* v, const
             const int64_t* o_strides, const int64_t* do_strides, const int64_t* dq_strides,
             const int64_t* dk_strides, const int64_t* dv_strides, float scale, int causal, int q_offset,
             int window, int sink, float softcap, const uint8_t* block_mask, int n_br, int n_bc, int mask_bq, int mask_bkv,
-            void* workspace, void* stream);
+            void* workspace, float* sink_ws, void* stream);
+
+// Backward with sinks: the `tile`-key tiles that hold them, [0, tiles), see
+// every later query, so `parts` CTAs share each one's queries: about as many
+// 64-query units per CTA as the window gives another key tile, so that no CTA
+// runs much longer than the rest.
+inline void bwd_sink_shape(int tile, int Sq, int Skv, int window, int sink, int& tiles, int& parts) {
+  const int keys = sink < Skv ? sink : Skv;
+  tiles = (keys + tile - 1) / tile;
+  const int64_t n_q = ((int64_t)Sq + 63) / 64;
+  const int64_t usual = ((int64_t)window + tile + 63) / 64 + 1;
+  const int64_t n = (n_q + usual - 1) / usual;
+  parts = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+}
 
 }  // namespace ffa
