@@ -146,7 +146,11 @@ enum : uint32_t {
 // SINK: a sliding window with the first p.sink keys visible outside it (as far
 // as causality allows).  The walk takes the key tiles that hold sinks and lie
 // left of the window's first, then the window's; sinks inside the window's
-// tiles are kept by the same per-element mask.  A kernel of its own, so the
+// tiles are kept by the same per-element mask.  A query tile skips the window
+// tiles that only the other one sees (under a short window they are a fair
+// share of the walk): prefill of 8192 tokens, 32/8 heads of 128, window 1024 + 4
+// 221 -> 214 us.  (A first step of 32 columns for few sinks measured slower, 225
+// us: its block costs the main loop registers.)  A kernel of its own, so the
 // others carry none of it.
 template <typename T, int D, int DV, int NQT, bool SINK>
 __global__ void __launch_bounds__(FwdShape<NQT>::THREADS, FwdShape<NQT>::MIN_BLOCKS)
@@ -269,6 +273,17 @@ __global__ void __launch_bounds__(FwdShape<NQT>::THREADS, FwdShape<NQT>::MIN_BLO
   auto tile_at = [&](int it) -> int {
     if (SINK) return it < n_sink ? it : j_lo + it;
     return use_list ? (int)list[it] : j_lo + it;
+  };
+  // SINK: query tile t takes part in steps [0, n_sink) and [w0(t), w1(t)) of
+  // the n, counted without gaps: step it is its own step it - gap(t) there.
+  auto step_range = [&](int t, int& w0, int& w1) {
+    const int a0 = a_lo + t * FWD_BM, a1 = min(a0 + FWD_BM - 1, a_hi);
+    const int first = a0 - p.window + 1;
+    w0 = n_sink;
+    w1 = n;
+    if (first > 0 && (j_lo + n_sink) * FWD_BN >= p.sink) w0 = max(n_sink, first / FWD_BN - j_lo);
+    if (p.causal) w1 = min(n, (a1 >= 0 ? a1 / FWD_BN + 1 : 0) - j_lo);
+    if (a0 > a_hi || w1 < w0) w0 = w1 = n_sink;  // past the last query, or no window tile
   };
   constexpr uint32_t FMT = DtypeFmt<T>::value;
 
@@ -395,12 +410,19 @@ __global__ void __launch_bounds__(FwdShape<NQT>::THREADS, FwdShape<NQT>::MIN_BLO
           mma_ts(d, a + ks * 8, vb + (uint64_t)((ks * 16 * 128) >> 4), idesc_pv, (acc || ks > 0) ? 1u : 0u);
         }
       };
+      int w0[NQT], w1[NQT];
+      if (SINK)
+        for (int t = 0; t < NQT; ++t) step_range(t, w0[t], w1[t]);
+      // whether query tile t takes part in step it, and the steps it skipped before
+      auto takes = [&](int t, int it) { return !SINK || it < n_sink || (it >= w0[t] && it < w1[t]); };
+      auto own = [&](int t, int it) { return SINK && it >= n_sink ? it - (w0[t] - n_sink) : it; };
       bool ok = n == 0 || mbar_wait_mma(&bars->q_full, 0, p.ec, abort_flag, SITE_FWD_Q);
       if (ok && n > 0) {
         ok = mbar_wait_mma(&bars->kv_full[0], 0, p.ec, abort_flag, SITE_FWD_KV_FULL);
         if (ok) {
           tc_fence_after();
           for (int t = 0; t < NQT; ++t) {
+            if (!takes(t, 0)) continue;
             issue_qk(t, 0);
             mma_commit(&bars->s_full[t]);
           }
@@ -423,16 +445,19 @@ __global__ void __launch_bounds__(FwdShape<NQT>::THREADS, FwdShape<NQT>::MIN_BLO
         const bool has_next = it + 1 < n;
         if (!mbar_wait_mma(&bars->kv_full[vbar], vph, p.ec, abort_flag, SITE_FWD_KV_FULL)) break;
         for (int t = 0; t < FWD_NQT && ok; ++t) {
-          for (int k = 0; k < FWD_PCH; ++k) {
-            if (!mbar_wait_mma(&bars->p_full[t][k], it & 1, p.ec, abort_flag, SITE_FWD_P_FULL)) {
-              ok = false;
-              break;
+          if (takes(t, it)) {
+            const int own_it = own(t, it);
+            for (int k = 0; k < FWD_PCH; ++k) {
+              if (!mbar_wait_mma(&bars->p_full[t][k], own_it & 1, p.ec, abort_flag, SITE_FWD_P_FULL)) {
+                ok = false;
+                break;
+              }
+              tc_fence_after();
+              issue_pv(t, vb, own_it > 0, k);
             }
-            tc_fence_after();
-            issue_pv(t, vb, it > 0, k);
+            if (!ok) break;
+            mma_commit(&bars->o_done[t]);
           }
-          if (!ok) break;
-          mma_commit(&bars->o_done[t]);
           // With two slots or a V ring of one, V of tile it is released as soon
           // as the last query tile's P·V retires (before the next S), so its
           // refill starts earlier; deeper shared rings release it below.
@@ -443,8 +468,10 @@ __global__ void __launch_bounds__(FwdShape<NQT>::THREADS, FwdShape<NQT>::MIN_BLO
               break;
             }
             tc_fence_after();
-            issue_qk(t, kb);
-            mma_commit(&bars->s_full[t]);
+            if (takes(t, it + 1)) {
+              issue_qk(t, kb);
+              mma_commit(&bars->s_full[t]);
+            }
           }
         }
         if (!ok) break;
@@ -469,8 +496,15 @@ __global__ void __launch_bounds__(FwdShape<NQT>::THREADS, FwdShape<NQT>::MIN_BLO
     const int arow = row + p.q_offset;
     float m = -INFINITY, l = 0.f;
     bool ok = true;
-    for (int it = 0; it < n; ++it) {
-      const int j = tile_at(it);
+    int own_n = n, gap = 0;  // this query tile's steps; the steps it skips after the sinks
+    if (SINK) {
+      int w0, w1;
+      step_range(t, w0, w1);
+      gap = w0 - n_sink;
+      own_n = n_sink + w1 - w0;
+    }
+    for (int it = 0; it < own_n; ++it) {
+      const int j = tile_at(SINK && it >= n_sink ? it + gap : it);
       ok = __all_sync(0xffffffffu, mbar_wait(&bars->s_full[t], it & 1, p.ec, abort_flag, SITE_FWD_S_FULL));
       if (!ok) break;
       tc_fence_after();
@@ -522,26 +556,28 @@ __global__ void __launch_bounds__(FwdShape<NQT>::THREADS, FwdShape<NQT>::MIN_BLO
         const int lo_c = p.window > 0 ? max(arow - p.window + 1 - c0, 0) : 0;
         const uint32_t span = hi >= lo_c ? (uint32_t)(hi - lo_c) : 0xffffffffu;
         const uint32_t ninf = __float_as_uint(-INFINITY);
-        if (SINK && c0 < p.sink) {
+        if (SINK) {
           // the window's range or the sinks before it, both up to `hi`: one
-          // keep bit for each column
+          // keep bit for each column, applied to the groups of 32 columns of
+          // which a row of the warp drops any
           const int n_keep = min(p.sink - c0, hi + 1);
-          uint32_t kb[4];
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
             const int a = max(lo_c - 32 * w, 0), e = min(hi - 32 * w, 31);
             const int z = min(n_keep - 32 * w, 32);
-            kb[w] = e >= a ? ((2u << (e - a)) - 1u) << a : 0u;
-            if (z > 0) kb[w] |= z == 32 ? ~0u : (1u << z) - 1u;
-          }
+            uint32_t kb = e >= a ? ((2u << (e - a)) - 1u) << a : 0u;
+            if (z > 0) kb |= z == 32 ? ~0u : (1u << z) - 1u;
+            if (!__all_sync(0xffffffffu, kb == ~0u)) {
 #pragma unroll
-          for (int c = 0; c < FWD_BN; ++c) s[c] = ((kb[c / 32] >> (c % 32)) & 1u) ? s[c] : ninf;
+              for (int c = 0; c < 32; ++c) s[32 * w + c] = ((kb >> c) & 1u) ? s[32 * w + c] : ninf;
+            }
+          }
         } else {
 #pragma unroll
-        for (int c = 0; c < FWD_BN; ++c) {
-          const bool keep = span != 0xffffffffu && (uint32_t)(c - lo_c) <= span;
-          s[c] = keep ? s[c] : ninf;
-        }
+          for (int c = 0; c < FWD_BN; ++c) {
+            const bool keep = span != 0xffffffffu && (uint32_t)(c - lo_c) <= span;
+            s[c] = keep ? s[c] : ninf;
+          }
         }
         if (!SINK && p.block_mask != nullptr) {
           // Column keep-bits of this row from the block mask (a runtime loop
@@ -642,8 +678,8 @@ __global__ void __launch_bounds__(FwdShape<NQT>::THREADS, FwdShape<NQT>::MIN_BLO
     }
     // ------------------------------ epilogue ------------------------------
     const bool have_o =
-        ok && n > 0 &&
-        __all_sync(0xffffffffu, mbar_wait(&bars->o_done[t], (n - 1) & 1, p.ec, abort_flag, SITE_FWD_O_DONE));
+        ok && own_n > 0 &&
+        __all_sync(0xffffffffu, mbar_wait(&bars->o_done[t], (own_n - 1) & 1, p.ec, abort_flag, SITE_FWD_O_DONE));
     if (have_o) tc_fence_after();
     const float inv_l = (l > 0.f) ? 1.f / l : 0.f;
     T* orow = reinterpret_cast<T*>(p.o) + (size_t)b * p.o_sb + (size_t)h * p.o_sh + (size_t)row * p.o_ss;
