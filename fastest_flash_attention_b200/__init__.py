@@ -22,6 +22,7 @@ from .decode import paged_decode
 from .fa4 import FA4AttnFunc, fa4_attn_func, fa4_forward_dispatch
 from .modules import FastestFlashMHA, FastestFlashGQA, FastestFlashMLA, FastestFlashFA4, RotaryEmbedding
 from .mla import MLADecoder, MLALatentCache, mla_decode, absorbed_weights
+from .streaming import FastestFlashStreamingGQA, StreamingDecoder
 from .utils import repeat_kv
 from .ring import ring_attention_forward, ring_attention_backward, ring_attention_func, zigzag_shard, zigzag_unshard
 
@@ -31,6 +32,6 @@ __all__ = [
     "FastestFlashGQA", "FastestFlashMLA", "FastestFlashFA4", "PagedKVCache", "ContinuousKVCache",
     "create_causal_block_mask", "create_sliding_window_block_mask", "create_local_block_mask",
     "auto_select_block_size", "check_triton_available", "paged_decode", "MLADecoder", "mla_decode",
-    "copy_pages", "move_tokens", "rotary_tables", "apply_rotary", "rotary_append",
+    "FastestFlashStreamingGQA", "StreamingDecoder", "copy_pages", "move_tokens", "rotary_tables", "apply_rotary", "rotary_append",
     "ring_attention_forward", "ring_attention_backward", "ring_attention_func", "zigzag_shard", "zigzag_unshard",
 ]

@@ -231,10 +231,21 @@ _HERE = contextlib.nullcontext()
 
 def device_of(t: torch.Tensor):
     """Context in which t's device is current (nothing to switch, and nothing to pay, where it already is)."""
-    return _HERE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _HERE if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
 _ERR_WORDS: dict[int, torch.Tensor] = {}
+
+
+_ERR_PTRS: dict[int, int] = {}
+
+
+def err_ptr(t: torch.Tensor) -> int:
+    """Address of the error word of t's device."""
+    p = _ERR_PTRS.get(t.device.index)
+    if p is None:
+        p = _ERR_PTRS[t.device.index] = err_word(t.device).data_ptr()
+    return p
 
 
 def err_word(device: torch.device) -> torch.Tensor:

@@ -137,13 +137,14 @@ def flash_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float
     operands = (q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr() if lse is not None else None,
                 _ATTN_DTYPE_CODE[dt], B, Hq, Hkv, Sq, Skv, D, Dv,
                 _strides_bhs(q), _strides_bhs(k), _strides_bhs(v), _strides_bhs(o),
-                float(scale), int(bool(causal)), int(q_offset), int(window or 0))
-    tail = (_lib.err_word(q.device).data_ptr(), _lib.stream_of(q))
+                scale, 1 if causal else 0, q_offset, window or 0)
+    cap = softcap or 0.0
+    tail = (_lib.err_ptr(q), _lib.stream_of(q))
     with _lib.device_of(q):
         if sink:
-            st = lib.ffa_fwd_sink(*operands, sink, float(softcap or 0.0), *tail)
+            st = lib.ffa_fwd_sink(*operands, sink, cap, *tail)
         else:
-            st = lib.ffa_fwd(*operands, float(softcap or 0.0), bm_ptr, n_br, n_bc, int(mask_block[0]),
+            st = lib.ffa_fwd(*operands, cap, bm_ptr, n_br, n_bc, int(mask_block[0]),
                              int(mask_block[1]), *tail)
     _lib.check(st, "ffa_fwd_sink" if sink else "ffa_fwd")
     if block_mask is not None:
@@ -288,7 +289,7 @@ def flash_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Ten
               _strides_bhs(dq), _strides_bhs(dk), _strides_bhs(dv),
               float(scale), int(bool(causal)), int(q_offset), int(window or 0))
     cap = float(softcap or 0.0)
-    tail = (ws.data_ptr(), ws_bytes, _lib.err_word(q.device).data_ptr(), _lib.stream_of(q))
+    tail = (ws.data_ptr(), ws_bytes, _lib.err_ptr(q), _lib.stream_of(q))
     with _lib.device_of(q):
         if sink:
             st = lib.ffa_bwd_sink(*common, sink, cap, *tail)

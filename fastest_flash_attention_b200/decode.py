@@ -140,7 +140,7 @@ def _window_decode(q, k_pages, v_pages, block_table, ctx_lens, scale, softcap, r
         raise ValueError("paged_decode needs fp16/bf16 q and pages of the same dtype")
     if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
         raise ValueError("page pools must be contiguous")
-    if block_table.dim() != 2 or block_table.shape[0] != R or tuple(ctx_lens.shape) != (R,):
+    if block_table.dim() != 2 or ctx_lens.dim() != 1 or block_table.shape[0] != R or ctx_lens.shape[0] != R:
         raise ValueError("block_table must be [R, max_pages] and ctx_lens [R]")
     bt, lens = _int32(block_table), _int32(ctx_lens)
     sr, sh, sd = q.stride()
@@ -157,7 +157,7 @@ def _window_decode(q, k_pages, v_pages, block_table, ctx_lens, scale, softcap, r
             q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), bt.data_ptr(), lens.data_ptr(), out.data_ptr(),
             lse.data_ptr() if return_lse else None, _lib.DTYPE_CODE[q.dtype], R, Hq, Hkv, D, P, page_size,
             bt.shape[1], _lib.i64arr(sr, sh), _lib.i64arr(Hq * D, D), scale, softcap or 0.0,
-            min(window, big), min(sinks, big), max_ctx or 0, _lib.err_word(q.device).data_ptr(), _lib.stream_of(q))
+            min(window, big), min(sinks, big), max_ctx or 0, _lib.err_ptr(q), _lib.stream_of(q))
     _lib.check(st, "ffa_window_decode")
     if _lib.sync_check_enabled():
         _lib.check_device_errors(q.device)

@@ -135,7 +135,7 @@ def copy_pages(k_pages: torch.Tensor, v_pages: Optional[torch.Tensor], src: Ids,
         st = _lib.load().ffa_page_copy(
             k_pages.data_ptr(), v_pages.data_ptr() if v_pages is not None else None, src.data_ptr(), dst.data_ptr(),
             src.numel(), k_pages.shape[0], k_pages.stride(0) * k_pages.element_size(),
-            _lib.err_word(k_pages.device).data_ptr(), _lib.stream_of(k_pages))
+            _lib.err_ptr(k_pages), _lib.stream_of(k_pages))
     _lib.check(st, "ffa_page_copy")
     if _lib.sync_check_enabled():
         _lib.check_device_errors(k_pages.device)
@@ -160,7 +160,7 @@ def move_tokens(k_pages: torch.Tensor, v_pages: Optional[torch.Tensor], src_slot
         st = _lib.load().ffa_token_move(
             k_pages.data_ptr(), v_pages.data_ptr() if v_pages is not None else None, src_slots.data_ptr(),
             dst_slots.data_ptr(), src_slots.numel(), k_pages.shape[1] if k_pages.dim() == 4 else 1, page_size, P,
-            D * k_pages.element_size(), _lib.err_word(k_pages.device).data_ptr(), _lib.stream_of(k_pages))
+            D * k_pages.element_size(), _lib.err_ptr(k_pages), _lib.stream_of(k_pages))
     _lib.check(st, "ffa_token_move")
     if _lib.sync_check_enabled():
         _lib.check_device_errors(k_pages.device)

@@ -106,7 +106,7 @@ def _rotate(q: torch.Tensor, k: Optional[torch.Tensor], cos: torch.Tensor, sin: 
         st = _lib.load().ffa_rotary(
             q.data_ptr(), qs, qo.data_ptr(), qd, kptr, ks, koptr, kd, cos.data_ptr(), sin.data_ptr(), cos.shape[0],
             pos.data_ptr(), _POS64[pos.dtype], pos.stride(0) if pos.dim() == 2 else 0, _lib.IN_DTYPE_CODE[q.dtype],
-            B, S, Hq, Hkv, D, 2 * cos.shape[1], layout, int(inverse), _lib.err_word(q.device).data_ptr(),
+            B, S, Hq, Hkv, D, 2 * cos.shape[1], layout, int(inverse), _lib.err_ptr(q),
             _lib.stream_of(q))
     _lib.check(st, "ffa_rotary")
     if _lib.sync_check_enabled():
@@ -193,16 +193,17 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.
         raise ValueError(f"incompatible shapes q {tuple(q.shape)} k {tuple(k.shape)} v {tuple(v.shape)} pools "
                          f"{tuple(k_pages.shape)} {tuple(v_pages.shape)}")
     dt = q.dtype
-    if dt not in _lib.IN_DTYPE_CODE or any(t.dtype != dt for t in (k, v, k_pages, v_pages)):
+    if dt not in _lib.IN_DTYPE_CODE or not (k.dtype == v.dtype == k_pages.dtype == v_pages.dtype == dt):
         raise ValueError("rotary_append needs q, k, v and both pools of one dtype (fp16, bf16 or fp32)")
     if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
         raise ValueError("page pools must be contiguous")
     rot = _check_tables(cos, sin, D, layout)
-    if positions.dtype not in _POS64 or tuple(positions.shape) != (T,):
+    if positions.dtype not in _POS64 or positions.dim() != 1 or positions.shape[0] != T:
         raise ValueError(f"positions must be int32 or int64 [T], got {positions.dtype} {tuple(positions.shape)}")
-    if slots.dtype != torch.int32 or tuple(slots.shape) != (T,):
+    if slots.dtype != torch.int32 or slots.dim() != 1 or slots.shape[0] != T:
         raise ValueError(f"slots must be int32 [T], got {slots.dtype} {tuple(slots.shape)}")
-    q, k, v, positions, slots = (_unit_last(t) for t in (q, k, v, positions, slots))
+    q, k, v = _unit_last(q), _unit_last(k), _unit_last(v)
+    positions, slots = _unit_last(positions), _unit_last(slots)
     out = q.new_empty((T, Hq, D))
     arr = _lib.i64arr
     with _lib.device_of(q):
@@ -211,7 +212,7 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.
             arr(k.stride(0), k.stride(1)), v.data_ptr(), arr(v.stride(0), v.stride(1)), cos.data_ptr(),
             sin.data_ptr(), cos.shape[0], positions.data_ptr(), _POS64[positions.dtype], slots.data_ptr(),
             k_pages.data_ptr(), v_pages.data_ptr(), _lib.IN_DTYPE_CODE[dt], T, Hq, Hkv, D, rot, _LAYOUTS[layout],
-            page_size, P, _lib.err_word(q.device).data_ptr(), _lib.stream_of(q))
+            page_size, P, _lib.err_ptr(q), _lib.stream_of(q))
     _lib.check(st, "ffa_rotary_append")
     if _lib.sync_check_enabled():
         _lib.check_device_errors(q.device)
