@@ -144,14 +144,19 @@ enum : uint32_t {
 
 
 // SINK: a sliding window with the first p.sink keys visible outside it (as far
-// as causality allows).  The walk takes the key tiles that hold sinks and lie
-// left of the window's first, then the window's; sinks inside the window's
-// tiles are kept by the same per-element mask.  A query tile skips the window
-// tiles that only the other one sees (under a short window they are a fair
-// share of the walk): prefill of 8192 tokens, 32/8 heads of 128, window 1024 + 4
-// 221 -> 214 us.  (A first step of 32 columns for few sinks measured slower, 225
-// us: its block costs the main loop registers.)  A kernel of its own, so the
-// others carry none of it.
+// as causality allows).  A kernel of its own, so the others carry none of it.
+// The plain walk takes the key tiles that hold sinks and lie left of the
+// window's first, then the window's; every query tile takes every step.  Where
+// one sink tile precedes a window whose tiles start and end one later for the
+// second query tile (the usual case), the walk is balanced instead: with
+// window tiles w0 .. w(m-1)
+//   query tile 0:  w0    w1 ... w(m-2)  sink
+//   query tile 1:  sink  w1 ... w(m-2)  w(m-1)
+// m steps without a tile that one of the two sees nothing of; the first and the
+// last step load a tile for each.  Prefill of 8192 tokens, 32/8 heads of 128,
+// window 1024 + 4 sinks: 221 us plain, 214 with steps skipped one-sidedly (the
+// second query tile then ends a step after the first), XXX balanced.  (A first
+// step of 32 columns for few sinks cost the main loop registers: 225 us.)
 template <typename T, int D, int DV, int NQT, bool SINK>
 __global__ void __launch_bounds__(FwdShape<NQT>::THREADS, FwdShape<NQT>::MIN_BLOCKS)
     ffa_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -274,17 +279,26 @@ __global__ void __launch_bounds__(FwdShape<NQT>::THREADS, FwdShape<NQT>::MIN_BLO
     if (SINK) return it < n_sink ? it : j_lo + it;
     return use_list ? (int)list[it] : j_lo + it;
   };
-  // SINK: query tile t takes part in steps [0, n_sink) and [w0(t), w1(t)) of
-  // the n, counted without gaps: step it is its own step it - gap(t) there.
-  auto step_range = [&](int t, int& w0, int& w1) {
-    const int a0 = a_lo + t * FWD_BM, a1 = min(a0 + FWD_BM - 1, a_hi);
-    const int first = a0 - p.window + 1;
-    w0 = n_sink;
-    w1 = n;
-    if (first > 0 && (j_lo + n_sink) * FWD_BN >= p.sink) w0 = max(n_sink, first / FWD_BN - j_lo);
-    if (p.causal) w1 = min(n, (a1 >= 0 ? a1 / FWD_BN + 1 : 0) - j_lo);
-    if (a0 > a_hi || w1 < w0) w0 = w1 = n_sink;  // past the last query, or no window tile
+  // SINK: the balanced walk (see above).  j_lo is n_sink short of the window's
+  // first tile here, so that is tile j_lo + 1 with one sink tile.
+  bool balanced = false;
+  if (SINK && NQT == 2 && n_sink == 1 && p.causal) {
+    const int first1 = a_lo + FWD_BM - p.window + 1, end0 = (a_lo + FWD_BM - 1) / FWD_BN + 1;
+    balanced = first1 / FWD_BN == j_lo + 2 && end0 == j_lo + n - 1 && a_hi >= a_lo + FWD_BM && end0 > j_lo + 1 &&
+               p.sink <= (j_lo + 1) * FWD_BN;
+  }
+  const int steps = balanced ? n - 1 : n;  // of each query tile
+  // the walk's key tile `x`, in the order they are loaded (steps + 2 of them
+  // when balanced), and which of them query tile t takes in step k
+  auto walk_tile = [&](int x) -> int {
+    if (!balanced) return tile_at(x);
+    return x == 1 || x == steps ? 0 : x == 0 ? j_lo + 1 : x == steps + 1 ? j_lo + steps : j_lo + x;
   };
+  auto walk_at = [&](int t, int k) -> int {
+    if (!balanced) return k;
+    return k == 0 ? t : k == steps - 1 ? steps + t : k + 1;
+  };
+  const int loads = balanced ? steps + 2 : n;
   constexpr uint32_t FMT = DtypeFmt<T>::value;
 
   if (warp >= 4 * NQT) {
@@ -311,8 +325,8 @@ __global__ void __launch_bounds__(FwdShape<NQT>::THREADS, FwdShape<NQT>::MIN_BLO
       const int bytes = is_v ? Cfg::VTILE : Cfg::TILE;
       uint8_t* ring = is_v ? sV : sKV;
       int issued = 0;  // slots armed so far
-      for (int it = 0; it < n; ++it) {
-        const int j = tile_at(it);
+      for (int it = 0; it < (SINK ? loads : n); ++it) {
+        const int j = SINK ? walk_tile(it) : tile_at(it);
         const int buf = it % nslot, use = it / nslot;
         if (use > 0 &&
             !mbar_wait(&bars->kv_empty[bar0 + buf], (use - 1) & 1, p.ec, abort_flag, SITE_FWD_KV_EMPTY))
@@ -345,8 +359,8 @@ __global__ void __launch_bounds__(FwdShape<NQT>::THREADS, FwdShape<NQT>::MIN_BLO
           tma_load_4d(&tmQ, &bars->q_full, sQ + t * Cfg::TILE + c * (FWD_BM * 128), c * 64, q_lo + t * FWD_BM,
                       h, b, pol_q);
       int issued = 0;  // key/value slots armed so far
-      for (int it = 0; it < n; ++it) {
-        const int j = tile_at(it);
+      for (int it = 0; it < (SINK ? loads : n); ++it) {
+        const int j = SINK ? walk_tile(it) : tile_at(it);
         bool ok = true;
         for (int kv = 0; kv < 2 && ok; ++kv) {
           const int s = 2 * it + kv;
@@ -410,26 +424,79 @@ __global__ void __launch_bounds__(FwdShape<NQT>::THREADS, FwdShape<NQT>::MIN_BLO
           mma_ts(d, a + ks * 8, vb + (uint64_t)((ks * 16 * 128) >> 4), idesc_pv, (acc || ks > 0) ? 1u : 0u);
         }
       };
-      int w0[NQT], w1[NQT];
-      if (SINK)
-        for (int t = 0; t < NQT; ++t) step_range(t, w0[t], w1[t]);
-      // whether query tile t takes part in step it, and the steps it skipped before
-      auto takes = [&](int t, int it) { return !SINK || it < n_sink || (it >= w0[t] && it < w1[t]); };
-      auto own = [&](int t, int it) { return SINK && it >= n_sink ? it - (w0[t] - n_sink) : it; };
+      // ring slot, barrier and phase of the K (or V) of load x
+      auto slot = [&](int x, bool v, int& buf, int& bar, uint32_t& phase) {
+        if constexpr (Cfg::SPLIT) {
+          const int ring = v ? Cfg::NV : Cfg::NK;
+          buf = x % ring;
+          bar = (v ? 4 : 0) + buf;
+          phase = (x / ring) & 1;
+        } else {
+          const int i = 2 * x + (v ? 1 : 0);
+          buf = bar = i % Cfg::NBUF;
+          phase = (i / Cfg::NBUF) & 1;
+        }
+      };
       bool ok = n == 0 || mbar_wait_mma(&bars->q_full, 0, p.ec, abort_flag, SITE_FWD_Q);
-      if (ok && n > 0) {
+      if constexpr (SINK) {
+        // Step k's load is k (+ 1 past the first when balanced); a first or last
+        // balanced step has a load for each query tile.  A slot is released once
+        // the last query tile that reads it has issued.
+        auto load_qk = [&](int x, int t, bool last) -> bool {
+          int buf, bar;
+          uint32_t phase;
+          slot(x, false, buf, bar, phase);
+          if (!mbar_wait_mma(&bars->kv_full[bar], phase, p.ec, abort_flag, SITE_FWD_KV_FULL)) return false;
+          tc_fence_after();
+          issue_qk(t, buf);
+          mma_commit(&bars->s_full[t]);
+          if (last) mma_commit(&bars->kv_empty[bar]);
+          return true;
+        };
+        for (int t = 0; t < NQT && ok && steps > 0; ++t)
+          ok = load_qk(balanced ? t : 0, t, balanced || t == NQT - 1);
+        int x = 0;
+        bool two = balanced;
+        for (int k = 0; k < steps && ok; ++k) {
+          const bool two_next = balanced && k + 2 == steps;
+          const int x_next = k + 1 + (balanced ? 1 : 0);
+#pragma unroll
+          for (int t = 0; t < NQT; ++t) {
+            int buf, bar;
+            uint32_t phase;
+            slot(x + (two ? t : 0), true, buf, bar, phase);
+            ok = mbar_wait_mma(&bars->kv_full[bar], phase, p.ec, abort_flag, SITE_FWD_KV_FULL);
+            for (int c = 0; c < FWD_PCH && ok; ++c) {
+              ok = mbar_wait_mma(&bars->p_full[t][c], k & 1, p.ec, abort_flag, SITE_FWD_P_FULL);
+              if (!ok) break;
+              tc_fence_after();
+              issue_pv(t, buf, k > 0, c);
+            }
+            if (!ok) break;
+            mma_commit(&bars->o_done[t]);
+            if ((Cfg::SPLIT || Cfg::NBUF == 2) && (two || t == NQT - 1)) mma_commit(&bars->kv_empty[bar]);
+            if (k + 1 < steps) {
+              ok = load_qk(x_next + (two_next ? t : 0), t, two_next || t == NQT - 1);
+              if (!ok) break;
+            }
+            // deeper rings release V after the next S is on its way
+            if (!(Cfg::SPLIT || Cfg::NBUF == 2) && (two || t == NQT - 1)) mma_commit(&bars->kv_empty[bar]);
+          }
+          x = x_next;
+          two = two_next;
+        }
+      } else if (ok && n > 0) {
         ok = mbar_wait_mma(&bars->kv_full[0], 0, p.ec, abort_flag, SITE_FWD_KV_FULL);
         if (ok) {
           tc_fence_after();
           for (int t = 0; t < NQT; ++t) {
-            if (!takes(t, 0)) continue;
             issue_qk(t, 0);
             mma_commit(&bars->s_full[t]);
           }
           mma_commit(&bars->kv_empty[0]);
         }
       }
-      for (int it = 0; it < n && ok; ++it) {
+      for (int it = 0; it < n && ok && !SINK; ++it) {
         // slot (vb: V of tile it, kb: K of tile it + 1), its barrier and phase
         int vb, kb, vbar, kbar;
         uint32_t vph, kph;
@@ -445,19 +512,16 @@ __global__ void __launch_bounds__(FwdShape<NQT>::THREADS, FwdShape<NQT>::MIN_BLO
         const bool has_next = it + 1 < n;
         if (!mbar_wait_mma(&bars->kv_full[vbar], vph, p.ec, abort_flag, SITE_FWD_KV_FULL)) break;
         for (int t = 0; t < FWD_NQT && ok; ++t) {
-          if (takes(t, it)) {
-            const int own_it = own(t, it);
-            for (int k = 0; k < FWD_PCH; ++k) {
-              if (!mbar_wait_mma(&bars->p_full[t][k], own_it & 1, p.ec, abort_flag, SITE_FWD_P_FULL)) {
-                ok = false;
-                break;
-              }
-              tc_fence_after();
-              issue_pv(t, vb, own_it > 0, k);
+          for (int k = 0; k < FWD_PCH; ++k) {
+            if (!mbar_wait_mma(&bars->p_full[t][k], it & 1, p.ec, abort_flag, SITE_FWD_P_FULL)) {
+              ok = false;
+              break;
             }
-            if (!ok) break;
-            mma_commit(&bars->o_done[t]);
+            tc_fence_after();
+            issue_pv(t, vb, it > 0, k);
           }
+          if (!ok) break;
+          mma_commit(&bars->o_done[t]);
           // With two slots or a V ring of one, V of tile it is released as soon
           // as the last query tile's P·V retires (before the next S), so its
           // refill starts earlier; deeper shared rings release it below.
@@ -468,10 +532,8 @@ __global__ void __launch_bounds__(FwdShape<NQT>::THREADS, FwdShape<NQT>::MIN_BLO
               break;
             }
             tc_fence_after();
-            if (takes(t, it + 1)) {
-              issue_qk(t, kb);
-              mma_commit(&bars->s_full[t]);
-            }
+            issue_qk(t, kb);
+            mma_commit(&bars->s_full[t]);
           }
         }
         if (!ok) break;
@@ -496,15 +558,9 @@ __global__ void __launch_bounds__(FwdShape<NQT>::THREADS, FwdShape<NQT>::MIN_BLO
     const int arow = row + p.q_offset;
     float m = -INFINITY, l = 0.f;
     bool ok = true;
-    int own_n = n, gap = 0;  // this query tile's steps; the steps it skips after the sinks
-    if (SINK) {
-      int w0, w1;
-      step_range(t, w0, w1);
-      gap = w0 - n_sink;
-      own_n = n_sink + w1 - w0;
-    }
+    const int own_n = SINK ? steps : n;
     for (int it = 0; it < own_n; ++it) {
-      const int j = tile_at(SINK && it >= n_sink ? it + gap : it);
+      const int j = SINK ? walk_tile(walk_at(t, it)) : tile_at(it);
       ok = __all_sync(0xffffffffu, mbar_wait(&bars->s_full[t], it & 1, p.ec, abort_flag, SITE_FWD_S_FULL));
       if (!ok) break;
       tc_fence_after();
