@@ -160,7 +160,8 @@ enum : uint32_t {
 template <typename T, int D, int DV, int NQT, bool SINK>
 __global__ void __launch_bounds__(FwdShape<NQT>::THREADS, FwdShape<NQT>::MIN_BLOCKS)
     ffa_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                   const __grid_constant__ CUtensorMap tmV, const FwdParams p) {
+                   const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO,
+                   const FwdParams p) {
   using Cfg = FwdCfg<D, DV, NQT>;
   using Shape = FwdShape<NQT>;
   constexpr int FWD_NQT = NQT;
@@ -314,8 +315,8 @@ __global__ void __launch_bounds__(FwdShape<NQT>::THREADS, FwdShape<NQT>::MIN_BLO
       if (!is_v) {
         tma_prefetch_desc(&tmQ);
         const uint64_t pol_q = policy_evict_first();
-        mbar_arrive_expect_tx(&bars->q_full, FWD_NQT * Cfg::TILE);
-        for (int t = 0; t < FWD_NQT; ++t)
+        if (n > 0) mbar_arrive_expect_tx(&bars->q_full, FWD_NQT * Cfg::TILE);
+        for (int t = 0; t < FWD_NQT && n > 0; ++t)
           for (int c = 0; c < D / 64; ++c)
             tma_load_4d(&tmQ, &bars->q_full, sQ + t * Cfg::TILE + c * (FWD_BM * 128), c * 64, q_lo + t * FWD_BM,
                         h, b, pol_q);
@@ -339,7 +340,7 @@ __global__ void __launch_bounds__(FwdShape<NQT>::THREADS, FwdShape<NQT>::MIN_BLO
       }
       if (*abort_flag) {
         // Let copies still in flight land before the CTA gives up its smem.
-        if (!is_v) mbar_wait(&bars->q_full, 0, p.ec, abort_flag, SITE_FWD_DRAIN, true);
+        if (!is_v && n > 0) mbar_wait(&bars->q_full, 0, p.ec, abort_flag, SITE_FWD_DRAIN, true);
         for (int s = max(0, issued - nslot); s < issued; ++s)
           mbar_wait(&bars->kv_full[bar0 + s % nslot], (s / nslot) & 1, p.ec, abort_flag, SITE_FWD_DRAIN, true);
       }
@@ -353,8 +354,9 @@ __global__ void __launch_bounds__(FwdShape<NQT>::THREADS, FwdShape<NQT>::MIN_BLO
       tma_prefetch_desc(&tmV);
       const uint64_t pol_q = policy_evict_first();
       const uint64_t pol_kv = policy_evict_last();
-      mbar_arrive_expect_tx(&bars->q_full, FWD_NQT * Cfg::TILE);
-      for (int t = 0; t < FWD_NQT; ++t)
+      // (without a key tile nothing would wait for Q before the CTA leaves)
+      if (n > 0) mbar_arrive_expect_tx(&bars->q_full, FWD_NQT * Cfg::TILE);
+      for (int t = 0; t < FWD_NQT && n > 0; ++t)
         for (int c = 0; c < D / 64; ++c)
           tma_load_4d(&tmQ, &bars->q_full, sQ + t * Cfg::TILE + c * (FWD_BM * 128), c * 64, q_lo + t * FWD_BM,
                       h, b, pol_q);
@@ -381,7 +383,7 @@ __global__ void __launch_bounds__(FwdShape<NQT>::THREADS, FwdShape<NQT>::MIN_BLO
       }
       if (*abort_flag) {
         // Let copies still in flight land before the CTA gives up its smem.
-        mbar_wait(&bars->q_full, 0, p.ec, abort_flag, SITE_FWD_DRAIN, true);
+        if (n > 0) mbar_wait(&bars->q_full, 0, p.ec, abort_flag, SITE_FWD_DRAIN, true);
         for (int s = max(0, issued - Cfg::NBUF); s < issued; ++s)
           mbar_wait(&bars->kv_full[s % Cfg::NBUF], (s / Cfg::NBUF) & 1, p.ec, abort_flag, SITE_FWD_DRAIN, true);
       }
@@ -756,11 +758,31 @@ __global__ void __launch_bounds__(FwdShape<NQT>::THREADS, FwdShape<NQT>::MIN_BLO
         const float2 v = fmul2(make_float2(__uint_as_float(ov[2 * e]), __uint_as_float(ov[2 * e + 1])), f2(inv_l));
         pk[e] = pack2<T>(v.x, v.y);
       }
-      if (store) {
+      if (SINK) {
+        // into the query tile's smem (idle: its last S is done), 128-byte
+        // swizzled in blocks of 64 columns, for one TMA store per warp and block
+        uint8_t* blk = sQ + t * Cfg::TILE + (c / 64) * (FWD_BM * 128) + r * 128;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          *reinterpret_cast<uint4*>(blk + (((c / 8 % 8 + e) ^ (r & 7)) << 4)) =
+              make_uint4(pk[4 * e], pk[4 * e + 1], pk[4 * e + 2], pk[4 * e + 3]);
+      } else if (store) {
         uint4* dst = reinterpret_cast<uint4*>(orow + c);
 #pragma unroll
         for (int e = 0; e < 4; ++e) dst[e] = make_uint4(pk[4 * e], pk[4 * e + 1], pk[4 * e + 2], pk[4 * e + 3]);
       }
+    }
+    if (SINK && (have_o || own_n == 0)) {  // nothing after a wait that gave up
+      fence_async_smem();
+      __syncwarp();
+      const int row0 = q_lo + t * FWD_BM + (warp % 4) * 32;
+      if (lane == 0 && row0 < p.Sq) {
+        for (int c = 0; c < DV / 64; ++c)
+          tma_store_4d(&tmO, sQ + t * Cfg::TILE + c * (FWD_BM * 128) + (warp % 4) * (32 * 128), c * 64, row0, h, b);
+        tma_store_commit();
+        tma_store_wait_read();
+      }
+      __syncwarp();
     }
     if (store && p.lse != nullptr) {
       const float mu = (m == -INFINITY) ? 0.f : m;
@@ -778,13 +800,13 @@ __global__ void __launch_bounds__(FwdShape<NQT>::THREADS, FwdShape<NQT>::MIN_BLO
 }
 
 template <typename T, int D, int DV, int NQT, bool SINK>
-static int launch_fwd(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const FwdParams& p,
-                      int grid, cudaStream_t stream) {
+static int launch_fwd(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mo,
+                      const FwdParams& p, int grid, cudaStream_t stream) {
   using Cfg = FwdCfg<D, DV, NQT>;
   auto kern = ffa_fwd_kernel<T, D, DV, NQT, SINK>;
   static std::atomic<uint64_t> attr_done{0};
   if (int st = smem_attr_once(kern, Cfg::SMEM, attr_done)) return st;
-  kern<<<grid, FwdShape<NQT>::THREADS, Cfg::SMEM, stream>>>(mq, mk, mv, p);
+  kern<<<grid, FwdShape<NQT>::THREADS, Cfg::SMEM, stream>>>(mq, mk, mv, mo, p);
   return launch_status();
 }
 
@@ -897,7 +919,7 @@ static int fwd_impl(const void* q, const void* k, const void* v, void* o, float*
 
   const CUtensorMapDataType dt =
       dtype == FFA_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  CUtensorMap mq, mk, mv;
+  CUtensorMap mq, mk, mv, mo{};
   const int skv_map = Skv > 0 ? Skv : 1;
   int st = make_tmap_4d(&mq, q, dt, 2, D, Sq, Hq, B, q_strides[2] * 2, q_strides[1] * 2, q_strides[0] * 2, 64,
                         FWD_BM);
@@ -907,6 +929,8 @@ static int fwd_impl(const void* q, const void* k, const void* v, void* o, float*
   if (!st)
     st = make_tmap_4d(&mv, v, dt, 2, Dv, skv_map, Hkv, B, v_strides[2] * 2, v_strides[1] * 2, v_strides[0] * 2, 64,
                       FWD_BN);
+  if (!st && sink > 0)  // O by TMA: one 32-row x 64-column box per warp and block of columns
+    st = make_tmap_4d(&mo, o, dt, 2, Dv, Sq, Hq, B, o_strides[2] * 2, o_strides[1] * 2, o_strides[0] * 2, 64, 32);
   if (st) return st;
 
   const long long grid = (long long)p.n_qblk * B * Hq;
@@ -919,12 +943,12 @@ static int fwd_impl(const void* q, const void* k, const void* v, void* o, float*
     auto typed = [&](auto t) -> int {
       using T = decltype(t);
       if (D == 64)
-        return nqt == 1 ? launch_fwd<T, 64, 64, 1, SINK>(mq, mk, mv, p, (int)grid, s)
-                        : launch_fwd<T, 64, 64, 2, SINK>(mq, mk, mv, p, (int)grid, s);
+        return nqt == 1 ? launch_fwd<T, 64, 64, 1, SINK>(mq, mk, mv, mo, p, (int)grid, s)
+                        : launch_fwd<T, 64, 64, 2, SINK>(mq, mk, mv, mo, p, (int)grid, s);
       if (D == 128)
-        return nqt == 1 ? launch_fwd<T, 128, 128, 1, SINK>(mq, mk, mv, p, (int)grid, s)
-                        : launch_fwd<T, 128, 128, 2, SINK>(mq, mk, mv, p, (int)grid, s);
-      return launch_fwd<T, 192, 128, 2, SINK>(mq, mk, mv, p, (int)grid, s);
+        return nqt == 1 ? launch_fwd<T, 128, 128, 1, SINK>(mq, mk, mv, mo, p, (int)grid, s)
+                        : launch_fwd<T, 128, 128, 2, SINK>(mq, mk, mv, mo, p, (int)grid, s);
+      return launch_fwd<T, 192, 128, 2, SINK>(mq, mk, mv, mo, p, (int)grid, s);
     };
     return dtype == FFA_DTYPE_BF16 ? typed(__nv_bfloat16{}) : typed(__half{});
   };
