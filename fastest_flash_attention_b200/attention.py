@@ -75,6 +75,7 @@ def _tma_ready(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
 
 
 _strides_bhs = _lib.strides3
+_MAX_WINDOW = 2 ** 30  # past any length: the kernels add positions to it in 32 bits
 
 
 def _sinks(window: Optional[int], sink: int, block_mask: Optional[torch.Tensor]) -> int:
@@ -113,6 +114,7 @@ def flash_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float
         raise ValueError(f"head dims (qk={D}, v={Dv}) not supported by the sm_100a forward kernel "
                          f"(supported: qk <= {MAX_HEAD_DIM}, v <= 128)")
     sink = _sinks(window, sink, block_mask)
+    window = min(window or 0, _MAX_WINDOW)
     dt = kernel_dtype(q, compute_dtype)
     if kdims != (D, Dv):
         o, lse = flash_fwd(_pad_last(q.to(dt), kdims[0]), _pad_last(k.to(dt), kdims[0]),
@@ -137,7 +139,7 @@ def flash_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float
     operands = (q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr() if lse is not None else None,
                 _ATTN_DTYPE_CODE[dt], B, Hq, Hkv, Sq, Skv, D, Dv,
                 _strides_bhs(q), _strides_bhs(k), _strides_bhs(v), _strides_bhs(o),
-                scale, 1 if causal else 0, q_offset, window or 0)
+                scale, 1 if causal else 0, q_offset, window)
     cap = softcap or 0.0
     tail = (_lib.err_ptr(q), _lib.stream_of(q))
     with _lib.device_of(q):
@@ -261,6 +263,7 @@ def flash_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Ten
     if Hq % Hkv != 0:
         raise ValueError(f"query heads ({Hq}) must be a multiple of key/value heads ({Hkv})")
     sink = _sinks(window, sink, block_mask)
+    window = min(window or 0, _MAX_WINDOW)
     dt = kernel_dtype(q, compute_dtype)
     if kdims != (D, Dv):
         # zero columns: Delta, dP and the kept gradient columns are unchanged
@@ -287,7 +290,7 @@ def flash_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Ten
               dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ATTN_DTYPE_CODE[dt], B, Hq, Hkv, Sq, Skv, D, v.shape[3],
               _strides_bhs(q), _strides_bhs(k), _strides_bhs(v), _strides_bhs(o), _strides_bhs(dout),
               _strides_bhs(dq), _strides_bhs(dk), _strides_bhs(dv),
-              float(scale), int(bool(causal)), int(q_offset), int(window or 0))
+              float(scale), int(bool(causal)), int(q_offset), int(window))
     cap = float(softcap or 0.0)
     tail = (ws.data_ptr(), ws_bytes, _lib.err_ptr(q), _lib.stream_of(q))
     with _lib.device_of(q):

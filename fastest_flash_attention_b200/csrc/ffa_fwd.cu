@@ -129,7 +129,6 @@ struct FwdBars {
   int n_tiles;
   int j_lo;
   int use_list;
-  int n_sink;
 };
 
 enum : uint32_t {
@@ -155,8 +154,10 @@ enum : uint32_t {
 // m steps without a tile that one of the two sees nothing of; the first and the
 // last step load a tile for each.  Prefill of 8192 tokens, 32/8 heads of 128,
 // window 1024 + 4 sinks: 221 us plain, 214 with steps skipped one-sidedly (the
-// second query tile then ends a step after the first), XXX balanced.  (A first
-// step of 32 columns for few sinks cost the main loop registers: 225 us.)
+// second query tile then ends a step after the first), 194 balanced, with O
+// stored by TMA and the first loads started before the CTA meets (211 without
+// these two).  A first step of 32 columns for few sinks cost the main loop
+// registers (225 us).
 template <typename T, int D, int DV, int NQT, bool SINK>
 __global__ void __launch_bounds__(FwdShape<NQT>::THREADS, FwdShape<NQT>::MIN_BLOCKS)
     ffa_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -204,7 +205,58 @@ __global__ void __launch_bounds__(FwdShape<NQT>::THREADS, FwdShape<NQT>::MIN_BLO
   const int a_hi = q_hi + p.q_offset;
   const int n_kv = (p.Skv + FWD_BN - 1) / FWD_BN;
 
-  if (threadIdx.x == 0) {
+  // Key-tile range [first, end) allowed by causal / window masks.
+  auto tile_range = [&]() -> int2 {
+    const int end = p.causal ? min(n_kv, a_hi >= 0 ? a_hi / FWD_BN + 1 : 0) : n_kv;
+    const int lo_col = p.window > 0 ? a_lo - p.window + 1 : 0;
+    return make_int2(lo_col > 0 ? min(lo_col / FWD_BN, end) : 0, end);
+  };
+  const int2 range = SINK ? tile_range() : make_int2(0, 0);
+  const int j_first = range.x, j_hi = range.y;
+  // SINK: the walk (see above): `loads` key tiles, `steps` of them for each
+  // query tile.  w0: the window's first tile, less the sink tiles before it.
+  const int n_sink = SINK ? min((p.sink + FWD_BN - 1) / FWD_BN, j_first) : 0;
+  const int w0 = j_first - n_sink, n_walk = max(0, j_hi - j_first) + n_sink;
+  bool balanced = false;
+  if (SINK && NQT == 2 && n_sink == 1 && p.causal) {
+    const int first1 = a_lo + FWD_BM - p.window + 1, end0 = (a_lo + FWD_BM - 1) / FWD_BN + 1;
+    balanced = first1 / FWD_BN == j_first + 1 && end0 == j_hi - 1 && a_hi >= a_lo + FWD_BM && end0 > j_first &&
+               p.sink <= j_first * FWD_BN;
+  }
+  const int steps = balanced ? n_walk - 1 : n_walk, loads = balanced ? steps + 2 : n_walk;
+  // the walk's key tile `x`, in the order they are loaded, and which of them
+  // query tile t takes in step k
+  auto walk_tile = [&](int x) -> int {
+    if (!balanced) return x < n_sink ? x : w0 + x;
+    return x == 1 || x == steps ? 0 : x == 0 ? w0 + 1 : x == steps + 1 ? w0 + steps : w0 + x;
+  };
+  auto walk_at = [&](int t, int k) -> int {
+    if (!balanced) return k;
+    return k == 0 ? t : k == steps - 1 ? steps + t : k + 1;
+  };
+  // Q, and (shared ring) the K or V of key tile j, the x-th, into its slot
+  auto load_q = [&]() {
+    const uint64_t pol_q = policy_evict_first();
+    mbar_arrive_expect_tx(&bars->q_full, FWD_NQT * Cfg::TILE);
+    for (int t = 0; t < FWD_NQT; ++t)
+      for (int c = 0; c < D / 64; ++c)
+        tma_load_4d(&tmQ, &bars->q_full, sQ + t * Cfg::TILE + c * (FWD_BM * 128), c * 64, q_lo + t * FWD_BM, h, b,
+                    pol_q);
+  };
+  auto load_kv = [&](int x, int j, int kv, uint64_t pol_kv) {
+    const int buf = (2 * x + kv) % Cfg::NBUF;
+    mbar_arrive_expect_tx(&bars->kv_full[buf], kv ? Cfg::VTILE : Cfg::TILE);
+    uint8_t* dst = sKV + buf * Cfg::BUF;
+    for (int c = 0; c < (kv ? DV : D) / 64; ++c)
+      tma_load_4d(kv ? &tmV : &tmK, &bars->kv_full[buf], dst + c * (FWD_BN * 128), c * 64, j * FWD_BN, hkv, b,
+                  pol_kv);
+  };
+  // SINK (whose walk needs no list): the producer sets the barriers up and
+  // starts Q and the first loads, while the CTA gets its TMEM and meets.
+  constexpr bool EARLY = SINK && !Cfg::SPLIT;
+  const int n_early = EARLY ? min(loads, Cfg::NBUF / 2) : 0;
+
+  if (EARLY ? warp == FWD_WARP_LOAD && lane == 0 : threadIdx.x == 0) {
     mbar_init(&bars->q_full, 1);
     for (int t = 0; t < NQT; ++t) {
       mbar_init(&bars->s_full[t], 1);
@@ -218,33 +270,33 @@ __global__ void __launch_bounds__(FwdShape<NQT>::THREADS, FwdShape<NQT>::MIN_BLO
     }
     bars->abort = 0;
     fence_mbar_init();
+    if (EARLY && loads > 0) {
+      load_q();
+      const uint64_t pol_kv = policy_evict_last();
+      for (int x = 0; x < n_early; ++x)
+        for (int kv = 0; kv < 2; ++kv) load_kv(x, walk_tile(x), kv, pol_kv);
+    }
   }
+  __syncwarp();
   if (warp == FWD_WARP_MMA) {
     tmem_alloc(&bars->tmem_base, Shape::TMEM_COLS);
     tmem_relinquish();
   }
-  if (warp == FWD_WARP_LOAD) {
-    // Key-tile range allowed by causal / window masks, then filtered by the
-    // block mask (a tile stays if any of its (row, col) pairs is kept).
-    int j_hi = n_kv;
-    if (p.causal) j_hi = min(n_kv, a_hi >= 0 ? a_hi / FWD_BN + 1 : 0);
-    int j_lo = 0;
-    if (p.window > 0) {
-      const int lo_col = a_lo - p.window + 1;
-      if (lo_col > 0) j_lo = min(lo_col / FWD_BN, j_hi);
-    }
+  if (!SINK && warp == FWD_WARP_LOAD) {
+    // The range, filtered by the block mask (a tile stays if any of its (row,
+    // col) pairs is kept).
+    const int2 range = tile_range();
+    const int j_first = range.x, j_hi = range.y;
     if (p.block_mask == nullptr) {
       if (lane == 0) {
-        const int n_sink = SINK ? min((p.sink + FWD_BN - 1) / FWD_BN, j_lo) : 0;
-        bars->j_lo = j_lo - n_sink;  // tile_at's offset past the sink tiles
-        bars->n_sink = n_sink;
-        bars->n_tiles = max(0, j_hi - j_lo) + n_sink;
+        bars->j_lo = j_first;
+        bars->n_tiles = max(0, j_hi - j_first);
         bars->use_list = 0;
       }
     } else {
       int count = 0;
       const int br_lo = q_lo / p.mask_bq, br_hi = q_hi / p.mask_bq;
-      for (int j0 = j_lo; j0 < j_hi; j0 += 32) {
+      for (int j0 = j_first; j0 < j_hi; j0 += 32) {
         const int j = j0 + lane;
         bool keep = false;
         if (j < j_hi) {
@@ -272,34 +324,10 @@ __global__ void __launch_bounds__(FwdShape<NQT>::THREADS, FwdShape<NQT>::MIN_BLO
   tc_fence_after();
 
   const uint32_t tmem = bars->tmem_base;
-  const int n = bars->n_tiles;
-  const int j_lo = bars->j_lo;
-  const bool use_list = bars->use_list != 0;
-  const int n_sink = SINK ? bars->n_sink : 0;
-  auto tile_at = [&](int it) -> int {
-    if (SINK) return it < n_sink ? it : j_lo + it;
-    return use_list ? (int)list[it] : j_lo + it;
-  };
-  // SINK: the balanced walk (see above).  j_lo is n_sink short of the window's
-  // first tile here, so that is tile j_lo + 1 with one sink tile.
-  bool balanced = false;
-  if (SINK && NQT == 2 && n_sink == 1 && p.causal) {
-    const int first1 = a_lo + FWD_BM - p.window + 1, end0 = (a_lo + FWD_BM - 1) / FWD_BN + 1;
-    balanced = first1 / FWD_BN == j_lo + 2 && end0 == j_lo + n - 1 && a_hi >= a_lo + FWD_BM && end0 > j_lo + 1 &&
-               p.sink <= (j_lo + 1) * FWD_BN;
-  }
-  const int steps = balanced ? n - 1 : n;  // of each query tile
-  // the walk's key tile `x`, in the order they are loaded (steps + 2 of them
-  // when balanced), and which of them query tile t takes in step k
-  auto walk_tile = [&](int x) -> int {
-    if (!balanced) return tile_at(x);
-    return x == 1 || x == steps ? 0 : x == 0 ? j_lo + 1 : x == steps + 1 ? j_lo + steps : j_lo + x;
-  };
-  auto walk_at = [&](int t, int k) -> int {
-    if (!balanced) return k;
-    return k == 0 ? t : k == steps - 1 ? steps + t : k + 1;
-  };
-  const int loads = balanced ? steps + 2 : n;
+  const int n = SINK ? n_walk : bars->n_tiles;
+  const int j_lo = SINK ? 0 : bars->j_lo;
+  const bool use_list = !SINK && bars->use_list != 0;
+  auto tile_at = [&](int it) -> int { return use_list ? (int)list[it] : j_lo + it; };
   constexpr uint32_t FMT = DtypeFmt<T>::value;
 
   if (warp >= 4 * NQT) {
@@ -314,12 +342,7 @@ __global__ void __launch_bounds__(FwdShape<NQT>::THREADS, FwdShape<NQT>::MIN_BLO
       const uint64_t pol_kv = policy_evict_last();
       if (!is_v) {
         tma_prefetch_desc(&tmQ);
-        const uint64_t pol_q = policy_evict_first();
-        if (n > 0) mbar_arrive_expect_tx(&bars->q_full, FWD_NQT * Cfg::TILE);
-        for (int t = 0; t < FWD_NQT && n > 0; ++t)
-          for (int c = 0; c < D / 64; ++c)
-            tma_load_4d(&tmQ, &bars->q_full, sQ + t * Cfg::TILE + c * (FWD_BM * 128), c * 64, q_lo + t * FWD_BM,
-                        h, b, pol_q);
+        if (n > 0) load_q();
       }
       const int nslot = is_v ? Cfg::NV : Cfg::NK;
       const int bar0 = is_v ? 4 : 0;
@@ -349,37 +372,43 @@ __global__ void __launch_bounds__(FwdShape<NQT>::THREADS, FwdShape<NQT>::MIN_BLO
    } else if (!Cfg::SPLIT && warp == FWD_WARP_LOAD) {
     // ------------------------------ producer ------------------------------
     if (lane == 0) {
-      tma_prefetch_desc(&tmQ);
-      tma_prefetch_desc(&tmK);
-      tma_prefetch_desc(&tmV);
-      const uint64_t pol_q = policy_evict_first();
-      const uint64_t pol_kv = policy_evict_last();
-      // (without a key tile nothing would wait for Q before the CTA leaves)
-      if (n > 0) mbar_arrive_expect_tx(&bars->q_full, FWD_NQT * Cfg::TILE);
-      for (int t = 0; t < FWD_NQT && n > 0; ++t)
-        for (int c = 0; c < D / 64; ++c)
-          tma_load_4d(&tmQ, &bars->q_full, sQ + t * Cfg::TILE + c * (FWD_BM * 128), c * 64, q_lo + t * FWD_BM,
-                      h, b, pol_q);
-      int issued = 0;  // key/value slots armed so far
-      for (int it = 0; it < (SINK ? loads : n); ++it) {
-        const int j = SINK ? walk_tile(it) : tile_at(it);
+      int issued = 2 * n_early;  // key/value slots armed so far
+      if constexpr (EARLY) {
+        const uint64_t pol_kv = policy_evict_last();
         bool ok = true;
-        for (int kv = 0; kv < 2 && ok; ++kv) {
-          const int s = 2 * it + kv;
-          const int buf = s % Cfg::NBUF;
-          const int use = s / Cfg::NBUF;
-          if (use > 0 && !mbar_wait(&bars->kv_empty[buf], (use - 1) & 1, p.ec, abort_flag, SITE_FWD_KV_EMPTY)) {
-            ok = false;
-            break;
+        for (int x = n_early; x < loads && ok; ++x) {
+          const int j = walk_tile(x);
+          for (int kv = 0; kv < 2 && ok; ++kv) {
+            const int s = 2 * x + kv;
+            ok = mbar_wait(&bars->kv_empty[s % Cfg::NBUF], (s / Cfg::NBUF - 1) & 1, p.ec, abort_flag,
+                           SITE_FWD_KV_EMPTY);
+            if (!ok) break;
+            load_kv(x, j, kv, pol_kv);
+            ++issued;
           }
-          mbar_arrive_expect_tx(&bars->kv_full[buf], kv ? Cfg::VTILE : Cfg::TILE);
-          ++issued;
-          uint8_t* dst = sKV + buf * Cfg::BUF;
-          for (int c = 0; c < (kv ? DV : D) / 64; ++c)
-            tma_load_4d(kv ? &tmV : &tmK, &bars->kv_full[buf], dst + c * (FWD_BN * 128), c * 64, j * FWD_BN,
-                        hkv, b, pol_kv);
         }
-        if (!ok) break;
+      } else {
+        tma_prefetch_desc(&tmQ);
+        tma_prefetch_desc(&tmK);
+        tma_prefetch_desc(&tmV);
+        const uint64_t pol_kv = policy_evict_last();
+        // (without a key tile nothing would wait for Q before the CTA leaves)
+        if (n > 0) load_q();
+        for (int it = 0; it < n; ++it) {
+          const int j = tile_at(it);
+          bool ok = true;
+          for (int kv = 0; kv < 2 && ok; ++kv) {
+            const int s = 2 * it + kv, use = s / Cfg::NBUF;
+            if (use > 0 && !mbar_wait(&bars->kv_empty[s % Cfg::NBUF], (use - 1) & 1, p.ec, abort_flag,
+                                      SITE_FWD_KV_EMPTY)) {
+              ok = false;
+              break;
+            }
+            ++issued;
+            load_kv(it, j, kv, pol_kv);
+          }
+          if (!ok) break;
+        }
       }
       if (*abort_flag) {
         // Let copies still in flight land before the CTA gives up its smem.

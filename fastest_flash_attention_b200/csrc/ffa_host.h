@@ -69,14 +69,15 @@ int f32_bwd(const void* dout, const void* q, const void* k, const void* v, const
 // Backward with sinks: the `tile`-key tiles that hold them, [0, tiles), see
 // every later query, so `parts` CTAs share each one's queries: about as many
 // 64-query units per CTA as the window gives another key tile, so that no CTA
-// runs much longer than the rest.
+// runs much longer than the rest; at most 64 shares in all, since many sink
+// tiles are parallel work enough and every share holds fp32 sums.
 inline void bwd_sink_shape(int tile, int Sq, int Skv, int window, int sink, int& tiles, int& parts) {
   const int keys = sink < Skv ? sink : Skv;
   tiles = (keys + tile - 1) / tile;
   const int64_t n_q = ((int64_t)Sq + 63) / 64;
   const int64_t usual = ((int64_t)window + tile + 63) / 64 + 1;
-  const int64_t n = (n_q + usual - 1) / usual;
-  parts = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+  const int64_t n = (n_q + usual - 1) / usual, most = tiles > 32 ? 1 : 64 / (tiles > 0 ? tiles : 1);
+  parts = (int)(n < 1 ? 1 : n > most ? most : n);
 }
 
 }  // namespace ffa

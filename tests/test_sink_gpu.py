@@ -192,6 +192,33 @@ def test_no_sinks_and_no_window_change_nothing():
     assert torch.equal(a, b)
 
 
+def test_windows_and_sinks_past_any_length():
+    from fastest_flash_attention_b200 import fastest_flash_attn_forward, fastest_flash_attn_func
+    q, k, v, do = _tensors(1, 4, 2, 300, 300, 64, 64, torch.float16, 2)
+    want, _ = fastest_flash_attn_forward(q, k, v, causal=True)
+    for kw in (dict(sliding_window=2 ** 40), dict(sliding_window=2 ** 31, sink_tokens=3),
+               dict(sliding_window=1, sink_tokens=2 ** 40)):
+        o, _ = fastest_flash_attn_forward(q, k, v, causal=True, **kw)
+        assert torch.equal(o, want)
+        x = [t.detach().requires_grad_() for t in (q, k, v)]
+        g = torch.autograd.grad(fastest_flash_attn_func(*x, causal=True, **kw), x, do)
+        ref = torch.autograd.grad(fastest_flash_attn_func(*x, causal=True), x, do)
+        for name, a, b in zip(("dq", "dk", "dv"), g, ref):  # both are one rounding of nearly the same sums
+            _near(a, b.double(), torch.float16, name)
+
+
+def test_many_sink_tiles():
+    """Sinks over dozens of key tiles: each tile's queries are shared by few CTAs."""
+    from fastest_flash_attention_b200 import fastest_flash_attn_func
+    q, k, v, do = _tensors(1, 2, 1, 6000, 6000, 64, 64, torch.bfloat16, 6)
+    x = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = fastest_flash_attn_func(*x, causal=True, sliding_window=60, sink_tokens=4500)
+    grads = torch.autograd.grad(out, x, do)
+    want = _exact(q, k, v, do, _visible(6000, 6000, 60, 4500, True, 0), None, 0.125)
+    for name, got, ref in zip(("o", "dq", "dk", "dv"), (out,) + grads, (want[0],) + want[2:5]):
+        _near(got, ref, torch.bfloat16, name, want[5])
+
+
 def test_refusals():
     from fastest_flash_attention_b200 import fastest_flash_attn_backward, fastest_flash_attn_forward
     q, k, v, do = _tensors(1, 2, 2, 64, 64, 64, 64, torch.bfloat16, 1)
