@@ -1302,13 +1302,12 @@ extern "C" size_t ffa_bwd_workspace_size(int B, int Hq, int Sq) {
 
 extern "C" size_t ffa_bwd_sink_workspace_size(int B, int Hq, int Hkv, int Sq, int Skv, int D, int Dv, int window,
                                               int sinks) {
-  size_t rows = 0;  // fp32 sums: of the tensor-core kernels' 128-key tiles, or of the fp32 kernels' 64-key ones
-  for (int tile : {64, ffa::BWD_BT}) {
-    int tiles = 0, parts = 0;
-    ffa::bwd_sink_shape(tile, Sq, Skv, window, sinks, tiles, parts);
-    const size_t n = (size_t)tiles * parts * tile;
-    if (n > rows) rows = n;
-  }
+  // fp32 sums: of the tensor-core kernels' 128-key tiles, or of the fp32 kernels' 64-key ones
+  int tiles = 0, parts = 0;
+  ffa::bwd_sink_shape(ffa::BWD_BT, Sq, Skv, window, sinks, tiles, parts);
+  size_t rows = (size_t)tiles * parts * ffa::BWD_BT;
+  ffa::f32_bwd_sink_shape(B, Hq, Hkv, Sq, Skv, window, sinks, tiles, parts);
+  if ((size_t)tiles * parts * 64 > rows) rows = (size_t)tiles * parts * 64;
   return ffa_bwd_workspace_size(B, Hq, Sq) + 16 + (size_t)B * Hkv * rows * ((size_t)D + Dv) * sizeof(float);
 }
 

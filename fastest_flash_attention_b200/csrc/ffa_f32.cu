@@ -45,9 +45,10 @@ struct F32Params {
   int64_t q_s[3], k_s[3], v_s[3], o_s[3], do_s[3], out_s[3], dq_s[3], dk_s[3], dv_s[3];
   int B, Hq, Hkv, Sq, Skv, q_offset, causal, window;
   int sink;  // keys [0, sink) stay visible outside the window
-  // backward: the first sink_tiles key tiles hold sinks and see every later
-  // query; sink_parts CTAs share each one's queries and leave their sums in
-  // sink_ws [B * Hkv, sink_tiles, sink_parts, 64, DQ + DV] (0 tiles: no sharing)
+  // backward with sinks: sink_parts CTAs share the queries of each of the first
+  // sink_tiles key tiles (f32_bwd_sink_shape) and leave their sums in sink_ws
+  // [B * Hkv, sink_tiles, sink_parts, 64, DQ + DV] (0 tiles: no sharing).
+  // B2 H8 S1024 D64 window 256: 250 us unshared, 124 with the sink tile shared.
   int sink_tiles, sink_parts;
   float* sink_ws;
   float scale, softcap;
@@ -669,7 +670,7 @@ int f32_bwd(const void* dout, const void* q, const void* k, const void* v, const
   f32_copy_strides(p.dv_s, dv_strides);
   f32_common(p, B, Hq, Hkv, Sq, Skv, scale, causal, q_offset, window, sink, softcap, block_mask, n_br, n_bc,
              mask_bq, mask_bkv);
-  if (p.sink > 0) bwd_sink_shape(F_BN, Sq, Skv, window, sink, p.sink_tiles, p.sink_parts);
+  if (p.sink > 0) f32_bwd_sink_shape(B, Hq, Hkv, Sq, Skv, window, sink, p.sink_tiles, p.sink_parts);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (D == 64) return f32_bwd_launch<64, 64>(p, s);
   if (D == 128) return f32_bwd_launch<128, 128>(p, s);

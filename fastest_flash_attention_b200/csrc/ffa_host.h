@@ -80,4 +80,19 @@ inline void bwd_sink_shape(int tile, int Sq, int Skv, int window, int sink, int&
   parts = (int)(n < 1 ? 1 : n > most ? most : n);
 }
 
+// The same for the fp32 kernels' 64-key tiles, whose units are many times
+// slower: where the key tiles would keep half of the SMs idle, every tile's
+// queries are shared (B1 H32/8 S216 D64: 32 CTAs of up to 16 units, about 230
+// us, against 45 shared).  Larger grids are not worth it, since a share also loads its K and V
+// and leaves its sums (256 CTAs of 5 units in three shares each: 124 -> 165 us).
+inline void f32_bwd_sink_shape(int B, int Hq, int Hkv, int Sq, int Skv, int window, int sink, int& tiles,
+                               int& parts) {
+  bwd_sink_shape(64, Sq, Skv, window, sink, tiles, parts);
+  const int64_t all = ((int64_t)Skv + 63) / 64, ctas = all * B * Hkv;
+  if (ctas > 74) return;
+  const int64_t units = ((int64_t)Sq + 63) / 64 * (Hq / Hkv), n = 4 * 148 / ctas;
+  tiles = (int)all;
+  parts = (int)(n < units ? n : units);
+}
+
 }  // namespace ffa
