@@ -89,6 +89,12 @@ def _sinks(window: Optional[int], sink: int, block_mask: Optional[torch.Tensor])
     return min(int(sink), 2 ** 31 - 1)
 
 
+def _narrow_ok(sink: int, dt: torch.dtype, D: int, Dv: int) -> bool:
+    """Whether the kernels take head dims below their tile's as they are: the
+    16-bit kernels with sinks do (multiples of 8); the others get padded copies."""
+    return sink > 0 and dt in _KERNEL_DTYPES and D % 8 == 0 and Dv % 8 == 0
+
+
 def flash_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float, causal: bool = False,
               q_offset: int = 0, window: Optional[int] = None, softcap: Optional[float] = None,
               block_mask: Optional[torch.Tensor] = None, mask_block: Tuple[int, int] = (64, 64),
@@ -116,7 +122,7 @@ def flash_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float
     sink = _sinks(window, sink, block_mask)
     window = min(window or 0, _MAX_WINDOW)
     dt = kernel_dtype(q, compute_dtype)
-    if kdims != (D, Dv):
+    if kdims != (D, Dv) and not _narrow_ok(sink, dt, D, Dv):
         o, lse = flash_fwd(_pad_last(q.to(dt), kdims[0]), _pad_last(k.to(dt), kdims[0]),
                            _pad_last(v.to(dt), kdims[1]), scale=scale, causal=causal, q_offset=q_offset,
                            window=window, softcap=softcap, block_mask=block_mask, mask_block=mask_block,
@@ -265,7 +271,7 @@ def flash_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Ten
     sink = _sinks(window, sink, block_mask)
     window = min(window or 0, _MAX_WINDOW)
     dt = kernel_dtype(q, compute_dtype)
-    if kdims != (D, Dv):
+    if kdims != (D, Dv) and not _narrow_ok(sink, dt, D, Dv):
         # zero columns: Delta, dP and the kept gradient columns are unchanged
         kd, kv = kdims
         dq, dk, dv = flash_bwd(_pad_last(dout.to(dt), kv), _pad_last(q.to(dt), kd), _pad_last(k.to(dt), kd),

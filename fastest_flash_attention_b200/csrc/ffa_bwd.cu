@@ -73,7 +73,9 @@ struct BwdParams {
   // CTAs share such a tile's queries and leave fp32 sums in sink_ws
   // [B * Hkv, n_sink_tiles, sink_parts, 128, DV + D], which a last launch adds
   // up in order.
+  // (one share: an ordinary tile).
   int sink, n_sink_tiles, sink_parts;
+  int D, Dv;  // head dims (SINK kernels: multiples of 8, at most the tile's)
   float* sink_ws;
   // optional tile mask [n_br, n_bc] of (mask_bq x mask_bkv) blocks, the one
   // the forward was given: masked pairs get P = 0 (nullptr: none)
@@ -334,6 +336,20 @@ __device__ __forceinline__ void store_row32(T* dst, const uint32_t* v, float mul
   }
 }
 
+// Stores the first `left` (a multiple of 8, may be past N or negative) of N
+// fp32 accumulator columns of one row (times mul) as T.
+template <typename T, int N>
+__device__ __forceinline__ void store_row_upto(T* dst, const uint32_t* v, float mul, bool store, int left) {
+#pragma unroll
+  for (int e = 0; e < N; e += 8) {
+    uint32_t pk[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      pk[i] = pack2<T>(__uint_as_float(v[e + 2 * i]) * mul, __uint_as_float(v[e + 2 * i + 1]) * mul);
+    if (store && e < left) *reinterpret_cast<uint4*>(dst + e) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+  }
+}
+
 // K-major smem descriptor offset of the ks-th 16-column K step in a tile of
 // `rows` rows stored as 64-column (128-byte) swizzled chunks.
 __device__ __forceinline__ uint64_t kstep(int ks, int rows) {
@@ -384,8 +400,8 @@ __global__ void ffa_bwd_pre_kernel(const T* __restrict__ o, const T* __restrict_
 template <typename T, int TPR>
 __global__ void __launch_bounds__(256) ffa_bwd_pre_vec_kernel(
     const T* __restrict__ o, const T* __restrict__ dout, const float* __restrict__ lse, float* __restrict__ nlse2,
-    float* __restrict__ delta, int Hq, int Sq, int Sq_pad, int64_t o_sb, int64_t o_sh, int64_t o_ss, int64_t d_sb,
-    int64_t d_sh, int64_t d_ss, int n_rows) {
+    float* __restrict__ delta, int Hq, int Sq, int Sq_pad, int D, int64_t o_sb, int64_t o_sh, int64_t o_ss,
+    int64_t d_sb, int64_t d_sh, int64_t d_ss, int n_rows) {
   const int t = blockIdx.x * blockDim.x + threadIdx.x;
   const int row_g = t / TPR;
   const int sub = t % TPR;
@@ -394,7 +410,7 @@ __global__ void __launch_bounds__(256) ffa_bwd_pre_vec_kernel(
   const int q = live ? row_g % Sq_pad : Sq;
   const int b = bh / Hq, h = bh % Hq;
   float acc = 0.f;
-  if (q < Sq) {
+  if (q < Sq && sub * 8 < D) {
     const uint4 ov = __ldg(reinterpret_cast<const uint4*>(o + b * o_sb + h * o_sh + (int64_t)q * o_ss) + sub);
     const uint4 dv = __ldg(reinterpret_cast<const uint4*>(dout + b * d_sb + h * d_sh + (int64_t)q * d_ss) + sub);
     const uint32_t ow[4] = {ov.x, ov.y, ov.z, ov.w}, dw[4] = {dv.x, dv.y, dv.z, dv.w};
@@ -615,7 +631,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
     if ((int)blockIdx.x < shares) {
       bhk = (int)blockIdx.x % BHk;
       j = (int)blockIdx.x / BHk % p.n_sink_tiles;
-      part = (int)blockIdx.x / BHk / p.n_sink_tiles;
+      if (p.sink_parts > 1) part = (int)blockIdx.x / BHk / p.n_sink_tiles;
     } else {
       const int rem = (int)blockIdx.x - shares;
       bhk = rem % BHk;
@@ -855,7 +871,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
       }
       fence_async_smem();
       __syncwarp();
-      if (lane == 0) {
+      if (lane == 0 && (!SINK || half * 64 < (pair ? p.D : p.Dv))) {
         tma_store_4d(pair == 0 ? &tmDV : &tmDK, tile, half * 64, j * BWD_BT + (warp % 4) * 32, hkv, b);
         tma_store_commit();
         tma_store_wait_read();
@@ -872,7 +888,10 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
 #pragma unroll
           for (int e = 0; e < 32; ++e) v[e] = 0u;
         }
-        store_row32<T>(row + c, v, mul, store);
+        if constexpr (SINK)
+          store_row_upto<T, 32>(row + c, v, mul, store, (pair ? p.D : p.Dv) - c);
+        else
+          store_row32<T>(row + c, v, mul, store);
       }
     }
   }
@@ -1159,7 +1178,10 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
 #pragma unroll
         for (int e = 0; e < 16; ++e) v[e] = 0u;
       }
-      store_row16<T>(dqrow + c, v, p.scale, store);
+      if constexpr (SINK)
+        store_row_upto<T, 16>(dqrow + c, v, p.scale, store, p.D - c);
+      else
+        store_row16<T>(dqrow + c, v, p.scale, store);
     }
   }
   tc_fence_before();
@@ -1183,7 +1205,7 @@ __global__ void __launch_bounds__(256) ffa_bwd_sink_sum_kernel(const BwdParams p
   if (tile >= (int64_t)p.B * p.Hkv * p.n_sink_tiles) return;
   const int j = (int)(tile % p.n_sink_tiles), bhk = (int)(tile / p.n_sink_tiles);
   const int r = (int)(row % BWD_BT), key = j * BWD_BT + r;
-  if (key >= p.Skv) return;
+  if (key >= p.Skv || (c >= DV ? c - DV >= p.D : c >= p.Dv)) return;
   const float* src = p.sink_ws + (tile * p.sink_parts * BWD_BT + r) * (D + DV) + c;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int i = 0; i < p.sink_parts; ++i) {
@@ -1257,12 +1279,12 @@ static int launch_bwd(const CUtensorMap* maps, const BwdParams& p, const void* o
     const int blocks = (int)(((int64_t)n_rows * TPR + threads - 1) / threads);
     ffa_bwd_pre_vec_kernel<T, TPR><<<blocks, threads, 0, st>>>(
         reinterpret_cast<const T*>(o), reinterpret_cast<const T*>(dout), lse, lse2, delta, p.Hq, p.Sq, p.Sq_pad,
-        o_str[0], o_str[1], o_str[2], do_str[0], do_str[1], do_str[2], n_rows);
+        p.Dv, o_str[0], o_str[1], o_str[2], do_str[0], do_str[1], do_str[2], n_rows);
   } else {
     const int blocks = (int)(((int64_t)n_rows * 32 + threads - 1) / threads);
     ffa_bwd_pre_kernel<T><<<blocks, threads, 0, st>>>(
         reinterpret_cast<const T*>(o), reinterpret_cast<const T*>(dout), lse, lse2, delta, p.Hq, p.Sq, p.Sq_pad,
-        DV, o_str[0], o_str[1], o_str[2], do_str[0], do_str[1], do_str[2], n_rows);
+        p.Dv, o_str[0], o_str[1], o_str[2], do_str[0], do_str[1], do_str[2], n_rows);
   }
   int s = launch_status();
   if (s) return s;
@@ -1275,7 +1297,7 @@ static int launch_bwd(const CUtensorMap* maps, const BwdParams& p, const void* o
     const int grid = (SINK ? tiles - p.n_sink_tiles + p.n_sink_tiles * p.sink_parts : tiles) * p.B * p.Hkv;
     kern<<<grid, BWD_THREADS, DkdvCfg<D, DV>::SMEM, st>>>(maps[0], maps[1], maps[2], maps[3], maps[4], maps[5], p);
     if ((s = launch_status())) return s;
-    if (SINK) {
+    if (SINK && p.sink_parts > 1) {
       const int64_t threads_sum = (int64_t)p.B * p.Hkv * p.n_sink_tiles * BWD_BT * ((D + DV) / 4);
       ffa_bwd_sink_sum_kernel<T, D, DV><<<(unsigned)((threads_sum + 255) / 256), 256, 0, st>>>(p);
       if ((s = launch_status())) return s;
@@ -1308,7 +1330,9 @@ extern "C" size_t ffa_bwd_sink_workspace_size(int B, int Hq, int Hkv, int Sq, in
   size_t rows = (size_t)tiles * parts * ffa::BWD_BT;
   ffa::f32_bwd_sink_shape(B, Hq, Hkv, Sq, Skv, window, sinks, tiles, parts);
   if ((size_t)tiles * parts * 64 > rows) rows = (size_t)tiles * parts * 64;
-  return ffa_bwd_workspace_size(B, Hq, Sq) + 16 + (size_t)B * Hkv * rows * ((size_t)D + Dv) * sizeof(float);
+  int KD = D, KV = Dv;
+  ffa::attention_tile(D, Dv, true, KD, KV);  // sums are kept at the tile's width
+  return ffa_bwd_workspace_size(B, Hq, Sq) + 16 + (size_t)B * Hkv * rows * ((size_t)KD + KV) * sizeof(float);
 }
 
 namespace ffa {
@@ -1329,7 +1353,8 @@ static int bwd_impl(const void* dout, const void* q, const void* k, const void* 
       !dv_strides)
     return FFA_ERR_INVALID_ARG;
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || Sq <= 0 || Skv <= 0 || Hq % Hkv != 0) return FFA_ERR_INVALID_ARG;
-  if (!((D == 64 && Dv == 64) || (D == 128 && Dv == 128) || (D == 192 && Dv == 128))) return FFA_ERR_UNSUPPORTED;
+  int KD = 0, KV = 0;
+  if (!attention_tile(D, Dv, sink > 0 && dtype != FFA_DTYPE_F32, KD, KV)) return FFA_ERR_UNSUPPORTED;
   if (dtype != FFA_DTYPE_BF16 && dtype != FFA_DTYPE_F16 && dtype != FFA_DTYPE_F32) return FFA_ERR_UNSUPPORTED;
   const size_t stats = ffa_bwd_workspace_size(B, Hq, Sq);
   const size_t need =
@@ -1373,6 +1398,8 @@ static int bwd_impl(const void* dout, const void* q, const void* k, const void* 
   p.Hkv = Hkv;
   p.Sq = Sq;
   p.Skv = Skv;
+  p.D = D;
+  p.Dv = Dv;
   p.q_offset = q_offset;
   p.scale = scale;
   p.scale_log2 = scale * 1.4426950408889634f;
@@ -1426,8 +1453,8 @@ static int bwd_impl(const void* dout, const void* q, const void* k, const void* 
     constexpr bool BM = decltype(bm)::value, SINK = decltype(sk)::value;
     auto typed = [&](auto t) -> int {
       using T = decltype(t);
-      if (D == 64) return launch_bwd<T, 64, 64, BM, SINK>(maps, p, o, dout, lse, lse2, delta, o_strides, do_strides, s);
-      if (D == 128)
+      if (KD == 64) return launch_bwd<T, 64, 64, BM, SINK>(maps, p, o, dout, lse, lse2, delta, o_strides, do_strides, s);
+      if (KD == 128)
         return launch_bwd<T, 128, 128, BM, SINK>(maps, p, o, dout, lse, lse2, delta, o_strides, do_strides, s);
       return launch_bwd<T, 192, 128, BM, SINK>(maps, p, o, dout, lse, lse2, delta, o_strides, do_strides, s);
     };

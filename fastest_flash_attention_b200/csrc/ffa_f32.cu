@@ -670,7 +670,10 @@ int f32_bwd(const void* dout, const void* q, const void* k, const void* v, const
   f32_copy_strides(p.dv_s, dv_strides);
   f32_common(p, B, Hq, Hkv, Sq, Skv, scale, causal, q_offset, window, sink, softcap, block_mask, n_br, n_bc,
              mask_bq, mask_bkv);
-  if (p.sink > 0) f32_bwd_sink_shape(B, Hq, Hkv, Sq, Skv, window, sink, p.sink_tiles, p.sink_parts);
+  if (p.sink > 0) {
+    f32_bwd_sink_shape(B, Hq, Hkv, Sq, Skv, window, sink, p.sink_tiles, p.sink_parts);
+    if (p.sink_parts == 1) p.sink_tiles = 0;  // nothing to share
+  }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (D == 64) return f32_bwd_launch<64, 64>(p, s);
   if (D == 128) return f32_bwd_launch<128, 128>(p, s);

@@ -111,6 +111,7 @@ struct FwdParams {
   int use_softcap;
   int causal, window;
   int sink;  // SINK kernels: keys [0, sink) stay visible outside the window
+  int Dv;    // SINK kernels: value columns (a multiple of 8, at most the tile's)
   const uint8_t* block_mask;
   int n_br, n_bc, mask_bq, mask_bkv;
   ErrCtx ec;
@@ -806,7 +807,7 @@ __global__ void __launch_bounds__(FwdShape<NQT>::THREADS, FwdShape<NQT>::MIN_BLO
       __syncwarp();
       const int row0 = q_lo + t * FWD_BM + (warp % 4) * 32;
       if (lane == 0 && row0 < p.Sq) {
-        for (int c = 0; c < DV / 64; ++c)
+        for (int c = 0; c * 64 < p.Dv; ++c)
           tma_store_4d(&tmO, sQ + t * Cfg::TILE + c * (FWD_BM * 128) + (warp % 4) * (32 * 128), c * 64, row0, h, b);
         tma_store_commit();
         tma_store_wait_read();
@@ -902,7 +903,8 @@ static int fwd_impl(const void* q, const void* k, const void* v, void* o, float*
   if (sink > Skv) sink = Skv;
   if (!q || !k || !v || !o || !q_strides || !k_strides || !v_strides || !o_strides) return FFA_ERR_INVALID_ARG;
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || Sq <= 0 || Skv < 0 || Hq % Hkv != 0) return FFA_ERR_INVALID_ARG;
-  if (!((D == 64 && Dv == 64) || (D == 128 && Dv == 128) || (D == 192 && Dv == 128))) return FFA_ERR_UNSUPPORTED;
+  int KD = 0, KV = 0;
+  if (!attention_tile(D, Dv, sink > 0 && dtype != FFA_DTYPE_F32, KD, KV)) return FFA_ERR_UNSUPPORTED;
   if (dtype != FFA_DTYPE_BF16 && dtype != FFA_DTYPE_F16 && dtype != FFA_DTYPE_F32) return FFA_ERR_UNSUPPORTED;
   if (Skv > 65535 * FWD_BN) return FFA_ERR_UNSUPPORTED;
   // with a block mask a CTA records its kept key tiles in shared memory
@@ -927,7 +929,7 @@ static int fwd_impl(const void* q, const void* k, const void* v, void* o, float*
   p.Sq = Sq;
   p.Skv = Skv;
   p.q_offset = q_offset;
-  const int nqt = fwd_query_tiles(D, Sq, Skv, causal, window, block_mask != nullptr);
+  const int nqt = fwd_query_tiles(KD, Sq, Skv, causal, window, block_mask != nullptr);
   p.n_qblk = (Sq + FWD_BM * nqt - 1) / (FWD_BM * nqt);
   p.head_group = fwd_head_group(B * Hq, Hq / Hkv, Skv, D, Dv, window, (long long)p.n_qblk * B * Hq);
   p.scale_log2 = scale * 1.4426950408889634f;
@@ -938,6 +940,7 @@ static int fwd_impl(const void* q, const void* k, const void* v, void* o, float*
   p.causal = causal;
   p.window = window > 0 ? window : 0;
   p.sink = sink;
+  p.Dv = Dv;
   p.block_mask = block_mask;
   p.n_br = n_br;
   p.n_bc = n_bc;
@@ -971,10 +974,10 @@ static int fwd_impl(const void* q, const void* k, const void* v, void* o, float*
     constexpr bool SINK = decltype(sk)::value;
     auto typed = [&](auto t) -> int {
       using T = decltype(t);
-      if (D == 64)
+      if (KD == 64)
         return nqt == 1 ? launch_fwd<T, 64, 64, 1, SINK>(mq, mk, mv, mo, p, (int)grid, s)
                         : launch_fwd<T, 64, 64, 2, SINK>(mq, mk, mv, mo, p, (int)grid, s);
-      if (D == 128)
+      if (KD == 128)
         return nqt == 1 ? launch_fwd<T, 128, 128, 1, SINK>(mq, mk, mv, mo, p, (int)grid, s)
                         : launch_fwd<T, 128, 128, 2, SINK>(mq, mk, mv, mo, p, (int)grid, s);
       return launch_fwd<T, 192, 128, 2, SINK>(mq, mk, mv, mo, p, (int)grid, s);

@@ -66,6 +66,17 @@ int f32_bwd(const void* dout, const void* q, const void* k, const void* v, const
             int window, int sink, float softcap, const uint8_t* block_mask, int n_br, int n_bc, int mask_bq, int mask_bkv,
             void* workspace, float* sink_ws, void* stream);
 
+// Head dims of the attention kernel that serves (D, Dv).  The sink kernels take
+// any multiples of 8 up to (192, 128): their TMA copies read zeros past the
+// true head dim and write nothing there, so narrower heads run on the next
+// wider tile without a padded copy.  The others take exactly these widths.
+inline bool attention_tile(int D, int Dv, bool sinks, int& KD, int& KV) {
+  KD = D <= 64 && Dv <= 64 ? 64 : D <= 128 ? 128 : 192;
+  KV = KD == 64 ? 64 : 128;
+  if (D <= 0 || Dv <= 0 || D > KD || Dv > KV) return false;
+  return sinks ? D % 8 == 0 && Dv % 8 == 0 : D == KD && Dv == KV;
+}
+
 // Backward with sinks: the `tile`-key tiles that hold them, [0, tiles), see
 // every later query, so `parts` CTAs share each one's queries: about as many
 // 64-query units per CTA as the window gives another key tile, so that no CTA

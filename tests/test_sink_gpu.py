@@ -89,7 +89,10 @@ CASES = [
     (1, 2, 1, 640, 640, 128, 128, 65, 700, True, None),   # every key a sink: plain causal
     (1, 2, 1, 500, 500, 128, 128, 4000, 4, True, None),   # a window that hides nothing
     (1, 4, 2, 600, 600, 192, 128, 150, 5, True, None),    # qk 192, v 128
-    (1, 2, 2, 513, 513, 96, 96, 64, 9, True, 20.0),       # a padded head dim
+    (1, 2, 2, 513, 513, 96, 96, 64, 9, True, 20.0),       # head dims below the tile's
+    (2, 4, 2, 300, 300, 40, 24, 50, 3, True, None),       # ... of q / k and v apart
+    (1, 2, 1, 777, 777, 136, 72, 128, 4, True, None),     # ... on the widest tile
+    (1, 2, 2, 200, 200, 20, 20, 30, 3, True, None),       # no multiple of 8: padded copies
     (1, 2, 1, 400, 1100, 64, 64, 90, 6, True, None),      # more keys than queries (offset 0)
     (1, 2, 1, 1100, 400, 128, 128, 90, 6, False, None),   # windows past the last key: sinks alone
 ]
