@@ -20,7 +20,7 @@
 // maximum and sum.  No warp waits for another before the join.
 //
 // HBM-bound: the K and V bytes of the visible tokens, read once per kv head;
-// 64 requests, window 4096 + 4, 32/8 heads, D 128: 165 us, 6.16 TB/s (0.94 of a
+// 64 requests, window 4096 + 4, 32/8 heads, D 128: 159 us, 6.38 TB/s (0.97 of a
 // measured copy).  One request alone is bound by latencies (11 us: the launch,
 // the length, the table, the rows, each warp's few chunks, two cluster barriers).
 // P is rounded to the data's type for the P V product (the tensor core's
@@ -41,11 +41,6 @@ namespace cg = cooperative_groups;
 // and left fewer warps for the same shared memory: 192 us against 165 on 64
 // requests of a 4096-token window, 32/8 heads, D 128.
 constexpr int WD_CHUNK = 16;
-// Warps per CTA.  8 leave one CTA per SM: 199 us on the case above; 2 with
-// three chunks in flight each: 159 us there, but 14.2 us against 11.1 for one
-// request alone.
-constexpr int WD_WARPS = 4;
-constexpr int WD_THREADS = WD_WARPS * 32;
 
 struct WdParams {
   const void* q;  // [R, Hq, D]
@@ -67,19 +62,24 @@ struct WdParams {
   uint32_t* err;
 };
 
-template <int DP>
+// WARPS per CTA, each with STAGES chunks in flight.  Two shapes:
+//   4 warps, 64 KB of rings (2 stages at 128 columns), three CTAs per SM;
+//   2 warps, 48 KB (3 stages), four CTAs per SM, for 128 columns: more requests
+//     run unsplit in one wave (at 64 columns the warps' instructions bound it).
+// 8 warps, or 4 with 3 stages, leave fewer CTAs per SM: 183 us and more on 64
+// requests of a 4096-token window, 32/8 heads, D 128, against 165 and less.
+template <int DP, int WARPS>
 struct WdCfg {
+  static constexpr int THREADS = WARPS * 32;
+  static constexpr int STAGES = (WARPS == 2 ? 3 : 2) * (128 / DP);
   static constexpr int HALF = WD_CHUNK * 128;        // a chunk's rows x 64 elements
   static constexpr int KV_BYTES = WD_CHUNK * DP * 2; // one chunk of K (or V)
   static constexpr int STAGE = 2 * KV_BYTES;
-  // chunks a warp has in flight: 64 KB of rings, three CTAs per SM (96 KB, two
-  // CTAs: 183 us on the case above)
-  static constexpr int STAGES = DP == 64 ? 4 : 2;
-  static constexpr int RING = WD_WARPS * STAGES * STAGE;
+  static constexpr int RING = WARPS * STAGES * STAGE;
   // the joins overlay the rings, idle by then: per warp, then per CTA,
   // 16 rows x (m, l, O[DP])
   static constexpr int STATE = 16 * (DP + 2);        // floats
-  static constexpr int CTA_OFF = WD_WARPS * STATE * 4;
+  static constexpr int CTA_OFF = WARPS * STATE * 4;
   static constexpr int MERGE = CTA_OFF + STATE * 4;
   static constexpr int SMEM = (RING > MERGE ? RING : MERGE) + 1024;
 };
@@ -123,9 +123,10 @@ __device__ __forceinline__ __nv_bfloat16 wd_round<__nv_bfloat16>(float x) { retu
 template <>
 __device__ __forceinline__ __half wd_round<__half>(float x) { return __float2half_rn(x); }
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(WD_THREADS) ffa_window_decode_kernel(const WdParams p) {
-  using Cfg = WdCfg<DP>;
+template <typename T, int DP, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32) ffa_window_decode_kernel(const WdParams p) {
+  using Cfg = WdCfg<DP, WARPS>;
+  constexpr int WD_WARPS = WARPS, WD_THREADS = Cfg::THREADS;
   constexpr int S = Cfg::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -382,29 +383,41 @@ __global__ void __launch_bounds__(WD_THREADS) ffa_window_decode_kernel(const WdP
   cluster.sync();  // no CTA leaves while another reads its shared memory
 }
 
-// CTAs per cluster (a power of two up to 16, no less than a chunk per warp):
-// the count with the least waves x (tokens per CTA + what a CTA costs beside
-// them).  Three CTAs fit an SM; a CTA's start and join cost about as much as
-// 19200 / D tokens (5 us against 35 ns a token of K and V at D = 128 with every
-// SM streaming).  Measured at 1, 2, 4, 8, 16: the case above 201, 177, 165, 195,
-// 295 us (it takes 4); one request 64, 36, 21, 13.6, 11.1 (16); 5 requests of up
-// to 3000 tokens, window 1000, 20 heads of 64: 15.3, 11.5, 9.1, 15.0, 26 (4).
-static int wd_splits(int64_t pairs, int64_t visible, int D) {
-  int best = 1;
-  double least = 0;
-  for (int s = 1; s <= 16 && (s == 1 || visible >= (int64_t)s * WD_WARPS * WD_CHUNK); s *= 2) {
-    double waves = (double)(pairs * s) / (148 * 3);
-    if (waves < 3) waves = ceil(waves);
-    const double cost = waves * ((double)visible / s + 19200.0 / D);
-    if (s == 1 || cost < least) best = s, least = cost;
-  }
-  return best;
+// Estimated time (us) of `pairs` clusters of s CTAs over `visible` tokens each.
+// Full waves of resident CTAs stream at the memory's rate and pay a start and a
+// join (4 us); the last, partial one takes that rate or one CTA's own speed
+// (13.6 ns a token with 4 warps at 128 columns, 10 at 64), whichever is longer,
+// and 5 us.  Measured against it (us, estimate in brackets), D 128, 512 pairs of
+// 4100 tokens: 4 warps split by 1, 2, 4, 8: 215 (208), 188 (184), 184 (186),
+// 218 (209); 2 warps split by 1, 2, 4: 167 (170), 178 (174), 189 (188).  8 pairs
+// of 4100 split by 8, 16: 13.6, 11.1; 512 pairs of 1028: 4 warps 64 (59), 2 warps
+// 51 (47); 296 pairs of 4100: 4 warps unsplit 100 (101), 2 warps split by 2 103.
+static double wd_time(int64_t pairs, int64_t visible, int D, int warps, int s) {
+  const double per_token = 4.0 * D / 6.5e6;  // K and V bytes over bytes per us
+  const double own = (D > 64 ? 0.0136 : 0.010) * 4 / warps, tokens = (double)visible / s;
+  const int64_t slots = 148 * (warps == 2 ? 4 : 3), ctas = pairs * s;
+  const int64_t full = ctas / slots, rest = ctas % slots;
+  double t = full * (slots * tokens * per_token + 4.0);
+  if (rest) t += fmax(rest * tokens * per_token, tokens * own) + 5.0;
+  return t;
 }
 
-template <typename T, int DP>
+// CTAs per cluster and warps per CTA with the least estimated time: powers of
+// two up to 16, no less than a chunk per warp.
+static void wd_shape(int64_t pairs, int64_t visible, int D, int& splits, int& warps) {
+  double least = 0;
+  splits = 0;
+  for (int w = 4; w >= (D > 64 ? 2 : 4); w -= 2)
+    for (int s = 1; s <= 16 && (s == 1 || visible >= (int64_t)s * w * WD_CHUNK); s *= 2) {
+      const double t = wd_time(pairs, visible, D, w, s);
+      if (!splits || t < least) splits = s, warps = w, least = t;
+    }
+}
+
+template <typename T, int DP, int WARPS>
 static int launch_window_decode(const WdParams& p, int64_t grid, cudaStream_t st) {
-  using Cfg = WdCfg<DP>;
-  auto kern = ffa_window_decode_kernel<T, DP>;
+  using Cfg = WdCfg<DP, WARPS>;
+  auto kern = ffa_window_decode_kernel<T, DP, WARPS>;
   static std::atomic<uint64_t> done{0}, wide{0};
   if (int s = smem_attr_once(kern, Cfg::SMEM, done)) return s;
   if (p.splits > 8) {  // clusters past 8 CTAs are opt-in
@@ -418,7 +431,7 @@ static int launch_window_decode(const WdParams& p, int64_t grid, cudaStream_t st
   }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3(WD_THREADS);
+  cfg.blockDim = dim3(Cfg::THREADS);
   cfg.dynamicSmemBytes = Cfg::SMEM;
   cfg.stream = st;
   cudaLaunchAttribute attr{};
@@ -485,12 +498,15 @@ extern "C" int ffa_window_decode(const void* q, const void* k_pages, const void*
   // the most tokens a request can see
   int64_t visible = max_ctx > 0 && max_ctx < p.max_ctx ? max_ctx : p.max_ctx;
   if (visible > (int64_t)window + sinks) visible = (int64_t)window + sinks;
-  p.splits = wd_splits(pairs, visible, D);
+  int warps = 4;
+  wd_shape(pairs, visible, D, p.splits, warps);
   const int64_t grid = pairs * p.splits;
   if (grid > 0x7fffffffLL) return FFA_ERR_UNSUPPORTED;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == FFA_DTYPE_BF16)
-    return D <= 64 ? launch_window_decode<__nv_bfloat16, 64>(p, grid, st)
-                   : launch_window_decode<__nv_bfloat16, 128>(p, grid, st);
-  return D <= 64 ? launch_window_decode<__half, 64>(p, grid, st) : launch_window_decode<__half, 128>(p, grid, st);
+  auto typed = [&](auto t) -> int {
+    using T = decltype(t);
+    if (D <= 64) return launch_window_decode<T, 64, 4>(p, grid, st);
+    return warps == 2 ? launch_window_decode<T, 128, 2>(p, grid, st) : launch_window_decode<T, 128, 4>(p, grid, st);
+  };
+  return dtype == FFA_DTYPE_BF16 ? typed(__nv_bfloat16{}) : typed(__half{});
 }
