@@ -20,7 +20,7 @@
 // maximum and sum.  No warp waits for another before the join.
 //
 // HBM-bound: the K and V bytes of the visible tokens, read once per kv head;
-// 64 requests, window 4096 + 4, 32/8 heads, D 128: 159 us, 6.38 TB/s (0.97 of a
+// 64 requests, window 4096 + 4, 32/8 heads, D 128: 154 us, 6.59 TB/s (1.0 of a
 // measured copy).  One request alone is bound by latencies (11 us: the launch,
 // the length, the table, the rows, each warp's few chunks, two cluster barriers).
 // P is rounded to the data's type for the P V product (the tensor core's
@@ -55,6 +55,8 @@ struct WdParams {
   int64_t o_sr, o_sh;
   float* lse;  // [R, Hq] or nullptr
   int R, Hq, Hkv, G, D, page_size, window, sinks;
+  uint32_t ps_mul;  // division by page_size (WdRows)
+  int ps_shift;
   int splits;       // CTAs per cluster
   int head_blocks;  // blocks of 16 query heads in a group
   float scale_log2, sc_pre, sc_post;
@@ -97,22 +99,28 @@ __device__ __forceinline__ void cp_wait() {
 struct WdRows {
   const int* table;
   int h, Hkv, page_size, num_pages, ns, skip, nv;  // skip: added to v >= ns
+  uint32_t ps_mul;
+  int ps_shift;
   uint32_t* err;
-  // table entry of virtual index v (any value for one past the end)
-  __device__ __forceinline__ int page(int v) const {
+  // Table entry of virtual index v, and the token's offset in its page (any
+  // values for one past the end).  Division by the page size as a product:
+  // ps_mul = floor(2^(31 + k) / d) + 1 with 2^k >= d is exact below 2^31.
+  __device__ __forceinline__ int page(int v, int& off) const {
+    off = 0;
     if (v >= nv) return 0;
     const uint32_t tok = v < ns ? v : v + skip;
-    return table[tok / (uint32_t)page_size];
+    const uint32_t i = (uint32_t)(((uint64_t)tok * ps_mul) >> ps_shift);
+    off = (int)(tok - i * page_size);
+    return table[i];
   }
   // pool row, or -1: past the end, or a page id outside the pool (recorded)
-  __device__ __forceinline__ int row(int v, int page) const {
+  __device__ __forceinline__ int row(int v, int page, int off) const {
     if (v >= nv) return -1;
     if ((unsigned)page >= (unsigned)num_pages) {
       if (err) atomicCAS(err, 0u, SITE_DEC_BAD_PAGE);
       return -1;
     }
-    const uint32_t tok = v < ns ? v : v + skip;
-    return (page * Hkv + h) * page_size + (int)(tok % (uint32_t)page_size);
+    return (page * Hkv + h) * page_size + off;
   }
 };
 
@@ -153,6 +161,8 @@ __global__ void __launch_bounds__(WARPS * 32) ffa_window_decode_kernel(const WdP
   rows.ns = min(p.sinks, w0);
   rows.skip = w0 - rows.ns;
   rows.nv = rows.ns + ctx - w0;
+  rows.ps_mul = p.ps_mul;
+  rows.ps_shift = p.ps_shift;
   rows.err = p.err;
   const int chunks = (rows.nv + WD_CHUNK - 1) / WD_CHUNK;
   const int c0 = (int)((int64_t)chunks * split / p.splits), c1 = (int)((int64_t)chunks * (split + 1) / p.splits);
@@ -186,9 +196,12 @@ __global__ void __launch_bounds__(WARPS * 32) ffa_window_decode_kernel(const WdP
   };
   auto vidx = [&](int i) { return (c0 + warp + i * WD_WARPS) * WD_CHUNK + lane % WD_CHUNK; };
   // table entries run one chunk ahead of the copies that need them
-  int pages[S + 1];
+  int pages[S + 1], offs[S + 1];
 #pragma unroll
-  for (int i = 0; i <= S; ++i) pages[i] = i < n ? rows.page(vidx(i)) : 0;
+  for (int i = 0; i <= S; ++i) {
+    pages[i] = offs[i] = 0;
+    if (i < n) pages[i] = rows.page(vidx(i), offs[i]);
+  }
 
   // Q as the A operand: rows = the block's query heads (rows past G are zero)
   const int g = lane >> 2, t = lane & 3;
@@ -205,10 +218,10 @@ __global__ void __launch_bounds__(WARPS * 32) ffa_window_decode_kernel(const WdP
   }
 #pragma unroll
   for (int i = 0; i < S; ++i) {
-    if (i < n) issue(i, rows.row(vidx(i), pages[i]));
+    if (i < n) issue(i, rows.row(vidx(i), pages[i], offs[i]));
     cp_commit();
   }
-  int next_page = pages[S];
+  int next_page = pages[S], next_off = offs[S];
 
   float o[DP / 8][4];
 #pragma unroll
@@ -239,15 +252,28 @@ __global__ void __launch_bounds__(WARPS * 32) ffa_window_decode_kernel(const WdP
       }
     }
     const int left = rows.nv - (c0 + warp + i * WD_WARPS) * WD_CHUNK;  // tokens of this chunk
+    float mul = p.scale_log2;
+    if (p.use_softcap) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[nt][e] = tanh_acc(x[nt][e] * p.sc_pre);
+      mul = p.sc_post;
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[nt][e] *= mul;
+    if (left < WD_CHUNK) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (nt * 8 + 2 * t + (e & 1) >= left) x[nt][e] = -INFINITY;
+    }
     float mx_lo = -INFINITY, mx_hi = -INFINITY;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float v = x[nt][e];
-        const float y = p.use_softcap ? tanh_acc(v * p.sc_pre) * p.sc_post : v * p.scale_log2;
-        x[nt][e] = nt * 8 + 2 * t + (e & 1) < left ? y : -INFINITY;
-      }
       mx_lo = fmaxf(mx_lo, fmaxf(x[nt][0], x[nt][1]));
       mx_hi = fmaxf(mx_hi, fmaxf(x[nt][2], x[nt][3]));
     }
@@ -300,9 +326,9 @@ __global__ void __launch_bounds__(WARPS * 32) ffa_window_decode_kernel(const WdP
       }
     }
     __syncwarp();  // every lane has read the stage before it is refilled
-    if (i + S < n) issue(i + S, rows.row(vidx(i + S), next_page));
+    if (i + S < n) issue(i + S, rows.row(vidx(i + S), next_page, next_off));
     cp_commit();
-    if (i + S + 1 < n) next_page = rows.page(vidx(i + S + 1));
+    if (i + S + 1 < n) next_page = rows.page(vidx(i + S + 1), next_off);
   }
   cp_wait<0>();
 
@@ -486,6 +512,10 @@ extern "C" int ffa_window_decode(const void* q, const void* k_pages, const void*
   p.G = Hq / Hkv;
   p.D = D;
   p.page_size = page_size;
+  int k = 0;
+  while ((1ll << k) < page_size) ++k;
+  p.ps_shift = 31 + k;
+  p.ps_mul = (uint32_t)((1ull << p.ps_shift) / (unsigned)page_size + 1);
   p.window = window;
   p.sinks = sinks;
   p.head_blocks = (p.G + 15) / 16;
