@@ -14,6 +14,7 @@ it and run on the tensor cores, and the result is cast back to fp32.
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import Optional, Tuple
 
@@ -244,6 +245,11 @@ def fastest_flash_attn_forward(
     return o, lse
 
 
+@functools.lru_cache(maxsize=1024)
+def _sink_workspace(*sizes: int) -> int:
+    return _lib.load().ffa_bwd_sink_workspace_size(*sizes)
+
+
 def flash_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor,
               lse: torch.Tensor, *, scale: float, causal: bool = False, q_offset: int = 0,
               window: Optional[int] = None, softcap: Optional[float] = None,
@@ -282,13 +288,14 @@ def flash_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Ten
     q, k, v, o, dout = (_tma_ready(t, dt) for t in (q, k, v, o, dout))
     if lse.dim() == 4:
         lse = lse[..., 0]
-    lse = lse.to(torch.float32).contiguous()
+    if lse.dtype is not torch.float32 or not lse.is_contiguous():
+        lse = lse.to(torch.float32).contiguous()
     dq = torch.empty_like(q)
     dk = torch.empty_like(k)
     dv = torch.empty_like(v)
     lib = _lib.load()
     if sink:
-        ws_bytes = lib.ffa_bwd_sink_workspace_size(B, Hq, Hkv, Sq, Skv, D, Dv, window, sink)
+        ws_bytes = _sink_workspace(B, Hq, Hkv, Sq, Skv, D, Dv, window, sink)
     else:
         ws_bytes = lib.ffa_bwd_workspace_size(B, Hq, Sq)
     ws = q.new_empty(ws_bytes, dtype=torch.uint8)
@@ -354,12 +361,10 @@ class FastestFlashAttnFunc(Function):
     Accepts GQA (fewer K/V heads than query heads) natively."""
 
     @staticmethod
-    def forward(ctx, q, k, v, scale, causal, block_size, softcap, sliding_window, two_pass, block_mask=None,
-                sink_tokens=0):
+    def forward(ctx, q, k, v, scale, causal, block_size, softcap, sliding_window, two_pass, block_mask=None):
         output, lse = fastest_flash_attn_forward(
             q, k, v, scale=scale, causal=causal, block_size=block_size, softcap=softcap,
-            sliding_window=sliding_window, two_pass=two_pass, block_mask=block_mask, return_lse=True,
-            sink_tokens=sink_tokens)
+            sliding_window=sliding_window, two_pass=two_pass, block_mask=block_mask, return_lse=True)
         ctx.save_for_backward(q, k, v, output, lse)
         ctx.block_mask = block_mask
         ctx.scale = scale
@@ -367,7 +372,6 @@ class FastestFlashAttnFunc(Function):
         ctx.block_size = block_size
         ctx.softcap = softcap
         ctx.sliding_window = sliding_window
-        ctx.sink_tokens = sink_tokens
         return output
 
     @staticmethod
@@ -378,11 +382,34 @@ class FastestFlashAttnFunc(Function):
             q, k, v, output, lse, grad_output = (t.unsqueeze(1) for t in (q, k, v, output, lse, grad_output))
         dq, dk, dv = fastest_flash_attn_backward(
             grad_output, q, k, v, output, lse, scale=ctx.scale, causal=ctx.causal, block_size=ctx.block_size,
-            softcap=ctx.softcap, sliding_window=ctx.sliding_window, block_mask=ctx.block_mask,
-            sink_tokens=ctx.sink_tokens)
+            softcap=ctx.softcap, sliding_window=ctx.sliding_window, block_mask=ctx.block_mask)
         if was_3d:
             dq, dk, dv = dq.squeeze(1), dk.squeeze(1), dv.squeeze(1)
-        return dq, dk, dv, None, None, None, None, None, None, None, None
+        return dq, dk, dv, None, None, None, None, None, None, None
+
+
+class SinkAttnFunc(Function):
+    """Autograd function of attention with a sliding window and sinks, on 4-D
+    q, k, v: ``options`` are flash_fwd's and flash_bwd's keyword arguments.
+    (The backward runs on autograd's own thread, where every Python call takes
+    several times longer; so it is one call.)"""
+
+    @staticmethod
+    def forward(ctx, q, k, v, options):
+        o, lse = flash_fwd(q, k, v, **options)
+        if o.dtype != q.dtype:
+            o = o.to(q.dtype)
+        ctx.save_for_backward(q, k, v, o, lse)
+        ctx.options = options
+        return o
+
+    @staticmethod
+    def backward(ctx, grad_output):
+        q, k, v, o, lse = ctx.saved_tensors
+        dq, dk, dv = flash_bwd(grad_output, q, k, v, o, lse, **ctx.options)
+        if dq.dtype != q.dtype or dk.dtype != k.dtype or dv.dtype != v.dtype:
+            dq, dk, dv = dq.to(q.dtype), dk.to(k.dtype), dv.to(v.dtype)
+        return dq, dk, dv, None
 
 
 def fastest_flash_attn_func(
@@ -402,5 +429,11 @@ def fastest_flash_attn_func(
     ``block_mask`` (tiles of ``block_size``) and ``sink_tokens`` (first keys
     that stay visible outside the window) are additions: the reference's
     autograd path has neither."""
+    if sink_tokens and _sinks(sliding_window, sink_tokens, block_mask):
+        q4, k4, v4, squeezed = maybe_unsqueeze_head(q, k, v)
+        o = SinkAttnFunc.apply(q4, k4, v4, dict(
+            scale=scale if scale is not None else 1.0 / math.sqrt(q.shape[-1]), causal=causal, window=sliding_window,
+            softcap=softcap, sink=sink_tokens))
+        return o.squeeze(1) if squeezed else o
     return FastestFlashAttnFunc.apply(q, k, v, scale, causal, block_size, softcap, sliding_window, two_pass,
-                                      block_mask, sink_tokens)
+                                      block_mask)

@@ -222,6 +222,20 @@ def test_many_sink_tiles():
         _near(got, ref, torch.bfloat16, name, want[5])
 
 
+def test_three_dimensional_tensors():
+    from fastest_flash_attention_b200 import fastest_flash_attn_forward, fastest_flash_attn_func
+    q, k, v, do = (t[:, 0] for t in _tensors(2, 1, 1, 200, 200, 64, 64, torch.bfloat16, 8))
+    kw = dict(causal=True, sliding_window=30, sink_tokens=4)
+    o, lse = fastest_flash_attn_forward(q, k, v, return_lse=True, **kw)
+    x = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = fastest_flash_attn_func(*x, **kw)
+    assert out.shape == q.shape and torch.equal(out, o) and lse.shape == (2, 200, 1)
+    got = torch.autograd.grad(out, x, do)
+    x = [t.detach().unsqueeze(1).requires_grad_() for t in (q, k, v)]
+    ref = torch.autograd.grad(fastest_flash_attn_func(*x, **kw), x, do.unsqueeze(1))
+    assert all(torch.equal(a, b[:, 0]) for a, b in zip(got, ref))
+
+
 def test_refusals():
     from fastest_flash_attention_b200 import fastest_flash_attn_backward, fastest_flash_attn_forward
     q, k, v, do = _tensors(1, 2, 2, 64, 64, 64, 64, torch.bfloat16, 1)
