@@ -658,7 +658,43 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
   }
   constexpr uint32_t FMT = DtypeFmt<T>::value;
 
-  if (threadIdx.x == 0) bwd_init_bars(bars, NS, 2 * 4);
+  // one 64-row query sub-tile's Q, dO and statistics into their stage
+  auto load_stage = [&](int u, uint64_t pol) {
+    const int s = u % NS;
+    const int g = (u_lo + u) / n_i, i = i_lo + (u_lo + u) % n_i;
+    const int h = hkv * group + g;
+    mbar_arrive_expect_tx(&bars->st_full[s], Cfg::STAGE + 2 * BWD_BS * 4);
+    uint8_t* dst = sStage + s * Cfg::STAGE;
+    for (int c = 0; c < D / 64; ++c)
+      tma_load_4d(&tmQ, &bars->st_full[s], dst + c * BWD_BS * 128, c * 64, i * BWD_BS, h, b, pol);
+    for (int c = 0; c < DV / 64; ++c)
+      tma_load_4d(&tmDO, &bars->st_full[s], dst + Cfg::SUB_Q + c * BWD_BS * 128, c * 64, i * BWD_BS, h, b, pol);
+    const int64_t row0 = (int64_t)(b * p.Hq + h) * p.Sq_pad + i * BWD_BS;
+    bulk_load(sStat + 2 * BWD_BS * s, p.nlse2 + row0, BWD_BS * 4, &bars->st_full[s]);
+    bulk_load(sStat + 2 * BWD_BS * s + BWD_BS, p.delta + row0, BWD_BS * 4, &bars->st_full[s]);
+  };
+  // The producer sets the barriers up and starts the first loads at once, so
+  // they run while the CTA gets its TMEM and meets (whole backward of B8 H16
+  // S4096 D128, window 1024, softcap: 1482 -> 1457 us).  The kept tile and one
+  // stage only: with every stage issued there the CTA waited for the issuing
+  // thread instead, and nothing was gained.
+  if (warp == BWD_WARP_LOAD && lane == 0) {
+    bwd_init_bars(bars, NS, 2 * 4);
+    if (n > 0) {
+      const uint64_t pol = policy_evict_last();
+      mbar_arrive_expect_tx(&bars->fixed_full, Cfg::TILE_K + Cfg::TILE_V);
+      for (int hf = 0; hf < 2; ++hf) {
+        for (int c = 0; c < D / 64; ++c)
+          tma_load_4d(&tmK, &bars->fixed_full, sK + c * BWD_BT * 128 + hf * BWD_BS * 128, c * 64,
+                      j * BWD_BT + hf * BWD_BS, hkv, b, pol);
+        for (int c = 0; c < DV / 64; ++c)
+          tma_load_4d(&tmV, &bars->fixed_full, sV + c * BWD_BT * 128 + hf * BWD_BS * 128, c * 64,
+                      j * BWD_BT + hf * BWD_BS, hkv, b, pol);
+      }
+      load_stage(0, pol);
+    }
+  }
+  __syncwarp();
   if (warp == BWD_WARP_MMA) {
     tmem_alloc(&bars->tmem_base, 512);
     tmem_relinquish();
@@ -671,30 +707,10 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
   if (warp == BWD_WARP_LOAD) {
     if (lane == 0 && n > 0) {
       const uint64_t pol = policy_evict_last();
-      mbar_arrive_expect_tx(&bars->fixed_full, Cfg::TILE_K + Cfg::TILE_V);
-      for (int hf = 0; hf < 2; ++hf) {
-        for (int c = 0; c < D / 64; ++c)
-          tma_load_4d(&tmK, &bars->fixed_full, sK + c * BWD_BT * 128 + hf * BWD_BS * 128, c * 64,
-                      j * BWD_BT + hf * BWD_BS, hkv, b, pol);
-        for (int c = 0; c < DV / 64; ++c)
-          tma_load_4d(&tmV, &bars->fixed_full, sV + c * BWD_BT * 128 + hf * BWD_BS * 128, c * 64,
-                      j * BWD_BT + hf * BWD_BS, hkv, b, pol);
-      }
-      int issued = 0;
-      for (int u = 0; u < n; ++u) {
-        const int s = u % NS, use = u / NS;
-        if (use > 0 && !mbar_wait(&bars->st_empty[s], (use - 1) & 1, p.ec, abort_flag, SITE_BWD_EMPTY)) break;
-        const int g = (u_lo + u) / n_i, i = i_lo + (u_lo + u) % n_i;
-        const int h = hkv * group + g;
-        mbar_arrive_expect_tx(&bars->st_full[s], Cfg::STAGE + 2 * BWD_BS * 4);
-        uint8_t* dst = sStage + s * Cfg::STAGE;
-        for (int c = 0; c < D / 64; ++c)
-          tma_load_4d(&tmQ, &bars->st_full[s], dst + c * BWD_BS * 128, c * 64, i * BWD_BS, h, b, pol);
-        for (int c = 0; c < DV / 64; ++c)
-          tma_load_4d(&tmDO, &bars->st_full[s], dst + Cfg::SUB_Q + c * BWD_BS * 128, c * 64, i * BWD_BS, h, b, pol);
-        const int64_t row0 = (int64_t)(b * p.Hq + h) * p.Sq_pad + i * BWD_BS;
-        bulk_load(sStat + 2 * BWD_BS * s, p.nlse2 + row0, BWD_BS * 4, &bars->st_full[s]);
-        bulk_load(sStat + 2 * BWD_BS * s + BWD_BS, p.delta + row0, BWD_BS * 4, &bars->st_full[s]);
+      int issued = 1;
+      for (int u = issued; u < n; ++u) {
+        if (u >= NS && !mbar_wait(&bars->st_empty[u % NS], (u / NS - 1) & 1, p.ec, abort_flag, SITE_BWD_EMPTY)) break;
+        load_stage(u, pol);
         ++issued;
       }
       if (*abort_flag) {  // let copies in flight land before the CTA exits
@@ -997,18 +1013,36 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
   auto unit_at = [&](int u) -> int { return SINK && u < n_sink ? u : j_lo + u; };
   constexpr uint32_t FMT = DtypeFmt<T>::value;
 
-  if (threadIdx.x == 0) bwd_init_bars(bars, 8, Cfg::WIDE ? 4 * 4 : 2 * 4);
-  if (warp == BWD_WARP_MMA) {
-    tmem_alloc(&bars->tmem_base, 512);
-    tmem_relinquish();
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = bars->tmem_base;
-
-  if (warp == BWD_WARP_LOAD) {
-    if (lane == 0 && n > 0) {
+  // unit u: V (SPLIT) into its own ring, since its slot frees first; then K (or
+  // {K, V}) into slot u % NSK
+  auto load_v = [&](int u, uint64_t pol) {
+    const int jj = unit_at(u), sv = 4 + u % (Cfg::SPLIT ? NSV : 1);
+    mbar_arrive_expect_tx(&bars->st_full[sv], Cfg::SUB_V);
+    uint8_t* dv = sStage + Cfg::v_off(u);
+    for (int hf = 0; hf < R; ++hf)
+      for (int c = 0; c < DV / 64; ++c)
+        tma_load_4d(&tmV, &bars->st_full[sv], dv + c * UK * 128 + hf * BWD_BS * 128, c * 64,
+                    jj * UK + hf * BWD_BS, hkv, b, pol);
+  };
+  auto load_k = [&](int u, uint64_t pol) {
+    const int jj = unit_at(u), s = u % NSK;
+    mbar_arrive_expect_tx(&bars->st_full[s], Cfg::SPLIT ? Cfg::SUB_K : Cfg::STAGE);
+    uint8_t* dk = sStage + Cfg::k_off(u);
+    uint8_t* dv = sStage + Cfg::v_off(u);
+    for (int hf = 0; hf < R; ++hf) {
+      for (int c = 0; c < D / 64; ++c)
+        tma_load_4d(&tmK, &bars->st_full[s], dk + c * UK * 128 + hf * BWD_BS * 128, c * 64, jj * UK + hf * BWD_BS,
+                    hkv, b, pol);
+      if (!Cfg::SPLIT)
+        for (int c = 0; c < DV / 64; ++c)
+          tma_load_4d(&tmV, &bars->st_full[s], dv + c * UK * 128 + hf * BWD_BS * 128, c * 64, jj * UK + hf * BWD_BS,
+                      hkv, b, pol);
+    }
+  };
+  // barriers and first loads by the producer, as in the dK/dV kernel
+  if (warp == BWD_WARP_LOAD && lane == 0) {
+    bwd_init_bars(bars, 8, Cfg::WIDE ? 4 * 4 : 2 * 4);
+    if (n > 0) {
       const uint64_t pol_q = policy_evict_first();
       const uint64_t pol_kv = policy_evict_last();
       mbar_arrive_expect_tx(&bars->fixed_full, Cfg::TILE_Q + Cfg::TILE_DO);
@@ -1020,43 +1054,42 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
           tma_load_4d(&tmDO, &bars->fixed_full, sDO + c * BWD_BT * 128 + hf * BWD_BS * 128, c * 64,
                       i * BWD_BT + hf * BWD_BS, h, b, pol_q);
       }
-      // unit u: V (SPLIT) into its own ring first, since its slot frees first;
-      // then K (or {K, V}) into slot u % NSK
-      int issued_k = 0, issued_v = 0;
-      for (int u = 0; u < n; ++u) {
-        const int jj = unit_at(u);
-        if (Cfg::SPLIT) {
-          const int sv = 4 + u % NSV, usev = u / NSV;
-          if (usev > 0 && !mbar_wait(&bars->st_empty[sv], (usev - 1) & 1, p.ec, abort_flag, SITE_BWD_EMPTY)) break;
-          mbar_arrive_expect_tx(&bars->st_full[sv], Cfg::SUB_V);
-          uint8_t* dv = sStage + Cfg::v_off(u);
-          for (int hf = 0; hf < R; ++hf)
-            for (int c = 0; c < DV / 64; ++c)
-              tma_load_4d(&tmV, &bars->st_full[sv], dv + c * UK * 128 + hf * BWD_BS * 128, c * 64,
-                          jj * UK + hf * BWD_BS, hkv, b, pol_kv);
+      if (Cfg::SPLIT) load_v(0, pol_kv);
+      load_k(0, pol_kv);
+    }
+  }
+  __syncwarp();
+  if (warp == BWD_WARP_MMA) {
+    tmem_alloc(&bars->tmem_base, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem_base;
+
+  if (warp == BWD_WARP_LOAD) {
+    if (lane == 0 && n > 0) {
+      const uint64_t pol_kv = policy_evict_last();
+      int issued_k = 1, issued_v = Cfg::SPLIT ? 1 : 0;
+      for (int u = 1; u < n; ++u) {
+        if constexpr (Cfg::SPLIT) {
+          if (u >= NSV &&
+              !mbar_wait(&bars->st_empty[4 + u % NSV], (u / NSV - 1) & 1, p.ec, abort_flag, SITE_BWD_EMPTY))
+            break;
+          load_v(u, pol_kv);
           ++issued_v;
         }
-        const int s = u % NSK, use = u / NSK;
-        if (use > 0 && !mbar_wait(&bars->st_empty[s], (use - 1) & 1, p.ec, abort_flag, SITE_BWD_EMPTY)) break;
-        mbar_arrive_expect_tx(&bars->st_full[s], Cfg::SPLIT ? Cfg::SUB_K : Cfg::STAGE);
-        uint8_t* dk = sStage + Cfg::k_off(u);
-        uint8_t* dv = sStage + Cfg::v_off(u);
-        for (int hf = 0; hf < R; ++hf) {
-          for (int c = 0; c < D / 64; ++c)
-            tma_load_4d(&tmK, &bars->st_full[s], dk + c * UK * 128 + hf * BWD_BS * 128, c * 64,
-                        jj * UK + hf * BWD_BS, hkv, b, pol_kv);
-          if (!Cfg::SPLIT)
-            for (int c = 0; c < DV / 64; ++c)
-              tma_load_4d(&tmV, &bars->st_full[s], dv + c * UK * 128 + hf * BWD_BS * 128, c * 64,
-                          jj * UK + hf * BWD_BS, hkv, b, pol_kv);
-        }
+        if (u >= NSK && !mbar_wait(&bars->st_empty[u % NSK], (u / NSK - 1) & 1, p.ec, abort_flag, SITE_BWD_EMPTY))
+          break;
+        load_k(u, pol_kv);
         ++issued_k;
       }
       if (*abort_flag) {
         mbar_wait(&bars->fixed_full, 0, p.ec, abort_flag, SITE_BWD_DRAIN, true);
         for (int u = max(0, issued_k - NSK); u < issued_k; ++u)
           mbar_wait(&bars->st_full[u % NSK], (u / NSK) & 1, p.ec, abort_flag, SITE_BWD_DRAIN, true);
-        if (Cfg::SPLIT)
+        if constexpr (Cfg::SPLIT)
           for (int u = max(0, issued_v - NSV); u < issued_v; ++u)
             mbar_wait(&bars->st_full[4 + u % NSV], (u / NSV) & 1, p.ec, abort_flag, SITE_BWD_DRAIN, true);
       }
