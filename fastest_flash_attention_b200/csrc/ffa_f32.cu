@@ -20,7 +20,7 @@
 #include <math.h>
 #include <stdint.h>
 
-#include "ffa_b200.h"
+#include "ffa_common.cuh"
 #include "ffa_host.h"
 
 namespace ffa {
@@ -168,10 +168,9 @@ __device__ __forceinline__ void f32_accumulate(const float* P, const float* M, i
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float pv = kk == 0 ? pr[i].x : kk == 1 ? pr[i].y : kk == 2 ? pr[i].z : pr[i].w;
-          acc[i][c].x = fmaf(pv, m.x, acc[i][c].x);
-          acc[i][c].y = fmaf(pv, m.y, acc[i][c].y);
-          acc[i][c].z = fmaf(pv, m.z, acc[i][c].z);
-          acc[i][c].w = fmaf(pv, m.w, acc[i][c].w);
+          const float2 lo = ffma2(make_float2(pv, pv), make_float2(m.x, m.y), make_float2(acc[i][c].x, acc[i][c].y));
+          const float2 hi = ffma2(make_float2(pv, pv), make_float2(m.z, m.w), make_float2(acc[i][c].z, acc[i][c].w));
+          acc[i][c] = make_float4(lo.x, lo.y, hi.x, hi.y);
         }
       }
     }
