@@ -155,7 +155,7 @@ __device__ __forceinline__ void f32_scores(const float* A, const float* Bm, int 
 template <int W>
 __device__ __forceinline__ void f32_accumulate(const float* P, const float* M, int ty, int tx,
                                                float4 acc[4][W / 64]) {
-#pragma unroll 2
+#pragma unroll 4
   for (int k = 0; k < 64; k += 4) {
     float4 pr[4];
 #pragma unroll
