@@ -15,6 +15,9 @@
 //   3. dQ: one CTA per (batch, query head, 128-row query tile), streaming
 //      key units (128 keys for D <= 128, 64 for D = 192):
 //        S = Q K^T, dP = dO V^T, dS as above, dQ += dS K.
+// Under a sliding window with sinks (SINK instances) the queries of the key
+// tiles that hold sinks are shared by several CTAs of launch 2, and one more
+// launch adds their fp32 sums in order.
 // The dK/dV kernel double-buffers the score tiles in TMEM (alternate sub-tiles
 // go to alternate buffers); the dQ kernel has one buffer of a wider unit.  A compute warpgroup loads its S / dP columns into
 // registers and releases the TMEM buffer at once, then writes the 16-bit P^T /
