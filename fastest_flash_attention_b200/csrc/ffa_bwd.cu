@@ -1360,6 +1360,8 @@ extern "C" size_t ffa_bwd_workspace_size(int B, int Hq, int Sq) {
 
 extern "C" size_t ffa_bwd_sink_workspace_size(int B, int Hq, int Hkv, int Sq, int Skv, int D, int Dv, int window,
                                               int sinks) {
+  // sizes that ffa_bwd_sink refuses: nothing to size (and nothing to divide by)
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || Sq <= 0 || Skv <= 0 || window <= 0 || sinks <= 0) return 0;
   // fp32 sums: of the tensor-core kernels' 128-key tiles, or of the fp32 kernels' 64-key ones
   int tiles = 0, parts = 0;
   ffa::bwd_sink_shape(ffa::BWD_BT, Sq, Skv, window, sinks, tiles, parts);

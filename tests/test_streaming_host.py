@@ -47,6 +47,44 @@ def test_rotary_tables_refusals(kw):
         ffa.rotary_tables(device="cpu", **kw)
 
 
+def test_c_entry_points_refuse_sizes_that_mean_nothing():
+    """No size crashes an entry point: it returns a status (no kernel is launched, so no GPU is needed)."""
+    from fastest_flash_attention_b200 import _lib
+    lib = _lib.load()
+    good = dict(B=1, Hq=4, Hkv=2, Sq=8, Skv=8, D=64, Dv=64, window=4, sinks=2)
+    assert lib.ffa_bwd_sink_workspace_size(*good.values()) > 0
+    for name in ("B", "Hq", "Hkv", "Sq", "Skv", "window", "sinks"):
+        for bad in (0, -1, -2 ** 31):
+            assert lib.ffa_bwd_sink_workspace_size(*dict(good, **{name: bad}).values()) == 0
+    s, p = _lib.i64arr(64, 64, 64), 4096  # never dereferenced: the sizes are refused first
+    for B, Hq, Hkv, Sq, Skv, D, Dv, w, n in ((0, 4, 2, 8, 8, 64, 64, 4, 2), (1, 4, 0, 8, 8, 64, 64, 4, 2),
+                                             (1, 3, 2, 8, 8, 64, 64, 4, 2), (1, 4, 2, -1, 8, 64, 64, 4, 2),
+                                             (1, 4, 2, 8, 8, 65, 64, 4, 2), (1, 4, 2, 8, 8, 64, 136, 4, 2),
+                                             (1, 4, 2, 8, 8, 64, 64, 0, 2), (1, 4, 2, 8, 8, 64, 64, 4, -1)):
+        assert lib.ffa_fwd_sink(p, p, p, p, p, 1, B, Hq, Hkv, Sq, Skv, D, Dv, s, s, s, s, 1.0, 1, 0, w, n, 0.0, None,
+                                None) in (_lib.FFA_ERR_INVALID_ARG, _lib.FFA_ERR_UNSUPPORTED)
+        assert lib.ffa_bwd_sink(p, p, p, p, p, p, p, p, p, 1, B, Hq, Hkv, Sq, Skv, D, Dv, s, s, s, s, s, s, s, s, 1.0,
+                                1, 0, w, n, 0.0, p, 1 << 30, None,
+                                None) in (_lib.FFA_ERR_INVALID_ARG, _lib.FFA_ERR_UNSUPPORTED)
+    for R, Hq, Hkv, D, P, page, width, w, n in ((-1, 4, 2, 64, 4, 16, 2, 4, 0), (1, 4, 0, 64, 4, 16, 2, 4, 0),
+                                                (1, 5, 2, 64, 4, 16, 2, 4, 0), (1, 4, 2, 60, 4, 16, 2, 4, 0),
+                                                (1, 4, 2, 136, 4, 16, 2, 4, 0), (1, 4, 2, 64, 0, 16, 2, 4, 0),
+                                                (1, 4, 2, 64, 4, 0, 2, 4, 0), (1, 4, 2, 64, 4, 16, 0, 4, 0),
+                                                (1, 4, 2, 64, 4, 16, 2, 0, 0), (1, 4, 2, 64, 4, 16, 2, 4, -1),
+                                                (1, 4, 2, 64, 2 ** 30, 2 ** 20, 2, 4, 0)):
+        assert lib.ffa_window_decode(p, p, p, p, p, p, None, 1, R, Hq, Hkv, D, P, page, width, s, s, 1.0, 0.0, w, n, 0,
+                                     None, None) in (_lib.FFA_ERR_INVALID_ARG, _lib.FFA_ERR_UNSUPPORTED)
+    assert lib.ffa_page_copy(p, None, p, p, -1, 4, 32, None, None) == _lib.FFA_ERR_INVALID_ARG
+    assert lib.ffa_page_copy(p, None, p, p, 1, 4, 33, None, None) == _lib.FFA_ERR_UNSUPPORTED
+    assert lib.ffa_token_move(p, None, p, p, 1, 2, 0, 4, 32, None, None) == _lib.FFA_ERR_INVALID_ARG
+    assert lib.ffa_rotary(p, s, p, s, None, None, None, None, p, p, 8, p, 0, 0, 1, 1, 1, 4, 0, 64, 63, 0, 0, None,
+                          None) == _lib.FFA_ERR_INVALID_ARG
+    assert lib.ffa_rotary(p, s, p, s, p, None, p, s, p, p, 8, p, 0, 0, 1, 1, 1, 4, 2, 64, 64, 0, 0, None,
+                          None) == _lib.FFA_ERR_INVALID_ARG
+    assert lib.ffa_rotary_append(p, s, p, s, p, s, p, s, p, p, 0, p, 0, p, p, p, 1, 1, 4, 2, 64, 64, 0, 16, 4, None,
+                                 None) == _lib.FFA_ERR_INVALID_ARG
+
+
 def test_new_operators_refuse_cpu_tensors():
     x = torch.zeros(1, 1, 2, 8)
     cos, sin = ffa.rotary_tables(8, 4, device="cpu")
