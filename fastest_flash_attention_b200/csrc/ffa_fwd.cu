@@ -274,8 +274,8 @@ __global__ void __launch_bounds__(FwdShape<NQT>::THREADS, FwdShape<NQT>::MIN_BLO
     if (EARLY && loads > 0) {
       load_q();
       const uint64_t pol_kv = policy_evict_last();
-      for (int x = 0; x < n_early; ++x)
-        for (int kv = 0; kv < 2; ++kv) load_kv(x, walk_tile(x), kv, pol_kv);
+      for (int kv = 0; kv < 2; ++kv)  // every K first: the two query tiles' first S need them
+        for (int x = 0; x < n_early; ++x) load_kv(x, walk_tile(x), kv, pol_kv);
     }
   }
   __syncwarp();
