@@ -195,6 +195,26 @@ def load() -> ctypes.CDLL:
     return lib
 
 
+_CALL = None
+
+
+def direct():
+    """The entry points that ``csrc/ffa_call.cpp`` calls without ctypes (the
+    same functions of the same library; strides are passed as tuples)."""
+    global _CALL
+    if _CALL is None:
+        lib = load()
+        try:
+            from . import _ffa_call
+        except ImportError as e:
+            raise RuntimeError("the _ffa_call module is not built; build it with "
+                               "`python -m fastest_flash_attention_b200.build`") from e
+        for name in _ffa_call.NAMES:
+            _ffa_call.bind(name, ctypes.cast(getattr(lib, name), ctypes.c_void_p).value)
+        _CALL = _ffa_call
+    return _CALL
+
+
 def register(name: str, restype, argtypes) -> None:
     SIGNATURES[name] = (restype, argtypes)
     if _LIB is not None:
@@ -219,6 +239,11 @@ def i64arr(*vals: int):
 def strides3(t: torch.Tensor):
     """The first three strides of a 4-D tensor, for an entry point's {batch, head, token} argument."""
     return i64arr(*t.stride()[:3])
+
+
+def three(t: torch.Tensor) -> tuple:
+    """The same as the tuple that the direct calls take."""
+    return t.stride()[:3]
 
 
 def stream_of(t: torch.Tensor) -> int:

@@ -142,18 +142,17 @@ def flash_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float
         bm = block_mask.to(device=q.device, dtype=torch.uint8).contiguous()
         n_br, n_bc = bm.shape
         bm_ptr = bm.data_ptr()
-    lib = _lib.load()
+    strides = _lib.three if sink else _strides_bhs
     operands = (q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr() if lse is not None else None,
-                _ATTN_DTYPE_CODE[dt], B, Hq, Hkv, Sq, Skv, D, Dv,
-                _strides_bhs(q), _strides_bhs(k), _strides_bhs(v), _strides_bhs(o),
+                _ATTN_DTYPE_CODE[dt], B, Hq, Hkv, Sq, Skv, D, Dv, strides(q), strides(k), strides(v), strides(o),
                 scale, 1 if causal else 0, q_offset, window)
     cap = softcap or 0.0
     tail = (_lib.err_ptr(q), _lib.stream_of(q))
     with _lib.device_of(q):
         if sink:
-            st = lib.ffa_fwd_sink(*operands, sink, cap, *tail)
+            st = _lib.direct().ffa_fwd_sink(*operands, sink, cap, *tail)
         else:
-            st = lib.ffa_fwd(*operands, cap, bm_ptr, n_br, n_bc, int(mask_block[0]),
+            st = _lib.load().ffa_fwd(*operands, cap, bm_ptr, n_br, n_bc, int(mask_block[0]),
                              int(mask_block[1]), *tail)
     _lib.check(st, "ffa_fwd_sink" if sink else "ffa_fwd")
     if block_mask is not None:
@@ -301,14 +300,13 @@ def flash_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Ten
     ws = q.new_empty(ws_bytes, dtype=torch.uint8)
     common = (dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(),
               dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ATTN_DTYPE_CODE[dt], B, Hq, Hkv, Sq, Skv, D, v.shape[3],
-              _strides_bhs(q), _strides_bhs(k), _strides_bhs(v), _strides_bhs(o), _strides_bhs(dout),
-              _strides_bhs(dq), _strides_bhs(dk), _strides_bhs(dv),
+              *map(_lib.three if sink else _strides_bhs, (q, k, v, o, dout, dq, dk, dv)),
               float(scale), int(bool(causal)), int(q_offset), int(window))
     cap = float(softcap or 0.0)
     tail = (ws.data_ptr(), ws_bytes, _lib.err_ptr(q), _lib.stream_of(q))
     with _lib.device_of(q):
         if sink:
-            st = lib.ffa_bwd_sink(*common, sink, cap, *tail)
+            st = _lib.direct().ffa_bwd_sink(*common, sink, cap, *tail)
         elif block_mask is None:
             st = lib.ffa_bwd(*common, cap, *tail)
         else:

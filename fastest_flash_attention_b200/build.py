@@ -2,7 +2,8 @@
 
 The library is a plain C-ABI shared object (``include/ffa_b200.h``); it is
 loaded through ctypes by :mod:`fastest_flash_attention_b200._lib`.  Building
-needs only nvcc (cross-compiles without a GPU).
+needs only nvcc (cross-compiles without a GPU) and, for the module that calls
+it from CPython directly (``csrc/ffa_call.cpp``), g++ and Python's headers.
 """
 from __future__ import annotations
 
@@ -10,6 +11,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -18,6 +20,8 @@ CSRC = PKG_DIR / "csrc"
 INCLUDE = REPO_DIR / "include"
 LIB_NAME = "libffa_b200.so"
 LIB_PATH = PKG_DIR / LIB_NAME
+CALL_SRC = CSRC / "ffa_call.cpp"
+CALL_PATH = PKG_DIR / ("_ffa_call" + sysconfig.get_config_var("EXT_SUFFIX"))
 BUILD_DIR = REPO_DIR / "_build"
 
 NVCC_FLAGS = [
@@ -46,8 +50,21 @@ def _stale(obj: Path, src: Path) -> bool:
     return any(d.stat().st_mtime > obj.stat().st_mtime for d in deps)
 
 
+def build_call(verbose: bool = False, force: bool = False) -> Path:
+    """Compile ``csrc/ffa_call.cpp``, the CPython side of the C ABI."""
+    if force or _stale(CALL_PATH, CALL_SRC):
+        tmp = CALL_PATH.with_suffix(".so.tmp")
+        cmd = [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-I", str(INCLUDE),
+               "-I", sysconfig.get_paths()["include"], str(CALL_SRC), "-o", str(tmp)]
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        subprocess.run(cmd, check=True)
+        os.replace(tmp, CALL_PATH)
+    return CALL_PATH
+
+
 def build(verbose: bool = False, force: bool = False, jobs: int | None = None) -> Path:
-    """Compile every ``csrc/*.cu`` for sm_100a and link ``libffa_b200.so``."""
+    """Compile every ``csrc/*.cu`` for sm_100a, link ``libffa_b200.so``, and build the module that calls it."""
     nvcc = _nvcc()
     BUILD_DIR.mkdir(exist_ok=True)
     objs = []
@@ -79,6 +96,7 @@ def build(verbose: bool = False, force: bool = False, jobs: int | None = None) -
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True)
         os.replace(tmp, LIB_PATH)
+    build_call(verbose, force)
     return LIB_PATH
 
 

@@ -153,10 +153,10 @@ def _window_decode(q, k_pages, v_pages, block_table, ctx_lens, scale, softcap, r
     out = q.new_empty((R, Hq, D))
     lse = q.new_empty((R, Hq), dtype=torch.float32) if return_lse else None
     with _lib.device_of(q):
-        st = _lib.load().ffa_window_decode(
+        st = _lib.direct().ffa_window_decode(
             q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), bt.data_ptr(), lens.data_ptr(), out.data_ptr(),
             lse.data_ptr() if return_lse else None, _lib.DTYPE_CODE[q.dtype], R, Hq, Hkv, D, P, page_size,
-            bt.shape[1], _lib.i64arr(sr, sh), _lib.i64arr(Hq * D, D), scale, softcap or 0.0,
+            bt.shape[1], (sr, sh), (Hq * D, D), scale, softcap or 0.0,
             min(window, big), min(sinks, big), max_ctx or 0, _lib.err_ptr(q), _lib.stream_of(q))
     _lib.check(st, "ffa_window_decode")
     if _lib.sync_check_enabled():

@@ -132,7 +132,7 @@ def copy_pages(k_pages: torch.Tensor, v_pages: Optional[torch.Tensor], src: Ids,
     if k_pages.numel() == 0 or src.numel() == 0:
         return
     with _lib.device_of(k_pages):
-        st = _lib.load().ffa_page_copy(
+        st = _lib.direct().ffa_page_copy(
             k_pages.data_ptr(), v_pages.data_ptr() if v_pages is not None else None, src.data_ptr(), dst.data_ptr(),
             src.numel(), k_pages.shape[0], k_pages.stride(0) * k_pages.element_size(),
             _lib.err_ptr(k_pages), _lib.stream_of(k_pages))
@@ -157,7 +157,7 @@ def move_tokens(k_pages: torch.Tensor, v_pages: Optional[torch.Tensor], src_slot
     if k_pages.numel() == 0 or src_slots.numel() == 0:
         return
     with _lib.device_of(k_pages):
-        st = _lib.load().ffa_token_move(
+        st = _lib.direct().ffa_token_move(
             k_pages.data_ptr(), v_pages.data_ptr() if v_pages is not None else None, src_slots.data_ptr(),
             dst_slots.data_ptr(), src_slots.numel(), k_pages.shape[1] if k_pages.dim() == 4 else 1, page_size, P,
             D * k_pages.element_size(), _lib.err_ptr(k_pages), _lib.stream_of(k_pages))

@@ -94,16 +94,16 @@ def _rotate(q: torch.Tensor, k: Optional[torch.Tensor], cos: torch.Tensor, sin: 
     B, Hq, S, D = q.shape
     q = _unit_last(q)
     qo = torch.empty_like(q)
-    qs, qd = _lib.strides3(q), _lib.strides3(qo)
+    qs, qd = _lib.three(q), _lib.three(qo)
     if k is not None:
         k = _unit_last(k)
         ko = torch.empty_like(k)
         Hkv, kptr, koptr = k.shape[1], k.data_ptr(), ko.data_ptr()
-        ks, kd = _lib.strides3(k), _lib.strides3(ko)
+        ks, kd = _lib.three(k), _lib.three(ko)
     else:
         ko, Hkv, kptr, koptr, ks, kd = None, 0, None, None, None, None
     with _lib.device_of(q):
-        st = _lib.load().ffa_rotary(
+        st = _lib.direct().ffa_rotary(
             q.data_ptr(), qs, qo.data_ptr(), qd, kptr, ks, koptr, kd, cos.data_ptr(), sin.data_ptr(), cos.shape[0],
             pos.data_ptr(), _POS64[pos.dtype], pos.stride(0) if pos.dim() == 2 else 0, _lib.IN_DTYPE_CODE[q.dtype],
             B, S, Hq, Hkv, D, 2 * cos.shape[1], layout, int(inverse), _lib.err_ptr(q),
@@ -205,11 +205,10 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.
     q, k, v = _unit_last(q), _unit_last(k), _unit_last(v)
     positions, slots = _unit_last(positions), _unit_last(slots)
     out = q.new_empty((T, Hq, D))
-    arr = _lib.i64arr
     with _lib.device_of(q):
-        st = _lib.load().ffa_rotary_append(
-            q.data_ptr(), arr(q.stride(0), q.stride(1)), out.data_ptr(), arr(Hq * D, D), k.data_ptr(),
-            arr(k.stride(0), k.stride(1)), v.data_ptr(), arr(v.stride(0), v.stride(1)), cos.data_ptr(),
+        st = _lib.direct().ffa_rotary_append(
+            q.data_ptr(), q.stride(), out.data_ptr(), (Hq * D, D), k.data_ptr(), k.stride(), v.data_ptr(), v.stride(),
+            cos.data_ptr(),
             sin.data_ptr(), cos.shape[0], positions.data_ptr(), _POS64[positions.dtype], slots.data_ptr(),
             k_pages.data_ptr(), v_pages.data_ptr(), _lib.IN_DTYPE_CODE[dt], T, Hq, Hkv, D, rot, _LAYOUTS[layout],
             page_size, P, _lib.err_ptr(q), _lib.stream_of(q))

@@ -85,6 +85,29 @@ def test_c_entry_points_refuse_sizes_that_mean_nothing():
                                  None) == _lib.FFA_ERR_INVALID_ARG
 
 
+def test_direct_calls_check_their_arguments():
+    """The module that calls the library without ctypes raises for what does not fit a parameter."""
+    from fastest_flash_attention_b200 import _lib
+    call = _lib.direct()
+    assert set(call.NAMES) <= set(_lib.SIGNATURES)
+    ok = (0, None, 0, 0, 0, 4, 32, None, None)  # n = 0: nothing to do
+    assert call.ffa_page_copy(*ok) == _lib.FFA_OK
+    with pytest.raises(TypeError):
+        call.ffa_page_copy(*ok[:-1])
+    with pytest.raises(TypeError):
+        call.ffa_page_copy(0, None, 0, 0, 0.5, 4, 32, None, None)
+    with pytest.raises(OverflowError):
+        call.ffa_page_copy(0, None, 0, 0, 0, 2 ** 31, 32, None, None)
+    with pytest.raises(KeyError):
+        call.bind("ffa_nothing", 0)
+    args = [4096] * 7 + [1, -1, 4, 2, 64, 4, 16, 2, (1, 1), (1, 1), 1.0, 0, 4, 0, 0, None, None]
+    assert call.ffa_window_decode(*args) == _lib.FFA_ERR_INVALID_ARG
+    for i, bad, err in ((15, [1, 1], TypeError), (15, (1,) * 5, TypeError), (16, (1, "a"), TypeError),
+                        (17, "x", TypeError), (0, 1.5, TypeError), (7, 2 ** 40, OverflowError)):
+        with pytest.raises(err):
+            call.ffa_window_decode(*args[:i], bad, *args[i + 1:])
+
+
 def test_new_operators_refuse_cpu_tensors():
     x = torch.zeros(1, 1, 2, 8)
     cos, sin = ffa.rotary_tables(8, 4, device="cpu")
