@@ -1,6 +1,6 @@
 // Direct calls of the C ABI from CPython, for the entry points whose time is
-// the call itself: ctypes spends 0.1 us on every argument of a call (2.8 us of
-// the 6 of a windowed decode), and needs an array object for every tuple of
+// the call itself: ctypes spends 0.1 us on every argument of a call (2.4 us of
+// the 6 of a windowed decode; 0.3 here), and needs an array object for every tuple of
 // strides.  The signatures come from include/ffa_b200.h, so an argument list
 // that does not fit it does not compile, and a Python value that does not fit
 // its parameter raises.  The library itself stays free of Python: the module is
