@@ -13,7 +13,7 @@
 //
 // HBM-bound: every value is read and written once; a token's table row is read
 // once per thread and serves all of its heads.  Measured on q [4, 32, 4096, 128]
-// and k [4, 8, 4096, 128] bf16: 58 us a launch, 5.87 TB/s (0.90 of a measured
+// and k [4, 8, 4096, 128] bf16: 56 us a launch, 6.06 TB/s (0.92 of a measured
 // copy); one thread per pair took 359 us, and addressing each head's row from
 // the operand table inside the loop 92 us (integer work).
 #include "ffa_common.cuh"
@@ -275,10 +275,11 @@ static bool rot_vec_ready(const RotParams& p) {
   return true;
 }
 
-// CTAs for each SM that a launch aims at before a thread walks more heads: 4,
-// 8 and 16 measured alike (58 us a launch below), 32 four microseconds more
-// (the table rows are read more often).
-constexpr int ROT_CTAS_PER_SM = 8;
+// CTAs for each SM that a launch aims at before a thread walks more heads: with
+// 2 a launch of the case above takes 56 us, with 4, 8 and 16 58, with 32 62 (the
+// table rows are read more often).  Evict-first loads, and batches of 2 heads at
+// four resident CTAs, measured 57 to 63 beside it.
+constexpr int ROT_CTAS_PER_SM = 2;
 
 template <typename T>
 static int launch_rotary(RotParams p, cudaStream_t st) {
