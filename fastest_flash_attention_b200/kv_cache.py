@@ -210,16 +210,17 @@ class PagedKVCache:
 
     def _assign_slots(self, seq_id: int, n: int) -> List[int]:
         """Slot (page * page_size + offset) of each appended token, allocating
-        pages exactly as the reference's per-token loop does (kv_cache.py:192-204)."""
-        seq = self.sequences.setdefault(seq_id, {"page_table": [], "len": 0})
-        slots = []
-        for _ in range(n):
-            idx, off = divmod(seq["len"], self.page_size)
-            while len(seq["page_table"]) <= idx:
-                seq["page_table"].append(self.allocate_page())
-            slots.append(seq["page_table"][idx] * self.page_size + off)
-            seq["len"] += 1
-        return slots
+        pages in the order of the reference's per-token loop (kv_cache.py:192-204);
+        without enough free pages nothing changes."""
+        seq = self.sequences.get(seq_id) or {"page_table": [], "len": 0}
+        start, end, table = seq["len"], seq["len"] + n, seq["page_table"]
+        more = -(-end // self.page_size) - len(table)
+        if more > len(self.free_pages):
+            raise RuntimeError("PagedKVCache: out of physical pages")
+        table.extend(self.allocate_page() for _ in range(more))
+        seq["len"] = end
+        self.sequences[seq_id] = seq
+        return [table[t // self.page_size] * self.page_size + t % self.page_size for t in range(start, end)]
 
     def append_tokens(self, seq_id: int, k_tokens: torch.Tensor, v_tokens: torch.Tensor) -> int:
         """Append [num_heads, S_new, head_dim] K/V; returns the new length (kv_cache.py:170-206)."""
