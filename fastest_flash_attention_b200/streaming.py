@@ -98,6 +98,13 @@ class StreamingDecoder:
             self._key = key
         return self._w, self._b
 
+    @staticmethod
+    def _check_ids(x: torch.Tensor, seq_ids: Sequence[int]) -> None:
+        if len(seq_ids) != x.shape[0]:
+            raise ValueError(f"{x.shape[0]} rows and {len(seq_ids)} sequences")
+        if len(set(seq_ids)) < len(seq_ids):
+            raise ValueError("a sequence is named twice")
+
     def _trim(self, seq_ids: Sequence[int]) -> None:
         for s in seq_ids:
             self.cache.trim_sequence(s, self.attn.sliding_window, self.attn.sink_tokens)
@@ -106,6 +113,7 @@ class StreamingDecoder:
     def prefill(self, x: torch.Tensor, seq_ids: Sequence[int]) -> torch.Tensor:
         """Run new sequences' prompts x [B, S, hidden] and cache their keys and
         values (pages outside the window and the first tokens come free at once)."""
+        self._check_ids(x, seq_ids)
         for s in seq_ids:
             if s in self.cache.sequences:
                 raise ValueError(f"sequence {s} has a context already")

@@ -28,3 +28,39 @@ def test_append_without_enough_pages_changes_nothing():
     assert c.sequences[0]["len"] == 5 and c.sequences[0]["page_table"] == [0, 1] and c.free_pages == [2]
     c.append_tokens(0, *_tokens(7, 5))  # what fits still does
     assert c.get_kv(0)[0][0, :, 0].tolist() == list(range(12))
+
+
+class _HostAttention(ffa.FastestFlashStreamingGQA):
+    """The module with plain projections for its two launches, so its decoder's bookkeeping runs on the host."""
+
+    def qkv(self, x, start=0):
+        B, S, _ = x.shape
+        return tuple(p(x).view(B, S, -1, self.head_dim).transpose(1, 2) for p in (self.q_proj, self.k_proj, self.v_proj))
+
+    def attend(self, q, k, v):
+        B, H, S, D = q.shape
+        return self.o_proj(q.transpose(1, 2).reshape(B, S, H * D))
+
+
+def _decoder(pages=8, ps=4, window=6, sinks=2, max_len=64):
+    torch.manual_seed(0)
+    m = _HostAttention(16, 2, 1, 8, sliding_window=window, sink_tokens=sinks, max_len=max_len).eval()
+    return ffa.StreamingDecoder(m, max_pages=pages, page_size=ps)
+
+
+def _unchanged(dec, call, err, match=None):
+    """`call` raises and leaves the decoder's cache as it was."""
+    c = dec.cache
+    before = ({s: dict(q, page_table=list(q["page_table"])) for s, q in c.sequences.items()}, list(c.free_pages),
+              dict(c._more_owners), c.k_pages.clone())
+    with pytest.raises(err, match=match):
+        call()
+    assert (c.sequences, c.free_pages, c._more_owners) == before[:3] and torch.equal(c.k_pages, before[3])
+
+
+@pytest.mark.parametrize("ids", [[0], [0, 1, 2], [3, 3], []])
+def test_prefill_takes_one_new_sequence_per_prompt(ids):
+    dec = _decoder()
+    _unchanged(dec, lambda: dec.prefill(torch.randn(2, 5, 16), ids), ValueError)
+    dec.prefill(torch.randn(2, 5, 16), [0, 1])
+    assert dec.cache.position(0) == dec.cache.position(1) == 5
