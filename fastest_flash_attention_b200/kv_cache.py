@@ -222,6 +222,13 @@ class PagedKVCache:
         self.sequences[seq_id] = seq
         return [table[t // self.page_size] * self.page_size + t % self.page_size for t in range(start, end)]
 
+    def _unassign_slot(self, seq_id: int) -> None:
+        """Take back the last slot that _assign_slots gave a sequence (its page too, if that began with it)."""
+        seq = self.sequences[seq_id]
+        seq["len"] -= 1
+        if seq["len"] % self.page_size == 0:
+            self.free_pages.insert(0, seq["page_table"].pop())
+
     def append_tokens(self, seq_id: int, k_tokens: torch.Tensor, v_tokens: torch.Tensor) -> int:
         """Append [num_heads, S_new, head_dim] K/V; returns the new length (kv_cache.py:170-206)."""
         S_new = k_tokens.size(1)

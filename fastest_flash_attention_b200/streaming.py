@@ -100,7 +100,7 @@ class StreamingDecoder:
 
     @staticmethod
     def _check_ids(x: torch.Tensor, seq_ids: Sequence[int]) -> None:
-        if len(seq_ids) != x.shape[0]:
+        if len(seq_ids) != x.shape[0] or len(seq_ids) == 0:
             raise ValueError(f"{x.shape[0]} rows and {len(seq_ids)} sequences")
         if len(set(seq_ids)) < len(seq_ids):
             raise ValueError("a sequence is named twice")
@@ -125,19 +125,35 @@ class StreamingDecoder:
 
     @torch.no_grad()
     def step(self, x: torch.Tensor, seq_ids: Sequence[int]) -> torch.Tensor:
-        """One new token for each sequence: x [R, 1, hidden] -> [R, 1, hidden]."""
+        """One new token for each sequence: x [R, 1, hidden] -> [R, 1, hidden].
+        A failing call changes nothing."""
         m, cache = self.attn, self.cache
-        R, dev = x.shape[0], x.device
-        H, Hkv, D = m.num_heads, m.num_kv_heads, m.head_dim
+        if x.dim() != 3 or x.shape[1] != 1:
+            raise ValueError(f"a step takes x [R, 1, hidden], got {tuple(x.shape)}")
+        self._check_ids(x, seq_ids)
         pos: List[int] = [cache.position(s) for s in seq_ids]
         if max(pos) >= m.max_len:
             raise ValueError(f"position {max(pos)} is past the rotary tables' {m.max_len}")
-        if len(set(seq_ids)) < R:
-            raise ValueError("a sequence is named twice")
         starts = sum(cache.sequences.get(s, {"len": 0})["len"] % cache.page_size == 0 for s in seq_ids)
         if starts > cache.num_free_pages:  # before anything changes
             raise RuntimeError("PagedKVCache: out of physical pages")
+        new = [s for s in seq_ids if s not in cache.sequences]
         slots = [cache._assign_slots(s, 1)[0] for s in seq_ids]
+        try:
+            out = self._step(x, seq_ids, pos, slots)
+        except BaseException:
+            for s in reversed(seq_ids):
+                cache._unassign_slot(s)
+            for s in new:
+                del cache.sequences[s]
+            raise
+        self._trim(seq_ids)
+        return out
+
+    def _step(self, x: torch.Tensor, seq_ids: Sequence[int], pos: List[int], slots: List[int]) -> torch.Tensor:
+        m, cache = self.attn, self.cache
+        R, dev = x.shape[0], x.device
+        H, Hkv, D = m.num_heads, m.num_kv_heads, m.head_dim
         meta = torch.tensor([pos, slots], dtype=torch.int32).to(dev, non_blocking=True)
         bt, lens = cache.block_table(seq_ids, dev, sliding_window=m.sliding_window, sink_tokens=m.sink_tokens)
         w, b = self._weights()
@@ -148,7 +164,6 @@ class StreamingDecoder:
         o = paged_decode(q, cache.k_pages, cache.v_pages, bt, lens, scale=m.scale, softcap=m.softcap,
                          sliding_window=m.sliding_window, sink_tokens=m.sink_tokens,
                          max_ctx=max(cache.sequences[s]["len"] for s in seq_ids))
-        self._trim(seq_ids)
         return m.o_proj(o.view(R, 1, H * D))
 
     def fork(self, pairs: Sequence[Tuple[int, int]]) -> None:

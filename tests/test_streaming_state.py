@@ -64,3 +64,25 @@ def test_prefill_takes_one_new_sequence_per_prompt(ids):
     _unchanged(dec, lambda: dec.prefill(torch.randn(2, 5, 16), ids), ValueError)
     dec.prefill(torch.randn(2, 5, 16), [0, 1])
     assert dec.cache.position(0) == dec.cache.position(1) == 5
+
+
+@pytest.mark.parametrize("rows,ids", [(1, [0, 1]), (2, [0]), (2, [1, 1]), (0, [])])
+def test_step_takes_one_sequence_per_row(rows, ids):
+    dec = _decoder()
+    dec.prefill(torch.randn(2, 5, 16), [0, 1])
+    _unchanged(dec, lambda: dec.step(torch.randn(rows, 1, 16), ids), ValueError, "sequence")
+
+
+def test_step_takes_one_token_per_row():
+    dec = _decoder()
+    dec.prefill(torch.randn(2, 5, 16), [0, 1])
+    _unchanged(dec, lambda: dec.step(torch.randn(2, 2, 16), [0, 1]), ValueError)
+
+
+@pytest.mark.parametrize("prompt", [3, 4, 5])
+def test_step_that_fails_changes_nothing(prompt):
+    """A launch that refuses (here: for tensors without a GPU) comes after the slots were assigned."""
+    dec = _decoder()
+    dec.prefill(torch.randn(2, prompt, 16), [0, 1])
+    _unchanged(dec, lambda: dec.step(torch.randn(3, 1, 16), [0, 5, 1]), RuntimeError, "CUDA")
+    _unchanged(dec, lambda: dec.step(torch.randn(2, 1, 16, dtype=torch.float64), [0, 1]), RuntimeError, "dtype")
