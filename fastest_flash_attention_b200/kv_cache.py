@@ -312,6 +312,11 @@ class PagedKVCache:
             self.k_pages[new] = self.k_pages[old]
             self.v_pages[new] = self.v_pages[old]
 
+    def _outside(self, n: int, sliding_window: int, sink_tokens: int) -> Tuple[int, int]:
+        """Pages [first, last) of n tokens: those without a token of the window or of the first sink_tokens."""
+        first = -(-sink_tokens // self.page_size)
+        return first, max(first, (n - sliding_window) // self.page_size)
+
     def trim_sequence(self, seq_id: int, sliding_window: int, sink_tokens: int = 0) -> int:
         """Free the pages whose tokens are all outside the last sliding_window
         tokens and the first sink_tokens (their table entries become -1; the
@@ -319,8 +324,7 @@ class PagedKVCache:
         check_window(sliding_window, sink_tokens)
         seq = self.sequences[seq_id]
         table, freed = seq["page_table"], 0
-        first = -(-sink_tokens // self.page_size)  # the first page without a sink token
-        for i in range(first, max(first, (seq["len"] - sliding_window) // self.page_size)):
+        for i in range(*self._outside(seq["len"], sliding_window, sink_tokens)):
             freed += self._release(table[i])
             table[i] = -1
         return freed

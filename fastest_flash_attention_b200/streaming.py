@@ -112,16 +112,26 @@ class StreamingDecoder:
     @torch.no_grad()
     def prefill(self, x: torch.Tensor, seq_ids: Sequence[int]) -> torch.Tensor:
         """Run new sequences' prompts x [B, S, hidden] and cache their keys and
-        values (pages outside the window and the first tokens come free at once)."""
+        values (pages outside the window and the first tokens come free at
+        once).  A failing call changes nothing."""
+        m, cache = self.attn, self.cache
         self._check_ids(x, seq_ids)
         for s in seq_ids:
-            if s in self.cache.sequences:
+            if s in cache.sequences:
                 raise ValueError(f"sequence {s} has a context already")
-        q, k, v = self.attn.qkv(x)
+        B, S, _ = x.shape
+        if S > m.max_len:
+            raise ValueError(f"{S} tokens are past the rotary tables' {m.max_len}")
+        pages = -(-S // cache.page_size)
+        first, last = cache._outside(S, m.sliding_window, m.sink_tokens)
+        if pages + (B - 1) * (pages - (last - first)) > cache.num_free_pages:
+            raise RuntimeError("PagedKVCache: out of physical pages")
+        q, k, v = m.qkv(x)
+        out = m.attend(q, k, v)
         for b, s in enumerate(seq_ids):
-            self.cache.append_tokens(s, k[b], v[b])
+            cache.append_tokens(s, k[b], v[b])
             self._trim([s])
-        return self.attn.attend(q, k, v)
+        return out
 
     @torch.no_grad()
     def step(self, x: torch.Tensor, seq_ids: Sequence[int]) -> torch.Tensor:

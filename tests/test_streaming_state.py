@@ -86,3 +86,15 @@ def test_step_that_fails_changes_nothing(prompt):
     dec.prefill(torch.randn(2, prompt, 16), [0, 1])
     _unchanged(dec, lambda: dec.step(torch.randn(3, 1, 16), [0, 5, 1]), RuntimeError, "CUDA")
     _unchanged(dec, lambda: dec.step(torch.randn(2, 1, 16, dtype=torch.float64), [0, 1]), RuntimeError, "dtype")
+
+
+def test_prefill_that_fails_changes_nothing():
+    dec = _decoder(pages=8, ps=4)
+    dec.prefill(torch.randn(1, 10, 16), [9])  # 3 pages
+    _unchanged(dec, lambda: dec.prefill(torch.randn(3, 8, 16), [0, 1, 2]), RuntimeError, "out of physical pages")
+    _unchanged(dec, lambda: dec.prefill(torch.randn(1, 65, 16), [0]), ValueError)  # past the rotary tables
+    dec.attn.attend = lambda q, k, v: (_ for _ in ()).throw(RuntimeError("refused"))
+    _unchanged(dec, lambda: dec.prefill(torch.randn(1, 8, 16), [0]), RuntimeError, "refused")
+    del dec.attn.attend
+    dec.prefill(torch.randn(2, 8, 16), [0, 1])
+    assert dec.cache.num_free_pages == 8 - 3 - 4
