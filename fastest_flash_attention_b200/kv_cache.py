@@ -233,8 +233,28 @@ class PagedKVCache:
         """Append [num_heads, S_new, head_dim] K/V; returns the new length (kv_cache.py:170-206)."""
         S_new = k_tokens.size(1)
         slots = self._assign_slots(seq_id, S_new)
-        if S_new == 0:
-            return self.sequences[seq_id]["len"]
+        if S_new > 0:
+            self._write(slots, k_tokens, v_tokens)
+        return self.sequences[seq_id]["len"]
+
+    def _append_visible(self, seq_id: int, k_tokens: torch.Tensor, v_tokens: torch.Tensor, sliding_window: int,
+                       sink_tokens: int = 0) -> int:
+        """A new sequence as append_tokens and trim_sequence leave it, without
+        pages for the tokens that the trim would free."""
+        check_window(sliding_window, sink_tokens)
+        if seq_id in self.sequences:
+            raise ValueError(f"PagedKVCache: sequence {seq_id} exists already")
+        n, ps = k_tokens.size(1), self.page_size
+        first, last = self._outside(n, sliding_window, sink_tokens)
+        if first < last:  # tokens [first * ps, last * ps) get no page
+            k_tokens, v_tokens = (torch.cat([t[:, :first * ps], t[:, last * ps:]], 1) for t in (k_tokens, v_tokens))
+        self.append_tokens(seq_id, k_tokens, v_tokens)
+        seq = self.sequences[seq_id]
+        seq["page_table"][first:first] = [-1] * (last - first)
+        seq["len"] = n
+        return n
+
+    def _write(self, slots: List[int], k_tokens: torch.Tensor, v_tokens: torch.Tensor) -> None:
         if self.k_pages.is_cuda and self.k_pages.dtype in _lib.DTYPE_CODE and self.head_dim % 8 == 0:
             k_new = k_tokens.to(self.k_pages.device, self.k_pages.dtype).contiguous()
             v_new = v_tokens.to(self.v_pages.device, self.v_pages.dtype).contiguous()
@@ -243,7 +263,7 @@ class PagedKVCache:
             with torch.cuda.device(self.k_pages.device):
                 st = lib.ffa_paged_append(k_new.data_ptr(), v_new.data_ptr(), self.k_pages.data_ptr(),
                                           self.v_pages.data_ptr(), slot_t.data_ptr(),
-                                          _lib.DTYPE_CODE[self.k_pages.dtype], S_new, self.num_heads,
+                                          _lib.DTYPE_CODE[self.k_pages.dtype], len(slots), self.num_heads,
                                           self.head_dim, self.page_size, self.max_pages,
                                           _lib.i64arr(k_new.stride(0), k_new.stride(1)),
                                           _lib.stream_of(self.k_pages))
@@ -254,7 +274,6 @@ class PagedKVCache:
             pages, offs = slot_t // self.page_size, slot_t % self.page_size
             self.k_pages[pages, :, offs, :] = k_tokens.permute(1, 0, 2).to(self.k_pages)
             self.v_pages[pages, :, offs, :] = v_tokens.permute(1, 0, 2).to(self.v_pages)
-        return self.sequences[seq_id]["len"]
 
     def get_kv(self, seq_id: int) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
         """Contiguous [num_heads, len, head_dim] copies of a sequence (kv_cache.py:208-232)."""

@@ -112,8 +112,8 @@ class StreamingDecoder:
     @torch.no_grad()
     def prefill(self, x: torch.Tensor, seq_ids: Sequence[int]) -> torch.Tensor:
         """Run new sequences' prompts x [B, S, hidden] and cache their keys and
-        values (pages outside the window and the first tokens come free at
-        once).  A failing call changes nothing."""
+        values (in pages for the window and the first tokens alone).  A failing
+        call changes nothing."""
         m, cache = self.attn, self.cache
         self._check_ids(x, seq_ids)
         for s in seq_ids:
@@ -122,15 +122,13 @@ class StreamingDecoder:
         B, S, _ = x.shape
         if S > m.max_len:
             raise ValueError(f"{S} tokens are past the rotary tables' {m.max_len}")
-        pages = -(-S // cache.page_size)
         first, last = cache._outside(S, m.sliding_window, m.sink_tokens)
-        if pages + (B - 1) * (pages - (last - first)) > cache.num_free_pages:
+        if B * (-(-S // cache.page_size) - (last - first)) > cache.num_free_pages:
             raise RuntimeError("PagedKVCache: out of physical pages")
         q, k, v = m.qkv(x)
         out = m.attend(q, k, v)
         for b, s in enumerate(seq_ids):
-            cache.append_tokens(s, k[b], v[b])
-            self._trim([s])
+            cache._append_visible(s, k[b], v[b], m.sliding_window, m.sink_tokens)
         return out
 
     @torch.no_grad()

@@ -98,3 +98,30 @@ def test_prefill_that_fails_changes_nothing():
     del dec.attn.attend
     dec.prefill(torch.randn(2, 8, 16), [0, 1])
     assert dec.cache.num_free_pages == 8 - 3 - 4
+
+
+@pytest.mark.parametrize("ps,window,sinks,n", [(4, 6, 2, 30), (4, 6, 0, 30), (4, 1, 9, 40), (4, 100, 2, 30), (4, 3, 50, 20),
+                                               (1, 3, 2, 9), (16, 5, 3, 15), (4, 6, 2, 1)])
+def test_prefill_leaves_what_append_and_trim_leave(ps, window, sinks, n):
+    x = torch.randn(1, n, 16)
+    a, b = _decoder(64, ps, window, sinks), _decoder(64, ps, window, sinks)
+    out = a.prefill(x, [0])
+    q, k, v = b.attn.qkv(x)
+    b.cache.append_tokens(0, k[0], v[0])
+    b.cache.trim_sequence(0, window, sinks)
+    ta, tb = a.cache.sequences[0]["page_table"], b.cache.sequences[0]["page_table"]
+    assert [p < 0 for p in ta] == [p < 0 for p in tb] and a.cache.position(0) == n == b.cache.position(0)
+    for pa, pb in zip(ta, tb):
+        if pa >= 0:
+            assert torch.equal(a.cache.k_pages[pa], b.cache.k_pages[pb])
+            assert torch.equal(a.cache.v_pages[pa], b.cache.v_pages[pb])
+    assert torch.equal(out, b.attn.attend(q, k, v)) and a.cache.num_free_pages == b.cache.num_free_pages
+
+
+def test_prefill_needs_pages_for_the_visible_tokens_alone():
+    dec = _decoder(pages=6, ps=4, window=6, sinks=2)
+    dec.prefill(torch.randn(2, 40, 16), [0, 1])  # each: the first page and the last two of ten
+    assert dec.cache.num_free_pages == 0
+    dec.cache.free_sequence(0)
+    dec.cache.free_sequence(1)
+    assert sorted(dec.cache.free_pages) == list(range(6))
