@@ -4,7 +4,7 @@ both (no counterpart in the reference, whose modules have neither rotary
 positions outside MLA nor a cache of their own).
 
 ``FastestFlashStreamingGQA`` trains and prefills; ``StreamingDecoder`` serves
-it: every step is one stacked projection, one launch that rotates the new
+it: every step is the three projections, one launch that rotates the new
 queries and keys and writes keys and values into their pages, one launch of
 the windowed decode, and the output projection.  Pages that leave the window
 are freed as it goes, so a sequence of any length holds
@@ -87,17 +87,6 @@ class StreamingDecoder:
         w = attn.q_proj.weight
         self.cache = PagedKVCache(max_pages, page_size, attn.num_kv_heads, attn.head_dim, w.dtype, w.device)
 
-    def _weights(self) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
-        """q_proj, k_proj and v_proj stacked, so a step's projections are one
-        GEMM (stacked again when a parameter changed)."""
-        ps = (self.attn.q_proj, self.attn.k_proj, self.attn.v_proj)
-        key = tuple((t.data_ptr(), t._version) for p in ps for t in (p.weight, p.bias) if t is not None)
-        if getattr(self, "_key", None) != key:
-            self._w = torch.cat([p.weight.detach() for p in ps])
-            self._b = torch.cat([p.bias.detach() for p in ps]) if ps[0].bias is not None else None
-            self._key = key
-        return self._w, self._b
-
     @staticmethod
     def _check_ids(x: torch.Tensor, seq_ids: Sequence[int]) -> None:
         if len(seq_ids) != x.shape[0] or len(seq_ids) == 0:
@@ -164,11 +153,9 @@ class StreamingDecoder:
         H, Hkv, D = m.num_heads, m.num_kv_heads, m.head_dim
         meta = torch.tensor([pos, slots], dtype=torch.int32).to(dev, non_blocking=True)
         bt, lens = cache.block_table(seq_ids, dev, sliding_window=m.sliding_window, sink_tokens=m.sink_tokens)
-        w, b = self._weights()
-        y = torch.nn.functional.linear(x[:, 0], w, b)  # [R, (H + 2 Hkv) D]
-        q = rotary_append(y[:, :H * D].view(R, H, D), y[:, H * D:(H + Hkv) * D].view(R, Hkv, D),
-                          y[:, (H + Hkv) * D:].view(R, Hkv, D), *m.tables(dev), meta[0], meta[1], cache.k_pages,
-                          cache.v_pages, layout=m.rotary_layout)
+        x = x[:, 0]
+        q = rotary_append(m.q_proj(x).view(R, H, D), m.k_proj(x).view(R, Hkv, D), m.v_proj(x).view(R, Hkv, D),
+                          *m.tables(dev), meta[0], meta[1], cache.k_pages, cache.v_pages, layout=m.rotary_layout)
         o = paged_decode(q, cache.k_pages, cache.v_pages, bt, lens, scale=m.scale, softcap=m.softcap,
                          sliding_window=m.sliding_window, sink_tokens=m.sink_tokens,
                          max_ctx=max(cache.sequences[s]["len"] for s in seq_ids))

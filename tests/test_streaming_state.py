@@ -125,3 +125,45 @@ def test_prefill_needs_pages_for_the_visible_tokens_alone():
     dec.cache.free_sequence(0)
     dec.cache.free_sequence(1)
     assert sorted(dec.cache.free_pages) == list(range(6))
+
+
+def _captured_step(monkeypatch, dec, x, ids):
+    """The q, k, v that a step projects (its launches replaced on the host)."""
+    from fastest_flash_attention_b200 import streaming
+    seen = {}
+
+    def append(q, k, v, *args, **kw):
+        seen.update(q=q, k=k, v=v)
+        return q
+    monkeypatch.setattr(streaming, "rotary_append", append)
+    monkeypatch.setattr(streaming, "paged_decode", lambda q, *args, **kw: q)
+    dec.step(x, ids)
+    return seen
+
+
+@pytest.mark.parametrize("bias", [False, True])
+def test_step_uses_the_weights_of_its_own_time(monkeypatch, bias):
+    """Weights written through .data change neither address nor version."""
+    dec = _decoder()
+    m = dec.attn
+    if bias:
+        for p in (m.q_proj, m.k_proj, m.v_proj):
+            p.bias = torch.nn.Parameter(torch.randn(p.out_features))
+    dec.prefill(torch.randn(2, 5, 16), [0, 1])
+    for change in (lambda t: None, lambda t: t.data.mul_(-2.0), lambda t: t.data.copy_(torch.randn_like(t))):
+        for p in (m.q_proj, m.k_proj, m.v_proj):
+            for t in p.parameters():
+                change(t)
+        x = torch.randn(2, 1, 16)
+        got = _captured_step(monkeypatch, dec, x, [0, 1])
+        for name, n in (("q", 2), ("k", 1), ("v", 1)):
+            want = getattr(m, name + "_proj")(x[:, 0]).view(2, n, 8)
+            # 16 products of fp32 values, summed in another order at most
+            torch.testing.assert_close(got[name], want, rtol=1e-5, atol=1e-5)
+
+
+def test_step_with_parameters_made_in_inference_mode(monkeypatch):
+    with torch.inference_mode():
+        dec = _decoder()
+        dec.prefill(torch.randn(1, 5, 16), [0])
+        assert _captured_step(monkeypatch, dec, torch.randn(1, 1, 16), [0])["q"].shape == (1, 2, 8)
