@@ -116,23 +116,30 @@ def _rotate(q: torch.Tensor, k: Optional[torch.Tensor], cos: torch.Tensor, sin: 
 
 class RotaryFunc(Function):
     """Autograd function of apply_rotary: the gradient of a rotation is the
-    rotation by the negative angle (the transpose, with scaled tables too)."""
+    rotation by the negative angle (the transpose, with scaled tables too),
+    itself through this function where it will be differentiated again."""
 
     @staticmethod
-    def forward(ctx, q, k, cos, sin, pos, layout):
+    def forward(ctx, q, k, cos, sin, pos, layout, inverse):
         ctx.save_for_backward(cos, sin, pos)
-        ctx.layout = layout
+        ctx.layout, ctx.inverse = layout, inverse
         ctx.set_materialize_grads(False)
-        return _rotate(q, k, cos, sin, pos, layout, False)
+        return _rotate(q, k, cos, sin, pos, layout, inverse)
 
     @staticmethod
     def backward(ctx, dq, dk):
-        cos, sin, pos = ctx.saved_tensors
         first, second = (dq, dk) if dq is not None else (dk, None)
         if first is None:
-            return None, None, None, None, None, None
-        a, b = _rotate(first, second, cos, sin, pos, ctx.layout, True)
-        return (a, b, None, None, None, None) if dq is not None else (None, a, None, None, None, None)
+            return (None,) * 7
+        a, b = _rotation(first, second, *ctx.saved_tensors, ctx.layout, not ctx.inverse)
+        return (a, b) + (None,) * 5 if dq is not None else (None, a) + (None,) * 5
+
+
+def _rotation(q, k, cos, sin, pos, layout: int, inverse: bool):
+    """The rotation, through autograd where an input is part of a graph (and only there: the function costs host time)."""
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return RotaryFunc.apply(q, k, cos, sin, pos, layout, inverse)
+    return _rotate(q, k, cos, sin, pos, layout, inverse)
 
 
 def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], cos: torch.Tensor, sin: torch.Tensor,
@@ -167,10 +174,7 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], cos: torch.Tensor, 
     if positions.dtype not in _POS64 or tuple(positions.shape) not in ((S,), (B, S)):
         raise ValueError(f"positions must be int32 or int64 [S] or [B, S], got {positions.dtype} "
                          f"{tuple(positions.shape)}")
-    positions = _unit_last(positions)
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        return RotaryFunc.apply(q, k, cos, sin, positions, _LAYOUTS[layout])
-    return _rotate(q, k, cos, sin, positions, _LAYOUTS[layout], False)
+    return _rotation(q, k, cos, sin, _unit_last(positions), _LAYOUTS[layout], False)
 
 
 def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
