@@ -13,7 +13,7 @@ import math
 from typing import Optional, Tuple, Union
 
 import torch
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 
 from . import _lib
 
@@ -136,8 +136,10 @@ class RotaryFunc(Function):
 
 
 def _rotation(q, k, cos, sin, pos, layout: int, inverse: bool):
-    """The rotation, through autograd where an input is part of a graph (and only there: the function costs host time)."""
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+    """The rotation, through autograd where an input is part of a graph or may
+    carry a tangent (which the function refuses), and only there: it costs host time."""
+    if (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))
+            or forward_ad._current_level >= 0):
         return RotaryFunc.apply(q, k, cos, sin, pos, layout, inverse)
     return _rotate(q, k, cos, sin, pos, layout, inverse)
 

@@ -50,3 +50,16 @@ def test_gradient_of_one_output_alone(host_rotation):
     assert dq is None or not bool(dq.any())
     torch.testing.assert_close(dk, 2 * k)  # a rotation keeps the norm, 2^-24 in the tables
     torch.testing.assert_close(torch.autograd.grad(dk.sum(), k)[0], torch.full_like(k, 2.0))
+
+
+def test_forward_mode_is_refused_not_dropped(host_rotation):
+    """A dual tensor requires no gradient; its tangent must not vanish."""
+    from torch.autograd import forward_ad
+    q, k, cos, sin = (t.detach() for t in _inputs())
+    with forward_ad.dual_level():
+        for a, b in ((forward_ad.make_dual(q, q), None), (forward_ad.make_dual(q, q), k), (q, forward_ad.make_dual(k, k))):
+            with pytest.raises((RuntimeError, NotImplementedError), match="jvp"):
+                rotary.apply_rotary(a, b, cos, sin, 2)
+            with torch.no_grad(), pytest.raises((RuntimeError, NotImplementedError), match="jvp"):
+                rotary.apply_rotary(a, b, cos, sin, 2)
+        rotary.apply_rotary(q, k, cos, sin, 2)
