@@ -386,6 +386,20 @@ class FastestFlashAttnFunc(Function):
         return dq, dk, dv, None, None, None, None, None, None, None
 
 
+class _NoSecondDerivative(Function):
+    """Passes gradients on and raises where they would be differentiated again
+    (they come from launches that autograd does not see; once_differentiable
+    looks at the incoming gradient alone, not at q, k and v)."""
+
+    @staticmethod
+    def forward(ctx, dq, dk, dv, *inputs):
+        return dq.view_as(dq), dk.view_as(dk), dv.view_as(dv)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("attention with sinks has no second derivative")
+
+
 class SinkAttnFunc(Function):
     """Autograd function of attention with a sliding window and sinks, on 4-D
     q, k, v: ``options`` are flash_fwd's and flash_bwd's keyword arguments.
@@ -407,6 +421,8 @@ class SinkAttnFunc(Function):
         dq, dk, dv = flash_bwd(grad_output, q, k, v, o, lse, **ctx.options)
         if dq.dtype != q.dtype or dk.dtype != k.dtype or dv.dtype != v.dtype:
             dq, dk, dv = dq.to(q.dtype), dk.to(k.dtype), dv.to(v.dtype)
+        if torch.is_grad_enabled():  # create_graph=True
+            dq, dk, dv = _NoSecondDerivative.apply(dq, dk, dv, grad_output, q, k, v)
         return dq, dk, dv, None
 
 
