@@ -121,7 +121,7 @@ def flash_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float
         raise ValueError(f"head dims (qk={D}, v={Dv}) not supported by the sm_100a forward kernel "
                          f"(supported: qk <= {MAX_HEAD_DIM}, v <= 128)")
     sink = _sinks(window, sink, block_mask)
-    window = min(window or 0, _MAX_WINDOW)
+    window = min(int(window or 0), _MAX_WINDOW)
     dt = kernel_dtype(q, compute_dtype)
     if kdims != (D, Dv) and not _narrow_ok(sink, dt, D, Dv):
         o, lse = flash_fwd(_pad_last(q.to(dt), kdims[0]), _pad_last(k.to(dt), kdims[0]),
@@ -145,8 +145,8 @@ def flash_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float
     strides = _lib.three if sink else _strides_bhs
     operands = (q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr() if lse is not None else None,
                 _ATTN_DTYPE_CODE[dt], B, Hq, Hkv, Sq, Skv, D, Dv, strides(q), strides(k), strides(v), strides(o),
-                scale, 1 if causal else 0, q_offset, window)
-    cap = softcap or 0.0
+                float(scale), 1 if causal else 0, int(q_offset), window)
+    cap = float(softcap or 0.0)
     tail = (_lib.err_ptr(q), _lib.stream_of(q))
     with _lib.device_of(q):
         if sink:
@@ -274,7 +274,7 @@ def flash_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Ten
     if Hq % Hkv != 0:
         raise ValueError(f"query heads ({Hq}) must be a multiple of key/value heads ({Hkv})")
     sink = _sinks(window, sink, block_mask)
-    window = min(window or 0, _MAX_WINDOW)
+    window = min(int(window or 0), _MAX_WINDOW)
     dt = kernel_dtype(q, compute_dtype)
     if kdims != (D, Dv) and not _narrow_ok(sink, dt, D, Dv):
         # zero columns: Delta, dP and the kept gradient columns are unchanged
@@ -301,7 +301,7 @@ def flash_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Ten
     common = (dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(),
               dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ATTN_DTYPE_CODE[dt], B, Hq, Hkv, Sq, Skv, D, v.shape[3],
               *map(_lib.three if sink else _strides_bhs, (q, k, v, o, dout, dq, dk, dv)),
-              float(scale), int(bool(causal)), int(q_offset), int(window))
+              float(scale), int(bool(causal)), int(q_offset), window)
     cap = float(softcap or 0.0)
     tail = (ws.data_ptr(), ws_bytes, _lib.err_ptr(q), _lib.stream_of(q))
     with _lib.device_of(q):
