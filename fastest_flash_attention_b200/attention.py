@@ -201,7 +201,7 @@ def fastest_flash_attn_forward(
         compute_dtype = config.compute_dtype
         num_kv_heads = config.num_kv_heads
         return_lse = config.return_lse
-        sink_tokens = config.sink_tokens
+        sink_tokens = getattr(config, "sink_tokens", sink_tokens)  # the reference's class has no such field
 
     in_dtype = q.dtype
     q, k, v, squeezed = maybe_unsqueeze_head(q, k, v)

@@ -63,3 +63,18 @@ def test_forward_and_backward(lib, kw, sink):
 def test_offset(lib, off, sink):
     attention.flash_fwd(*_qkv(), scale=0.125, causal=True, q_offset=off, window=8, sink=sink)
     assert lib.last[1][19] == 5
+
+
+def test_configuration_of_another_class(lib):
+    """A configuration with the fields of the reference's, which has no sink_tokens."""
+    from types import SimpleNamespace
+    from fastest_flash_attention_b200 import AttentionConfig
+    fields = {f: getattr(AttentionConfig(causal=True, sliding_window=8), f) for f in (
+        "block_size_q", "block_size_kv", "causal", "sliding_window", "softcap", "num_kv_heads", "compute_dtype",
+        "two_pass", "return_lse")}
+    attention.fastest_flash_attn_forward(*_qkv(), config=SimpleNamespace(**fields))
+    assert lib.last[0] == "ffa_fwd" and lib.last[1][18] == 1 and lib.last[1][20] == 8
+    attention.fastest_flash_attn_forward(*_qkv(), config=SimpleNamespace(**fields), sink_tokens=2)
+    assert lib.last[0] == "ffa_fwd_sink" and lib.last[1][21] == 2
+    attention.fastest_flash_attn_forward(*_qkv(), config=AttentionConfig(**fields, sink_tokens=3), sink_tokens=2)
+    assert lib.last[0] == "ffa_fwd_sink" and lib.last[1][21] == 3
