@@ -53,8 +53,9 @@ class FastestFlashStreamingGQA(FastestFlashGQA):
     def tables(self, device: torch.device) -> Tuple[torch.Tensor, torch.Tensor]:
         """The rotary tables on `device`, built at their first use."""
         if device not in self._tables:
-            self._tables[device] = rotary_tables(self.rotary_dim, self.max_len, self.rotary_base, device=device,
-                                                 **self.rotary_scaling)
+            with torch.inference_mode(False):  # a training step may save them for its backward later
+                self._tables[device] = rotary_tables(self.rotary_dim, self.max_len, self.rotary_base, device=device,
+                                                     **self.rotary_scaling)
         return self._tables[device]
 
     def qkv(self, x: torch.Tensor, start: int = 0) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:

@@ -167,3 +167,11 @@ def test_step_with_parameters_made_in_inference_mode(monkeypatch):
         dec = _decoder()
         dec.prefill(torch.randn(1, 5, 16), [0])
         assert _captured_step(monkeypatch, dec, torch.randn(1, 1, 16), [0])["q"].shape == (1, 2, 8)
+
+
+def test_tables_built_in_inference_mode_serve_training_too():
+    m = _decoder().attn
+    with torch.inference_mode():
+        first = m.tables(torch.device("cpu"))
+    assert not any(t.is_inference() for t in m.tables(torch.device("cpu")))
+    assert all(a is b for a, b in zip(first, m.tables(torch.device("cpu"))))
