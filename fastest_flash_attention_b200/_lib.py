@@ -318,8 +318,17 @@ def check_device_errors(device: torch.device | None = None) -> None:
 
 
 def require_cuda(*ts: torch.Tensor) -> None:
+    """Raise unless the tensors (those that are not None) are on one GPU."""
+    one = None
     for t in ts:
-        if t is not None and not t.is_cuda:
+        if t is None:
+            continue
+        at = t.get_device()  # -1: on the CPU
+        if at < 0:
             raise RuntimeError(
                 "fastest_flash_attention_b200 runs only on CUDA tensors (sm_100a); got a tensor on "
                 f"{t.device}. There is no CPU fallback.")
+        if one is None:
+            one = at
+        elif at != one:
+            raise ValueError(f"all operands must be on one device, got cuda:{one} and cuda:{at}")

@@ -87,8 +87,9 @@ def _id_pair(src: Ids, dst: Ids, limit: int, device: torch.device, what: str) ->
     host are checked: each in [0, limit), destinations distinct and none of
     them a source.  Ids on the device are taken as they are (the kernels skip
     and report those outside the pool)."""
-    if (isinstance(src, torch.Tensor) and isinstance(dst, torch.Tensor) and src.is_cuda and dst.is_cuda
-            and src.dtype is torch.int32 and dst.dtype is torch.int32 and src.dim() == dst.dim() == 1
+    if (isinstance(src, torch.Tensor) and isinstance(dst, torch.Tensor) and src.is_cuda
+            and src.device == device == dst.device and src.dtype is torch.int32 and dst.dtype is torch.int32
+            and src.dim() == dst.dim() == 1
             and src.numel() == dst.numel()):  # nothing to convert, nothing to check on the host
         return src.contiguous(), dst.contiguous()
     pair = []

@@ -172,7 +172,7 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], cos: torch.Tensor, 
         if positions < 0 or positions + S > cos.shape[0]:
             raise ValueError(f"positions [{positions}, {positions + S}) are outside the tables' {cos.shape[0]}")
         positions = torch.arange(positions, positions + S, dtype=torch.int32, device=q.device)
-    _lib.require_cuda(positions)
+    _lib.require_cuda(q, positions)
     if positions.dtype not in _POS64 or tuple(positions.shape) not in ((S,), (B, S)):
         raise ValueError(f"positions must be int32 or int64 [S] or [B, S], got {positions.dtype} "
                          f"{tuple(positions.shape)}")
