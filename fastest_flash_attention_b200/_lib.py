@@ -215,6 +215,15 @@ def direct():
     return _CALL
 
 
+def int32(t: torch.Tensor, limit: int = 2 ** 31 - 1) -> torch.Tensor:
+    """Contiguous int32 form of ids or lengths below `limit`; 64-bit values
+    outside [0, limit) become one outside too (-1 or limit, which the kernels
+    report) instead of wrapping into it."""
+    if t.dtype is torch.int64:
+        t = t.clamp(-1, limit)
+    return t if t.dtype is torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+
+
 def register(name: str, restype, argtypes) -> None:
     SIGNATURES[name] = (restype, argtypes)
     if _LIB is not None:

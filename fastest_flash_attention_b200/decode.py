@@ -119,10 +119,6 @@ def paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     return (out, lse) if return_lse else out
 
 
-def _int32(t: torch.Tensor) -> torch.Tensor:
-    return t if t.dtype is torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
-
-
 def _window_decode(q, k_pages, v_pages, block_table, ctx_lens, scale, softcap, return_lse, max_ctx, window, sinks):
     _lib.require_cuda(q, k_pages, v_pages, block_table, ctx_lens)
     if q.dim() != 3 or k_pages.dim() != 4:
@@ -142,7 +138,7 @@ def _window_decode(q, k_pages, v_pages, block_table, ctx_lens, scale, softcap, r
         raise ValueError("page pools must be contiguous")
     if block_table.dim() != 2 or ctx_lens.dim() != 1 or block_table.shape[0] != R or ctx_lens.shape[0] != R:
         raise ValueError("block_table must be [R, max_pages] and ctx_lens [R]")
-    bt, lens = _int32(block_table), _int32(ctx_lens)
+    bt, lens = _lib.int32(block_table), _lib.int32(ctx_lens)
     sr, sh, sd = q.stride()
     if sd != 1 or (sr | sh) % 2 or q.data_ptr() % 4:
         q = q.contiguous()

@@ -107,8 +107,9 @@ def _id_pair(src: Ids, dst: Ids, limit: int, device: torch.device, what: str) ->
             raise ValueError(f"{what} {bad[0]} is outside [0, {limit})")
         if len(set(d)) < len(d) or not set(s).isdisjoint(d):
             raise ValueError(f"destination {what}s must be distinct and none of them a source")
-    out = [t.to(device, torch.int32) for t in pair]
-    return tuple(t if t.is_contiguous() else t.contiguous() for t in out)
+    if limit > 2 ** 31 - 1 and any(t.dtype is torch.int64 for t in pair):
+        raise ValueError(f"{what}s are 32-bit numbers: a pool of {limit} takes int32 ones alone")
+    return tuple(_lib.int32(t, limit).to(device) for t in pair)
 
 
 def _check_pools(k_pages: torch.Tensor, v_pages: Optional[torch.Tensor]) -> None:

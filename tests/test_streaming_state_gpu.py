@@ -1,0 +1,37 @@
+"""The streaming operators at arguments of unusual type, layout or size on the
+GPU: the same results, bit for bit, as the ordinary form of the same call."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _pools(P=8, Hkv=2, page=16, D=64, dtype=torch.bfloat16, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return tuple(torch.randn(P, Hkv, page, D, generator=g, device="cuda").to(dtype) for _ in range(2))
+
+
+def _reports(call):
+    """Whether the call's bad ids were reported (tests read the error word after every call)."""
+    with pytest.raises(RuntimeError, match="FFA_ERR_INVALID_ARG"):
+        call()
+
+
+@pytest.mark.parametrize("bad", [2 ** 32 + 5, 2 ** 33, -2 ** 32 + 5, 2 ** 31, 2 ** 62])
+def test_64_bit_ids_do_not_wrap(bad):
+    """An id outside 32 bits must not turn into one inside the pool."""
+    import fastest_flash_attention_b200 as ffa
+    k, v = _pools()
+    k0, v0 = k.clone(), v.clone()
+    for fn in (ffa.copy_pages, ffa.move_tokens):
+        for src, dst in (([bad, 1], [2, 3]), ([1, 2], [3, bad])):
+            _reports(lambda: fn(k, v, torch.tensor(src, device="cuda"), torch.tensor(dst, device="cuda")))
+    # only what the good ids name has changed: page 2 or 3 (pages), token 2 or 3 of page 0 (tokens)
+    for now, then in ((k, k0), (v, v0)):
+        assert torch.equal(now[4:], then[4:]) and torch.equal(now[1], then[1]) and torch.equal(now[0, :, 4:], then[0, :, 4:])
+    q = torch.randn(1, 4, 64, device="cuda").to(torch.bfloat16)
+    bt, lens = torch.tensor([[1, 2]], device="cuda"), torch.tensor([20], device="cuda")
+    want = ffa.paged_decode(q, k, v, bt.int(), lens.int(), sliding_window=8, sink_tokens=2)
+    assert torch.equal(ffa.paged_decode(q, k, v, bt, lens, sliding_window=8, sink_tokens=2), want)
+    _reports(lambda: ffa.paged_decode(q, k, v, torch.tensor([[1, bad]], device="cuda"), lens, sliding_window=8))
+    _reports(lambda: ffa.paged_decode(q, k, v, bt, torch.tensor([bad], device="cuda"), sliding_window=8))
