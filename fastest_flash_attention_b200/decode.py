@@ -141,7 +141,8 @@ def _window_decode(q, k_pages, v_pages, block_table, ctx_lens, scale, softcap, r
     bt, lens = _lib.int32(block_table), _lib.int32(ctx_lens)
     sr, sh, sd = q.stride()
     if sd != 1 or (sr | sh) % 2 or q.data_ptr() % 4:
-        q = q.contiguous()
+        # (contiguous() keeps a tensor whose axes of one element have odd strides, or whose base is odd)
+        q = q.clone(memory_format=torch.contiguous_format)
         sr, sh, _ = q.stride()
     if scale is None:
         scale = 1.0 / math.sqrt(D)

@@ -35,3 +35,20 @@ def test_64_bit_ids_do_not_wrap(bad):
     assert torch.equal(ffa.paged_decode(q, k, v, bt, lens, sliding_window=8, sink_tokens=2), want)
     _reports(lambda: ffa.paged_decode(q, k, v, torch.tensor([[1, bad]], device="cuda"), lens, sliding_window=8))
     _reports(lambda: ffa.paged_decode(q, k, v, bt, torch.tensor([bad], device="cuda"), sliding_window=8))
+
+
+@pytest.mark.parametrize("form", ["odd strides", "odd base"])
+def test_decode_of_queries_that_only_look_contiguous(form):
+    """A tensor of one row counts as contiguous whatever its outer strides are, and at any address."""
+    import fastest_flash_attention_b200 as ffa
+    k, v = _pools(Hkv=1)
+    bt = torch.tensor([[1, 2]], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([20], dtype=torch.int32, device="cuda")
+    src = torch.randn(1, 1, 64, device="cuda").to(torch.bfloat16)
+    if form == "odd strides":
+        q = torch.empty(200, dtype=torch.bfloat16, device="cuda").as_strided((1, 1, 64), (67, 65, 1)).copy_(src)
+    else:
+        q = torch.empty(65, dtype=torch.bfloat16, device="cuda")[1:].view(1, 1, 64).copy_(src)
+    assert q.is_contiguous()
+    want = ffa.paged_decode(src, k, v, bt, lens, sliding_window=8, sink_tokens=2)
+    assert torch.equal(ffa.paged_decode(q, k, v, bt, lens, sliding_window=8, sink_tokens=2), want)
