@@ -72,6 +72,9 @@ def _tma_ready(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     sb, sh, ss, sd = t.stride()
     if sd != 1 or (sb | sh | ss) % 8 or t.data_ptr() % 16 or not (sb and sh and ss):
         t = t.contiguous()
+        sb, sh, ss, _ = t.stride()
+        if (sb | sh | ss) % 8 or t.data_ptr() % 16:  # axes of one element and the base do not count for contiguous()
+            t = t.clone(memory_format=torch.contiguous_format)
     return t
 
 

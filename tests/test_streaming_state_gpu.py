@@ -52,3 +52,25 @@ def test_decode_of_queries_that_only_look_contiguous(form):
     assert q.is_contiguous()
     want = ffa.paged_decode(src, k, v, bt, lens, sliding_window=8, sink_tokens=2)
     assert torch.equal(ffa.paged_decode(q, k, v, bt, lens, sliding_window=8, sink_tokens=2), want)
+
+
+@pytest.mark.parametrize("form", ["odd strides", "zero strides", "odd base"])
+def test_attention_of_operands_that_only_look_contiguous(form):
+    from fastest_flash_attention_b200 import fastest_flash_attn_func
+    g = torch.Generator(device="cuda").manual_seed(1)
+    src = [torch.randn(1, 1, 40, 64, generator=g, device="cuda").to(torch.bfloat16) for _ in range(4)]
+
+    def odd(t):
+        if form == "odd strides":
+            return torch.empty(4000, dtype=t.dtype, device="cuda").as_strided(t.shape, (2601, 2567, 64, 1)).copy_(t)
+        if form == "zero strides":
+            return torch.empty(4000, dtype=t.dtype, device="cuda").as_strided(t.shape, (0, 0, 64, 1)).copy_(t)
+        return torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")[1:].view(t.shape).copy_(t)
+
+    def run(q, k, v, do, **kw):
+        q, k, v = (t.detach().requires_grad_() for t in (q, k, v))
+        o = fastest_flash_attn_func(q, k, v, causal=True, sliding_window=16, **kw)
+        return (o,) + torch.autograd.grad(o, (q, k, v), do)
+    for kw in (dict(sink_tokens=3), dict()):
+        for a, b in zip(run(*map(odd, src), **kw), run(*src, **kw)):
+            assert torch.equal(a, b)
