@@ -1362,6 +1362,7 @@ extern "C" size_t ffa_bwd_sink_workspace_size(int B, int Hq, int Hkv, int Sq, in
                                               int sinks) {
   // sizes that ffa_bwd_sink refuses: nothing to size (and nothing to divide by)
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || Sq <= 0 || Skv <= 0 || window <= 0 || sinks <= 0) return 0;
+  window = ffa::bounded_window(window);
   // fp32 sums: of the tensor-core kernels' 128-key tiles, or of the fp32 kernels' 64-key ones
   int tiles = 0, parts = 0;
   ffa::bwd_sink_shape(ffa::BWD_BT, Sq, Skv, window, sinks, tiles, parts);
@@ -1383,6 +1384,7 @@ static int bwd_impl(const void* dout, const void* q, const void* k, const void* 
                     int window, int sink, float softcap, const uint8_t* block_mask, int n_br, int n_bc, int mask_bq,
                     int mask_bkv, void* workspace, size_t workspace_bytes, uint32_t* dev_err, void* stream) {
   if (sink > Skv) sink = Skv;
+  window = bounded_window(window);
   if (!dout || !q || !k || !v || !o || !lse || !dq || !dk || !dv) return FFA_ERR_INVALID_ARG;
   if (block_mask && (n_br <= 0 || n_bc <= 0 || mask_bq <= 0 || mask_bkv <= 0 ||
                      (int64_t)n_br * mask_bq < Sq || (int64_t)n_bc * mask_bkv < Skv))

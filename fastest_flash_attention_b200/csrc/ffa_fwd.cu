@@ -901,6 +901,7 @@ static int fwd_impl(const void* q, const void* k, const void* v, void* o, float*
                     int window, int sink, float softcap, const uint8_t* block_mask, int n_br, int n_bc, int mask_bq,
                     int mask_bkv, uint32_t* dev_err, void* stream) {
   if (sink > Skv) sink = Skv;
+  window = bounded_window(window);
   if (!q || !k || !v || !o || !q_strides || !k_strides || !v_strides || !o_strides) return FFA_ERR_INVALID_ARG;
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || Sq <= 0 || Skv < 0 || Hq % Hkv != 0) return FFA_ERR_INVALID_ARG;
   int KD = 0, KV = 0;

@@ -66,6 +66,9 @@ int f32_bwd(const void* dout, const void* q, const void* k, const void* v, const
             int window, int sink, float softcap, const uint8_t* block_mask, int n_br, int n_bc, int mask_bq, int mask_bkv,
             void* workspace, float* sink_ws, void* stream);
 
+// A window past any length: the kernels add positions to it in 32 bits.
+inline int bounded_window(int window) { return window < (1 << 30) ? window : 1 << 30; }
+
 // Head dims of the attention kernel that serves (D, Dv).  The sink kernels take
 // any multiples of 8 up to (192, 128): their TMA copies read zeros past the
 // true head dim and write nothing there, so narrower heads run on the next

@@ -74,3 +74,39 @@ def test_attention_of_operands_that_only_look_contiguous(form):
     for kw in (dict(sink_tokens=3), dict()):
         for a, b in zip(run(*map(odd, src), **kw), run(*src, **kw)):
             assert torch.equal(a, b)
+
+
+def _sink_call(lib, _lib, q, k, v, window, sinks, do=None, skv=None):
+    """ffa_fwd_sink (and, with do, ffa_bwd_sink) through the C entry points."""
+    B, Hq, Sq, D = q.shape
+    Hkv, Skv, Dv = k.shape[1], k.shape[2] if skv is None else skv, v.shape[3]
+    o = torch.empty(B, Hq, Sq, Dv, dtype=q.dtype, device="cuda")
+    lse = torch.empty(B, Hq, Sq, device="cuda")
+    st = [_lib.strides3(t) for t in (q, k, v, o)]
+    stream = _lib.stream_of(q)
+    sizes = (_lib.DTYPE_CODE[q.dtype], B, Hq, Hkv, Sq, Skv, D, Dv)
+    _lib.check(lib.ffa_fwd_sink(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), *sizes, *st,
+                                0.125, 1, 0, window, sinks, 0.0, None, stream), "ffa_fwd_sink")
+    if do is None:
+        return o, lse
+    grads = [torch.empty_like(t) for t in (q, k, v)]
+    ws = torch.empty(lib.ffa_bwd_sink_workspace_size(B, Hq, Hkv, Sq, Skv, D, Dv, window, sinks), dtype=torch.uint8,
+                     device="cuda")
+    _lib.check(lib.ffa_bwd_sink(
+        do.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(),
+        *(t.data_ptr() for t in grads), *sizes, *st, _lib.strides3(do), *map(_lib.strides3, grads), 0.125, 1, 0, window,
+        sinks, 0.0, ws.data_ptr(), ws.numel(), None, stream), "ffa_bwd_sink")
+    return (o, lse, *grads)
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 100, 2 ** 30 + 1])
+def test_c_entry_points_with_windows_near_2_31(window):
+    """A window past every length hides nothing: the same as one of 2^20."""
+    from fastest_flash_attention_b200 import _lib
+    g = torch.Generator(device="cuda").manual_seed(2)
+    q, k, v, do = (torch.randn(1, 2, 300, 64, generator=g, device="cuda").to(torch.bfloat16) for _ in range(4))
+    lib = _lib.load()
+    want = _sink_call(lib, _lib, q, k, v, 2 ** 20, 4, do)
+    assert bool(want[3][0, :, 4:].any(-1).all())  # every key has a gradient
+    for a, b in zip(_sink_call(lib, _lib, q, k, v, window, 4, do), want):
+        assert torch.equal(a, b)
