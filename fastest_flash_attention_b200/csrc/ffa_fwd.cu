@@ -900,12 +900,13 @@ static int fwd_impl(const void* q, const void* k, const void* v, void* o, float*
                     const int64_t* v_strides, const int64_t* o_strides, float scale, int causal, int q_offset,
                     int window, int sink, float softcap, const uint8_t* block_mask, int n_br, int n_bc, int mask_bq,
                     int mask_bkv, uint32_t* dev_err, void* stream) {
+  const bool sinks = sink > 0;  // which kernels (with no keys there is no sink either, but any of their head dims)
   if (sink > Skv) sink = Skv;
   window = bounded_window(window);
   if (!q || !k || !v || !o || !q_strides || !k_strides || !v_strides || !o_strides) return FFA_ERR_INVALID_ARG;
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || Sq <= 0 || Skv < 0 || Hq % Hkv != 0) return FFA_ERR_INVALID_ARG;
   int KD = 0, KV = 0;
-  if (!attention_tile(D, Dv, sink > 0 && dtype != FFA_DTYPE_F32, KD, KV)) return FFA_ERR_UNSUPPORTED;
+  if (!attention_tile(D, Dv, sinks && dtype != FFA_DTYPE_F32, KD, KV)) return FFA_ERR_UNSUPPORTED;
   if (dtype != FFA_DTYPE_BF16 && dtype != FFA_DTYPE_F16 && dtype != FFA_DTYPE_F32) return FFA_ERR_UNSUPPORTED;
   if (Skv > 65535 * FWD_BN) return FFA_ERR_UNSUPPORTED;
   // with a block mask a CTA records its kept key tiles in shared memory
@@ -962,7 +963,7 @@ static int fwd_impl(const void* q, const void* k, const void* v, void* o, float*
   if (!st)
     st = make_tmap_4d(&mv, v, dt, 2, Dv, skv_map, Hkv, B, v_strides[2] * 2, v_strides[1] * 2, v_strides[0] * 2, 64,
                       FWD_BN);
-  if (!st && sink > 0)  // O by TMA: one 32-row x 64-column box per warp and block of columns
+  if (!st && sinks)  // O by TMA: one 32-row x 64-column box per warp and block of columns
     st = make_tmap_4d(&mo, o, dt, 2, Dv, Sq, Hq, B, o_strides[2] * 2, o_strides[1] * 2, o_strides[0] * 2, 64, 32);
   if (st) return st;
 
@@ -985,7 +986,7 @@ static int fwd_impl(const void* q, const void* k, const void* v, void* o, float*
     };
     return dtype == FFA_DTYPE_BF16 ? typed(__nv_bfloat16{}) : typed(__half{});
   };
-  return sink > 0 ? run(std::true_type{}) : run(std::false_type{});
+  return sinks ? run(std::true_type{}) : run(std::false_type{});
 }
 
 }  // namespace ffa

@@ -110,3 +110,12 @@ def test_c_entry_points_with_windows_near_2_31(window):
     assert bool(want[3][0, :, 4:].any(-1).all())  # every key has a gradient
     for a, b in zip(_sink_call(lib, _lib, q, k, v, window, 4, do), want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("D,Dv", [(64, 64), (40, 24), (136, 72)])
+def test_c_forward_of_no_keys(D, Dv):
+    """No key: 0 and -inf, at every head dim that the entry point takes."""
+    from fastest_flash_attention_b200 import _lib
+    q, k, v = (torch.randn(1, 2, 8, d, device="cuda").to(torch.bfloat16) for d in (D, D, Dv))
+    o, lse = _sink_call(_lib.load(), _lib, q, k, v, 4, 2, skv=0)
+    assert not bool(o.any()) and bool((lse == -float("inf")).all())
