@@ -1540,7 +1540,10 @@ extern "C" int ffa_bwd_sink(const void* dout, const void* q, const void* k, cons
                             const int64_t* dq_strides, const int64_t* dk_strides, const int64_t* dv_strides,
                             float scale, int causal, int q_offset, int window, int sinks, float softcap,
                             void* workspace, size_t workspace_bytes, uint32_t* dev_err, void* stream) {
-  if (window <= 0 || sinks < 0) return FFA_ERR_INVALID_ARG;
+  if (window <= 0 || sinks <= 0) {
+    ffa::set_last_error("ffa_bwd_sink takes a positive window and sinks (ffa_bwd serves the rest)");
+    return FFA_ERR_INVALID_ARG;
+  }
   return ffa::bwd_impl(dout, q, k, v, o, lse, dq, dk, dv, dtype, B, Hq, Hkv, Sq, Skv, D, Dv, q_strides, k_strides,
                        v_strides, o_strides, do_strides, dq_strides, dk_strides, dv_strides, scale, causal, q_offset,
                        window, sinks, softcap, nullptr, 0, 0, 0, 0, workspace, workspace_bytes, dev_err, stream);

@@ -136,9 +136,11 @@ int ffa_bwd_masked(const void* dout, const void* q, const void* k, const void* v
  * are visible outside the window too, as far as causality allows:
  *   j visible iff (j <= i + q_offset if causal) and
  *                 (j >= i + q_offset - window + 1 or j < sinks).
- * Same types, shapes, strides, softcap and determinism (no block mask); D and
- * Dv may be any multiples of 8 up to (192, 128) in the 16-bit types.  The
- * backward's workspace comes from ffa_bwd_sink_workspace_size: a sink sees
+ * Same types, shapes, strides, softcap and determinism (no block mask); with
+ * sinks > 0, D and Dv may be any multiples of 8 up to (192, 128) in the 16-bit
+ * types.  ffa_fwd_sink takes sinks = 0 too (ffa_fwd's result); ffa_bwd_sink
+ * does not, its gradients are ffa_bwd's.  The backward's workspace comes from
+ * ffa_bwd_sink_workspace_size (0 for sizes that the call refuses): a sink sees
  * every later query, so the queries of the key tiles that hold sinks are
  * shared by several CTAs, whose fp32 sums one more launch adds up in order.
  * ------------------------------------------------------------------------- */
