@@ -82,6 +82,7 @@ SIGNATURES: dict[str, tuple] = {
         _c_float, _c_int, _c_int, _c_int, _c_int, _c_float,  # scale causal q_offset window sinks softcap
         _c_u32p, _c_void_p,  # err stream
     ]),
+    "ffa_bwd_sink_workspace_size_of": (_c_size_t, [_c_int] * 10),  # dtype, then as below
     "ffa_bwd_sink_workspace_size": (_c_size_t, [_c_int] * 9),  # B Hq Hkv Sq Skv D Dv window sinks
     "ffa_bwd_sink": (_c_int, [
         _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,  # dout q k v o lse

@@ -249,7 +249,7 @@ def fastest_flash_attn_forward(
 
 @functools.lru_cache(maxsize=1024)
 def _sink_workspace(*sizes: int) -> int:
-    return _lib.load().ffa_bwd_sink_workspace_size(*sizes)
+    return _lib.load().ffa_bwd_sink_workspace_size_of(*sizes)
 
 
 def flash_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor,
@@ -297,7 +297,7 @@ def flash_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Ten
     dv = torch.empty_like(v)
     lib = _lib.load()
     if sink:
-        ws_bytes = _sink_workspace(B, Hq, Hkv, Sq, Skv, D, Dv, window, sink)
+        ws_bytes = _sink_workspace(_ATTN_DTYPE_CODE[dt], B, Hq, Hkv, Sq, Skv, D, Dv, window, sink)
     else:
         ws_bytes = lib.ffa_bwd_workspace_size(B, Hq, Sq)
     ws = q.new_empty(ws_bytes, dtype=torch.uint8)

@@ -1358,20 +1358,31 @@ extern "C" size_t ffa_bwd_workspace_size(int B, int Hq, int Sq) {
   return 2 * (size_t)B * Hq * sq_pad * sizeof(float) + 256;
 }
 
-extern "C" size_t ffa_bwd_sink_workspace_size(int B, int Hq, int Hkv, int Sq, int Skv, int D, int Dv, int window,
-                                              int sinks) {
+extern "C" size_t ffa_bwd_sink_workspace_size_of(int dtype, int B, int Hq, int Hkv, int Sq, int Skv, int D, int Dv,
+                                                 int window, int sinks) {
   // sizes that ffa_bwd_sink refuses: nothing to size (and nothing to divide by)
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || Sq <= 0 || Skv <= 0 || window <= 0 || sinks <= 0) return 0;
+  if (dtype != FFA_DTYPE_BF16 && dtype != FFA_DTYPE_F16 && dtype != FFA_DTYPE_F32) return 0;
+  const bool f32 = dtype == FFA_DTYPE_F32;
+  int KD = 0, KV = 0;  // the sums are kept at the tile's width
+  if (!ffa::attention_tile(D, Dv, !f32, KD, KV)) return 0;
   window = ffa::bounded_window(window);
-  // fp32 sums: of the tensor-core kernels' 128-key tiles, or of the fp32 kernels' 64-key ones
+  const size_t stats = ffa_bwd_workspace_size(B, Hq, Sq);
   int tiles = 0, parts = 0;
-  ffa::bwd_sink_shape(ffa::BWD_BT, Sq, Skv, window, sinks, tiles, parts);
-  size_t rows = (size_t)tiles * parts * ffa::BWD_BT;
-  ffa::f32_bwd_sink_shape(B, Hq, Hkv, Sq, Skv, window, sinks, tiles, parts);
-  if ((size_t)tiles * parts * 64 > rows) rows = (size_t)tiles * parts * 64;
-  int KD = D, KV = Dv;
-  ffa::attention_tile(D, Dv, true, KD, KV);  // sums are kept at the tile's width
-  return ffa_bwd_workspace_size(B, Hq, Sq) + 16 + (size_t)B * Hkv * rows * ((size_t)KD + KV) * sizeof(float);
+  if (f32)
+    ffa::f32_bwd_sink_shape(B, Hq, Hkv, Sq, Skv, window, sinks, tiles, parts);
+  else
+    ffa::bwd_sink_shape(ffa::BWD_BT, Sq, Skv, window, sinks, tiles, parts);
+  if (parts <= 1) return stats;  // nothing is shared
+  const size_t rows = (size_t)tiles * parts * (f32 ? 64 : ffa::BWD_BT);
+  return stats + 16 + (size_t)B * Hkv * rows * ((size_t)KD + KV) * sizeof(float);
+}
+
+extern "C" size_t ffa_bwd_sink_workspace_size(int B, int Hq, int Hkv, int Sq, int Skv, int D, int Dv, int window,
+                                              int sinks) {
+  const size_t half = ffa_bwd_sink_workspace_size_of(FFA_DTYPE_F16, B, Hq, Hkv, Sq, Skv, D, Dv, window, sinks);
+  const size_t f32 = ffa_bwd_sink_workspace_size_of(FFA_DTYPE_F32, B, Hq, Hkv, Sq, Skv, D, Dv, window, sinks);
+  return half > f32 ? half : f32;
 }
 
 namespace ffa {
@@ -1398,7 +1409,7 @@ static int bwd_impl(const void* dout, const void* q, const void* k, const void* 
   if (dtype != FFA_DTYPE_BF16 && dtype != FFA_DTYPE_F16 && dtype != FFA_DTYPE_F32) return FFA_ERR_UNSUPPORTED;
   const size_t stats = ffa_bwd_workspace_size(B, Hq, Sq);
   const size_t need =
-      sink > 0 ? ffa_bwd_sink_workspace_size(B, Hq, Hkv, Sq, Skv, D, Dv, window, sink) : stats;
+      sink > 0 ? ffa_bwd_sink_workspace_size_of(dtype, B, Hq, Hkv, Sq, Skv, D, Dv, window, sink) : stats;
   if (!workspace || workspace_bytes < need) return FFA_ERR_WORKSPACE;
   float* sink_ws = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(workspace) + stats + 15) & ~uintptr_t(15));
   if (dtype == FFA_DTYPE_F32)

@@ -139,16 +139,19 @@ int ffa_bwd_masked(const void* dout, const void* q, const void* k, const void* v
  * Same types, shapes, strides, softcap and determinism (no block mask); with
  * sinks > 0, D and Dv may be any multiples of 8 up to (192, 128) in the 16-bit
  * types.  ffa_fwd_sink takes sinks = 0 too (ffa_fwd's result); ffa_bwd_sink
- * does not, its gradients are ffa_bwd's.  The backward's workspace comes from
- * ffa_bwd_sink_workspace_size (0 for sizes that the call refuses): a sink sees
- * every later query, so the queries of the key tiles that hold sinks are
- * shared by several CTAs, whose fp32 sums one more launch adds up in order.
+ * does not, its gradients are ffa_bwd's.  A sink sees every later query, so
+ * the queries of the key tiles that hold sinks are shared by several CTAs,
+ * whose fp32 sums one more launch adds up in order: the backward's workspace
+ * is ffa_bwd_sink_workspace_size_of for one type, ffa_bwd_sink_workspace_size
+ * for any (0 for sizes that the call refuses).
  * ------------------------------------------------------------------------- */
 int ffa_fwd_sink(const void* q, const void* k, const void* v, void* o, float* lse, int dtype, int B, int Hq,
                  int Hkv, int Sq, int Skv, int D, int Dv, const int64_t* q_strides, const int64_t* k_strides,
                  const int64_t* v_strides, const int64_t* o_strides, float scale, int causal, int q_offset,
                  int window, int sinks, float softcap, uint32_t* dev_err, void* stream);
 
+size_t ffa_bwd_sink_workspace_size_of(int dtype, int B, int Hq, int Hkv, int Sq, int Skv, int D, int Dv, int window,
+                                      int sinks);
 size_t ffa_bwd_sink_workspace_size(int B, int Hq, int Hkv, int Sq, int Skv, int D, int Dv, int window, int sinks);
 
 int ffa_bwd_sink(const void* dout, const void* q, const void* k, const void* v, const void* o, const float* lse,

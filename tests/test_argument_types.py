@@ -20,7 +20,7 @@ class _Signatures:
                 if not isinstance(a, tuple):
                     t.from_param(a)
             self.last = name, args
-            return 1 << 10 if name.endswith("workspace_size") else _lib.FFA_OK
+            return 1 << 10 if "workspace_size" in name else _lib.FFA_OK
         return call
 
 

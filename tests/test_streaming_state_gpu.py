@@ -119,3 +119,30 @@ def test_c_forward_of_no_keys(D, Dv):
     q, k, v = (torch.randn(1, 2, 8, d, device="cuda").to(torch.bfloat16) for d in (D, D, Dv))
     o, lse = _sink_call(_lib.load(), _lib, q, k, v, 4, 2, skv=0)
     assert not bool(o.any()) and bool((lse == -float("inf")).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("B,Hq,Hkv,S,D,Dv,window,sinks", [
+    (1, 8, 1, 1024, 128, 128, 256, 4), (1, 4, 2, 216, 64, 64, 48, 4), (2, 2, 2, 1300, 64, 64, 100, 300),
+    (1, 2, 1, 640, 192, 128, 65, 700), (1, 2, 2, 5000, 64, 64, 50, 4500)])
+def test_backward_stays_inside_its_workspace(B, Hq, Hkv, S, D, Dv, window, sinks, dtype):
+    """Nothing past the bytes that the size function of the type names is written."""
+    from fastest_flash_attention_b200 import _lib, attention
+    lib = _lib.load()
+    g = torch.Generator(device="cuda").manual_seed(S)
+    q, k, v, do = (torch.randn(B, h, S, d, generator=g, device="cuda").to(dtype)
+                   for h, d in ((Hq, D), (Hkv, D), (Hkv, Dv), (Hq, Dv)))
+    o, lse = attention.flash_fwd(q, k, v, scale=0.125, causal=True, window=window, sink=sinks)
+    want = attention.flash_bwd(do, q, k, v, o, lse, scale=0.125, causal=True, window=window, sink=sinks)
+    sizes = (attention._ATTN_DTYPE_CODE[dtype], B, Hq, Hkv, S, S, D, Dv)
+    size = lib.ffa_bwd_sink_workspace_size_of(*sizes, window, sinks)
+    ws = torch.full((size + 1024,), 0xAB, dtype=torch.uint8, device="cuda")
+    grads = [torch.empty_like(t) for t in (q, k, v)]
+    ts = (q, k, v, o, do, *grads)
+    _lib.check(lib.ffa_bwd_sink(do.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(),
+                                *(t.data_ptr() for t in grads), *sizes, *map(_lib.strides3, ts), 0.125, 1, 0, window,
+                                sinks, 0.0, ws.data_ptr(), size, None, _lib.stream_of(q)), "ffa_bwd_sink")
+    assert bool((ws[size:] == 0xAB).all()) and all(torch.equal(a, b) for a, b in zip(grads, want))
+    assert lib.ffa_bwd_sink(do.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(),
+                            *(t.data_ptr() for t in grads), *sizes, *map(_lib.strides3, ts), 0.125, 1, 0, window,
+                            sinks, 0.0, ws.data_ptr(), size - 1, None, _lib.stream_of(q)) == _lib.FFA_ERR_WORKSPACE
