@@ -136,7 +136,7 @@ def copy_pages(k_pages: torch.Tensor, v_pages: Optional[torch.Tensor], src: Ids,
     with _lib.device_of(k_pages):
         st = _lib.direct().ffa_page_copy(
             k_pages.data_ptr(), v_pages.data_ptr() if v_pages is not None else None, src.data_ptr(), dst.data_ptr(),
-            src.numel(), k_pages.shape[0], k_pages.stride(0) * k_pages.element_size(),
+            src.numel(), k_pages.shape[0], k_pages.numel() // k_pages.shape[0] * k_pages.element_size(),
             _lib.err_ptr(k_pages), _lib.stream_of(k_pages))
     _lib.check(st, "ffa_page_copy")
     if _lib.sync_check_enabled():

@@ -78,3 +78,19 @@ def test_configuration_of_another_class(lib):
     assert lib.last[0] == "ffa_fwd_sink" and lib.last[1][21] == 2
     attention.fastest_flash_attn_forward(*_qkv(), config=AttentionConfig(**fields, sink_tokens=3), sink_tokens=2)
     assert lib.last[0] == "ffa_fwd_sink" and lib.last[1][21] == 3
+
+
+def test_pools_of_one_page(lib):
+    """A single page's stride says nothing about its size."""
+    from fastest_flash_attention_b200 import copy_pages
+    pool = torch.zeros(4096).as_strided((1, 2, 4, 8), (1 << 40, 32, 8, 1))
+    assert pool.is_contiguous()
+    copy_pages(pool, None, torch.zeros(0, dtype=torch.int32), torch.zeros(0, dtype=torch.int32))
+    import fastest_flash_attention_b200.kv_cache as kv
+    ids = torch.zeros(1, dtype=torch.int32)
+    original, kv._id_pair = kv._id_pair, lambda *a: (ids, ids)
+    try:
+        copy_pages(pool, None, ids, ids)
+    finally:
+        kv._id_pair = original
+    assert lib.last[0] == "ffa_page_copy" and lib.last[1][6] == 2 * 4 * 8 * 4
