@@ -124,8 +124,8 @@ def _check_pools(k_pages: torch.Tensor, v_pages: Optional[torch.Tensor]) -> None
 def copy_pages(k_pages: torch.Tensor, v_pages: Optional[torch.Tensor], src: Ids, dst: Ids) -> None:
     """Copy whole pages src[i] -> dst[i] inside the pools, in one launch.
 
-    Pools [P, ...] contiguous, any dtype; v_pages may be None (a latent cache
-    has one pool).  src, dst: page ids, int32 / int64 on the device (or on the
+    Pools [P, ...] contiguous, of any dtype whose page is an even number of
+    bytes; v_pages may be None (a latent cache has one pool).  src, dst: page ids, int32 / int64 on the device (or on the
     host, where they are checked); destinations are distinct and none of them
     is a source.
     """
@@ -149,7 +149,8 @@ def move_tokens(k_pages: torch.Tensor, v_pages: Optional[torch.Tensor], src_slot
     offset.
 
     Pools [P, Hkv, page_size, D], or [P, page_size, D] (a latent cache),
-    contiguous, any dtype; v_pages may be None.  Slots as copy_pages' page ids.
+    contiguous, of any dtype whose row of D is an even number of bytes; v_pages
+    may be None.  Slots as copy_pages' page ids.
     """
     _check_pools(k_pages, v_pages)
     if k_pages.dim() not in (3, 4):

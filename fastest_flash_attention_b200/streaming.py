@@ -1,14 +1,17 @@
-"""Attention for conversations without end: rotary positions, a sliding window
-with the first tokens kept visible, and a paged cache that holds no more than
-both (no counterpart in the reference, whose modules have neither rotary
+"""Attention for long conversations: rotary positions, a sliding window with the
+first tokens kept visible, and a paged cache that holds the pages of both and
+no others (no counterpart in the reference, whose modules have neither rotary
 positions outside MLA nor a cache of their own).
 
 ``FastestFlashStreamingGQA`` trains and prefills; ``StreamingDecoder`` serves
 it: every step is the three projections, one launch that rotates the new
 queries and keys and writes keys and values into their pages, one launch of
 the windowed decode, and the output projection.  Pages that leave the window
-are freed as it goes, so a sequence of any length holds
-window + sinks tokens.
+are freed as it goes, so the pool holds window + sinks tokens of a sequence,
+rounded to pages.  What does grow with a sequence is its page table (an entry
+for every page so far, until ``compact``), and with it a step's host time; and
+positions are absolute, so a sequence ends at ``max_len``, the length of the
+rotary tables, compacted or not.
 """
 from __future__ import annotations
 
