@@ -235,9 +235,22 @@ class PagedKVCache:
     def append_tokens(self, seq_id: int, k_tokens: torch.Tensor, v_tokens: torch.Tensor) -> int:
         """Append [num_heads, S_new, head_dim] K/V; returns the new length (kv_cache.py:170-206)."""
         S_new = k_tokens.size(1)
+        try:  # (axes of one are repeated, as the reference's assignment does)
+            k_tokens, v_tokens = (t.expand(self.num_heads, S_new, self.head_dim) for t in (k_tokens, v_tokens))
+        except RuntimeError:
+            raise ValueError(f"append takes k and v [{self.num_heads}, tokens, {self.head_dim}], got "
+                             f"{tuple(k_tokens.shape)} and {tuple(v_tokens.shape)}") from None
+        new = seq_id not in self.sequences
         slots = self._assign_slots(seq_id, S_new)
-        if S_new > 0:
-            self._write(slots, k_tokens, v_tokens)
+        try:
+            if S_new > 0:
+                self._write(slots, k_tokens, v_tokens)
+        except BaseException:  # nothing is cached that was not written
+            for _ in slots:
+                self._unassign_slot(seq_id)
+            if new:
+                del self.sequences[seq_id]
+            raise
         return self.sequences[seq_id]["len"]
 
     def _append_visible(self, seq_id: int, k_tokens: torch.Tensor, v_tokens: torch.Tensor, sliding_window: int,

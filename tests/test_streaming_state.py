@@ -175,3 +175,34 @@ def test_tables_built_in_inference_mode_serve_training_too():
         first = m.tables(torch.device("cpu"))
     assert not any(t.is_inference() for t in m.tables(torch.device("cpu")))
     assert all(a is b for a, b in zip(first, m.tables(torch.device("cpu"))))
+
+
+@pytest.mark.parametrize("k,v", [((2, 5, 4), (2, 3, 4)), ((2, 3, 4), (2, 5, 4)), ((3, 5, 4), (3, 5, 4)),
+                                 ((2, 5, 3), (2, 5, 3)), ((2, 5, 4), (2, 5, 8))])
+def test_append_of_mismatched_shapes_changes_nothing(k, v):
+    """The kernel reads both by one shape: a shorter one would be read past its end."""
+    c = _cache()
+    c.append_tokens(0, *_tokens(3))
+    before = list(c.free_pages), c.k_pages.clone()
+    with pytest.raises(ValueError, match="append"):
+        c.append_tokens(0, torch.zeros(k), torch.zeros(v))
+    with pytest.raises(ValueError, match="append"):
+        c.append_tokens(1, torch.zeros(k), torch.zeros(v))
+    assert list(c.sequences) == [0] and c.sequences[0]["len"] == 3
+    assert c.free_pages == before[0] and torch.equal(c.k_pages, before[1])
+    c.append_tokens(0, torch.full((1, 2, 4), 7.0), torch.full((2, 1, 4), 8.0))  # repeated over heads, over tokens
+    assert bool((c.get_kv(0)[0][:, 3:] == 7).all()) and bool((c.get_kv(0)[1][:, 3:] == 8).all())
+
+
+def test_append_whose_write_fails_changes_nothing(monkeypatch):
+    c = _cache()
+    c.append_tokens(0, *_tokens(3))
+
+    def fail(*args):
+        raise RuntimeError("refused")
+    monkeypatch.setattr(c, "_write", fail)
+    for s in (0, 1):
+        with pytest.raises(RuntimeError, match="refused"):
+            c.append_tokens(s, *_tokens(9))
+        assert list(c.sequences) == [0] and c.sequences[0] == {"page_table": [0], "len": 3}
+        assert c.free_pages == list(range(1, 8))
