@@ -325,27 +325,25 @@ class PagedKVCache:
                 raise KeyError(f"PagedKVCache: no sequence {s} to fork")
             if d in self.sequences or made.count(d) > 1:
                 raise ValueError(f"PagedKVCache: sequence {d} exists already")
-        parts = sum(self.sequences[s]["len"] % self.page_size != 0 for s, _ in pairs)
-        if parts > len(self.free_pages):
+        old = [self.sequences[s]["page_table"][-1] for s, _ in pairs if self.sequences[s]["len"] % self.page_size]
+        new = self.free_pages[:len(old)]
+        if len(new) < len(old):
             raise RuntimeError("PagedKVCache: out of physical pages")
-        old, new = [], []
-        for s, d in pairs:
-            seq = self.sequences[s]
-            table = list(seq["page_table"])
-            if seq["len"] % self.page_size:
-                old.append(table.pop())
-                new.append(self.allocate_page())
-            for page in table:
-                if page >= 0:
-                    self._more_owners[page] = self._more_owners.get(page, 0) + 1
-            if seq["len"] % self.page_size:
-                table.append(new[-1])
-            self.sequences[d] = dict(seq, page_table=table)
         if old and self.k_pages.is_cuda:
             copy_pages(self.k_pages, self.v_pages, old, new)
         elif old:  # host-side pool
             self.k_pages[new] = self.k_pages[old]
             self.v_pages[new] = self.v_pages[old]
+        for s, d in pairs:
+            seq = self.sequences[s]
+            table = list(seq["page_table"])
+            last = [self.allocate_page()] if seq["len"] % self.page_size else []  # new's pages, in order
+            if last:
+                table.pop()
+            for page in table:
+                if page >= 0:
+                    self._more_owners[page] = self._more_owners.get(page, 0) + 1
+            self.sequences[d] = dict(seq, page_table=table + last)
 
     def _outside(self, n: int, sliding_window: int, sink_tokens: int) -> Tuple[int, int]:
         """Pages [first, last) of n tokens: those without a token of the window or of the first sink_tokens."""
@@ -388,17 +386,15 @@ class PagedKVCache:
             src.append(old[kept // ps] * ps + kept % ps)
             if src[-1].min() < 0:
                 raise RuntimeError(f"PagedKVCache: pages of sequence {s} in this window were freed")
-        if sum(-(-len(kept) // ps) for _, kept in work) > len(self.free_pages):
+        pages = [-(-len(kept) // ps) for _, kept in work]
+        if sum(pages) > len(self.free_pages):
             raise RuntimeError("PagedKVCache: out of physical pages")
-        for (s, kept), _ in zip(work, src):
-            seq = self.sequences[s]
-            fresh = [self.allocate_page() for _ in range(-(-len(kept) // ps))]
+        first = 0
+        for (_, kept), count in zip(work, pages):
+            fresh = np.asarray(self.free_pages[first:first + count], dtype=np.int64)
             at = np.arange(len(kept))
-            dst.append(np.asarray(fresh, dtype=np.int64)[at // ps] * ps + at % ps)
-            seq["old_pages"], seq["page_table"] = seq["page_table"], fresh
-            dropped += seq["len"] - len(kept)
-            seq["dropped"] = seq.get("dropped", 0) + seq["len"] - len(kept)
-            seq["len"] = len(kept)
+            dst.append(fresh[at // ps] * ps + at % ps)
+            first += count
         if work:
             src_t, dst_t = (torch.from_numpy(np.concatenate(x)) for x in (src, dst))
             if self.k_pages.is_cuda:
@@ -406,8 +402,15 @@ class PagedKVCache:
             else:  # host-side pool
                 for pool in (self.k_pages, self.v_pages):
                     pool[dst_t // ps, :, dst_t % ps] = pool[src_t // ps, :, src_t % ps]
-        for s, _ in work:
-            for page in self.sequences[s].pop("old_pages"):
+        old = [self.sequences[s]["page_table"] for s, _ in work]
+        for (s, kept), count in zip(work, pages):
+            seq = self.sequences[s]
+            seq["page_table"] = [self.allocate_page() for _ in range(count)]  # the fresh ones, in order
+            dropped += seq["len"] - len(kept)
+            seq["dropped"] = seq.get("dropped", 0) + seq["len"] - len(kept)
+            seq["len"] = len(kept)
+        for table in old:
+            for page in table:
                 self._release(page)
         return dropped
 

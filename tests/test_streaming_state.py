@@ -206,3 +206,24 @@ def test_append_whose_write_fails_changes_nothing(monkeypatch):
             c.append_tokens(s, *_tokens(9))
         assert list(c.sequences) == [0] and c.sequences[0] == {"page_table": [0], "len": 3}
         assert c.free_pages == list(range(1, 8))
+
+
+@pytest.mark.parametrize("call", ["fork", "compact"])
+def test_fork_or_compaction_whose_copy_fails_changes_nothing(call):
+    c = _cache(pages=12)
+    c.append_tokens(0, *_tokens(30))
+    c.append_tokens(1, *_tokens(6))
+    before = {s: dict(q, page_table=list(q["page_table"])) for s, q in c.sequences.items()}
+    kept, free, v_pages = c.k_pages[:10].clone(), list(c.free_pages), c.v_pages
+    c.v_pages = torch.zeros(1)  # the copy of the values fails
+    with pytest.raises((IndexError, RuntimeError)):
+        c.fork_sequences([(0, 5), (1, 6)]) if call == "fork" else c.compact_sequences([0, 1], 3, 2)
+    c.v_pages = v_pages
+    assert c.sequences == before and c.free_pages == free and not c._more_owners
+    assert torch.equal(c.k_pages[:10], kept)
+    if call == "fork":
+        c.fork_sequences([(0, 5), (1, 6)])
+        assert c.get_kv(5)[0][0, :, 0].tolist() == list(range(30)) and c.get_kv(6)[1][0, :, 0].tolist()[1:] == [-1, -2, -3, -4, -5]
+    else:
+        assert c.compact_sequences([0, 1], 3, 2) == 26
+        assert c.get_kv(0)[0][0, :, 0].tolist() == [0, 1, 27, 28, 29] and c.get_kv(1)[0][0, :, 0].tolist() == [0, 1, 3, 4, 5]
