@@ -210,7 +210,7 @@ def test_append_whose_write_fails_changes_nothing(monkeypatch):
 
 @pytest.mark.parametrize("call", ["fork", "compact"])
 def test_fork_or_compaction_whose_copy_fails_changes_nothing(call):
-    c = _cache(pages=12)
+    c = _cache(pages=16)
     c.append_tokens(0, *_tokens(30))
     c.append_tokens(1, *_tokens(6))
     before = {s: dict(q, page_table=list(q["page_table"])) for s, q in c.sequences.items()}
