@@ -155,6 +155,16 @@ SIGNATURES: dict[str, tuple] = {
         _c_void_p, _c_void_p, _c_void_p, _c_void_p,  # k_pages v_pages src_slots dst_slots
         _c_int, _c_int, _c_int, _c_int, _c_int, _c_u32p, _c_void_p,  # n Hkv page_size num_pages row_bytes err stream
     ]),
+    "ffa_assign_slots": (_c_int, [
+        _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p,  # block_table width lens new ring state
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,  # slots positions starts lens_out state_out
+        _c_int, _c_int, _c_int, _c_int, _c_u32p, _c_void_p,  # R num_pages page_size max_tokens err stream
+    ]),
+    "ffa_release_pages": (_c_int, [
+        _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p,  # block_table width lens done keep
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p,  # ring state lens_out state_out
+        _c_int, _c_int, _c_int, _c_u32p, _c_void_p,  # R num_pages page_size err stream
+    ]),
     "ffa_rotary": (_c_int, [
         _c_void_p, _c_i64p, _c_void_p, _c_i64p, _c_void_p, _c_i64p, _c_void_p, _c_i64p,  # q s qo s k s ko s
         _c_void_p, _c_void_p, ctypes.c_int64, _c_void_p, _c_int, ctypes.c_int64,  # cos sin len pos pos64 pos_sb
@@ -300,6 +310,8 @@ _DATA_ERRORS = {
     0x3E1: "paged decode: a block-table entry is outside [0, num_pages)",
     0x3E2: "page copy: a page id or token slot is outside the pool",
     0x3E3: "rotary: a position is outside the cos / sin tables",
+    0x3E4: "assign_slots: too few free pages, too many tokens, or a length, page id or free list out of range",
+    0x3E5: "release_pages: more pages than places, or a length, page id or free list out of range",
 }
 
 

@@ -57,7 +57,8 @@ const char* ffa_last_error(void);
  * invalid data they find: 0x3E0 a decode context length outside
  * [0, max_pages_per_req * page_size], 0x3E1 a block-table page id outside
  * [0, num_pages), 0x3E2 a page id or slot of a copy outside the pool, 0x3E3 a
- * rotary position outside the tables, 0x1FF a block mask keeping more key tiles than the forward's
+ * rotary position outside the tables, 0x3E4 / 0x3E5 a page assignment /
+ * release that cannot be done, 0x3E6 request boundaries or a prefix that mean nothing, 0x1FF a block mask keeping more key tiles than the forward's
  * tile list holds (the offending loads are skipped; treat the call as failed).
  * ffa_read_error copies it to *out (synchronising `stream`). */
 int ffa_read_error(const uint32_t* dev_err, uint32_t* out, void* stream);
@@ -310,6 +311,33 @@ int ffa_page_copy(void* k_pages, void* v_pages, const int* src, const int* dst, 
 
 int ffa_token_move(void* k_pages, void* v_pages, const int* src_slots, const int* dst_slots, int n, int Hkv,
                    int page_size, int num_pages, int row_bytes, uint32_t* dev_err, void* stream);
+
+/* ----------------------------------------------------------------------------
+ * Block tables and slot maps built from request lengths on the device (no
+ * counterpart in the reference, whose tables are Python lists).  free_pages
+ * [num_pages] is a ring of page ids with free_state = {head, count}: the free
+ * pages are free_pages[(head + i) % num_pages], i < count.  R <= 16384; all
+ * arrays int32, block_table [R, width].  One launch each.
+ *   ffa_assign_slots   new_lens[r] tokens join request r's ctx_lens[r]: pages
+ *     from the ring's head, requests in order, written to the table behind the
+ *     request's own; slots, positions [max_tokens] of the new tokens in order
+ *     (-1 and 0 behind the last), starts [R + 1] their prefix sums,
+ *     ctx_lens_out, free_state_out (either may be the input itself).
+ *   ffa_release_pages  the pages of the rows with done[r] != 0, but those that
+ *     hold the first keep[r] tokens (keep NULL: none), go behind the ring's
+ *     last; ctx_lens_out of those rows is 0.
+ * What cannot be done (too few pages or places, more than max_tokens tokens, a
+ * length outside [0, width * page_size], an id outside the pool) records 0x3E4
+ * / 0x3E5 in *dev_err and changes nothing (slots -1, starts 0).
+ * ------------------------------------------------------------------------- */
+int ffa_assign_slots(int* block_table, int width, const int* ctx_lens, const int* new_lens, const int* free_pages,
+                     const int* free_state, int* slots, int* positions, int* starts, int* ctx_lens_out,
+                     int* free_state_out, int R, int num_pages, int page_size, int max_tokens, uint32_t* dev_err,
+                     void* stream);
+
+int ffa_release_pages(const int* block_table, int width, const int* ctx_lens, const uint8_t* done, const int* keep,
+                      int* free_pages, const int* free_state, int* ctx_lens_out, int* free_state_out, int R,
+                      int num_pages, int page_size, uint32_t* dev_err, void* stream);
 
 /* ----------------------------------------------------------------------------
  * Rotary positions.  The reference's rotary (modules/flash_mla.py:29-52) is a
