@@ -147,6 +147,15 @@ SIGNATURES: dict[str, tuple] = {
         _c_i64p, _c_i64p, _c_float, _c_float,  # q_strides o_strides scale softcap
         _c_int, _c_int, _c_int, _c_u32p, _c_void_p,  # window sinks max_ctx err stream
     ]),
+    "ffa_paged_prefill_workspace_size": (_c_size_t, [_c_int] * 6),  # R T Hq Hkv D max_ctx
+    "ffa_paged_prefill": (_c_int, [
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,  # q k_pages v_pages block_table lens starts
+        _c_void_p, _c_void_p,  # out lse
+        _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,  # dtype R T Hq Hkv D
+        _c_int, _c_int, _c_int,  # num_pages page_size max_pages_per_req
+        _c_i64p, _c_i64p, _c_float, _c_float, _c_int,  # q_strides o_strides scale softcap max_ctx
+        _c_void_p, _c_size_t, _c_u32p, _c_void_p,  # workspace bytes err stream
+    ]),
     "ffa_page_copy": (_c_int, [
         _c_void_p, _c_void_p, _c_void_p, _c_void_p,  # k_pages v_pages src dst
         _c_int, _c_int, ctypes.c_int64, _c_u32p, _c_void_p,  # n num_pages page_bytes err stream
@@ -310,6 +319,7 @@ _DATA_ERRORS = {
     0x3E1: "paged decode: a block-table entry is outside [0, num_pages)",
     0x3E2: "page copy: a page id or token slot is outside the pool",
     0x3E3: "rotary: a position is outside the cos / sin tables",
+    0x3E6: "request boundaries decrease or pass the batch, or a shared prefix's length is out of range",
     0x3E4: "assign_slots: too few free pages, too many tokens, or a length, page id or free list out of range",
     0x3E5: "release_pages: more pages than places, or a length, page id or free list out of range",
 }

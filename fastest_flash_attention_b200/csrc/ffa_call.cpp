@@ -109,11 +109,11 @@ struct Arg<const int64_t*> {
 // The entry points, in the order of their slots.
 enum Slot {
   FWD_SINK, BWD_SINK, WINDOW_DECODE, ROTARY, ROTARY_APPEND, PAGE_COPY, TOKEN_MOVE, ASSIGN_SLOTS,
-  RELEASE_PAGES, SLOTS
+  RELEASE_PAGES, PAGED_PREFILL, SLOTS
 };
 const char* const kNames[SLOTS] = {"ffa_fwd_sink",      "ffa_bwd_sink",  "ffa_window_decode", "ffa_rotary",
                                    "ffa_rotary_append", "ffa_page_copy", "ffa_token_move",    "ffa_assign_slots",
-                                   "ffa_release_pages"};
+                                   "ffa_release_pages", "ffa_paged_prefill"};
 void* g_fn[SLOTS];
 
 template <int ID, typename F>
@@ -168,6 +168,7 @@ PyMethodDef kMethods[] = {FFA_ENTRY(FWD_SINK, ffa_fwd_sink),
                           FFA_ENTRY(TOKEN_MOVE, ffa_token_move),
                           FFA_ENTRY(ASSIGN_SLOTS, ffa_assign_slots),
                           FFA_ENTRY(RELEASE_PAGES, ffa_release_pages),
+                          FFA_ENTRY(PAGED_PREFILL, ffa_paged_prefill),
                           {"bind", bind, METH_VARARGS, "bind(name, address)"},
                           {nullptr, nullptr, 0, nullptr}};
 #undef FFA_ENTRY

@@ -34,7 +34,7 @@ static EncodeTiledFn encode_fn() {
 
 int make_tmap_4d(CUtensorMap* map, const void* base, CUtensorMapDataType dt, uint32_t elem_bytes, uint64_t d0,
                  uint64_t d1, uint64_t d2, uint64_t d3, uint64_t s1_bytes, uint64_t s2_bytes, uint64_t s3_bytes,
-                 uint32_t b0, uint32_t b1) {
+                 uint32_t b0, uint32_t b1, uint32_t b2) {
   // The driver-level encode needs the device's primary context current on
   // this thread (host threads such as autograd workers may not have it yet).
   int dev = 0;
@@ -53,7 +53,7 @@ int make_tmap_4d(CUtensorMap* map, const void* base, CUtensorMapDataType dt, uin
   }
   cuuint64_t dims[4] = {d0, d1, d2, d3};
   cuuint64_t strides[3] = {s1_bytes, s2_bytes, s3_bytes};
-  cuuint32_t box[4] = {b0, b1, 1, 1};
+  cuuint32_t box[4] = {b0, b1, b2, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   (void)elem_bytes;
   CUresult r = fn(map, dt, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,

@@ -28,10 +28,10 @@ inline int launch_status() { return cuda_status(cudaGetLastError()); }
 
 // Encodes a 4-D tiled TMA map over a row-major tensor whose innermost dim is
 // contiguous: dims {d0 (contiguous), d1, d2, d3}, byte strides for d1..d3,
-// box {b0, b1, 1, 1}, 128-byte swizzle, zero fill out of bounds.
+// box {b0, b1, b2, 1}, 128-byte swizzle, zero fill out of bounds.
 int make_tmap_4d(CUtensorMap* map, const void* base, CUtensorMapDataType dt, uint32_t elem_bytes, uint64_t d0,
                  uint64_t d1, uint64_t d2, uint64_t d3, uint64_t s1_bytes, uint64_t s2_bytes, uint64_t s3_bytes,
-                 uint32_t b0, uint32_t b1);
+                 uint32_t b0, uint32_t b1, uint32_t b2 = 1);
 
 // Raises a kernel's dynamic shared-memory limit once per device.  The
 // attribute belongs to the device's context, so the "done" record is a bit

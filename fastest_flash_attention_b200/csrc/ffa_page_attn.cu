@@ -1,0 +1,796 @@
+// Attention of many query rows over the pages of a paged cache, on the tensor
+// cores (tcgen05):
+//   prefill  several new tokens of each request attend its pages, causally
+//   prefix   one token of each request of a group attends the pages of the
+//            prefix that the group shares (a partial result: the requests' own
+//            tokens are added by the windowed decode kernel's PREFIX form)
+//
+// The query rows of one kv head are packed: row = token * G + (head in its
+// group), G = Hq / Hkv, so a tile of 128 rows holds floor(128 / G) tokens and
+// every K and V tile is read once for all query heads that share it.  In the
+// prefix form the tokens are the requests of a group: that is the whole gain,
+// 128 rows for each byte of the prefix instead of G.
+//
+// One CTA owns NQT tiles of 128 rows of one (segment, kv head), a segment being
+// a request or a group, and walks key tiles of 128 tokens of one share of the
+// context:
+//   warp LOAD  TMA producer: Q once (one box of G x floor(128 / G) rows for
+//              each 64 columns), then K_j and V_j into a ring of slots, in boxes
+//              of `box` rows, the largest power of two that divides the page
+//              size (a box never leaves its page); a lane each looks its box's
+//              page up one tile ahead
+//   warp MMA   S_t = Q_t K_j^T into TMEM, O_t += P_t V_j with P_t from TMEM
+//   4 warps for each query tile: thread = row = TMEM lane.  Two passes over S
+//              in TMEM (maximum, then 2^(s - m) written back as 16-bit P), so
+//              that a row never lives in registers whole.
+// Rows and warps past the segment's last token do nothing and store nothing.
+// Keys past the last visible one: scores are masked by selection, and the rows
+// of V are zeroed in shared memory before the product, because 0 * NaN of
+// memory that was never written would reach O.
+//
+// Shares of a long context (few rows: one tile for each kv head would leave most
+// SMs idle) leave fp32 partial results, normalised, with their base-2 LSE; a
+// merge kernel (prefill) or the decode kernel (prefix) joins them.
+// P is rounded to the data's type once, as the tensor core's operand; the row
+// sums add the unrounded values; statistics, O and the join are fp32.
+#include "ffa_common.cuh"
+#include "ffa_host.h"
+#include "ffa_page_attn.h"
+
+#include <type_traits>
+
+namespace ffa {
+
+constexpr int PA_BM = 128, PA_BN = 128;
+
+struct PaParams {
+  const int* starts;  // [N + 1] first query token of each segment
+  const int* kv_lens; // causal: [N] context lengths; else [N] prefix lengths
+  const int* lens;    // [R] context lengths (prefix form: which members share)
+  const int* table;   // [R, width]
+  int64_t bt_stride;
+  void* out;          // [T, Hq, D] (causal)
+  int64_t o_st, o_sh;
+  float* lse;         // [T, Hq] or nullptr (causal)
+  float* o_part;      // [shares, T, Hq, D]
+  float* lse_part;    // [shares, T, Hq], base 2
+  int N, T, Hq, Hkv, G, TQ, D;
+  int num_pages, page_size, box, max_ctx;
+  int shares, chunk;  // a segment's tokens [s * chunk, (s + 1) * chunk), the last share the rest
+  float scale_log2, sc_pre, sc_post, sc_poly[3];
+  int use_softcap, keep_kv;  // keep_kv: other CTAs read the same K and V
+  ErrCtx ec;
+};
+
+template <int D, int NQT>
+struct PaCfg {
+  // NQT = 1: 6 warps, two CTAs per SM (each half the TMEM; the two interleave on
+  // the tensor core).  NQT = 2: 10 warps, one CTA, K and V read once for both tiles.
+  static constexpr int THREADS = (4 * NQT + 2) * 32;
+  static constexpr int MIN_BLOCKS = NQT == 1 ? 2 : 1;
+  static constexpr int TMEM_COLS = NQT == 1 ? 256 : 512;
+  static constexpr int TILE = PA_BM * D * 2;  // a tile of Q, K or V
+  static constexpr int NBUF = NQT == 1 ? (D == 64 ? 4 : 2) : (D == 64 ? 8 : 4);
+  static constexpr int KV_OFF = NQT * TILE;
+  static constexpr int BAR_OFF = KV_OFF + NBUF * TILE;
+  static constexpr int SMEM = BAR_OFF + 512 + 1024;
+  static_assert(SMEM <= (NQT == 1 ? 113 : 227) * 1024, "shared memory budget");
+};
+
+struct PaBars {
+  uint64_t q_full;
+  uint64_t s_full[2];
+  uint64_t p_full[2][2];
+  uint64_t o_done[2];
+  uint64_t drain;
+  uint64_t kv_full[8];
+  uint64_t kv_empty[8];
+  uint32_t tmem_base;
+  int abort;
+};
+
+enum : uint32_t {
+  SITE_PA_Q = 0x501,
+  SITE_PA_KV_EMPTY = 0x502,
+  SITE_PA_KV_FULL = 0x503,
+  SITE_PA_P_FULL = 0x504,
+  SITE_PA_S_FULL = 0x505,
+  SITE_PA_O_DONE = 0x506,
+  SITE_PA_DRAIN = 0x507,
+};
+
+// The item-th block of `per` query tokens over all segments, found by one warp:
+// its segment, the segment's first token and tokens, and the block within it
+// (blocks of a segment in reverse, the one with the most keys first).
+__device__ __forceinline__ bool pa_find(const PaParams& p, int per, int item, int lane, int& seg, int& first, int& n,
+                                        int& block) {
+  int base = 0;
+  for (int i0 = 0; i0 < p.N; i0 += 32) {
+    const int i = i0 + lane;
+    int lo = 0, hi = 0;
+    if (i < p.N) {
+      lo = p.starts[i];
+      hi = p.starts[i + 1];
+      if (lo < 0 || hi < lo || hi > p.T) {
+        if (p.ec.err) atomicCAS(p.ec.err, 0u, SITE_PA_BAD_STARTS);
+        lo = hi = 0;
+      }
+    }
+    const int blocks = (hi - lo + per - 1) / per;
+    int incl = blocks;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int a = __shfl_up_sync(0xffffffffu, incl, off);
+      if (lane >= off) incl += a;
+    }
+    const uint32_t past = __ballot_sync(0xffffffffu, base + incl > item);
+    if (past) {
+      const int o = __ffs(past) - 1;
+      seg = i0 + o;
+      first = __shfl_sync(0xffffffffu, lo, o);
+      n = __shfl_sync(0xffffffffu, hi - lo, o);
+      block = __shfl_sync(0xffffffffu, base + incl, o) - 1 - item;
+      return true;
+    }
+    base += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  return false;
+}
+
+template <typename T, int D, int NQT, bool CAUSAL>
+__global__ void __launch_bounds__(PaCfg<D, NQT>::THREADS, PaCfg<D, NQT>::MIN_BLOCKS)
+    ffa_page_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                         const __grid_constant__ CUtensorMap tmV, const PaParams p) {
+  using Cfg = PaCfg<D, NQT>;
+  constexpr int WARP_LOAD = 4 * NQT, WARP_MMA = 4 * NQT + 1;
+  constexpr uint32_t O_COL = NQT * 128;  // TMEM: S_t / P_t at [128 t, ...), O_t at O_COL + 128 t
+  constexpr int HALVES = D / 64, HALF = PA_BN * 128;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;
+  uint8_t* sKV = smem + Cfg::KV_OFF;
+  PaBars* bars = reinterpret_cast<PaBars*>(smem + Cfg::BAR_OFF);
+  volatile int* abort_flag = &bars->abort;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+  // a kernel launched behind this one may start once every CTA has come here
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  // ---------------- what this CTA works on (the same in every warp) ----------------
+  const int h = blockIdx.x % p.Hkv;
+  const int share = blockIdx.x / p.Hkv % p.shares;
+  const int item = blockIdx.x / p.Hkv / p.shares;
+  const int per = p.TQ * NQT;
+  int seg, first, n, block;
+  if (!pa_find(p, per, item, lane, seg, first, n, block)) return;
+  const int tok0 = block * per;              // of the segment's query tokens
+  const int toks = min(per, n - tok0);       // this CTA's
+  const int tiles_q = NQT == 1 || toks <= p.TQ ? 1 : 2;
+  const int kv = p.kv_lens[seg];
+  int row, past;  // table row; tokens before the segment's first query (causal)
+  bool direct = false;
+  int limit;      // keys [0, limit) are visible to some row of this CTA
+  if (CAUSAL) {
+    if (kv < n || kv > p.max_ctx) {
+      if (lane == 0 && p.ec.err) atomicCAS(p.ec.err, 0u, SITE_DEC_BAD_CTX);
+      return;
+    }
+    row = seg;
+    past = kv - n;
+    limit = past + tok0 + toks;
+    direct = p.shares == 1 || kv <= p.chunk;
+  } else {
+    if (kv < 0 || kv > p.max_ctx) {
+      if (lane == 0 && p.ec.err) atomicCAS(p.ec.err, 0u, SITE_PA_BAD_STARTS);
+      return;
+    }
+    // the first member long enough lends its pages
+    row = -1;
+    past = 0;
+    for (int i0 = 0; i0 < n && row < 0; i0 += 32) {
+      const int len = i0 + lane < n ? p.lens[first + i0 + lane] : -1;
+      const uint32_t has = __ballot_sync(0xffffffffu, len >= kv && len <= p.max_ctx);
+      if (has) row = first + i0 + __ffs(has) - 1;
+    }
+    if (row < 0) return;
+    limit = kv;
+  }
+  const int kv0 = share * p.chunk;
+  const int kv1 = share + 1 == p.shares ? limit : min(limit, kv0 + p.chunk);
+  if (kv0 >= kv1) return;
+  const int n_tiles = (kv1 - kv0 + PA_BN - 1) / PA_BN;
+
+  if (threadIdx.x == 0) {
+    mbar_init(&bars->q_full, 1);
+    for (int t = 0; t < NQT; ++t) {
+      mbar_init(&bars->s_full[t], 1);
+      for (int k = 0; k < 2; ++k) mbar_init(&bars->p_full[t][k], 4);  // one arrival per warp
+      mbar_init(&bars->o_done[t], 1);
+    }
+    mbar_init(&bars->drain, 1);
+    for (int i = 0; i < Cfg::NBUF; ++i) {
+      mbar_init(&bars->kv_full[i], 1);
+      mbar_init(&bars->kv_empty[i], 1);
+    }
+    bars->abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == WARP_MMA) {
+    tmem_alloc(&bars->tmem_base, Cfg::TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem_base;
+
+  if (warp == WARP_LOAD) {
+    // ------------------------------- producer -------------------------------
+    const uint64_t pol = p.keep_kv ? policy_evict_last() : policy_evict_first();
+    if (lane == 0) {
+      const int q_rows = p.TQ * p.G;
+      mbar_arrive_expect_tx(&bars->q_full, tiles_q * HALVES * q_rows * 128);
+      for (int t = 0; t < tiles_q; ++t)
+        for (int c = 0; c < HALVES; ++c)
+          tma_load_4d(&tmQ, &bars->q_full, sQ + t * Cfg::TILE + c * HALF, c * 64, 0, first + tok0 + t * p.TQ, h, pol);
+    }
+    __syncwarp();
+    const int* table = p.table + (int64_t)row * p.bt_stride;
+    // pool row of this lane's box of a tile, or -1 (past the last key, or a page
+    // id outside the pool, which is recorded)
+    auto box_row = [&](int j) -> int {
+      const int tok = kv0 + j * PA_BN + lane * p.box;
+      if (lane * p.box >= PA_BN || tok >= kv1) return -1;
+      const int i = tok / p.page_size;
+      const int page = table[i];
+      if ((unsigned)page >= (unsigned)p.num_pages) {
+        if (p.ec.err) atomicCAS(p.ec.err, 0u, SITE_DEC_BAD_PAGE);
+        return -1;
+      }
+      return (page * p.Hkv + h) * p.page_size + tok - i * p.page_size;
+    };
+    int at = box_row(0);
+    int issued = 0;
+    bool ok = true;
+    for (int j = 0; j < n_tiles && ok; ++j) {
+      const int next = j + 1 < n_tiles ? box_row(j + 1) : -1;
+      const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, at >= 0));
+      for (int v = 0; v < 2 && ok; ++v) {
+        const int s = 2 * j + v, buf = s % Cfg::NBUF, use = s / Cfg::NBUF;
+        if (use > 0) ok = mbar_wait(&bars->kv_empty[buf], (use - 1) & 1, p.ec, abort_flag, SITE_PA_KV_EMPTY);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(&bars->kv_full[buf], boxes * p.box * 128 * HALVES);
+        ++issued;
+        __syncwarp();
+        if (at >= 0) {
+          uint8_t* dst = sKV + buf * Cfg::TILE + lane * p.box * 128;
+#pragma unroll
+          for (int c = 0; c < HALVES; ++c)
+            tma_load_4d(v ? &tmV : &tmK, &bars->kv_full[buf], dst + c * HALF, c * 64, at, 0, 0, pol);
+        }
+      }
+      at = next;
+    }
+    if (*abort_flag && lane == 0) {
+      // let copies still in flight land before the CTA gives up its smem
+      mbar_wait(&bars->q_full, 0, p.ec, abort_flag, SITE_PA_DRAIN, true);
+      for (int s = max(0, issued - Cfg::NBUF); s < issued; ++s)
+        mbar_wait(&bars->kv_full[s % Cfg::NBUF], (s / Cfg::NBUF) & 1, p.ec, abort_flag, SITE_PA_DRAIN, true);
+    }
+    __syncwarp();
+  } else if (warp == WARP_MMA) {
+    // ------------------------------ MMA issuer ------------------------------
+    if (lane == 0) {
+      constexpr uint32_t FMT = DtypeFmt<T>::value;
+      const uint32_t idesc_qk = make_idesc_f16(PA_BM, PA_BN, FMT, 0, 0);
+      const uint32_t idesc_pv = make_idesc_f16(PA_BM, D, FMT, 0, 1);
+      const uint64_t q_base = make_sdesc_sw128(smem_u32(sQ), 16, 1024);
+      const uint64_t k_base = make_sdesc_sw128(smem_u32(sKV), 16, 1024);
+      const uint64_t v_base = make_sdesc_sw128(smem_u32(sKV), HALF, 1024);
+      auto issue_qk = [&](int t, int buf) {
+        const uint64_t qa = q_base + (uint64_t)((t * Cfg::TILE) >> 4);
+        const uint64_t kb = k_base + (uint64_t)((buf * Cfg::TILE) >> 4);
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          const uint32_t off = ((ks / 4) * HALF + (ks % 4) * 32) >> 4;
+          mma_ss(tmem + t * 128, qa + off, kb + off, idesc_qk, ks > 0);
+        }
+        mma_commit(&bars->s_full[t]);
+      };
+      auto issue_pv = [&](int t, int buf, bool acc, int half) {
+        const uint64_t vb = v_base + (uint64_t)((buf * Cfg::TILE) >> 4);
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          const int ks = half * 4 + kk;
+          mma_ts(tmem + O_COL + t * 128, tmem + t * 128 + ks * 8, vb + (uint64_t)((ks * 16 * 128) >> 4), idesc_pv,
+                 (acc || ks > 0) ? 1u : 0u);
+        }
+      };
+      bool ok = mbar_wait_mma(&bars->q_full, 0, p.ec, abort_flag, SITE_PA_Q) &&
+                mbar_wait_mma(&bars->kv_full[0], 0, p.ec, abort_flag, SITE_PA_KV_FULL);
+      if (ok) {
+        tc_fence_after();
+        for (int t = 0; t < tiles_q; ++t) issue_qk(t, 0);
+        mma_commit(&bars->kv_empty[0]);
+      }
+      for (int j = 0; j < n_tiles && ok; ++j) {
+        const int vs = 2 * j + 1, ks = 2 * j + 2;
+        const int vb = vs % Cfg::NBUF, kb = ks % Cfg::NBUF;
+        ok = mbar_wait_mma(&bars->kv_full[vb], (vs / Cfg::NBUF) & 1, p.ec, abort_flag, SITE_PA_KV_FULL);
+        for (int t = 0; t < tiles_q && ok; ++t) {
+          for (int half = 0; half < 2 && ok; ++half) {
+            ok = mbar_wait_mma(&bars->p_full[t][half], j & 1, p.ec, abort_flag, SITE_PA_P_FULL);
+            if (!ok) break;
+            tc_fence_after();
+            issue_pv(t, vb, j > 0, half);
+          }
+          if (!ok) break;
+          mma_commit(&bars->o_done[t]);
+          if (t == tiles_q - 1) mma_commit(&bars->kv_empty[vb]);
+          if (j + 1 < n_tiles) {
+            if (t == 0)
+              ok = mbar_wait_mma(&bars->kv_full[kb], (ks / Cfg::NBUF) & 1, p.ec, abort_flag, SITE_PA_KV_FULL);
+            if (!ok) break;
+            tc_fence_after();
+            issue_qk(t, kb);
+            if (t == tiles_q - 1) mma_commit(&bars->kv_empty[kb]);
+          }
+        }
+      }
+      // every MMA must retire before TMEM is released
+      mma_commit(&bars->drain);
+      mbar_wait_mma(&bars->drain, 0, p.ec, abort_flag, SITE_PA_DRAIN, true);
+    }
+    __syncwarp();
+  } else if (warp / 4 < tiles_q) {
+    // -------------------------------- softmax --------------------------------
+    const int t = warp / 4, r = threadIdx.x % PA_BM;
+    const uint32_t lane_off = (uint32_t)((warp % 4) * 32) << 16;
+    const uint32_t tS = tmem + lane_off + t * 128;
+    const uint32_t tO = tmem + lane_off + O_COL + t * 128;
+    const int t_toks = min(p.TQ, toks - t * p.TQ);   // tokens of this tile
+    const bool live = (warp % 4) * 32 < t_toks * p.G;  // any row of this warp
+    const int tl = r / p.G, g = r - tl * p.G;        // this row's token in the tile, and head
+    // keys [0, vis) are visible to this row (a row past the segment's last token is computed like the last)
+    const int vis = CAUSAL ? past + tok0 + t * p.TQ + min(tl, t_toks - 1) + 1 : limit;
+    const int vis_min = CAUSAL ? past + tok0 + t * p.TQ + 1 : limit;
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int j = 0; j < n_tiles; ++j) {
+      const int c0 = kv0 + j * PA_BN;
+      ok = __all_sync(0xffffffffu, mbar_wait(&bars->s_full[t], j & 1, p.ec, abort_flag, SITE_PA_S_FULL));
+      if (!ok) break;
+      tc_fence_after();
+      if (t == 0 && c0 + PA_BN > limit) {
+        // The last tile ends past the visible keys: V's rows there become zeros.
+        // (Only now: S_j is issued after V_(j-1) was waited for, so the barrier
+        // is in this tile's phase; before that its parity would not tell.)
+        const int s = 2 * j + 1;
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars->kv_full[s % Cfg::NBUF], (s / Cfg::NBUF) & 1, p.ec, abort_flag,
+                                               SITE_PA_KV_FULL));
+        if (!ok) break;
+        uint8_t* vt = sKV + s % Cfg::NBUF * Cfg::TILE;
+        const int drop = (limit - c0) * 8, all = PA_BN * 8;  // 16-byte pieces of a half
+        for (int i = drop + r; i < all; i += PA_BM)
+#pragma unroll
+          for (int c = 0; c < HALVES; ++c) *reinterpret_cast<uint4*>(vt + c * HALF + i * 16) = make_uint4(0, 0, 0, 0);
+        fence_async_smem();
+        __syncwarp();
+      }
+      if (!live) {  // P of rows that nobody reads: whatever TMEM holds
+        if (lane == 0) {
+          mbar_arrive(&bars->p_full[t][0]);
+          mbar_arrive(&bars->p_full[t][1]);
+        }
+        continue;
+      }
+      const bool masked = c0 + PA_BN > vis_min;
+      const int hi = vis - c0;  // columns [0, hi) of this tile are visible to this row
+      // first pass: the row's maximum (of raw scores: scale is positive and the
+      // softcap monotone), and with a softcap the minimum too
+      float mx = -INFINITY, mn = INFINITY;
+#pragma unroll
+      for (int c = 0; c < PA_BN; c += 32) {
+        uint32_t s[32];
+        tmem_ld32(tS + c, s);
+        tmem_ld_wait32(s);
+        if (masked) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (c + e >= hi) s[e] = __float_as_uint(-INFINITY);
+        }
+        float a[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] = fmaxf(__uint_as_float(s[i]), __uint_as_float(s[i + 4]));
+#pragma unroll
+        for (int e = 8; e < 32; e += 8)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) a[i] = fmax3(a[i], __uint_as_float(s[e + i]), __uint_as_float(s[e + i + 4]));
+        mx = fmax3(mx, fmaxf(a[0], a[1]), fmaxf(a[2], a[3]));
+        if (p.use_softcap) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (!masked || c + e < hi) mn = fminf(mn, __uint_as_float(s[e]));
+        }
+      }
+      // scores in base-2 units: s * mul, or with a softcap softcap * log2 e * tanh(s * sc_pre)
+      float mul = p.scale_log2, top = mx * mul;
+      bool small = true;
+      if (p.use_softcap) {
+        const float lo = mx == -INFINITY ? 0.f : fmaxf(fabsf(mx), fabsf(mn));
+        small = __all_sync(0xffffffffu, lo * p.sc_pre <= 0.5f);
+        if (small) {
+          top = mx == -INFINITY ? mx
+                                : softcap_small2(make_float2(mx, mx), p.sc_poly[0], p.sc_poly[1], p.sc_poly[2]).x * mul;
+        } else {
+          mul = p.sc_post;
+          top = mx == -INFINITY ? mx : tanh_acc(mx * p.sc_pre) * mul;
+        }
+      }
+      const float m_new = fmaxf(m, top);
+      if (__any_sync(0xffffffffu, m_new > m + 8.f)) {
+        // lazy rescale: exact, numerator and denominator share the stale maximum
+        const float alpha = m_new == -INFINITY ? 1.f : ex2(m - m_new);
+        l *= alpha;
+        m = m_new;
+        if (j > 0) {
+          ok = __all_sync(0xffffffffu,
+                          mbar_wait(&bars->o_done[t], (j - 1) & 1, p.ec, abort_flag, SITE_PA_O_DONE));
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < D; c += 32) {
+            uint32_t ov[32];
+            tmem_ld32(tO + c, ov);
+            tmem_ld_wait32(ov);
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const float2 v = fmul2(make_float2(__uint_as_float(ov[e]), __uint_as_float(ov[e + 1])), f2(alpha));
+              ov[e] = __float_as_uint(v.x);
+              ov[e + 1] = __float_as_uint(v.y);
+            }
+            tmem_st32(tO + c, ov);
+          }
+        }
+      }
+      // second pass: P over S, handed over in two halves of 64 keys
+      const float mu = m == -INFINITY ? 0.f : m;
+      const float2 mul2 = f2(mul), nmu2 = f2(-mu);
+      float2 acc[2] = {f2(0.f), f2(0.f)};
+#pragma unroll
+      for (int c = 0; c < PA_BN; c += 32) {
+        uint32_t s[32], pk[16];
+        tmem_ld32(tS + c, s);
+        tmem_ld_wait32(s);
+        if (p.use_softcap) {
+          if (small) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const float2 y = softcap_small2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])),
+                                              p.sc_poly[0], p.sc_poly[1], p.sc_poly[2]);
+              s[e] = __float_as_uint(y.x);
+              s[e + 1] = __float_as_uint(y.y);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(tanh_acc(__uint_as_float(s[e]) * p.sc_pre));
+          }
+        }
+        if (masked) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (c + e >= hi) s[e] = __float_as_uint(-INFINITY);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float2 a = ffma2(make_float2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), mul2, nmu2);
+          const float2 pv = make_float2(ex2(a.x), ex2(a.y));
+          acc[e & 1] = fadd2(acc[e & 1], pv);
+          pk[e] = pack2<T>(pv.x, pv.y);
+        }
+        tmem_st16(tS + c / 2, pk);
+        if (c == 32 || c == 96) {
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->p_full[t][c / 64]);
+        }
+      }
+      const float2 a = fadd2(acc[0], acc[1]);
+      l += a.x + a.y;
+    }
+    // -------------------------------- epilogue --------------------------------
+    if (ok && live) {
+      ok = __all_sync(0xffffffffu,
+                      mbar_wait(&bars->o_done[t], (n_tiles - 1) & 1, p.ec, abort_flag, SITE_PA_O_DONE));
+      if (ok) {
+        tc_fence_after();
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+        const bool store = tl < t_toks;
+        const int64_t tok = first + tok0 + t * p.TQ + tl;
+        const int head = h * p.G + g;
+        const int64_t part = ((int64_t)share * p.T + tok) * p.Hq + head;
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          uint32_t ov[32];
+          tmem_ld32(tO + c, ov);
+          tmem_ld_wait32(ov);
+          if (!store) continue;
+          if (CAUSAL && direct) {
+            T* dst = reinterpret_cast<T*>(p.out) + tok * p.o_st + head * p.o_sh + c;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if (c + 8 * e >= p.D) break;
+              uint32_t pk[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                pk[i] = pack2<T>(__uint_as_float(ov[8 * e + 2 * i]) * inv, __uint_as_float(ov[8 * e + 2 * i + 1]) * inv);
+              reinterpret_cast<uint4*>(dst)[e] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+            }
+          } else {
+            float* dst = p.o_part + part * p.D + c;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              if (c + 4 * e >= p.D) break;
+              reinterpret_cast<float4*>(dst)[e] =
+                  make_float4(__uint_as_float(ov[4 * e]) * inv, __uint_as_float(ov[4 * e + 1]) * inv,
+                              __uint_as_float(ov[4 * e + 2]) * inv, __uint_as_float(ov[4 * e + 3]) * inv);
+            }
+          }
+        }
+        if (store) {
+          const float lse = l > 0.f ? m + lg2(l) : -INFINITY;
+          if (!(CAUSAL && direct)) p.lse_part[part] = lse;
+          else if (p.lse) p.lse[tok * p.Hq + head] = lse * 0.6931471805599453f;
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == WARP_MMA) {
+    tc_fence_after();
+    tmem_dealloc(tmem, Cfg::TMEM_COLS);
+  }
+}
+
+// Joins the shares of a prefill: one warp for each (token, query head) of the
+// requests longer than a share.
+template <typename T>
+__global__ void ffa_page_attn_merge_kernel(const PaParams p) {
+  const int64_t w = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / 32;
+  const int lane = threadIdx.x % 32;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (w >= (int64_t)p.T * p.Hq) return;
+  const int tok = (int)(w / p.Hq), head = (int)(w % p.Hq);
+  // the request: the last one that starts at or before the token
+  int seg = -1;
+  for (int i0 = 0; i0 < p.N; i0 += 32) {
+    const uint32_t has = __ballot_sync(0xffffffffu, i0 + lane < p.N && p.starts[i0 + lane] <= tok);
+    if (has) seg = i0 + 31 - __clz(has);
+  }
+  if (seg < 0) return;
+  const int first = p.starts[seg], end = p.starts[seg + 1], kv = p.kv_lens[seg], n = end - first;
+  if (first < 0 || tok >= end || end > p.T || kv < n || kv > p.max_ctx || kv <= p.chunk) return;
+  const int vis = kv - n + tok - first + 1;
+  const int parts = min(p.shares, (vis + p.chunk - 1) / p.chunk);
+  const int64_t step = (int64_t)p.T * p.Hq;
+  float M = -INFINITY;
+  for (int s = 0; s < parts; ++s) M = fmaxf(M, p.lse_part[w + s * step]);
+  float L = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s = 0; s < parts; ++s) {
+    const float x = p.lse_part[w + s * step];
+    const float f = x == -INFINITY ? 0.f : ex2(x - M);
+    L += f;
+    if (lane * 4 < p.D) {
+      const float4 v = *reinterpret_cast<const float4*>(p.o_part + (w + s * step) * p.D + lane * 4);
+      acc.x += f * v.x;
+      acc.y += f * v.y;
+      acc.z += f * v.z;
+      acc.w += f * v.w;
+    }
+  }
+  const float inv = L > 0.f ? 1.f / L : 0.f;
+  if (lane * 4 < p.D) {
+    T* dst = reinterpret_cast<T*>(p.out) + tok * p.o_st + head * p.o_sh + lane * 4;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+  }
+  if (lane == 0 && p.lse) p.lse[w] = L > 0.f ? (M + lg2(L)) * 0.6931471805599453f : -INFINITY;
+}
+
+// Shares of the context and query tiles per CTA.
+//   segments * blocks: CTAs of one kv head and share, at most
+PaShape pa_shape(int64_t tokens, int64_t segments, int64_t kv, int Hkv, int G) {
+  PaShape s;
+  const int tq = 128 / G;
+  const int64_t mean = (tokens + segments - 1) / segments;  // tokens of a segment
+  s.nqt = mean > tq ? 2 : 1;
+  const int64_t per = (int64_t)tq * s.nqt, slots = s.nqt == 1 ? 296 : 148;
+  const int64_t base = segments * ((mean + per - 1) / per) * Hkv;
+  const int64_t tiles = (kv + PA_BN - 1) / PA_BN;
+  // time of a CTA: 4 us of start and end, and a key tile at a time; a partial
+  // result costs its writing and reading
+  double least = 0;
+  int64_t best = 1;
+  for (int64_t n = 1; n <= tiles && n <= 64; ++n) {
+    const int64_t each = (tiles + n - 1) / n, used = (tiles + each - 1) / each;
+    if (used != n) continue;
+    const int64_t waves = (base * n + slots - 1) / slots;
+    double t = waves * (4.0 + each * (s.nqt == 1 ? 2.0 : 2.2));
+    if (n > 1) t += 2.0 + (double)n * tokens * Hkv * G * 1024 / 4.0e6;
+    if (n == 1 || t < least) least = t, best = n;
+  }
+  const int64_t each = (tiles + best - 1) / best;
+  s.shares = (int)best;
+  s.chunk = each > 0 && each < (1 << 24) ? (int)each * PA_BN : 0x7fffff80;  // (past any context: one share)
+  return s;
+}
+
+template <typename T, int D, int NQT, bool CAUSAL>
+static int launch_page_attn(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const PaParams& p,
+                            int64_t grid, cudaStream_t st) {
+  using Cfg = PaCfg<D, NQT>;
+  auto kern = ffa_page_attn_kernel<T, D, NQT, CAUSAL>;
+  static std::atomic<uint64_t> done{0};
+  if (int s = smem_attr_once(kern, Cfg::SMEM, done)) return s;
+  kern<<<(unsigned)grid, Cfg::THREADS, Cfg::SMEM, st>>>(mq, mk, mv, p);
+  return launch_status();
+}
+
+// Tensor maps and the launch, for either form.
+int page_attn(const PaCall& c, const PaShape& shape, void* stream) {
+  PaParams p{};
+  p.starts = c.starts;
+  p.kv_lens = c.kv_lens;
+  p.lens = c.lens;
+  p.table = c.block_table;
+  p.bt_stride = c.width;
+  p.out = c.out;
+  if (c.out) {
+    p.o_st = c.o_strides[0];
+    p.o_sh = c.o_strides[1];
+  }
+  p.lse = c.lse;
+  p.N = c.N;
+  p.T = c.T;
+  p.Hq = c.Hq;
+  p.Hkv = c.Hkv;
+  p.G = c.Hq / c.Hkv;
+  p.TQ = 128 / p.G;
+  p.D = c.D;
+  p.num_pages = c.num_pages;
+  p.page_size = c.page_size;
+  p.box = 8;
+  while (p.box < 128 && c.page_size % (2 * p.box) == 0) p.box *= 2;
+  p.max_ctx = c.width * c.page_size;
+  p.shares = shape.shares;
+  p.chunk = shape.chunk;
+  const int64_t rows = (int64_t)c.T * c.Hq;
+  p.o_part = static_cast<float*>(c.workspace);
+  p.lse_part = p.o_part + rows * shape.shares * c.D;
+  p.scale_log2 = c.scale * 1.4426950408889634f;
+  p.use_softcap = c.softcap > 0.f;
+  p.sc_pre = p.use_softcap ? c.scale / c.softcap : 0.f;
+  p.sc_post = p.use_softcap ? c.softcap * 1.4426950408889634f : 0.f;
+  softcap_poly_coeffs(p.sc_pre, p.sc_poly);
+  const int64_t per = (int64_t)p.TQ * shape.nqt;
+  const int64_t items = c.N + c.T / per;  // the sum of ceil(n / per) over segments of c.T tokens is at most this
+  p.keep_kv = c.T > c.N * per;
+  p.ec.err = c.dev_err;
+  p.ec.limit_ns = wait_limit_ns();
+  const int64_t grid = items * p.Hkv * p.shares;
+  if (grid > 0x7fffffffLL) return FFA_ERR_UNSUPPORTED;
+
+  const CUtensorMapDataType dt =
+      c.dtype == FFA_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUtensorMap mq, mk, mv;
+  const uint64_t pool = (uint64_t)c.num_pages * c.Hkv * c.page_size, line = (uint64_t)c.D * 2;
+  int st = make_tmap_4d(&mq, c.q, dt, 2, c.D, p.G, c.T, c.Hkv, c.q_strides[1] * 2, c.q_strides[0] * 2,
+                        (uint64_t)p.G * c.q_strides[1] * 2, 64, p.G, p.TQ);
+  if (!st) st = make_tmap_4d(&mk, c.k_pages, dt, 2, c.D, pool, 1, 1, line, pool * line, pool * line, 64, p.box);
+  if (!st) st = make_tmap_4d(&mv, c.v_pages, dt, 2, c.D, pool, 1, 1, line, pool * line, pool * line, 64, p.box);
+  if (st) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  auto typed = [&](auto t) -> int {
+    using T = decltype(t);
+    auto shaped = [&](auto causal) -> int {
+      constexpr bool C = decltype(causal)::value;
+      if (c.D <= 64)
+        return shape.nqt == 1 ? launch_page_attn<T, 64, 1, C>(mq, mk, mv, p, grid, s)
+                              : launch_page_attn<T, 64, 2, C>(mq, mk, mv, p, grid, s);
+      return shape.nqt == 1 ? launch_page_attn<T, 128, 1, C>(mq, mk, mv, p, grid, s)
+                            : launch_page_attn<T, 128, 2, C>(mq, mk, mv, p, grid, s);
+    };
+    if (!c.causal) return shaped(std::false_type{});
+    int status = shaped(std::true_type{});
+    if (status || p.shares == 1) return status;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)((rows + 7) / 8));
+    cfg.blockDim = dim3(256);
+    cfg.stream = s;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cuda_status(cudaLaunchKernelEx(&cfg, ffa_page_attn_merge_kernel<T>, p));
+  };
+  return c.dtype == FFA_DTYPE_BF16 ? typed(__nv_bfloat16{}) : typed(__half{});
+}
+
+// Sizes, strides and pointers that both forms need.
+int pa_check(const PaCall& c) {
+  if (!c.q || !c.k_pages || !c.v_pages || !c.block_table || !c.starts || !c.kv_lens || !c.q_strides)
+    return FFA_ERR_INVALID_ARG;
+  if (c.T <= 0 || c.N <= 0 || c.Hq <= 0 || c.Hkv <= 0 || c.Hq % c.Hkv || c.D <= 0 || c.num_pages <= 0 ||
+      c.page_size <= 0 || c.width <= 0 || !(c.scale > 0.f))
+    return FFA_ERR_INVALID_ARG;
+  if (c.dtype != FFA_DTYPE_BF16 && c.dtype != FFA_DTYPE_F16) return FFA_ERR_UNSUPPORTED;
+  if (c.D % 8 || c.D > 128 || c.page_size % 8 || c.Hq / c.Hkv > 128) return FFA_ERR_UNSUPPORTED;
+  // pool rows and positions are 32-bit indexes (a box reaches up to 128 past the last)
+  if ((int64_t)c.num_pages * c.Hkv * c.page_size > 0x7fffffffLL || (int64_t)c.width * c.page_size > 0x7fffff00LL ||
+      (int64_t)c.T * (c.Hq / c.Hkv) > 0x7fffff00LL)
+    return FFA_ERR_UNSUPPORTED;
+  if (!aligned16(c.q) || !aligned16(c.k_pages) || !aligned16(c.v_pages) || c.q_strides[0] % 8 || c.q_strides[1] % 8 ||
+      c.q_strides[0] < 0 || c.q_strides[1] < 0)
+    return FFA_ERR_INVALID_ARG;
+  return FFA_OK;
+}
+
+size_t pa_workspace(int64_t T, int Hq, int D, int shares) {
+  return shares > 1 ? (size_t)T * Hq * shares * (D + 1) * 4 : 0;
+}
+
+}  // namespace ffa
+
+extern "C" size_t ffa_paged_prefill_workspace_size(int R, int T, int Hq, int Hkv, int D, int max_ctx) {
+  using namespace ffa;
+  if (R <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || Hq / Hkv > 128 || D <= 0 || D > 128 || max_ctx < 0)
+    return 0;
+  return pa_workspace(T, Hq, D, pa_shape(T, R, max_ctx, Hkv, Hq / Hkv).shares);
+}
+
+extern "C" int ffa_paged_prefill(const void* q, const void* k_pages, const void* v_pages, const int* block_table,
+                                 const int* ctx_lens, const int* query_starts, void* out, float* lse, int dtype, int R,
+                                 int T, int Hq, int Hkv, int D, int num_pages, int page_size, int max_pages_per_req,
+                                 const int64_t* q_strides, const int64_t* o_strides, float scale, float softcap,
+                                 int max_ctx, void* workspace, size_t workspace_bytes, uint32_t* dev_err,
+                                 void* stream) {
+  using namespace ffa;
+  if (R == 0 || T == 0) return FFA_OK;
+  PaCall c{};
+  c.q = q;
+  c.k_pages = k_pages;
+  c.v_pages = v_pages;
+  c.block_table = block_table;
+  c.starts = query_starts;
+  c.kv_lens = ctx_lens;
+  c.out = out;
+  c.lse = lse;
+  c.dtype = dtype;
+  c.N = R;
+  c.T = T;
+  c.Hq = Hq;
+  c.Hkv = Hkv;
+  c.D = D;
+  c.num_pages = num_pages;
+  c.page_size = page_size;
+  c.width = max_pages_per_req;
+  c.q_strides = q_strides;
+  c.o_strides = o_strides;
+  c.scale = scale;
+  c.softcap = softcap;
+  c.causal = true;
+  c.workspace = workspace;
+  c.dev_err = dev_err;
+  if (int s = pa_check(c)) return s;
+  if (!out || !o_strides || max_ctx < 0 || !aligned16(out) || o_strides[0] % 8 || o_strides[1] % 8)
+    return FFA_ERR_INVALID_ARG;
+  const PaShape shape = pa_shape(T, R, max_ctx, Hkv, Hq / Hkv);
+  const size_t need = pa_workspace(T, Hq, D, shape.shares);
+  if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return FFA_ERR_WORKSPACE;
+  return page_attn(c, shape, stream);
+}

@@ -1,0 +1,40 @@
+// Attention of many query rows over a paged cache (ffa_page_attn.cu): the call
+// that ffa_paged_prefill and the first launch of ffa_prefix_decode share.
+#pragma once
+
+#include <stddef.h>
+#include <stdint.h>
+
+namespace ffa {
+
+// Request boundaries or a prefix length that mean nothing (not an expired wait).
+enum : uint32_t { SITE_PA_BAD_STARTS = 0x3E6 };
+
+struct PaCall {
+  const void *q, *k_pages, *v_pages;
+  const int* block_table;
+  const int* starts;   // [N + 1]
+  const int* kv_lens;  // [N]
+  const int* lens;     // prefix form: [R] context lengths
+  void* out;           // causal form
+  float* lse;
+  int dtype, N, T, Hq, Hkv, D, num_pages, page_size, width;
+  const int64_t *q_strides, *o_strides;  // {token, head}
+  float scale, softcap;
+  bool causal;
+  void* workspace;
+  uint32_t* dev_err;
+};
+
+// Query tiles per CTA, and the shares that a context is cut into: share s takes
+// tokens [s * chunk, (s + 1) * chunk), the last one all that follow.
+struct PaShape {
+  int nqt, shares, chunk;
+};
+
+PaShape pa_shape(int64_t tokens, int64_t segments, int64_t kv, int Hkv, int G);
+int pa_check(const PaCall& c);
+size_t pa_workspace(int64_t T, int Hq, int D, int shares);
+int page_attn(const PaCall& c, const PaShape& shape, void* stream);
+
+}  // namespace ffa

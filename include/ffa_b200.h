@@ -229,6 +229,28 @@ int ffa_window_decode(const void* q, const void* k_pages, const void* v_pages, c
                       uint32_t* dev_err, void* stream);
 
 /* ----------------------------------------------------------------------------
+ * Several new tokens of each request against its pages (replaces the gather of
+ * ops/kv_cache.py:208 and the forward with a cache, ops/attention_forward.py:
+ * 80-89).  Request r's queries are rows [query_starts[r], query_starts[r + 1])
+ * of q [T, Hq, D] (strides {token, head}), the last of its ctx_lens[r] tokens;
+ * query i of n sees the first ctx_lens[r] - n + i + 1.  Pools, block table and
+ * lse [T, Hq] as ffa_paged_decode; query_starts [R + 1] int32.  Rows of no
+ * request are not written.  D a multiple of 8 up to 128, page_size a multiple
+ * of 8, Hq / Hkv <= 128, scale > 0; q's base and strides multiples of 16 bytes,
+ * out's too.  max_ctx (the longest context; a smaller one is not an error)
+ * decides how contexts are split, and with it the workspace.
+ * query_starts that decrease or pass T record 0x3E6 in *dev_err.  One launch,
+ * or two where contexts are split.
+ * ------------------------------------------------------------------------- */
+size_t ffa_paged_prefill_workspace_size(int R, int T, int Hq, int Hkv, int D, int max_ctx);
+
+int ffa_paged_prefill(const void* q, const void* k_pages, const void* v_pages, const int* block_table,
+                      const int* ctx_lens, const int* query_starts, void* out, float* lse, int dtype, int R, int T,
+                      int Hq, int Hkv, int D, int num_pages, int page_size, int max_pages_per_req,
+                      const int64_t* q_strides, const int64_t* o_strides, float scale, float softcap, int max_ctx,
+                      void* workspace, size_t workspace_bytes, uint32_t* dev_err, void* stream);
+
+/* ----------------------------------------------------------------------------
  * MLA absorbed decode.  Replaces modules/flash_mla.py:116 FastestFlashMLA
  * forward for one new token per request (the reference re-runs the whole
  * prefix through up-projections; here W_UK is folded into the query and
