@@ -20,6 +20,7 @@ from .kv_cache import PagedKVCache, ContinuousKVCache, copy_pages, move_tokens
 from .rotary import apply_rotary, rotary_append, rotary_tables
 from .decode import paged_decode
 from .paged_prefill import paged_prefill
+from .prefix import prefix_decode
 from .page_table import DevicePageTable, SlotPlan, assign_slots, release_pages
 from .fa4 import FA4AttnFunc, fa4_attn_func, fa4_forward_dispatch
 from .modules import FastestFlashMHA, FastestFlashGQA, FastestFlashMLA, FastestFlashFA4, RotaryEmbedding
@@ -35,6 +36,6 @@ __all__ = [
     "create_causal_block_mask", "create_sliding_window_block_mask", "create_local_block_mask",
     "auto_select_block_size", "check_triton_available", "paged_decode", "MLADecoder", "mla_decode",
     "FastestFlashStreamingGQA", "StreamingDecoder", "copy_pages", "move_tokens", "rotary_tables", "apply_rotary", "rotary_append",
-    "DevicePageTable", "SlotPlan", "assign_slots", "release_pages", "paged_prefill",
+    "DevicePageTable", "SlotPlan", "assign_slots", "release_pages", "paged_prefill", "prefix_decode",
     "ring_attention_forward", "ring_attention_backward", "ring_attention_func", "zigzag_shard", "zigzag_unshard",
 ]

@@ -156,6 +156,15 @@ SIGNATURES: dict[str, tuple] = {
         _c_i64p, _c_i64p, _c_float, _c_float, _c_int,  # q_strides o_strides scale softcap max_ctx
         _c_void_p, _c_size_t, _c_u32p, _c_void_p,  # workspace bytes err stream
     ]),
+    "ffa_prefix_decode_workspace_size": (_c_size_t, [_c_int] * 6),  # R groups Hq Hkv D max_prefix
+    "ffa_prefix_decode": (_c_int, [
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,  # q k_pages v_pages block_table ctx_lens
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p,  # group_starts prefix_lens out lse
+        _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,  # dtype R groups Hq Hkv D
+        _c_int, _c_int, _c_int,  # num_pages page_size max_pages_per_req
+        _c_i64p, _c_i64p, _c_float, _c_float, _c_int, _c_int,  # q_strides o_strides scale softcap max_prefix max_own
+        _c_void_p, _c_size_t, _c_u32p, _c_void_p,  # workspace bytes err stream
+    ]),
     "ffa_page_copy": (_c_int, [
         _c_void_p, _c_void_p, _c_void_p, _c_void_p,  # k_pages v_pages src dst
         _c_int, _c_int, ctypes.c_int64, _c_u32p, _c_void_p,  # n num_pages page_bytes err stream

@@ -109,11 +109,11 @@ struct Arg<const int64_t*> {
 // The entry points, in the order of their slots.
 enum Slot {
   FWD_SINK, BWD_SINK, WINDOW_DECODE, ROTARY, ROTARY_APPEND, PAGE_COPY, TOKEN_MOVE, ASSIGN_SLOTS,
-  RELEASE_PAGES, PAGED_PREFILL, SLOTS
+  RELEASE_PAGES, PAGED_PREFILL, PREFIX_DECODE, SLOTS
 };
 const char* const kNames[SLOTS] = {"ffa_fwd_sink",      "ffa_bwd_sink",  "ffa_window_decode", "ffa_rotary",
                                    "ffa_rotary_append", "ffa_page_copy", "ffa_token_move",    "ffa_assign_slots",
-                                   "ffa_release_pages", "ffa_paged_prefill"};
+                                   "ffa_release_pages", "ffa_paged_prefill", "ffa_prefix_decode"};
 void* g_fn[SLOTS];
 
 template <int ID, typename F>
@@ -169,6 +169,7 @@ PyMethodDef kMethods[] = {FFA_ENTRY(FWD_SINK, ffa_fwd_sink),
                           FFA_ENTRY(ASSIGN_SLOTS, ffa_assign_slots),
                           FFA_ENTRY(RELEASE_PAGES, ffa_release_pages),
                           FFA_ENTRY(PAGED_PREFILL, ffa_paged_prefill),
+                          FFA_ENTRY(PREFIX_DECODE, ffa_prefix_decode),
                           {"bind", bind, METH_VARARGS, "bind(name, address)"},
                           {nullptr, nullptr, 0, nullptr}};
 #undef FFA_ENTRY

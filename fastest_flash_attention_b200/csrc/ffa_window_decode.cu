@@ -26,11 +26,18 @@
 // P is rounded to the data's type for the P V product (the tensor core's
 // operand), the row sums add the unrounded values; statistics, O and the join
 // are fp32.
+//
+// The PREFIX form (ffa_prefix_decode) is the second launch of decoding behind a
+// shared prefix: a request that shares attends its own tokens alone, those
+// behind the prefix, and joins the partial results that ffa_page_attn.cu left
+// for its rows.  It starts while that kernel still runs (programmatic launch:
+// its loads need nothing of it) and waits for it only before the join.
 #include <cooperative_groups.h>
 #include <math.h>
 
 #include "ffa_common.cuh"
 #include "ffa_host.h"
+#include "ffa_page_attn.h"
 
 namespace ffa {
 
@@ -62,6 +69,12 @@ struct WdParams {
   float scale_log2, sc_pre, sc_post;
   int use_softcap;
   uint32_t* err;
+  // PREFIX: requests [starts[g], starts[g + 1]) share their first prefix_lens[g]
+  // tokens, whose partial results lie in o_part [shares, R, Hq, D] (normalised)
+  // and lse_part [shares, R, Hq] (base 2), one for every `chunk` tokens
+  const int *starts, *prefix_lens;
+  int groups, shares, chunk;
+  const float *o_part, *lse_part;
 };
 
 // WARPS per CTA, each with STAGES chunks in flight.  Two shapes:
@@ -131,7 +144,24 @@ __device__ __forceinline__ __nv_bfloat16 wd_round<__nv_bfloat16>(float x) { retu
 template <>
 __device__ __forceinline__ __half wd_round<__half>(float x) { return __float2half_rn(x); }
 
-template <typename T, int DP, int WARPS>
+// Tokens of request r that its group's partial results cover: the group's
+// prefix, unless the request is shorter (it then shares nothing).  One warp.
+__device__ __forceinline__ int wd_prefix(const WdParams& p, int r, int ctx, int lane) {
+  if (p.groups == 0) return 0;
+  int before = 0, len = 0;  // groups that start at or before r; this lane's prefix length
+  for (int i0 = 0; i0 <= p.groups; i0 += 32) {
+    const int i = i0 + lane;
+    const bool le = i <= p.groups && p.starts[i] <= r;
+    if (p.groups < 32 && i < p.groups) len = p.prefix_lens[i];  // (asked for with the starts, not after them)
+    before += __popc(__ballot_sync(0xffffffffu, le));
+  }
+  const int g = before - 1;
+  if (g < 0 || g >= p.groups) return 0;
+  len = p.groups < 32 ? __shfl_sync(0xffffffffu, len, g) : p.prefix_lens[g];
+  return len > 0 && len <= ctx ? len : 0;
+}
+
+template <typename T, int DP, int WARPS, bool PREFIX>
 __global__ void __launch_bounds__(WARPS * 32) ffa_window_decode_kernel(const WdParams p) {
   using Cfg = WdCfg<DP, WARPS>;
   constexpr int WD_WARPS = WARPS, WD_THREADS = Cfg::THREADS;
@@ -151,14 +181,15 @@ __global__ void __launch_bounds__(WARPS * 32) ffa_window_decode_kernel(const WdP
     if (threadIdx.x == 0 && p.err) atomicCAS(p.err, 0u, SITE_DEC_BAD_CTX);
     ctx = 0;
   }
-  const int w0 = max(ctx - p.window, 0);
+  const int shared = PREFIX ? wd_prefix(p, r, ctx, lane) : 0;
+  const int w0 = PREFIX ? shared : max(ctx - p.window, 0);
   WdRows rows;
   rows.table = p.block_table + (int64_t)r * p.bt_stride;
   rows.h = h;
   rows.Hkv = p.Hkv;
   rows.page_size = p.page_size;
   rows.num_pages = p.num_pages;
-  rows.ns = min(p.sinks, w0);
+  rows.ns = PREFIX ? 0 : min(p.sinks, w0);
   rows.skip = w0 - rows.ns;
   rows.nv = rows.ns + ctx - w0;
   rows.ps_mul = p.ps_mul;
@@ -369,8 +400,28 @@ __global__ void __launch_bounds__(WARPS * 32) ffa_window_decode_kernel(const WdP
       acc.y += v.y * f;
     }
   };
+  const int parts = PREFIX && shared ? min(p.shares, (shared + p.chunk - 1) / p.chunk) : 0;
+  if (PREFIX) asm volatile("griddepcontrol.wait;" ::: "memory");  // the partial results are complete
   auto store = [&](int row, int d, float M, float L, float2 acc) {
     const int head = h * p.G + g0 + row;
+    if (PREFIX && parts) {  // the prefix's shares join the request's own tokens
+      const int64_t at = (int64_t)r * p.Hq + head, step = (int64_t)p.R * p.Hq;
+      float top = M;
+      for (int s = 0; s < parts; ++s) top = fmaxf(top, p.lse_part[at + s * step]);
+      const float own = M == -INFINITY ? 0.f : ex2(M - top);
+      L *= own;
+      acc.x *= own;
+      acc.y *= own;
+      for (int s = 0; s < parts; ++s) {
+        const float x = p.lse_part[at + s * step];
+        const float f = x == -INFINITY ? 0.f : ex2(x - top);
+        const float2 v = *reinterpret_cast<const float2*>(p.o_part + (at + s * step) * p.D + d);
+        L += f;
+        acc.x += v.x * f;
+        acc.y += v.y * f;
+      }
+      M = top;
+    }
     const float inv = L > 0.f ? 1.f / L : 0.f;
     T* dst = reinterpret_cast<T*>(p.out) + (int64_t)r * p.o_sr + (int64_t)head * p.o_sh + d;
     dst[0] = wd_round<T>(acc.x * inv);
@@ -440,10 +491,10 @@ static void wd_shape(int64_t pairs, int64_t visible, int D, int& splits, int& wa
     }
 }
 
-template <typename T, int DP, int WARPS>
+template <typename T, int DP, int WARPS, bool PREFIX>
 static int launch_window_decode(const WdParams& p, int64_t grid, cudaStream_t st) {
   using Cfg = WdCfg<DP, WARPS>;
-  auto kern = ffa_window_decode_kernel<T, DP, WARPS>;
+  auto kern = ffa_window_decode_kernel<T, DP, WARPS, PREFIX>;
   static std::atomic<uint64_t> done{0}, wide{0};
   if (int s = smem_attr_once(kern, Cfg::SMEM, done)) return s;
   if (p.splits > 8) {  // clusters past 8 CTAs are opt-in
@@ -460,13 +511,39 @@ static int launch_window_decode(const WdParams& p, int64_t grid, cudaStream_t st
   cfg.blockDim = dim3(Cfg::THREADS);
   cfg.dynamicSmemBytes = Cfg::SMEM;
   cfg.stream = st;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = (unsigned)p.splits;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute attr[2]{};
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)p.splits;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  // (with groups the launch before this one is their partial results')
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = PREFIX && p.groups ? 2 : 1;
   return cuda_status(cudaLaunchKernelEx(&cfg, kern, p));
+}
+
+// The launch for either form; `visible`: the most tokens a request sees here.
+template <bool PREFIX>
+static int window_decode(WdParams& p, int dtype, int64_t visible, cudaStream_t st) {
+  int k = 0;
+  while ((1ll << k) < p.page_size) ++k;
+  p.ps_shift = 31 + k;
+  p.ps_mul = (uint32_t)((1ull << p.ps_shift) / (unsigned)p.page_size + 1);
+  p.G = p.Hq / p.Hkv;
+  p.head_blocks = (p.G + 15) / 16;
+  const int64_t pairs = (int64_t)p.R * p.Hkv * p.head_blocks;
+  int warps = 4;
+  wd_shape(pairs, visible, p.D, p.splits, warps);
+  const int64_t grid = pairs * p.splits;
+  if (grid > 0x7fffffffLL) return FFA_ERR_UNSUPPORTED;
+  auto typed = [&](auto t) -> int {
+    using T = decltype(t);
+    if (p.D <= 64) return launch_window_decode<T, 64, 4, PREFIX>(p, grid, st);
+    return warps == 2 ? launch_window_decode<T, 128, 2, PREFIX>(p, grid, st)
+                      : launch_window_decode<T, 128, 4, PREFIX>(p, grid, st);
+  };
+  return dtype == FFA_DTYPE_BF16 ? typed(__nv_bfloat16{}) : typed(__half{});
 }
 
 }  // namespace ffa
@@ -509,34 +586,103 @@ extern "C" int ffa_window_decode(const void* q, const void* k_pages, const void*
   p.R = R;
   p.Hq = Hq;
   p.Hkv = Hkv;
-  p.G = Hq / Hkv;
   p.D = D;
   p.page_size = page_size;
-  int k = 0;
-  while ((1ll << k) < page_size) ++k;
-  p.ps_shift = 31 + k;
-  p.ps_mul = (uint32_t)((1ull << p.ps_shift) / (unsigned)page_size + 1);
   p.window = window;
   p.sinks = sinks;
-  p.head_blocks = (p.G + 15) / 16;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.use_softcap = softcap > 0.f;
   p.sc_pre = p.use_softcap ? scale / softcap : 0.f;
   p.sc_post = p.use_softcap ? softcap * 1.4426950408889634f : 0.f;
   p.err = dev_err;
-  const int64_t pairs = (int64_t)R * Hkv * p.head_blocks;
   // the most tokens a request can see
   int64_t visible = max_ctx > 0 && max_ctx < p.max_ctx ? max_ctx : p.max_ctx;
   if (visible > (int64_t)window + sinks) visible = (int64_t)window + sinks;
-  int warps = 4;
-  wd_shape(pairs, visible, D, p.splits, warps);
-  const int64_t grid = pairs * p.splits;
-  if (grid > 0x7fffffffLL) return FFA_ERR_UNSUPPORTED;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  auto typed = [&](auto t) -> int {
-    using T = decltype(t);
-    if (D <= 64) return launch_window_decode<T, 64, 4>(p, grid, st);
-    return warps == 2 ? launch_window_decode<T, 128, 2>(p, grid, st) : launch_window_decode<T, 128, 4>(p, grid, st);
-  };
-  return dtype == FFA_DTYPE_BF16 ? typed(__nv_bfloat16{}) : typed(__half{});
+  return window_decode<false>(p, dtype, visible, static_cast<cudaStream_t>(stream));
+}
+
+// The shares of a prefix: ffa_page_attn.cu's shape, with a workspace for every one.
+static ffa::PaShape prefix_shape(int R, int groups, int Hq, int Hkv, int max_prefix) {
+  return ffa::pa_shape(R, groups, max_prefix, Hkv, Hq / Hkv);
+}
+
+extern "C" size_t ffa_prefix_decode_workspace_size(int R, int groups, int Hq, int Hkv, int D, int max_prefix) {
+  if (R <= 0 || groups <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || Hq / Hkv > 128 || D <= 0 || D > 128 ||
+      max_prefix < 0)
+    return 0;
+  return (size_t)R * Hq * prefix_shape(R, groups, Hq, Hkv, max_prefix).shares * (D + 1) * 4;
+}
+
+extern "C" int ffa_prefix_decode(const void* q, const void* k_pages, const void* v_pages, const int* block_table,
+                                 const int* ctx_lens, const int* group_starts, const int* prefix_lens, void* out,
+                                 float* lse, int dtype, int R, int groups, int Hq, int Hkv, int D, int num_pages,
+                                 int page_size, int max_pages_per_req, const int64_t* q_strides,
+                                 const int64_t* o_strides, float scale, float softcap, int max_prefix, int max_own,
+                                 void* workspace, size_t workspace_bytes, uint32_t* dev_err, void* stream) {
+  using namespace ffa;
+  if (R == 0) return FFA_OK;
+  PaCall c{};
+  c.q = q;
+  c.k_pages = k_pages;
+  c.v_pages = v_pages;
+  c.block_table = block_table;
+  c.starts = groups ? group_starts : ctx_lens;  // (no group: neither is read)
+  c.kv_lens = groups ? prefix_lens : ctx_lens;
+  c.lens = ctx_lens;
+  c.dtype = dtype;
+  c.N = groups ? groups : 1;
+  c.T = R;
+  c.Hq = Hq;
+  c.Hkv = Hkv;
+  c.D = D;
+  c.num_pages = num_pages;
+  c.page_size = page_size;
+  c.width = max_pages_per_req;
+  c.q_strides = q_strides;
+  c.scale = scale;
+  c.softcap = softcap;
+  c.workspace = workspace;
+  c.dev_err = dev_err;
+  if (int s = pa_check(c)) return s;
+  if (!ctx_lens || !out || !o_strides || groups < 0 || max_prefix < 0 || max_own < 0) return FFA_ERR_INVALID_ARG;
+  WdParams p{};
+  if (groups) {
+    const PaShape shape = prefix_shape(R, groups, Hq, Hkv, max_prefix);
+    const size_t need = ffa_prefix_decode_workspace_size(R, groups, Hq, Hkv, D, max_prefix);
+    if (!workspace || workspace_bytes < need || !aligned16(workspace)) return FFA_ERR_WORKSPACE;
+    if (int s = page_attn(c, shape, stream)) return s;
+    p.starts = group_starts;
+    p.prefix_lens = prefix_lens;
+    p.groups = groups;
+    p.shares = shape.shares;
+    p.chunk = shape.chunk;
+    p.o_part = static_cast<float*>(workspace);
+    p.lse_part = p.o_part + (int64_t)R * Hq * shape.shares * D;
+  }
+  p.q = q;
+  p.q_sr = q_strides[0];
+  p.q_sh = q_strides[1];
+  p.kp = k_pages;
+  p.vp = v_pages;
+  p.block_table = block_table;
+  p.bt_stride = max_pages_per_req;
+  p.ctx_lens = ctx_lens;
+  p.num_pages = num_pages;
+  p.max_ctx = max_pages_per_req * page_size;
+  p.out = out;
+  p.o_sr = o_strides[0];
+  p.o_sh = o_strides[1];
+  p.lse = lse;
+  p.R = R;
+  p.Hq = Hq;
+  p.Hkv = Hkv;
+  p.D = D;
+  p.page_size = page_size;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.use_softcap = softcap > 0.f;
+  p.sc_pre = p.use_softcap ? scale / softcap : 0.f;
+  p.sc_post = p.use_softcap ? softcap * 1.4426950408889634f : 0.f;
+  p.err = dev_err;
+  const int64_t visible = max_own > 0 && max_own < p.max_ctx ? max_own : p.max_ctx;
+  return window_decode<true>(p, dtype, visible, static_cast<cudaStream_t>(stream));
 }

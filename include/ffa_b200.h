@@ -229,6 +229,32 @@ int ffa_window_decode(const void* q, const void* k_pages, const void* v_pages, c
                       uint32_t* dev_err, void* stream);
 
 /* ----------------------------------------------------------------------------
+ * Paged decode of requests that share a prefix, the prefix computed once for
+ * all (no counterpart in the reference).  As ffa_paged_decode, but requests
+ * [group_starts[g], group_starts[g + 1]) of the batch share their first
+ * prefix_lens[g] tokens: those are read through the table row of the group's
+ * first request that is long enough, once for the group, on the tensor cores;
+ * a request's own tokens through its own row.  A request shorter than its
+ * group's prefix, or in no group, is computed by itself.  group_starts
+ * [groups + 1] and prefix_lens [groups] int32 on the device; groups may be 0.
+ * D a multiple of 8 up to 128, page_size a multiple of 8, Hq / Hkv <= 128,
+ * scale > 0; q's base and strides multiples of 16 bytes.  max_prefix and
+ * max_own (0: not known) bound the prefixes and the tokens behind them for the
+ * choice of the split (larger ones are no error); max_prefix sets the
+ * workspace.  Boundaries that decrease or pass R, and a prefix length outside
+ * [0, max_pages_per_req * page_size], record 0x3E6 in *dev_err.  Two launches,
+ * the second overlapping the first.
+ * ------------------------------------------------------------------------- */
+size_t ffa_prefix_decode_workspace_size(int R, int groups, int Hq, int Hkv, int D, int max_prefix);
+
+int ffa_prefix_decode(const void* q, const void* k_pages, const void* v_pages, const int* block_table,
+                      const int* ctx_lens, const int* group_starts, const int* prefix_lens, void* out, float* lse,
+                      int dtype, int R, int groups, int Hq, int Hkv, int D, int num_pages, int page_size,
+                      int max_pages_per_req, const int64_t* q_strides, const int64_t* o_strides, float scale,
+                      float softcap, int max_prefix, int max_own, void* workspace, size_t workspace_bytes,
+                      uint32_t* dev_err, void* stream);
+
+/* ----------------------------------------------------------------------------
  * Several new tokens of each request against its pages (replaces the gather of
  * ops/kv_cache.py:208 and the forward with a cache, ops/attention_forward.py:
  * 80-89).  Request r's queries are rows [query_starts[r], query_starts[r + 1])
