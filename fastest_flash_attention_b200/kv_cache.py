@@ -11,7 +11,9 @@ assignment is host bookkeeping; the K/V bytes are scattered on the device
 by ``ffa_paged_append`` in one launch per call instead of a per-token loop.
 Beyond the reference API, ``block_table()`` exports the tables as an int32
 tensor and ``decode()`` runs the sm_100a split-KV decode directly on the
-pool, with no gather.  For long conversations, sequences are forked (full
+pool, with no gather; ``prefill()`` attends several new tokens of each
+sequence, and ``decode(share_prefix=True)`` reads the pages that forks share
+once for all of them.  For long conversations, sequences are forked (full
 pages shared, counted), trimmed (pages that left a sliding window freed) and
 compacted (first tokens and window moved to fresh pages); the bytes move in
 one launch of ``copy_pages`` / ``move_tokens``.
@@ -438,15 +440,68 @@ class PagedKVCache:
         check_block_table(bt, lens, self.max_pages, self.page_size, sliding_window, sink_tokens)
         return bt.to(device), lens.to(device)
 
+    def prefix_groups(self, seq_ids: Sequence[int]) -> Tuple[List[int], List[int]]:
+        """(group_starts, prefix_lens) of neighbours in seq_ids whose tables begin with the same pages (forks of
+        one sequence; sequences given the same pages), as ``prefix_decode`` takes them.  A sequence joins the
+        group before it unless that would lose more shared tokens than it adds."""
+        tables = [self.sequences[s]["page_table"] for s in seq_ids]
+        starts, pages = [], []  # pages: those that every member of the group has in common
+        for i, table in enumerate(tables):
+            common = 0
+            if starts:
+                first, members = tables[starts[-1]], i - starts[-1]
+                for a, b in zip(first[:pages[-1]], table):
+                    if a != b or a < 0:
+                        break
+                    common += 1
+                if common and common * members >= pages[-1] * (members - 1):
+                    pages[-1] = common
+                    continue
+            starts.append(i)
+            pages.append(self.sequences[seq_ids[i]]["len"] // self.page_size)
+        ends = starts[1:] + [len(tables)]
+        return starts + ends[-1:], [n * self.page_size if e - b > 1 else 0 for b, e, n in zip(starts, ends, pages)]
+
+    def prefill(self, q: torch.Tensor, seq_ids: Sequence[int], new_lens: Sequence[int], *,
+                scale: Optional[float] = None, softcap: Optional[float] = None, return_lse: bool = False):
+        """Causal attention of the last new_lens[i] cached tokens of each sequence (appended before) over its
+        cached K/V: q [sum(new_lens), Hq, D], the sequences' queries behind one another."""
+        from .paged_prefill import paged_prefill
+
+        if len(new_lens) != len(seq_ids) or sum(new_lens) != q.shape[0]:
+            raise ValueError(f"{q.shape[0]} queries for {len(seq_ids)} sequences with {list(new_lens)} new tokens")
+        for s, n in zip(seq_ids, new_lens):
+            if not 0 <= n <= self.sequences[s]["len"]:
+                raise ValueError(f"sequence {s} has {self.sequences[s]['len']} tokens, not {n}")
+        bt, lens = self.block_table(seq_ids, q.device)
+        starts = torch.from_numpy(np.r_[0, np.cumsum(new_lens, dtype=np.int32)].astype(np.int32)).to(q.device)
+        max_ctx = max(self.sequences[s]["len"] for s in seq_ids)
+        return paged_prefill(q, self.k_pages, self.v_pages, bt, lens, starts, scale=scale, softcap=softcap,
+                             return_lse=return_lse, max_ctx=max_ctx)
+
     def decode(self, q: torch.Tensor, seq_ids: Sequence[int], *, scale: Optional[float] = None,
                softcap: Optional[float] = None, return_lse: bool = False, sliding_window: Optional[int] = None,
-               sink_tokens: int = 0):
+               sink_tokens: int = 0, share_prefix: bool = False):
         """One-token attention of q [R, Hq, D] over each sequence's cached K/V
-        (with a window: over its last tokens and the first sink_tokens)."""
+        (with a window: over its last tokens and the first sink_tokens).
+        share_prefix: pages that neighbouring sequences share (``prefix_groups``)
+        are read once for all of them; not with a window."""
         from .decode import paged_decode
 
+        if share_prefix and sliding_window:
+            raise ValueError("PagedKVCache: a window moves along each sequence, so no prefix is shared under it")
         bt, lens = self.block_table(seq_ids, q.device, sliding_window=sliding_window, sink_tokens=sink_tokens)
         max_ctx = max(self.sequences[s]["len"] for s in seq_ids)
+        if share_prefix:
+            from .prefix import prefix_decode
+
+            starts, prefixes = self.prefix_groups(seq_ids)
+            own = max(self.sequences[s]["len"] - n for b, e, n in zip(starts, starts[1:], prefixes)
+                      for s in seq_ids[b:e])
+            meta = torch.tensor(starts + prefixes, dtype=torch.int32).to(q.device)
+            return prefix_decode(q, self.k_pages, self.v_pages, bt, lens, meta[:len(starts)], meta[len(starts):],
+                                 scale=scale, softcap=softcap, return_lse=return_lse, max_prefix=max(prefixes),
+                                 max_own=own)
         return paged_decode(q, self.k_pages, self.v_pages, bt, lens, scale=scale, softcap=softcap,
                             return_lse=return_lse, max_ctx=max_ctx, sliding_window=sliding_window,
                             sink_tokens=sink_tokens)
