@@ -66,6 +66,7 @@ template <int D, int NQT>
 struct PaCfg {
   // NQT = 1: 6 warps, two CTAs per SM (each half the TMEM; the two interleave on
   // the tensor core).  NQT = 2: 10 warps, one CTA, K and V read once for both tiles.
+  // At most 168 registers a thread either way.
   static constexpr int THREADS = (4 * NQT + 2) * 32;
   static constexpr int MIN_BLOCKS = NQT == 1 ? 2 : 1;
   static constexpr int TMEM_COLS = NQT == 1 ? 256 : 512;
@@ -355,6 +356,48 @@ __global__ void __launch_bounds__(PaCfg<D, NQT>::THREADS, PaCfg<D, NQT>::MIN_BLO
     // keys [0, vis) are visible to this row (a row past the segment's last token is computed like the last)
     const int vis = CAUSAL ? past + tok0 + t * p.TQ + min(tl, t_toks - 1) + 1 : limit;
     const int vis_min = CAUSAL ? past + tok0 + t * p.TQ + 1 : limit;
+    // S with a softcap applied and columns from `hi` on at -inf, written back;
+    // returns the factor that takes it to base-2 units
+    auto rewrite = [&](int hi) -> float {
+      bool small = true;
+      if (p.use_softcap) {
+        // tanh by its polynomial where every argument of the warp is within 1/2
+        float top = 0.f;
+#pragma unroll 1
+        for (int c = 0; c < PA_BN; c += 32) {
+          uint32_t s[32];
+          tmem_ld32(tS + c, s);
+          tmem_ld_wait32(s);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) top = c + e < hi ? fmaxf(top, fabsf(__uint_as_float(s[e]))) : top;
+        }
+        small = __all_sync(0xffffffffu, top * p.sc_pre <= 0.5f);
+      }
+#pragma unroll 1
+      for (int c = 0; c < PA_BN; c += 32) {
+        uint32_t s[32];
+        tmem_ld32(tS + c, s);
+        tmem_ld_wait32(s);
+        if (p.use_softcap && small) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float2 y = softcap_small2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), p.sc_poly[0],
+                                            p.sc_poly[1], p.sc_poly[2]);
+            s[e] = __float_as_uint(y.x);
+            s[e + 1] = __float_as_uint(y.y);
+          }
+        } else if (p.use_softcap) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(tanh_acc(__uint_as_float(s[e]) * p.sc_pre));
+        }
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          if (c + e >= hi) s[e] = __float_as_uint(-INFINITY);
+        tmem_st32(tS + c, s);
+      }
+      tmem_st_wait();
+      return p.use_softcap && !small ? p.sc_post : p.scale_log2;
+    };
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int j = 0; j < n_tiles; ++j) {
@@ -385,49 +428,26 @@ __global__ void __launch_bounds__(PaCfg<D, NQT>::THREADS, PaCfg<D, NQT>::MIN_BLO
         }
         continue;
       }
-      const bool masked = c0 + PA_BN > vis_min;
-      const int hi = vis - c0;  // columns [0, hi) of this tile are visible to this row
-      // first pass: the row's maximum (of raw scores: scale is positive and the
-      // softcap monotone), and with a softcap the minimum too
-      float mx = -INFINITY, mn = INFINITY;
+      // Tiles with masked keys, and softcaps: a pass of its own that writes the
+      // scores back to TMEM, so that the two passes below stay free of both.
+      // Scores are then in base-2 units as s * mul.
+      float mul = p.scale_log2;
+      if (p.use_softcap || c0 + PA_BN > vis_min) mul = rewrite(vis - c0);
+      // first pass: the row's maximum (scale is positive)
+      uint32_t sc[64];  // two pieces of 32 columns: the next is on its way while one is worked on
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      tmem_ld32(tS, sc);
 #pragma unroll
       for (int c = 0; c < PA_BN; c += 32) {
-        uint32_t s[32];
-        tmem_ld32(tS + c, s);
+        uint32_t* s = sc + c % 64;
         tmem_ld_wait32(s);
-        if (masked) {
+        tmem_ld32(tS + (c + 32) % PA_BN, sc + (c + 32) % 64);  // (the last one: the second pass's first)
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (c + e >= hi) s[e] = __float_as_uint(-INFINITY);
-        }
-        float a[4];
+        for (int e = 0; e < 32; e += 8)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) a[i] = fmaxf(__uint_as_float(s[i]), __uint_as_float(s[i + 4]));
-#pragma unroll
-        for (int e = 8; e < 32; e += 8)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) a[i] = fmax3(a[i], __uint_as_float(s[e + i]), __uint_as_float(s[e + i + 4]));
-        mx = fmax3(mx, fmaxf(a[0], a[1]), fmaxf(a[2], a[3]));
-        if (p.use_softcap) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (!masked || c + e < hi) mn = fminf(mn, __uint_as_float(s[e]));
-        }
+          for (int i = 0; i < 4; ++i) mx[i] = fmax3(mx[i], __uint_as_float(s[e + i]), __uint_as_float(s[e + i + 4]));
       }
-      // scores in base-2 units: s * mul, or with a softcap softcap * log2 e * tanh(s * sc_pre)
-      float mul = p.scale_log2, top = mx * mul;
-      bool small = true;
-      if (p.use_softcap) {
-        const float lo = mx == -INFINITY ? 0.f : fmaxf(fabsf(mx), fabsf(mn));
-        small = __all_sync(0xffffffffu, lo * p.sc_pre <= 0.5f);
-        if (small) {
-          top = mx == -INFINITY ? mx
-                                : softcap_small2(make_float2(mx, mx), p.sc_poly[0], p.sc_poly[1], p.sc_poly[2]).x * mul;
-        } else {
-          mul = p.sc_post;
-          top = mx == -INFINITY ? mx : tanh_acc(mx * p.sc_pre) * mul;
-        }
-      }
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * mul;
       const float m_new = fmaxf(m, top);
       if (__any_sync(0xffffffffu, m_new > m + 8.f)) {
         // lazy rescale: exact, numerator and denominator share the stale maximum
@@ -460,28 +480,10 @@ __global__ void __launch_bounds__(PaCfg<D, NQT>::THREADS, PaCfg<D, NQT>::MIN_BLO
       float2 acc[2] = {f2(0.f), f2(0.f)};
 #pragma unroll
       for (int c = 0; c < PA_BN; c += 32) {
-        uint32_t s[32], pk[16];
-        tmem_ld32(tS + c, s);
+        uint32_t pk[16];
+        uint32_t* s = sc + c % 64;
         tmem_ld_wait32(s);
-        if (p.use_softcap) {
-          if (small) {
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              const float2 y = softcap_small2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])),
-                                              p.sc_poly[0], p.sc_poly[1], p.sc_poly[2]);
-              s[e] = __float_as_uint(y.x);
-              s[e + 1] = __float_as_uint(y.y);
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(tanh_acc(__uint_as_float(s[e]) * p.sc_pre));
-          }
-        }
-        if (masked) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (c + e >= hi) s[e] = __float_as_uint(-INFINITY);
-        }
+        if (c + 32 < PA_BN) tmem_ld32(tS + c + 32, sc + (c + 32) % 64);
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const float2 a = ffma2(make_float2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), mul2, nmu2);
@@ -615,7 +617,7 @@ PaShape pa_shape(int64_t tokens, int64_t segments, int64_t kv, int Hkv, int G) {
   // result costs its writing and reading
   double least = 0;
   int64_t best = 1;
-  for (int64_t n = 1; n <= tiles && n <= 64; ++n) {
+  for (int64_t n = 1; n <= tiles && n <= PA_MAX_SHARES; ++n) {
     const int64_t each = (tiles + n - 1) / n, used = (tiles + each - 1) / each;
     if (used != n) continue;
     const int64_t waves = (base * n + slots - 1) / slots;

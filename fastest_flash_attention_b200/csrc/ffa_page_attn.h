@@ -10,6 +10,8 @@ namespace ffa {
 // Request boundaries or a prefix length that mean nothing (not an expired wait).
 enum : uint32_t { SITE_PA_BAD_STARTS = 0x3E6 };
 
+constexpr int PA_MAX_SHARES = 64;
+
 struct PaCall {
   const void *q, *k_pages, *v_pages;
   const int* block_table;

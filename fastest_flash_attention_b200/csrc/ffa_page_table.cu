@@ -26,7 +26,8 @@ namespace cg = cooperative_groups;
 
 enum : uint32_t { SITE_ASSIGN = 0x3E4, SITE_RELEASE = 0x3E5 };
 
-constexpr int PT_THREADS = 512;
+constexpr int PT_THREADS = 1024;
+constexpr int PT_ILP = 4;  // items that a thread works on at a time
 constexpr int PT_MAX_ROWS = 16384;  // three ints a row in shared memory
 
 struct PtParams {
@@ -40,18 +41,41 @@ struct PtParams {
   int *slots, *positions, *starts;
   int *lens_out, *state_out;
   int R, P, page_size, max_tokens;
+  int vec;          // slots and positions are 16-byte aligned
+  uint32_t ps_mul;  // division by page_size: floor(x / d) = x * mul >> shift with mul = floor(2^shift / d) + 1,
+  int ps_shift;     // shift = 31 + k, 2^k >= d, exact below 2^31
   uint32_t* err;
 };
 
-// Row that owns item i: the last one with first[row] <= i.
-__device__ __forceinline__ int pt_row(const int* first, int R, int i) {
-  int lo = 0, hi = R;  // first[lo] <= i < first[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (first[mid] <= i) lo = mid;
-    else hi = mid;
+// Rows that own items i[k] (the last ones with first[row] <= i[k]) for the lanes
+// of a warp whose items all lie in [from, to]: the warp finds those two's rows by
+// probing 32 places at a time, each lane its own between them by bisection (of N
+// items side by side, without branches: their loads overlap).
+__device__ __forceinline__ int pt_row(const int* first, int R, int i, int lane) {
+  int lo = 0;
+  for (int len = R; len > 1;) {
+    const int step = (len + 31) / 32, at = lo + lane * step;
+    const uint32_t below = __ballot_sync(0xffffffffu, lane * step < len && first[min(at, R - 1)] <= i);
+    const int skip = max(__popc(below) - 1, 0) * step;
+    lo += skip;
+    len = min(step, len - skip);
   }
   return lo;
+}
+template <int N>
+__device__ __forceinline__ void pt_rows(const int* first, int R, int from, int to, const int* i, int* row, int lane) {
+  const int lo = pt_row(first, R, from, lane), hi = from == to ? lo : pt_row(first, R, to, lane);
+#pragma unroll
+  for (int k = 0; k < N; ++k) row[k] = lo;
+  if (hi == lo) return;
+  for (int step = 1 << (31 - __clz(hi - lo)); step > 0; step >>= 1) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int next = row[k] + step;
+      const bool up = (next <= hi) & (first[min(next, hi)] <= i[k]);
+      row[k] = up ? next : row[k];
+    }
+  }
 }
 
 template <bool ASSIGN>
@@ -60,23 +84,22 @@ __global__ void __launch_bounds__(PT_THREADS) ffa_page_table_kernel(const PtPara
   int* page0 = smem;           // [R] pages of the rows before
   int* own = smem + p.R;       // [R] assign: the row's length; release: its first page index to give back
   int* tok0 = smem + 2 * p.R;  // [R] (assign) tokens of the rows before
-  auto base = [&](int r) { return ASSIGN ? (own[r] + p.page_size - 1) / p.page_size : own[r]; };
-  __shared__ long long warp_sum[2][PT_THREADS / 32];
-  __shared__ long long carry[2];
-  __shared__ int bad_flag, any_bad;
-  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  auto div_ps = [&](int x) { return (int)(((uint64_t)(uint32_t)x * p.ps_mul) >> p.ps_shift); };
+  auto ceil_ps = [&](int x) { return x > 0 ? div_ps(x - 1) + 1 : 0; };
+  auto base = [&](int r) { return ASSIGN ? ceil_ps(own[r]) : own[r]; };
+  __shared__ long long warp_sum[2][32];
+  __shared__ int bad_flag;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, threads = blockDim.x;
   const int ctas = gridDim.x, cta = blockIdx.x;  // one cluster
-  if (tid == 0) {
-    carry[0] = carry[1] = 0;
-    bad_flag = 0;
-  }
+  if (tid == 0) bad_flag = 0;
+  if (tid < 64) warp_sum[tid / 32][lane] = 0;  // (of warps that are not there)
   const int head = p.state[0], count = p.state[1];
   bool bad = head < 0 || head >= p.P || count < 0 || count > p.P;
   const long long room = (long long)p.width * p.page_size;
-  __syncthreads();
-  // exclusive sums over the rows, PT_THREADS of them at a time (64-bit: the
+  // exclusive sums over the rows, a row for each thread at a time (64-bit: the
   // sum of any 32-bit lengths fits; only sums found small enough are used)
-  for (int r0 = 0; r0 < p.R; r0 += PT_THREADS) {
+  long long pages64 = 0, toks64 = 0;  // of the rows so far, in every thread
+  for (int r0 = 0; r0 < p.R; r0 += threads) {
     const int r = r0 + tid;
     long long pages = 0, toks = 0;
     int first = 0;
@@ -90,19 +113,19 @@ __global__ void __launch_bounds__(PT_THREADS) ffa_page_table_kernel(const PtPara
           bad = true;
         } else {
           first = (int)len;
-          pages = (len + n + p.page_size - 1) / p.page_size - (len + p.page_size - 1) / p.page_size;
+          const int had = ceil_ps(first), i = div_ps(first);
+          pages = ceil_ps((int)(len + n)) - had;
           toks = n;
           // tokens that go on in a page begun earlier
-          if (n && len % p.page_size)
-            bad |= (unsigned)p.table[(int64_t)r * p.width + len / p.page_size] >= (unsigned)p.P;
+          if (n && i < had) bad |= (unsigned)p.table[(int64_t)r * p.width + i] >= (unsigned)p.P;
         }
       } else if (p.done[r]) {
         const long long keep = p.counts ? p.counts[r] : 0;
         if (keep < 0) {
           bad = true;
         } else {
-          first = (int)((keep + p.page_size - 1) / p.page_size);
-          pages = (len + p.page_size - 1) / p.page_size - first;
+          first = ceil_ps((int)keep);
+          pages = ceil_ps((int)len) - first;
           if (pages < 0) pages = 0;
         }
       }
@@ -116,59 +139,71 @@ __global__ void __launch_bounds__(PT_THREADS) ffa_page_table_kernel(const PtPara
         it += b;
       }
     }
+    __syncthreads();  // (the sums of the rows before have been read)
     if (lane == 31) {
       warp_sum[0][warp] = ip;
       warp_sum[1][warp] = it;
     }
     __syncthreads();
-    long long bp = carry[0], bt = carry[1];
-    for (int w = 0; w < warp; ++w) {
-      bp += warp_sum[0][w];
-      bt += warp_sum[1][w];
+    // every warp sums up the warps' totals
+    long long wp = warp_sum[0][lane], wt = warp_sum[1][lane];
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const long long a = __shfl_up_sync(0xffffffffu, wp, off), b = ASSIGN ? __shfl_up_sync(0xffffffffu, wt, off) : 0;
+      if (lane >= off) {
+        wp += a;
+        wt += b;
+      }
     }
+    const long long bp = warp ? __shfl_sync(0xffffffffu, wp, warp - 1) : 0;
+    const long long bt = ASSIGN && warp ? __shfl_sync(0xffffffffu, wt, warp - 1) : 0;
     if (r < p.R) {
-      page0[r] = (int)(bp + ip - pages);
+      page0[r] = (int)(pages64 + bp + ip - pages);
       own[r] = first;
-      if (ASSIGN) tok0[r] = (int)(bt + it - toks);
+      if (ASSIGN) tok0[r] = (int)(toks64 + bt + it - toks);
     }
-    __syncthreads();
-    if (tid == PT_THREADS - 1) {
-      carry[0] = bp + ip;
-      carry[1] = bt + it;
-    }
-    __syncthreads();
+    pages64 += __shfl_sync(0xffffffffu, wp, 31);
+    toks64 += ASSIGN ? __shfl_sync(0xffffffffu, wt, 31) : 0;
   }
-  const long long pages64 = carry[0], toks64 = carry[1];
   if (ASSIGN) bad |= pages64 > count || toks64 > p.max_tokens;
   else bad |= pages64 + count > p.P;
   // (the row sums are valid below 2^31 only; every thread knows both totals)
   const int pages = pages64 <= p.P ? (int)pages64 : 0, toks = (int)toks64;
   bad |= pages64 > p.P;
-  const int step = ctas * PT_THREADS, i0 = cta * PT_THREADS + tid;
+  const int step = ctas * threads, i0 = cta * threads + tid;
   const bool sums_ok = __syncthreads_or(bad) == 0;
-  // the page ids concerned, each checked by one thread of the cluster
+  // the page ids concerned, each checked by one thread of the cluster; `ids`
+  // (release): the first PT_ILP of this thread
+  int ids[PT_ILP];
+  auto entry = [&](int j, int r) { return p.table + (int64_t)r * p.width + base(r) + j - page0[r]; };
+  auto place = [&](int j) {  // j-th place behind the ring's first free page (assign) or last (release)
+    const long long at = (long long)head + j + (ASSIGN ? 0 : count);
+    return p.ring + (at >= p.P ? at - p.P : at);
+  };
+  // (a warp's PT_ILP pieces of 32 items follow one another)
+  const int w0 = (cta * threads / 32 + warp) * 32 * PT_ILP;
+  auto items = [&](int j0, int n, int* j) {  // this lane's of the warp's items from j0 on, all below n
+#pragma unroll
+    for (int k = 0; k < PT_ILP; ++k) j[k] = min(j0 + 32 * k + lane, n - 1);
+  };
   if (sums_ok) {
-    for (int j = i0; j < pages; j += step) {
-      int id;
-      if (ASSIGN) {
-        long long at = (long long)head + j;
-        id = p.ring[at >= p.P ? at - p.P : at];
-      } else {
-        const int r = pt_row(page0, p.R, j);
-        id = p.table[(int64_t)r * p.width + base(r) + j - page0[r]];
+    for (int j0 = w0; j0 < pages; j0 += PT_ILP * step) {
+      int j[PT_ILP], row[PT_ILP], id[PT_ILP];
+      items(j0, pages, j);
+      if (!ASSIGN) pt_rows<PT_ILP>(page0, p.R, j0, min(j0 + 32 * PT_ILP, pages) - 1, j, row, lane);
+#pragma unroll
+      for (int k = 0; k < PT_ILP; ++k) id[k] = ASSIGN ? *place(j[k]) : *entry(j[k], row[k]);
+#pragma unroll
+      for (int k = 0; k < PT_ILP; ++k) {
+        bad |= (unsigned)id[k] >= (unsigned)p.P;
+        if (j0 == w0) ids[k] = id[k];
       }
-      bad |= (unsigned)id >= (unsigned)p.P;
     }
   }
   if (bad) bad_flag = 1;
   cg::cluster_group cluster = cg::this_cluster();
   cluster.sync();
-  if (tid == 0) {
-    any_bad = 0;
-    for (int c = 0; c < ctas; ++c) any_bad |= *cluster.map_shared_rank(&bad_flag, c);
-  }
-  __syncthreads();
-  const bool ok = !any_bad;
+  const bool ok = !__syncthreads_or(tid < ctas && *cluster.map_shared_rank(&bad_flag, tid));
 
   // rows: where results are written over the inputs, each row is read and
   // written by one thread
@@ -194,46 +229,90 @@ __global__ void __launch_bounds__(PT_THREADS) ffa_page_table_kernel(const PtPara
     if (!ok && p.err) atomicCAS(p.err, 0u, ASSIGN ? SITE_ASSIGN : SITE_RELEASE);
   }
   if (ok) {
-    for (int j = i0; j < pages; j += step) {
-      const int r = pt_row(page0, p.R, j);
-      int* entry = p.table + (int64_t)r * p.width + base(r) + j - page0[r];
-      long long at = (long long)head + j + (ASSIGN ? 0 : count);
-      if (at >= p.P) at -= p.P;
-      if (ASSIGN) *entry = p.ring[at];
-      else p.ring[at] = *entry;
+    for (int j0 = w0; j0 < pages; j0 += PT_ILP * step) {
+      int j[PT_ILP], row[PT_ILP];
+      items(j0, pages, j);
+      if (ASSIGN || j0 > w0) pt_rows<PT_ILP>(page0, p.R, j0, min(j0 + 32 * PT_ILP, pages) - 1, j, row, lane);
+#pragma unroll
+      for (int k = 0; k < PT_ILP; ++k) {
+        if (j0 > w0) ids[k] = ASSIGN ? *place(j[k]) : *entry(j[k], row[k]);
+        if (j0 + 32 * k + lane >= pages) continue;
+        if (ASSIGN) *entry(j[k], row[k]) = ids[k];
+        else *place(j[k]) = ids[k];
+      }
     }
   }
   if (ASSIGN) {
-    for (int t = i0; t < p.max_tokens; t += step) {
-      int slot = -1, pos = 0;
-      if (ok && t < toks) {
-        const int r = pt_row(tok0, p.R, t);
-        pos = own[r] + t - tok0[r];
-        const int i = pos / p.page_size, k = i - base(r);
-        int page;
-        if (k >= 0) {
-          long long at = (long long)head + page0[r] + k;
-          page = p.ring[at >= p.P ? at - p.P : at];
-        } else {
-          page = p.table[(int64_t)r * p.width + i];
-        }
-        slot = page * p.page_size + pos - i * p.page_size;
+    // PT_ILP tokens in a row for each thread: one store
+    for (int tw = w0; tw < p.max_tokens; tw += PT_ILP * step) {
+      const int t0 = tw + PT_ILP * lane;
+      int pos[PT_ILP], slot[PT_ILP];
+#pragma unroll
+      for (int k = 0; k < PT_ILP; ++k) {
+        pos[k] = 0;
+        slot[k] = -1;
       }
-      p.slots[t] = slot;
-      p.positions[t] = pos;
+      if (ok && tw < toks) {
+        int t[PT_ILP], row[PT_ILP];
+#pragma unroll
+        for (int k = 0; k < PT_ILP; ++k) t[k] = min(t0 + k, toks - 1);
+        pt_rows<PT_ILP>(tok0, p.R, tw, min(tw + 32 * PT_ILP, toks) - 1, t, row, lane);
+#pragma unroll
+        for (int k = 0; k < PT_ILP; ++k) {
+          const int r = row[k], x = own[r] + t[k] - tok0[r];
+          const int i = div_ps(x), n = i - base(r);
+          const int page = *(n >= 0 ? place(page0[r] + n) : p.table + (int64_t)r * p.width + i);
+          if (t0 + k < toks) {
+            pos[k] = x;
+            slot[k] = page * p.page_size + x - i * p.page_size;
+          }
+        }
+      }
+      if (p.vec && t0 + PT_ILP <= p.max_tokens) {
+        *reinterpret_cast<int4*>(p.slots + t0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+        *reinterpret_cast<int4*>(p.positions + t0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < PT_ILP; ++k)
+          if (t0 + k < p.max_tokens) {
+            p.slots[t0 + k] = slot[k];
+            p.positions[t0 + k] = pos[k];
+          }
+      }
     }
   }
   cluster.sync();  // no CTA leaves while another reads its flag
 }
 
+// CTAs of the cluster, and threads of a CTA, for so many rows, tokens or table entries.
+static void pt_shape(int64_t items, unsigned& ctas, unsigned& threads) {
+  ctas = items <= PT_THREADS ? 1 : items <= 8 * PT_THREADS ? 4 : 16;
+  threads = items >= PT_THREADS ? PT_THREADS : items < 64 ? 64 : (unsigned)(items + 31) / 32 * 32;
+}
+
 template <bool ASSIGN>
-static int launch_page_table(const PtParams& p, int64_t items, cudaStream_t st) {
+static int launch_page_table(PtParams& p, int64_t items, cudaStream_t st) {
+  int k = 0;
+  while ((1ll << k) < p.page_size) ++k;
+  p.ps_shift = 31 + k;
+  p.ps_mul = (uint32_t)((1ull << p.ps_shift) / (unsigned)p.page_size + 1);
   auto kern = ffa_page_table_kernel<ASSIGN>;
-  static std::atomic<uint64_t> done{0};
+  static std::atomic<uint64_t> done{0}, wide{0};
   if (int s = smem_attr_once(kern, 3 * 4 * PT_MAX_ROWS, done)) return s;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(items > 4 * PT_THREADS ? 8 : 1);
-  cfg.blockDim = dim3(PT_THREADS);
+  unsigned ctas, threads;
+  pt_shape(items, ctas, threads);
+  cfg.gridDim = dim3(ctas);
+  if (cfg.gridDim.x > 8) {  // clusters past 8 CTAs are opt-in
+    int dev = 0;
+    if (int s = cuda_status(cudaGetDevice(&dev))) return s;
+    const uint64_t bit = dev < 64 ? (1ull << dev) : 0ull;
+    if (!bit || !(wide.load(std::memory_order_acquire) & bit)) {
+      if (int s = cuda_status(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1))) return s;
+      if (bit) wide.fetch_or(bit, std::memory_order_acq_rel);
+    }
+  }
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = (ASSIGN ? 3 : 2) * 4 * (size_t)p.R;
   cfg.stream = st;
   cudaLaunchAttribute attr{};
@@ -281,6 +360,7 @@ extern "C" int ffa_assign_slots(int* block_table, int width, const int* ctx_lens
   p.P = num_pages;
   p.page_size = page_size;
   p.max_tokens = max_tokens;
+  p.vec = aligned16(slots) && aligned16(positions);
   p.err = dev_err;
   return launch_page_table<true>(p, max_tokens > R ? max_tokens : R, static_cast<cudaStream_t>(stream));
 }

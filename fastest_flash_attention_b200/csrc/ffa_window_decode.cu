@@ -97,6 +97,7 @@ struct WdCfg {
   static constexpr int CTA_OFF = WARPS * STATE * 4;
   static constexpr int MERGE = CTA_OFF + STATE * 4;
   static constexpr int SMEM = (RING > MERGE ? RING : MERGE) + 1024;
+  static_assert(MERGE + 16 * PA_MAX_SHARES * 4 <= RING, "the partial results' LSEs lie behind the states");
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
@@ -400,25 +401,39 @@ __global__ void __launch_bounds__(WARPS * 32) ffa_window_decode_kernel(const WdP
       acc.y += v.y * f;
     }
   };
+  // PREFIX: the LSEs of the prefix's partial results, asked for at once, behind the states
   const int parts = PREFIX && shared ? min(p.shares, (shared + p.chunk - 1) / p.chunk) : 0;
-  if (PREFIX) asm volatile("griddepcontrol.wait;" ::: "memory");  // the partial results are complete
+  float* part_lse = reinterpret_cast<float*>(smem + Cfg::MERGE);  // [16 rows][PA_MAX_SHARES]
+  const int64_t part0 = (int64_t)r * p.Hq + h * p.G + g0, part_step = (int64_t)p.R * p.Hq;
+  if constexpr (PREFIX) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // they are complete
+    for (int i = threadIdx.x; i < G * parts; i += WD_THREADS)
+      part_lse[i / parts * PA_MAX_SHARES + i % parts] = p.lse_part[part0 + i / parts + i % parts * part_step];
+    __syncthreads();
+  }
   auto store = [&](int row, int d, float M, float L, float2 acc) {
     const int head = h * p.G + g0 + row;
     if (PREFIX && parts) {  // the prefix's shares join the request's own tokens
-      const int64_t at = (int64_t)r * p.Hq + head, step = (int64_t)p.R * p.Hq;
+      const float* x = part_lse + row * PA_MAX_SHARES;
+      const float* o = p.o_part + (part0 + row) * p.D + d;
       float top = M;
-      for (int s = 0; s < parts; ++s) top = fmaxf(top, p.lse_part[at + s * step]);
+      for (int s = 0; s < parts; ++s) top = fmaxf(top, x[s]);
       const float own = M == -INFINITY ? 0.f : ex2(M - top);
       L *= own;
       acc.x *= own;
       acc.y *= own;
-      for (int s = 0; s < parts; ++s) {
-        const float x = p.lse_part[at + s * step];
-        const float f = x == -INFINITY ? 0.f : ex2(x - top);
-        const float2 v = *reinterpret_cast<const float2*>(p.o_part + (at + s * step) * p.D + d);
-        L += f;
-        acc.x += v.x * f;
-        acc.y += v.y * f;
+      for (int s0 = 0; s0 < parts; s0 += 8) {  // eight loads in flight
+        float2 v[8];
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+          v[s] = s0 + s < parts ? *reinterpret_cast<const float2*>(o + (s0 + s) * part_step * p.D) : make_float2(0.f, 0.f);
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+          const float f = s0 + s < parts && x[s0 + s] != -INFINITY ? ex2(x[s0 + s] - top) : 0.f;
+          L += f;
+          acc.x += v[s].x * f;
+          acc.y += v[s].y * f;
+        }
       }
       M = top;
     }

@@ -71,11 +71,13 @@ def assign_slots(block_table: torch.Tensor, ctx_lens: torch.Tensor, new_lens: to
     if max_tokens < 0:
         raise ValueError(f"max_tokens must not be negative, got {max_tokens}")
     new_lens = _lib.int32(new_lens)
-    # one allocation: slots, positions, starts, and the lengths and state where they are not written over
-    sizes = [max_tokens, max_tokens, R + 1] + ([] if advance else [R, 2])
-    parts = ctx_lens.new_empty(sum(sizes)).split(sizes)
-    lens_out, state_out = (ctx_lens, free_state) if advance else parts[3:]
-    plan = SlotPlan(*parts[:3], lens_out, state_out)
+    # one allocation: slots and positions (each at a multiple of 16 bytes), starts, and the lengths and state where
+    # they are not written over
+    room = (max_tokens + 3) // 4 * 4
+    buf = ctx_lens.new_empty(2 * room + R + 1 + (0 if advance else R + 2))
+    slots, positions, starts = buf[:max_tokens], buf[room:room + max_tokens], buf[2 * room:2 * room + R + 1]
+    lens_out, state_out = (ctx_lens, free_state) if advance else buf[2 * room + R + 1:].split([R, 2])
+    plan = SlotPlan(slots, positions, starts, lens_out, state_out)
     with _lib.device_of(ctx_lens):
         st = _lib.direct().ffa_assign_slots(
             block_table.data_ptr(), width, ctx_lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr(),
