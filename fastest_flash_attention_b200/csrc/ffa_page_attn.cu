@@ -19,7 +19,9 @@
 //              of `box` rows, the largest power of two that divides the page
 //              size (a box never leaves its page); a lane each looks its box's
 //              page up one tile ahead
-//   warp MMA   S_t = Q_t K_j^T into TMEM, O_t += P_t V_j with P_t from TMEM
+//   warp MMA   S_t = Q_t K_j^T into TMEM, O_t += P_t V_j with P_t from TMEM; the
+//              whole warp in step, one lane issuing (2048 tokens behind 30 720, 32/8
+//              heads of 128: 1061 us issued by a single thread's code, 959 so)
 //   4 warps for each query tile: thread = row = TMEM lane.  Two passes over S
 //              in TMEM (maximum, then 2^(s - m) written back as 16-bit P), so
 //              that a row never lives in registers whole.
@@ -143,7 +145,7 @@ __global__ void __launch_bounds__(PaCfg<D, NQT>::THREADS, PaCfg<D, NQT>::MIN_BLO
     ffa_page_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                          const __grid_constant__ CUtensorMap tmV, const PaParams p) {
   using Cfg = PaCfg<D, NQT>;
-  constexpr int WARP_LOAD = 4 * NQT, WARP_MMA = 4 * NQT + 1;
+  constexpr int WARP_MMA = 0, WARP_LOAD = 1;  // then four softmax warps for each query tile
   constexpr uint32_t O_COL = NQT * 128;  // TMEM: S_t / P_t at [128 t, ...), O_t at O_COL + 128 t
   constexpr int HALVES = D / 64, HALF = PA_BN * 128;
   extern __shared__ uint8_t smem_raw[];
@@ -282,71 +284,83 @@ __global__ void __launch_bounds__(PaCfg<D, NQT>::THREADS, PaCfg<D, NQT>::MIN_BLO
     __syncwarp();
   } else if (warp == WARP_MMA) {
     // ------------------------------ MMA issuer ------------------------------
-    if (lane == 0) {
+    {
+      // (the lanes agree on a wait's outcome: each product needs all of them)
+      auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t site) -> bool {
+        return __all_sync(0xffffffffu, mbar_wait_mma(bar, parity, p.ec, abort_flag, site));
+      };
       constexpr uint32_t FMT = DtypeFmt<T>::value;
       const uint32_t idesc_qk = make_idesc_f16(PA_BM, PA_BN, FMT, 0, 0);
       const uint32_t idesc_pv = make_idesc_f16(PA_BM, D, FMT, 0, 1);
       const uint64_t q_base = make_sdesc_sw128(smem_u32(sQ), 16, 1024);
       const uint64_t k_base = make_sdesc_sw128(smem_u32(sKV), 16, 1024);
       const uint64_t v_base = make_sdesc_sw128(smem_u32(sKV), HALF, 1024);
-      auto issue_qk = [&](int t, int buf) {
-        const uint64_t qa = q_base + (uint64_t)((t * Cfg::TILE) >> 4);
-        const uint64_t kb = k_base + (uint64_t)((buf * Cfg::TILE) >> 4);
+      // every operand but the ring slot is a constant of the unrolled code
+      auto issue_qk = [&](auto tile, uint64_t kb) {
+        constexpr int t = decltype(tile)::value;
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
-          const uint32_t off = ((ks / 4) * HALF + (ks % 4) * 32) >> 4;
-          mma_ss(tmem + t * 128, qa + off, kb + off, idesc_qk, ks > 0);
+          const int off = (ks / 4) * HALF + (ks % 4) * 32;
+          mma_ss_warp(tmem + t * 128, q_base + (uint64_t)((t * Cfg::TILE + off) >> 4), kb + (uint64_t)(off >> 4),
+                      idesc_qk, ks > 0);
         }
-        mma_commit(&bars->s_full[t]);
+        mma_commit_warp(&bars->s_full[t]);
       };
-      auto issue_pv = [&](int t, int buf, bool acc, int half) {
-        const uint64_t vb = v_base + (uint64_t)((buf * Cfg::TILE) >> 4);
+      auto issue_pv = [&](auto tile, uint64_t vb, bool acc, auto hf) {
+        constexpr int t = decltype(tile)::value, half = decltype(hf)::value;
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
           const int ks = half * 4 + kk;
-          mma_ts(tmem + O_COL + t * 128, tmem + t * 128 + ks * 8, vb + (uint64_t)((ks * 16 * 128) >> 4), idesc_pv,
-                 (acc || ks > 0) ? 1u : 0u);
+          mma_ts_warp(tmem + O_COL + t * 128, tmem + t * 128 + ks * 8, vb + (uint64_t)((ks * 16 * 128) >> 4), idesc_pv,
+                      (acc || ks > 0) ? 1u : 0u);
         }
       };
-      bool ok = mbar_wait_mma(&bars->q_full, 0, p.ec, abort_flag, SITE_PA_Q) &&
-                mbar_wait_mma(&bars->kv_full[0], 0, p.ec, abort_flag, SITE_PA_KV_FULL);
+      auto tiles = [&](auto f) {  // f(tile) for the query tiles in use
+        f(std::integral_constant<int, 0>{});
+        if constexpr (NQT == 2) {
+          if (tiles_q == 2) f(std::integral_constant<int, 1>{});
+        }
+      };
+      using H0 = std::integral_constant<int, 0>;
+      using H1 = std::integral_constant<int, 1>;
+      bool ok = wait(&bars->q_full, 0, SITE_PA_Q) && wait(&bars->kv_full[0], 0, SITE_PA_KV_FULL);
       if (ok) {
         tc_fence_after();
-        for (int t = 0; t < tiles_q; ++t) issue_qk(t, 0);
-        mma_commit(&bars->kv_empty[0]);
+        tiles([&](auto t) { issue_qk(t, k_base); });
+        mma_commit_warp(&bars->kv_empty[0]);
       }
       for (int j = 0; j < n_tiles && ok; ++j) {
-        const int vs = 2 * j + 1, ks = 2 * j + 2;
-        const int vb = vs % Cfg::NBUF, kb = ks % Cfg::NBUF;
-        ok = mbar_wait_mma(&bars->kv_full[vb], (vs / Cfg::NBUF) & 1, p.ec, abort_flag, SITE_PA_KV_FULL);
-        for (int t = 0; t < tiles_q && ok; ++t) {
-          for (int half = 0; half < 2 && ok; ++half) {
-            ok = mbar_wait_mma(&bars->p_full[t][half], j & 1, p.ec, abort_flag, SITE_PA_P_FULL);
-            if (!ok) break;
-            tc_fence_after();
-            issue_pv(t, vb, j > 0, half);
-          }
-          if (!ok) break;
-          mma_commit(&bars->o_done[t]);
-          if (t == tiles_q - 1) mma_commit(&bars->kv_empty[vb]);
-          if (j + 1 < n_tiles) {
-            if (t == 0)
-              ok = mbar_wait_mma(&bars->kv_full[kb], (ks / Cfg::NBUF) & 1, p.ec, abort_flag, SITE_PA_KV_FULL);
-            if (!ok) break;
-            tc_fence_after();
-            issue_qk(t, kb);
-            if (t == tiles_q - 1) mma_commit(&bars->kv_empty[kb]);
-          }
-        }
+        const int vs = 2 * j + 1, ks = 2 * j + 2, vi = vs % Cfg::NBUF, ki = ks % Cfg::NBUF;
+        const uint64_t vb = v_base + (uint64_t)((vi * Cfg::TILE) >> 4), kb = k_base + (uint64_t)((ki * Cfg::TILE) >> 4);
+        ok = wait(&bars->kv_full[vi], (vs / Cfg::NBUF) & 1, SITE_PA_KV_FULL);
+        tiles([&](auto t) {
+          constexpr int n = decltype(t)::value;  // (the query tile)
+          ok = ok && wait(&bars->p_full[n][0], j & 1, SITE_PA_P_FULL);
+          if (!ok) return;
+          tc_fence_after();
+          issue_pv(t, vb, j > 0, H0{});
+          ok = wait(&bars->p_full[n][1], j & 1, SITE_PA_P_FULL);
+          if (!ok) return;
+          tc_fence_after();
+          issue_pv(t, vb, j > 0, H1{});
+          mma_commit_warp(&bars->o_done[n]);
+          if (n == tiles_q - 1) mma_commit_warp(&bars->kv_empty[vi]);
+          if (j + 1 == n_tiles) return;
+          if (n == 0) ok = wait(&bars->kv_full[ki], (ks / Cfg::NBUF) & 1, SITE_PA_KV_FULL);
+          if (!ok) return;
+          tc_fence_after();
+          issue_qk(t, kb);
+          if (n == tiles_q - 1) mma_commit_warp(&bars->kv_empty[ki]);
+        });
       }
       // every MMA must retire before TMEM is released
-      mma_commit(&bars->drain);
+      mma_commit_warp(&bars->drain);
       mbar_wait_mma(&bars->drain, 0, p.ec, abort_flag, SITE_PA_DRAIN, true);
     }
     __syncwarp();
-  } else if (warp / 4 < tiles_q) {
+  } else if ((warp - 2) / 4 < tiles_q) {
     // -------------------------------- softmax --------------------------------
-    const int t = warp / 4, r = threadIdx.x % PA_BM;
+    const int t = (warp - 2) / 4, r = warp % 4 * 32 + lane;  // (TMEM lanes go by the warp's number)
     const uint32_t lane_off = (uint32_t)((warp % 4) * 32) << 16;
     const uint32_t tS = tmem + lane_off + t * 128;
     const uint32_t tO = tmem + lane_off + O_COL + t * 128;
@@ -513,38 +527,63 @@ __global__ void __launch_bounds__(PaCfg<D, NQT>::THREADS, PaCfg<D, NQT>::MIN_BLO
         const int64_t tok = first + tok0 + t * p.TQ + tl;
         const int head = h * p.G + g;
         const int64_t part = ((int64_t)share * p.T + tok) * p.Hq + head;
-#pragma unroll
-        for (int c = 0; c < D; c += 32) {
-          uint32_t ov[32];
-          tmem_ld32(tO + c, ov);
-          tmem_ld_wait32(ov);
-          if (!store) continue;
-          if (CAUSAL && direct) {
-            T* dst = reinterpret_cast<T*>(p.out) + tok * p.o_st + head * p.o_sh + c;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if (c + 8 * e >= p.D) break;
-              uint32_t pk[4];
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                pk[i] = pack2<T>(__uint_as_float(ov[8 * e + 2 * i]) * inv, __uint_as_float(ov[8 * e + 2 * i + 1]) * inv);
-              reinterpret_cast<uint4*>(dst)[e] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
-            }
-          } else {
-            float* dst = p.o_part + part * p.D + c;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              if (c + 4 * e >= p.D) break;
-              reinterpret_cast<float4*>(dst)[e] =
-                  make_float4(__uint_as_float(ov[4 * e]) * inv, __uint_as_float(ov[4 * e + 1]) * inv,
-                              __uint_as_float(ov[4 * e + 2]) * inv, __uint_as_float(ov[4 * e + 3]) * inv);
-            }
-          }
-        }
         if (store) {
           const float lse = l > 0.f ? m + lg2(l) : -INFINITY;
           if (!(CAUSAL && direct)) p.lse_part[part] = lse;
           else if (p.lse) p.lse[tok * p.Hq + head] = lse * 0.6931471805599453f;
+        }
+        // O leaves through the query tile's place in shared memory (its S are all
+        // done), so that a warp's store covers whole rows of the output: a thread's
+        // own row at a time took 8200 cycles for fp32 partial results, 2200 for
+        // 16-bit ones.  A row of W 16-byte pieces, piece k of row r at k ^ (r % W):
+        // no bank conflicts either way.  fp32 rows go in two halves.
+        constexpr int W = D / 8;
+        uint8_t* buf = sQ + t * Cfg::TILE + warp % 4 * (W * 16 * 32);
+        uint8_t* mine = buf + lane * (W * 16);
+        auto leave = [&](auto* dst, int64_t own, int per, int col0) {
+          __syncwarp();
+#pragma unroll 4
+          for (int i = 0; i < W; ++i) {
+            const int row = i * (32 / W) + lane / W, k = lane % W;
+            const int64_t to = __shfl_sync(0xffffffffu, own, row);
+            if (to >= 0 && col0 + k * per < p.D)
+              *reinterpret_cast<uint4*>(dst + to + col0 + k * per) =
+                  *reinterpret_cast<const uint4*>(buf + row * (W * 16) + ((k ^ (row % W)) << 4));
+          }
+          __syncwarp();
+        };
+        if (CAUSAL && direct) {
+#pragma unroll
+          for (int c = 0; c < D; c += 32) {
+            uint32_t ov[32];
+            tmem_ld32(tO + c, ov);
+            tmem_ld_wait32(ov);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              uint32_t pk[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                pk[i] = pack2<T>(__uint_as_float(ov[8 * e + 2 * i]) * inv, __uint_as_float(ov[8 * e + 2 * i + 1]) * inv);
+              *reinterpret_cast<uint4*>(mine + (((c / 8 + e) ^ (lane % W)) << 4)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+            }
+          }
+          leave(reinterpret_cast<T*>(p.out), store ? tok * p.o_st + head * p.o_sh : -1, 8, 0);
+        } else {
+#pragma unroll
+          for (int c0 = 0; c0 < D; c0 += D / 2) {
+#pragma unroll
+            for (int c = 0; c < D / 2; c += 32) {
+              uint32_t ov[32];
+              tmem_ld32(tO + c0 + c, ov);
+              tmem_ld_wait32(ov);
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                *reinterpret_cast<float4*>(mine + (((c / 4 + e) ^ (lane % W)) << 4)) =
+                    make_float4(__uint_as_float(ov[4 * e]) * inv, __uint_as_float(ov[4 * e + 1]) * inv,
+                                __uint_as_float(ov[4 * e + 2]) * inv, __uint_as_float(ov[4 * e + 3]) * inv);
+            }
+            leave(p.o_part, store ? part * p.D : -1, 4, c0);
+          }
         }
       }
     }

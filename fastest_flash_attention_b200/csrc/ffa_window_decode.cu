@@ -49,6 +49,9 @@ namespace cg = cooperative_groups;
 // requests of a 4096-token window, 32/8 heads, D 128.
 constexpr int WD_CHUNK = 16;
 
+// PREFIX: partial results that a thread asks for at a time.
+constexpr int FOLD = 8;
+
 struct WdParams {
   const void* q;  // [R, Hq, D]
   int64_t q_sr, q_sh;
@@ -94,10 +97,9 @@ struct WdCfg {
   // the joins overlay the rings, idle by then: per warp, then per CTA,
   // 16 rows x (m, l, O[DP])
   static constexpr int STATE = 16 * (DP + 2);        // floats
-  static constexpr int CTA_OFF = WARPS * STATE * 4;
+  static constexpr int CTA_OFF = (WARPS + 1) * STATE * 4;  // (one more for PREFIX)
   static constexpr int MERGE = CTA_OFF + STATE * 4;
   static constexpr int SMEM = (RING > MERGE ? RING : MERGE) + 1024;
-  static_assert(MERGE + 16 * PA_MAX_SHARES * 4 <= RING, "the partial results' LSEs lie behind the states");
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
@@ -385,6 +387,50 @@ __global__ void __launch_bounds__(WARPS * 32) ffa_window_decode_kernel(const WdP
     *reinterpret_cast<float2*>(wm + g * P2 + d) = make_float2(o[nt][0], o[nt][1]);
     *reinterpret_cast<float2*>(wm + (g + 8) * P2 + d) = make_float2(o[nt][2], o[nt][3]);
   }
+  // PREFIX: the prefix's shares, which the cluster's CTAs divide, are one more state
+  constexpr int STATES = WARPS + (PREFIX ? 1 : 0);
+  if constexpr (PREFIX) {
+    const int parts = shared ? min(p.shares, (shared + p.chunk - 1) / p.chunk) : 0;
+    const int64_t step = (int64_t)p.R * p.Hq;
+    float* fold = reinterpret_cast<float*>(smem) + WARPS * Cfg::STATE;
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // they are complete
+    for (int it = threadIdx.x; it < G * (p.D / 4); it += WD_THREADS) {
+      const int row = it / (p.D / 4), d = it % (p.D / 4) * 4;
+      const int64_t at = (int64_t)r * p.Hq + h * p.G + g0 + row;
+      float M = -INFINITY, L = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int s0 = split; s0 < parts; s0 += FOLD * p.splits) {  // FOLD loads in flight
+        float x[FOLD], top = M;
+        float4 v[FOLD];
+#pragma unroll
+        for (int k = 0; k < FOLD; ++k) {
+          const int s = s0 + k * p.splits;
+          x[k] = s < parts ? p.lse_part[at + s * step] : -INFINITY;
+          v[k] = s < parts ? *reinterpret_cast<const float4*>(p.o_part + (at + s * step) * p.D + d)
+                           : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int k = 0; k < FOLD; ++k) top = fmaxf(top, x[k]);
+        const float keep = M == -INFINITY ? 0.f : ex2(M - top);
+        L *= keep;
+        acc = make_float4(acc.x * keep, acc.y * keep, acc.z * keep, acc.w * keep);
+#pragma unroll
+        for (int k = 0; k < FOLD; ++k) {
+          const float f = x[k] == -INFINITY ? 0.f : ex2(x[k] - top);
+          L += f;
+          acc.x += v[k].x * f;
+          acc.y += v[k].y * f;
+          acc.z += v[k].z * f;
+          acc.w += v[k].w * f;
+        }
+        M = top;
+      }
+      float* to = fold + row * P2;
+      *reinterpret_cast<float2*>(to + 2 + d) = make_float2(acc.x, acc.y);
+      *reinterpret_cast<float2*>(to + 4 + d) = make_float2(acc.z, acc.w);
+      if (d == 0) to[0] = M, to[1] = L;
+    }
+  }
   __syncthreads();
   // `state(s)`: the s-th partial state; joins two columns of one row
   auto join = [&](int parts, auto state, int row, int d, float& M, float& L, float2& acc) {
@@ -401,42 +447,8 @@ __global__ void __launch_bounds__(WARPS * 32) ffa_window_decode_kernel(const WdP
       acc.y += v.y * f;
     }
   };
-  // PREFIX: the LSEs of the prefix's partial results, asked for at once, behind the states
-  const int parts = PREFIX && shared ? min(p.shares, (shared + p.chunk - 1) / p.chunk) : 0;
-  float* part_lse = reinterpret_cast<float*>(smem + Cfg::MERGE);  // [16 rows][PA_MAX_SHARES]
-  const int64_t part0 = (int64_t)r * p.Hq + h * p.G + g0, part_step = (int64_t)p.R * p.Hq;
-  if constexpr (PREFIX) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // they are complete
-    for (int i = threadIdx.x; i < G * parts; i += WD_THREADS)
-      part_lse[i / parts * PA_MAX_SHARES + i % parts] = p.lse_part[part0 + i / parts + i % parts * part_step];
-    __syncthreads();
-  }
   auto store = [&](int row, int d, float M, float L, float2 acc) {
     const int head = h * p.G + g0 + row;
-    if (PREFIX && parts) {  // the prefix's shares join the request's own tokens
-      const float* x = part_lse + row * PA_MAX_SHARES;
-      const float* o = p.o_part + (part0 + row) * p.D + d;
-      float top = M;
-      for (int s = 0; s < parts; ++s) top = fmaxf(top, x[s]);
-      const float own = M == -INFINITY ? 0.f : ex2(M - top);
-      L *= own;
-      acc.x *= own;
-      acc.y *= own;
-      for (int s0 = 0; s0 < parts; s0 += 8) {  // eight loads in flight
-        float2 v[8];
-#pragma unroll
-        for (int s = 0; s < 8; ++s)
-          v[s] = s0 + s < parts ? *reinterpret_cast<const float2*>(o + (s0 + s) * part_step * p.D) : make_float2(0.f, 0.f);
-#pragma unroll
-        for (int s = 0; s < 8; ++s) {
-          const float f = s0 + s < parts && x[s0 + s] != -INFINITY ? ex2(x[s0 + s] - top) : 0.f;
-          L += f;
-          acc.x += v[s].x * f;
-          acc.y += v[s].y * f;
-        }
-      }
-      M = top;
-    }
     const float inv = L > 0.f ? 1.f / L : 0.f;
     T* dst = reinterpret_cast<T*>(p.out) + (int64_t)r * p.o_sr + (int64_t)head * p.o_sh + d;
     dst[0] = wd_round<T>(acc.x * inv);
@@ -450,7 +462,7 @@ __global__ void __launch_bounds__(WARPS * 32) ffa_window_decode_kernel(const WdP
     const int row = it / (p.D / 2), d = it % (p.D / 2) * 2;
     float M, L;
     float2 acc;
-    join(WD_WARPS, [&](int s) { return warps + s * Cfg::STATE; }, row, d, M, L, acc);
+    join(STATES, [&](int s) { return warps + s * Cfg::STATE; }, row, d, M, L, acc);
     if (p.splits == 1) {
       store(row, d, M, L, acc);
     } else {
@@ -494,14 +506,26 @@ static double wd_time(int64_t pairs, int64_t visible, int D, int warps, int s) {
   return t;
 }
 
+// The same for the PREFIX form, whose requests hold anything up to `visible`
+// tokens: the CTAs' throughput at the mean length, or the longest one's own
+// time.  Measured against it (us, estimate in brackets), D 128, 512 pairs of 1
+// to 1024 tokens: 4 warps split by 1, 2, 4: 32 (31), 37 (47), 52 (78); 2 warps 39
+// (34), 41, 47.  2048 pairs of 1 to 512: 4 warps 54 (66), 91 (123); 2 warps 59 (66), 88.
+static double wd_time_ragged(int64_t pairs, int64_t visible, int D, int warps, int s) {
+  const double per_token = 4.0 * D / 6.5e6, own = (D > 64 ? 0.0136 : 0.010) * 4 / warps;
+  const double slots = 148 * (warps == 2 ? 4 : 3), mean = 0.5 * visible / s;
+  const double start = s > 1 ? 8.0 : warps == 2 ? 5.5 : 4.0;
+  return fmax(pairs * s / slots * (start + mean * slots * per_token), (double)visible / s * own) + (s > 1 ? 7.5 : 6.0);
+}
+
 // CTAs per cluster and warps per CTA with the least estimated time: powers of
 // two up to 16, no less than a chunk per warp.
-static void wd_shape(int64_t pairs, int64_t visible, int D, int& splits, int& warps) {
+static void wd_shape(bool ragged, int64_t pairs, int64_t visible, int D, int& splits, int& warps) {
   double least = 0;
   splits = 0;
   for (int w = 4; w >= (D > 64 ? 2 : 4); w -= 2)
     for (int s = 1; s <= 16 && (s == 1 || visible >= (int64_t)s * w * WD_CHUNK); s *= 2) {
-      const double t = wd_time(pairs, visible, D, w, s);
+      const double t = ragged ? wd_time_ragged(pairs, visible, D, w, s) : wd_time(pairs, visible, D, w, s);
       if (!splits || t < least) splits = s, warps = w, least = t;
     }
 }
@@ -549,7 +573,7 @@ static int window_decode(WdParams& p, int dtype, int64_t visible, cudaStream_t s
   p.head_blocks = (p.G + 15) / 16;
   const int64_t pairs = (int64_t)p.R * p.Hkv * p.head_blocks;
   int warps = 4;
-  wd_shape(pairs, visible, p.D, p.splits, warps);
+  wd_shape(PREFIX, pairs, visible, p.D, p.splits, warps);
   const int64_t grid = pairs * p.splits;
   if (grid > 0x7fffffffLL) return FFA_ERR_UNSUPPORTED;
   auto typed = [&](auto t) -> int {
