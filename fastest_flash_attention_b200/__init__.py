@@ -19,7 +19,7 @@ __version__ = "1.0.0"
 from .kv_cache import PagedKVCache, ContinuousKVCache, copy_pages, move_tokens
 from .rotary import apply_rotary, rotary_append, rotary_tables
 from .decode import paged_decode
-from .paged_prefill import paged_prefill
+from .prefill import paged_prefill
 from .prefix import prefix_decode
 from .page_table import DevicePageTable, SlotPlan, assign_slots, release_pages
 from .fa4 import FA4AttnFunc, fa4_attn_func, fa4_forward_dispatch

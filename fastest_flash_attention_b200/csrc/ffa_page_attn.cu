@@ -73,7 +73,7 @@ struct PaCfg {
   static constexpr int MIN_BLOCKS = NQT == 1 ? 2 : 1;
   static constexpr int TMEM_COLS = NQT == 1 ? 256 : 512;
   static constexpr int TILE = PA_BM * D * 2;  // a tile of Q, K or V
-  static constexpr int NBUF = NQT == 1 ? (D == 64 ? 4 : 2) : (D == 64 ? 8 : 4);
+  static constexpr int NBUF = NQT == 1 && D == 128 ? 2 : 4;
   static constexpr int KV_OFF = NQT * TILE;
   static constexpr int BAR_OFF = KV_OFF + NBUF * TILE;
   static constexpr int SMEM = BAR_OFF + 512 + 1024;
@@ -86,8 +86,8 @@ struct PaBars {
   uint64_t p_full[2][2];
   uint64_t o_done[2];
   uint64_t drain;
-  uint64_t kv_full[8];
-  uint64_t kv_empty[8];
+  uint64_t kv_full[4];
+  uint64_t kv_empty[4];
   uint32_t tmem_base;
   int abort;
 };
@@ -138,6 +138,23 @@ __device__ __forceinline__ bool pa_find(const PaParams& p, int per, int item, in
     base += __shfl_sync(0xffffffffu, incl, 31);
   }
   return false;
+}
+
+
+// 2^x for two lanes on the FMA and integer pipes: x = n + f with n whole and f in
+// [-1/2, 1/2] (adding 1.5 2^23 rounds, and leaves n in the low bits), 2^f by a
+// quartic fitted to it (least squares on Chebyshev nodes, reweighted towards
+// minimax: relative error 2.7e-6 in fp32), n added to the exponent.
+__device__ __forceinline__ float2 exp2_fma2(float2 x) {
+  const float2 t = fadd2(x, f2(12582912.f));
+  const float2 f = ffma2(fadd2(t, f2(-12582912.f)), f2(-1.f), x);
+  float2 p = ffma2(f2(0.009570098975f), f, f2(0.05591786009f));
+  p = ffma2(p, f, f2(0.240247449f));
+  p = ffma2(p, f, f2(0.6931218148f));
+  p = ffma2(p, f, f2(0.9999992614f));
+  // (below 2^-125, -inf among them, exactly 0: a masked key must not count)
+  return make_float2(x.x < -125.f ? 0.f : __int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
+                     x.y < -125.f ? 0.f : __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
 }
 
 template <typename T, int D, int NQT, bool CAUSAL>
@@ -501,7 +518,9 @@ __global__ void __launch_bounds__(PaCfg<D, NQT>::THREADS, PaCfg<D, NQT>::MIN_BLO
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const float2 a = ffma2(make_float2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), mul2, nmu2);
-          const float2 pv = make_float2(ex2(a.x), ex2(a.y));
+          // three pairs of sixteen leave the special-function unit (D 128: 256 requests
+          // behind 32 768 tokens 193 -> 184 us, two pairs 188; 64 of 4 drafted tokens 386 -> 382)
+          const float2 pv = D > 64 && e % 5 == 3 ? exp2_fma2(a) : make_float2(ex2(a.x), ex2(a.y));
           acc[e & 1] = fadd2(acc[e & 1], pv);
           pk[e] = pack2<T>(pv.x, pv.y);
         }
@@ -642,13 +661,16 @@ __global__ void ffa_page_attn_merge_kernel(const PaParams p) {
   if (lane == 0 && p.lse) p.lse[w] = L > 0.f ? (M + lg2(L)) * 0.6931471805599453f : -INFINITY;
 }
 
-// Shares of the context and query tiles per CTA.
-//   segments * blocks: CTAs of one kv head and share, at most
-PaShape pa_shape(int64_t tokens, int64_t segments, int64_t kv, int Hkv, int G) {
+// Shares of the context and query tiles per CTA.  Two tiles where a segment's rows
+// fill more than one and the head dim is above 64 (chunk of 2048 tokens, D 128: 965
+// us against 1007 with one; at D 64, whose K and V are half the bytes and whose CTAs
+// are half as long, one tile and two CTAs an SM: nine ragged prompts 180 us against
+// 202).
+PaShape pa_shape(int64_t tokens, int64_t segments, int64_t kv, int Hkv, int G, int D) {
   PaShape s;
   const int tq = 128 / G;
   const int64_t mean = (tokens + segments - 1) / segments;  // tokens of a segment
-  s.nqt = mean > tq ? 2 : 1;
+  s.nqt = D > 64 && mean > tq ? 2 : 1;
   const int64_t per = (int64_t)tq * s.nqt, slots = s.nqt == 1 ? 296 : 148;
   const int64_t base = segments * ((mean + per - 1) / per) * Hkv;
   const int64_t tiles = (kv + PA_BN - 1) / PA_BN;
@@ -740,8 +762,7 @@ int page_attn(const PaCall& c, const PaShape& shape, void* stream) {
     auto shaped = [&](auto causal) -> int {
       constexpr bool C = decltype(causal)::value;
       if (c.D <= 64)
-        return shape.nqt == 1 ? launch_page_attn<T, 64, 1, C>(mq, mk, mv, p, grid, s)
-                              : launch_page_attn<T, 64, 2, C>(mq, mk, mv, p, grid, s);
+        return launch_page_attn<T, 64, 1, C>(mq, mk, mv, p, grid, s);
       return shape.nqt == 1 ? launch_page_attn<T, 128, 1, C>(mq, mk, mv, p, grid, s)
                             : launch_page_attn<T, 128, 2, C>(mq, mk, mv, p, grid, s);
     };
@@ -791,7 +812,7 @@ extern "C" size_t ffa_paged_prefill_workspace_size(int R, int T, int Hq, int Hkv
   using namespace ffa;
   if (R <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || Hq / Hkv > 128 || D <= 0 || D > 128 || max_ctx < 0)
     return 0;
-  return pa_workspace(T, Hq, D, pa_shape(T, R, max_ctx, Hkv, Hq / Hkv).shares);
+  return pa_workspace(T, Hq, D, pa_shape(T, R, max_ctx, Hkv, Hq / Hkv, D).shares);
 }
 
 extern "C" int ffa_paged_prefill(const void* q, const void* k_pages, const void* v_pages, const int* block_table,
@@ -830,7 +851,7 @@ extern "C" int ffa_paged_prefill(const void* q, const void* k_pages, const void*
   if (int s = pa_check(c)) return s;
   if (!out || !o_strides || max_ctx < 0 || !aligned16(out) || o_strides[0] % 8 || o_strides[1] % 8)
     return FFA_ERR_INVALID_ARG;
-  const PaShape shape = pa_shape(T, R, max_ctx, Hkv, Hq / Hkv);
+  const PaShape shape = pa_shape(T, R, max_ctx, Hkv, Hq / Hkv, D);
   const size_t need = pa_workspace(T, Hq, D, shape.shares);
   if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return FFA_ERR_WORKSPACE;
   return page_attn(c, shape, stream);

@@ -34,7 +34,7 @@ struct PaShape {
   int nqt, shares, chunk;
 };
 
-PaShape pa_shape(int64_t tokens, int64_t segments, int64_t kv, int Hkv, int G);
+PaShape pa_shape(int64_t tokens, int64_t segments, int64_t kv, int Hkv, int G, int D);
 int pa_check(const PaCall& c);
 size_t pa_workspace(int64_t T, int Hq, int D, int shares);
 int page_attn(const PaCall& c, const PaShape& shape, void* stream);

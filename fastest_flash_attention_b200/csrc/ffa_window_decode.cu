@@ -641,15 +641,15 @@ extern "C" int ffa_window_decode(const void* q, const void* k_pages, const void*
 }
 
 // The shares of a prefix: ffa_page_attn.cu's shape, with a workspace for every one.
-static ffa::PaShape prefix_shape(int R, int groups, int Hq, int Hkv, int max_prefix) {
-  return ffa::pa_shape(R, groups, max_prefix, Hkv, Hq / Hkv);
+static ffa::PaShape prefix_shape(int R, int groups, int Hq, int Hkv, int D, int max_prefix) {
+  return ffa::pa_shape(R, groups, max_prefix, Hkv, Hq / Hkv, D);
 }
 
 extern "C" size_t ffa_prefix_decode_workspace_size(int R, int groups, int Hq, int Hkv, int D, int max_prefix) {
   if (R <= 0 || groups <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || Hq / Hkv > 128 || D <= 0 || D > 128 ||
       max_prefix < 0)
     return 0;
-  return (size_t)R * Hq * prefix_shape(R, groups, Hq, Hkv, max_prefix).shares * (D + 1) * 4;
+  return (size_t)R * Hq * prefix_shape(R, groups, Hq, Hkv, D, max_prefix).shares * (D + 1) * 4;
 }
 
 extern "C" int ffa_prefix_decode(const void* q, const void* k_pages, const void* v_pages, const int* block_table,
@@ -686,7 +686,7 @@ extern "C" int ffa_prefix_decode(const void* q, const void* k_pages, const void*
   if (!ctx_lens || !out || !o_strides || groups < 0 || max_prefix < 0 || max_own < 0) return FFA_ERR_INVALID_ARG;
   WdParams p{};
   if (groups) {
-    const PaShape shape = prefix_shape(R, groups, Hq, Hkv, max_prefix);
+    const PaShape shape = prefix_shape(R, groups, Hq, Hkv, D, max_prefix);
     const size_t need = ffa_prefix_decode_workspace_size(R, groups, Hq, Hkv, D, max_prefix);
     if (!workspace || workspace_bytes < need || !aligned16(workspace)) return FFA_ERR_WORKSPACE;
     if (int s = page_attn(c, shape, stream)) return s;

@@ -466,7 +466,7 @@ class PagedKVCache:
                 scale: Optional[float] = None, softcap: Optional[float] = None, return_lse: bool = False):
         """Causal attention of the last new_lens[i] cached tokens of each sequence (appended before) over its
         cached K/V: q [sum(new_lens), Hq, D], the sequences' queries behind one another."""
-        from .paged_prefill import paged_prefill
+        from .prefill import paged_prefill
 
         if len(new_lens) != len(seq_ids) or sum(new_lens) != q.shape[0]:
             raise ValueError(f"{q.shape[0]} queries for {len(seq_ids)} sequences with {list(new_lens)} new tokens")

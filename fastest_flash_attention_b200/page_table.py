@@ -30,19 +30,19 @@ class SlotPlan(NamedTuple):
 
 def _check(block_table: torch.Tensor, ctx_lens: torch.Tensor, free_pages: torch.Tensor, free_state: torch.Tensor,
            rows: torch.Tensor, what: str, page_size: int) -> Tuple[int, int, int]:
-    if block_table.dim() != 2 or block_table.shape[1] == 0 or free_pages.dim() != 1 or free_pages.numel() == 0:
+    table, ring = block_table.shape, free_pages.shape
+    if len(table) != 2 or table[1] == 0 or len(ring) != 1 or ring[0] == 0:
         raise ValueError("block_table must be [R, max_pages] and free_pages [num_pages]")
-    R, width = block_table.shape
-    if tuple(ctx_lens.shape) != (R,) or tuple(rows.shape) != (R,) or tuple(free_state.shape) != (2,):
+    R, width = table
+    if ctx_lens.shape != (R,) or rows.shape != (R,) or free_state.shape != (2,):
         raise ValueError(f"ctx_lens and {what} must be [{R}] and free_state [2], got {tuple(ctx_lens.shape)}, "
                          f"{tuple(rows.shape)} and {tuple(free_state.shape)}")
-    for name, t in (("block_table", block_table), ("ctx_lens", ctx_lens), ("free_pages", free_pages),
-                    ("free_state", free_state)):
+    for t in (block_table, ctx_lens, free_pages, free_state):
         if t.dtype is not torch.int32 or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous int32 tensor")
+            raise ValueError("block_table, ctx_lens, free_pages and free_state must be contiguous int32 tensors")
     if page_size <= 0:
         raise ValueError(f"page_size must be positive, got {page_size}")
-    return R, width, free_pages.numel()
+    return R, width, ring[0]
 
 
 def assign_slots(block_table: torch.Tensor, ctx_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: torch.Tensor,
@@ -73,21 +73,19 @@ def assign_slots(block_table: torch.Tensor, ctx_lens: torch.Tensor, new_lens: to
     new_lens = _lib.int32(new_lens)
     # one allocation: slots and positions (each at a multiple of 16 bytes), starts, and the lengths and state where
     # they are not written over
-    room = (max_tokens + 3) // 4 * 4
-    buf = ctx_lens.new_empty(2 * room + R + 1 + (0 if advance else R + 2))
-    slots, positions, starts = buf[:max_tokens], buf[room:room + max_tokens], buf[2 * room:2 * room + R + 1]
-    lens_out, state_out = (ctx_lens, free_state) if advance else buf[2 * room + R + 1:].split([R, 2])
-    plan = SlotPlan(slots, positions, starts, lens_out, state_out)
+    sizes = [max_tokens, -max_tokens % 4, max_tokens, -max_tokens % 4, R + 1] + ([] if advance else [R, 2])
+    slots, _, positions, _, starts, *rest = ctx_lens.new_empty(sum(sizes)).split_with_sizes(sizes)
+    lens_out, state_out = rest or (ctx_lens, free_state)
     with _lib.device_of(ctx_lens):
         st = _lib.direct().ffa_assign_slots(
             block_table.data_ptr(), width, ctx_lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr(),
-            free_state.data_ptr(), plan.slots.data_ptr(), plan.positions.data_ptr(), plan.starts.data_ptr(),
+            free_state.data_ptr(), slots.data_ptr(), positions.data_ptr(), starts.data_ptr(),
             lens_out.data_ptr(), state_out.data_ptr(), R, P, page_size, max_tokens, _lib.err_ptr(ctx_lens),
             _lib.stream_of(ctx_lens))
     _lib.check(st, "ffa_assign_slots")
     if _lib.sync_check_enabled():
         _lib.check_device_errors(ctx_lens.device)
-    return plan
+    return SlotPlan(slots, positions, starts, lens_out, state_out)
 
 
 def release_pages(block_table: torch.Tensor, ctx_lens: torch.Tensor, done: torch.Tensor, free_pages: torch.Tensor,

@@ -18,14 +18,16 @@ import torch
 from . import _lib
 
 
-def check_pools(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, what: str) -> None:
-    """Raise unless q [tokens, Hq, D] and the pools [P, Hkv, page_size, D] fit the tensor-core kernels over pages."""
-    if q.dim() != 3 or k_pages.dim() != 4:
-        raise ValueError(f"q must be [tokens, Hq, D] and the pools [P, Hkv, page_size, D], got {tuple(q.shape)} and "
-                         f"{tuple(k_pages.shape)}")
-    Hq, D = q.shape[1:]
-    P, Hkv, page_size, Dk = k_pages.shape
-    if Dk != D or v_pages.shape != k_pages.shape:
+def check_pools(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, what: str) -> tuple:
+    """(tokens, Hq, D, P, Hkv, page_size) of q [tokens, Hq, D] and the pools [P, Hkv, page_size, D]; raises unless
+    they fit the tensor-core kernels over pages."""
+    qs, ks = q.shape, k_pages.shape
+    if len(qs) != 3 or len(ks) != 4:
+        raise ValueError(f"q must be [tokens, Hq, D] and the pools [P, Hkv, page_size, D], got {tuple(qs)} and "
+                         f"{tuple(ks)}")
+    T, Hq, D = qs
+    P, Hkv, page_size, Dk = ks
+    if Dk != D or v_pages.shape != ks:
         raise ValueError("q / page pool head dims disagree")
     if P == 0 or Hkv == 0 or Hq == 0 or Hq % Hkv or Hq // Hkv > 128:
         raise ValueError(f"query heads ({Hq}) must be a multiple of key/value heads ({Hkv}), at most 128 times")
@@ -33,10 +35,12 @@ def check_pools(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, w
         raise ValueError(f"{what} takes head dims up to 128 that are multiples of 8, got {D}")
     if page_size == 0 or page_size % 8:
         raise ValueError(f"{what} takes page sizes that are multiples of 8, got {page_size}")
-    if q.dtype not in _lib.DTYPE_CODE or k_pages.dtype != q.dtype or v_pages.dtype != q.dtype:
+    dt = q.dtype
+    if dt not in _lib.DTYPE_CODE or k_pages.dtype is not dt or v_pages.dtype is not dt:
         raise ValueError(f"{what} needs fp16/bf16 q and pages of the same dtype")
     if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
         raise ValueError("page pools must be contiguous")
+    return T, Hq, D, P, Hkv, page_size
 
 
 def check_scale(scale: Optional[float], softcap: Optional[float], D: int) -> tuple:
@@ -83,19 +87,17 @@ def paged_prefill(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     device error word.
     """
     _lib.require_cuda(q, k_pages, v_pages, block_table, ctx_lens, query_starts, out)
-    check_pools(q, k_pages, v_pages, "paged_prefill")
-    T, Hq, D = q.shape
-    P, Hkv, page_size, _ = k_pages.shape
-    if block_table.dim() != 2 or block_table.shape[1] == 0 or tuple(ctx_lens.shape) != (block_table.shape[0],) \
-            or tuple(query_starts.shape) != (block_table.shape[0] + 1,):
+    T, Hq, D, P, Hkv, page_size = check_pools(q, k_pages, v_pages, "paged_prefill")
+    table = block_table.shape
+    if len(table) != 2 or table[1] == 0 or ctx_lens.shape != (table[0],) or query_starts.shape != (table[0] + 1,):
         raise ValueError(f"block_table must be [R, max_pages], ctx_lens [R] and query_starts [R + 1], got "
-                         f"{tuple(block_table.shape)}, {tuple(ctx_lens.shape)} and {tuple(query_starts.shape)}")
+                         f"{tuple(table)}, {tuple(ctx_lens.shape)} and {tuple(query_starts.shape)}")
     if max_ctx is not None and max_ctx < 0:
         raise ValueError(f"max_ctx must not be negative, got {max_ctx}")
     scale, softcap = check_scale(scale, softcap, D)
-    R, width = block_table.shape
+    R, width = table
     if out is None:
-        out = q.new_empty((T, Hq, D))
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 or (out.stride(0) | out.stride(1)) % 8 \
             or out.data_ptr() % 16:
         raise ValueError("out must be like q, with contiguous heads and other strides and the base multiples of 16 bytes")

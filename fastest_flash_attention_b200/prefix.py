@@ -15,7 +15,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .paged_prefill import check_pools, check_scale, tma_rows
+from .prefill import check_pools, check_scale, tma_rows
 
 
 @functools.lru_cache(maxsize=1024)
@@ -45,20 +45,19 @@ def prefix_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     outside the pool set the device error word.
     """
     _lib.require_cuda(q, k_pages, v_pages, block_table, ctx_lens, group_starts, prefix_lens)
-    check_pools(q, k_pages, v_pages, "prefix_decode")
-    R, Hq, D = q.shape
-    P, Hkv, page_size, _ = k_pages.shape
-    if block_table.dim() != 2 or block_table.shape[0] != R or block_table.shape[1] == 0 or tuple(ctx_lens.shape) != (R,):
-        raise ValueError(f"block_table must be [{R}, max_pages] and ctx_lens [{R}], got {tuple(block_table.shape)} and "
+    R, Hq, D, P, Hkv, page_size = check_pools(q, k_pages, v_pages, "prefix_decode")
+    table, groups = block_table.shape, prefix_lens.shape
+    if len(table) != 2 or table[0] != R or table[1] == 0 or ctx_lens.shape != (R,):
+        raise ValueError(f"block_table must be [{R}, max_pages] and ctx_lens [{R}], got {tuple(table)} and "
                          f"{tuple(ctx_lens.shape)}")
-    if prefix_lens.dim() != 1 or tuple(group_starts.shape) != (prefix_lens.shape[0] + 1,):
+    if len(groups) != 1 or group_starts.shape != (groups[0] + 1,):
         raise ValueError(f"group_starts must be [G + 1] and prefix_lens [G], got {tuple(group_starts.shape)} and "
-                         f"{tuple(prefix_lens.shape)}")
+                         f"{tuple(groups)}")
     if (max_prefix or 0) < 0 or (max_own or 0) < 0:
         raise ValueError(f"max_prefix and max_own must not be negative, got {max_prefix} and {max_own}")
     scale, softcap = check_scale(scale, softcap, D)
-    width, groups = block_table.shape[1], prefix_lens.shape[0]
-    out = q.new_empty((R, Hq, D))
+    width, groups = table[1], groups[0]
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = q.new_empty((R, Hq), dtype=torch.float32) if return_lse else None
     if R == 0:
         return (out, lse) if return_lse else out
