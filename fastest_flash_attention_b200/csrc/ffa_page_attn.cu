@@ -43,7 +43,7 @@
 
 namespace ffa {
 
-constexpr int PA_BM = 128, PA_BN = 128;
+constexpr int PA_BM = 128, PA_BN = 128;  // rows of a query tile; the unit of a context's shares
 
 struct PaParams {
   const int* starts;  // [N + 1] first query token of each segment
@@ -66,18 +66,23 @@ struct PaParams {
 
 template <int D, int NQT>
 struct PaCfg {
-  // NQT = 1: 6 warps, two CTAs per SM (each half the TMEM; the two interleave on
-  // the tensor core).  NQT = 2: 10 warps, one CTA, K and V read once for both tiles.
-  // At most 168 registers a thread either way.
+  // D = 128, NQT = 1: 6 warps, two CTAs per SM (each half the TMEM; the two
+  // interleave on the tensor core).  NQT = 2: 10 warps, one CTA, K and V read once
+  // for both tiles.  At most 168 registers a thread either way.
+  // D = 64, where the exponentials outweigh the products: key tiles of 64, a quarter
+  // of the TMEM, four CTAs per SM, so that some softmax always has its scores.
+  static constexpr int BN = D == 64 ? 64 : 128;  // keys of a tile
   static constexpr int THREADS = (4 * NQT + 2) * 32;
-  static constexpr int MIN_BLOCKS = NQT == 1 ? 2 : 1;
-  static constexpr int TMEM_COLS = NQT == 1 ? 256 : 512;
-  static constexpr int TILE = PA_BM * D * 2;  // a tile of Q, K or V
+  static constexpr int MIN_BLOCKS = NQT == 2 ? 1 : D == 64 ? 4 : 2;
+  static constexpr int TMEM_COLS = 512 / MIN_BLOCKS;
+  static constexpr int O_COL = NQT * BN;      // TMEM: S_t / P_t at [128 t, ...), O_t at O_COL + 128 t
+  static constexpr int TILE = PA_BM * D * 2;  // a tile of Q
+  static constexpr int KV_TILE = BN * D * 2;  // a tile of K or V
   static constexpr int NBUF = NQT == 1 && D == 128 ? 2 : 4;
   static constexpr int KV_OFF = NQT * TILE;
-  static constexpr int BAR_OFF = KV_OFF + NBUF * TILE;
+  static constexpr int BAR_OFF = KV_OFF + NBUF * KV_TILE;
   static constexpr int SMEM = BAR_OFF + 512 + 1024;
-  static_assert(SMEM <= (NQT == 1 ? 113 : 227) * 1024, "shared memory budget");
+  static_assert(MIN_BLOCKS * (SMEM + 1024) <= 228 * 1024, "shared memory budget");
 };
 
 struct PaBars {
@@ -163,8 +168,9 @@ __global__ void __launch_bounds__(PaCfg<D, NQT>::THREADS, PaCfg<D, NQT>::MIN_BLO
                          const __grid_constant__ CUtensorMap tmV, const PaParams p) {
   using Cfg = PaCfg<D, NQT>;
   constexpr int WARP_MMA = 0, WARP_LOAD = 1;  // then four softmax warps for each query tile
-  constexpr uint32_t O_COL = NQT * 128;  // TMEM: S_t / P_t at [128 t, ...), O_t at O_COL + 128 t
-  constexpr int HALVES = D / 64, HALF = PA_BN * 128;
+  constexpr int O_COL = Cfg::O_COL, BN = Cfg::BN;
+  constexpr int HALVES = D / 64, HALF = 128 * 128;  // 64-column halves of a tile (two only where BN = 128)
+  static_assert(HALVES == 1 || BN == 128, "a half's bytes");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;
@@ -218,7 +224,7 @@ __global__ void __launch_bounds__(PaCfg<D, NQT>::THREADS, PaCfg<D, NQT>::MIN_BLO
   const int kv0 = share * p.chunk;
   const int kv1 = share + 1 == p.shares ? limit : min(limit, kv0 + p.chunk);
   if (kv0 >= kv1) return;
-  const int n_tiles = (kv1 - kv0 + PA_BN - 1) / PA_BN;
+  const int n_tiles = (kv1 - kv0 + BN - 1) / BN;
 
   if (threadIdx.x == 0) {
     mbar_init(&bars->q_full, 1);
@@ -259,8 +265,8 @@ __global__ void __launch_bounds__(PaCfg<D, NQT>::THREADS, PaCfg<D, NQT>::MIN_BLO
     // pool row of this lane's box of a tile, or -1 (past the last key, or a page
     // id outside the pool, which is recorded)
     auto box_row = [&](int j) -> int {
-      const int tok = kv0 + j * PA_BN + lane * p.box;
-      if (lane * p.box >= PA_BN || tok >= kv1) return -1;
+      const int tok = kv0 + j * BN + lane * p.box;
+      if (lane * p.box >= BN || tok >= kv1) return -1;
       const int i = tok / p.page_size;
       const int page = table[i];
       if ((unsigned)page >= (unsigned)p.num_pages) {
@@ -284,7 +290,7 @@ __global__ void __launch_bounds__(PaCfg<D, NQT>::THREADS, PaCfg<D, NQT>::MIN_BLO
         ++issued;
         __syncwarp();
         if (at >= 0) {
-          uint8_t* dst = sKV + buf * Cfg::TILE + lane * p.box * 128;
+          uint8_t* dst = sKV + buf * Cfg::KV_TILE + lane * p.box * 128;
 #pragma unroll
           for (int c = 0; c < HALVES; ++c)
             tma_load_4d(v ? &tmV : &tmK, &bars->kv_full[buf], dst + c * HALF, c * 64, at, 0, 0, pol);
@@ -307,7 +313,7 @@ __global__ void __launch_bounds__(PaCfg<D, NQT>::THREADS, PaCfg<D, NQT>::MIN_BLO
         return __all_sync(0xffffffffu, mbar_wait_mma(bar, parity, p.ec, abort_flag, site));
       };
       constexpr uint32_t FMT = DtypeFmt<T>::value;
-      const uint32_t idesc_qk = make_idesc_f16(PA_BM, PA_BN, FMT, 0, 0);
+      const uint32_t idesc_qk = make_idesc_f16(PA_BM, BN, FMT, 0, 0);
       const uint32_t idesc_pv = make_idesc_f16(PA_BM, D, FMT, 0, 1);
       const uint64_t q_base = make_sdesc_sw128(smem_u32(sQ), 16, 1024);
       const uint64_t k_base = make_sdesc_sw128(smem_u32(sKV), 16, 1024);
@@ -326,8 +332,8 @@ __global__ void __launch_bounds__(PaCfg<D, NQT>::THREADS, PaCfg<D, NQT>::MIN_BLO
       auto issue_pv = [&](auto tile, uint64_t vb, bool acc, auto hf) {
         constexpr int t = decltype(tile)::value, half = decltype(hf)::value;
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          const int ks = half * 4 + kk;
+        for (int kk = 0; kk < BN / 32; ++kk) {
+          const int ks = half * (BN / 32) + kk;
           mma_ts_warp(tmem + O_COL + t * 128, tmem + t * 128 + ks * 8, vb + (uint64_t)((ks * 16 * 128) >> 4), idesc_pv,
                       (acc || ks > 0) ? 1u : 0u);
         }
@@ -348,7 +354,7 @@ __global__ void __launch_bounds__(PaCfg<D, NQT>::THREADS, PaCfg<D, NQT>::MIN_BLO
       }
       for (int j = 0; j < n_tiles && ok; ++j) {
         const int vs = 2 * j + 1, ks = 2 * j + 2, vi = vs % Cfg::NBUF, ki = ks % Cfg::NBUF;
-        const uint64_t vb = v_base + (uint64_t)((vi * Cfg::TILE) >> 4), kb = k_base + (uint64_t)((ki * Cfg::TILE) >> 4);
+        const uint64_t vb = v_base + (uint64_t)((vi * Cfg::KV_TILE) >> 4), kb = k_base + (uint64_t)((ki * Cfg::KV_TILE) >> 4);
         ok = wait(&bars->kv_full[vi], (vs / Cfg::NBUF) & 1, SITE_PA_KV_FULL);
         tiles([&](auto t) {
           constexpr int n = decltype(t)::value;  // (the query tile)
@@ -395,7 +401,7 @@ __global__ void __launch_bounds__(PaCfg<D, NQT>::THREADS, PaCfg<D, NQT>::MIN_BLO
         // tanh by its polynomial where every argument of the warp is within 1/2
         float top = 0.f;
 #pragma unroll 1
-        for (int c = 0; c < PA_BN; c += 32) {
+        for (int c = 0; c < BN; c += 32) {
           uint32_t s[32];
           tmem_ld32(tS + c, s);
           tmem_ld_wait32(s);
@@ -405,7 +411,7 @@ __global__ void __launch_bounds__(PaCfg<D, NQT>::THREADS, PaCfg<D, NQT>::MIN_BLO
         small = __all_sync(0xffffffffu, top * p.sc_pre <= 0.5f);
       }
 #pragma unroll 1
-      for (int c = 0; c < PA_BN; c += 32) {
+      for (int c = 0; c < BN; c += 32) {
         uint32_t s[32];
         tmem_ld32(tS + c, s);
         tmem_ld_wait32(s);
@@ -432,11 +438,11 @@ __global__ void __launch_bounds__(PaCfg<D, NQT>::THREADS, PaCfg<D, NQT>::MIN_BLO
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int j = 0; j < n_tiles; ++j) {
-      const int c0 = kv0 + j * PA_BN;
+      const int c0 = kv0 + j * BN;
       ok = __all_sync(0xffffffffu, mbar_wait(&bars->s_full[t], j & 1, p.ec, abort_flag, SITE_PA_S_FULL));
       if (!ok) break;
       tc_fence_after();
-      if (t == 0 && c0 + PA_BN > limit) {
+      if (t == 0 && c0 + BN > limit) {
         // The last tile ends past the visible keys: V's rows there become zeros.
         // (Only now: S_j is issued after V_(j-1) was waited for, so the barrier
         // is in this tile's phase; before that its parity would not tell.)
@@ -444,8 +450,8 @@ __global__ void __launch_bounds__(PaCfg<D, NQT>::THREADS, PaCfg<D, NQT>::MIN_BLO
         ok = __all_sync(0xffffffffu, mbar_wait(&bars->kv_full[s % Cfg::NBUF], (s / Cfg::NBUF) & 1, p.ec, abort_flag,
                                                SITE_PA_KV_FULL));
         if (!ok) break;
-        uint8_t* vt = sKV + s % Cfg::NBUF * Cfg::TILE;
-        const int drop = (limit - c0) * 8, all = PA_BN * 8;  // 16-byte pieces of a half
+        uint8_t* vt = sKV + s % Cfg::NBUF * Cfg::KV_TILE;
+        const int drop = (limit - c0) * 8, all = BN * 8;  // 16-byte pieces of a half
         for (int i = drop + r; i < all; i += PA_BM)
 #pragma unroll
           for (int c = 0; c < HALVES; ++c) *reinterpret_cast<uint4*>(vt + c * HALF + i * 16) = make_uint4(0, 0, 0, 0);
@@ -463,16 +469,18 @@ __global__ void __launch_bounds__(PaCfg<D, NQT>::THREADS, PaCfg<D, NQT>::MIN_BLO
       // scores back to TMEM, so that the two passes below stay free of both.
       // Scores are then in base-2 units as s * mul.
       float mul = p.scale_log2;
-      if (p.use_softcap || c0 + PA_BN > vis_min) mul = rewrite(vis - c0);
+      if (p.use_softcap || c0 + BN > vis_min) mul = rewrite(vis - c0);
       // first pass: the row's maximum (scale is positive)
-      uint32_t sc[64];  // two pieces of 32 columns: the next is on its way while one is worked on
+      constexpr bool AHEAD = D > 64;  // the next 32 columns are on their way while these are worked on
+      uint32_t sc[AHEAD ? 64 : 32];   // (D = 64: other CTAs fill the wait, and registers are few)
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      tmem_ld32(tS, sc);
+      if (AHEAD) tmem_ld32(tS, sc);
 #pragma unroll
-      for (int c = 0; c < PA_BN; c += 32) {
-        uint32_t* s = sc + c % 64;
+      for (int c = 0; c < BN; c += 32) {
+        uint32_t* s = sc + (AHEAD ? c % 64 : 0);
+        if (!AHEAD) tmem_ld32(tS + c, s);
         tmem_ld_wait32(s);
-        tmem_ld32(tS + (c + 32) % PA_BN, sc + (c + 32) % 64);  // (the last one: the second pass's first)
+        if (AHEAD) tmem_ld32(tS + (c + 32) % BN, sc + (c + 32) % 64);  // (the last one: the second pass's first)
 #pragma unroll
         for (int e = 0; e < 32; e += 8)
 #pragma unroll
@@ -510,11 +518,12 @@ __global__ void __launch_bounds__(PaCfg<D, NQT>::THREADS, PaCfg<D, NQT>::MIN_BLO
       const float2 mul2 = f2(mul), nmu2 = f2(-mu);
       float2 acc[2] = {f2(0.f), f2(0.f)};
 #pragma unroll
-      for (int c = 0; c < PA_BN; c += 32) {
+      for (int c = 0; c < BN; c += 32) {
         uint32_t pk[16];
-        uint32_t* s = sc + c % 64;
+        uint32_t* s = sc + (AHEAD ? c % 64 : 0);
+        if (!AHEAD) tmem_ld32(tS + c, s);
         tmem_ld_wait32(s);
-        if (c + 32 < PA_BN) tmem_ld32(tS + c + 32, sc + (c + 32) % 64);
+        if (AHEAD && c + 32 < BN) tmem_ld32(tS + c + 32, sc + (c + 32) % 64);
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const float2 a = ffma2(make_float2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), mul2, nmu2);
@@ -525,11 +534,11 @@ __global__ void __launch_bounds__(PaCfg<D, NQT>::THREADS, PaCfg<D, NQT>::MIN_BLO
           pk[e] = pack2<T>(pv.x, pv.y);
         }
         tmem_st16(tS + c / 2, pk);
-        if (c == 32 || c == 96) {
+        if ((c + 32) % (BN / 2) == 0) {
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bars->p_full[t][c / 64]);
+          if (lane == 0) mbar_arrive(&bars->p_full[t][c / (BN / 2)]);
         }
       }
       const float2 a = fadd2(acc[0], acc[1]);
@@ -671,7 +680,7 @@ PaShape pa_shape(int64_t tokens, int64_t segments, int64_t kv, int Hkv, int G, i
   const int tq = 128 / G;
   const int64_t mean = (tokens + segments - 1) / segments;  // tokens of a segment
   s.nqt = D > 64 && mean > tq ? 2 : 1;
-  const int64_t per = (int64_t)tq * s.nqt, slots = s.nqt == 1 ? 296 : 148;
+  const int64_t per = (int64_t)tq * s.nqt, slots = s.nqt == 2 ? 148 : D > 64 ? 296 : 592;
   const int64_t base = segments * ((mean + per - 1) / per) * Hkv;
   const int64_t tiles = (kv + PA_BN - 1) / PA_BN;
   // time of a CTA: 4 us of start and end, and a key tile at a time; a partial
@@ -727,7 +736,7 @@ int page_attn(const PaCall& c, const PaShape& shape, void* stream) {
   p.num_pages = c.num_pages;
   p.page_size = c.page_size;
   p.box = 8;
-  while (p.box < 128 && c.page_size % (2 * p.box) == 0) p.box *= 2;
+  while (p.box < (c.D <= 64 ? 64 : 128) && c.page_size % (2 * p.box) == 0) p.box *= 2;  // (at most a key tile)
   p.max_ctx = c.width * c.page_size;
   p.shares = shape.shares;
   p.chunk = shape.chunk;
