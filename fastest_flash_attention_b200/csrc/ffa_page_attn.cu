@@ -59,7 +59,7 @@ struct PaParams {
   int N, T, Hq, Hkv, G, TQ, D;
   int num_pages, page_size, box, max_ctx;
   int shares, chunk;  // a segment's tokens [s * chunk, (s + 1) * chunk), the last share the rest
-  float scale_log2, sc_pre, sc_post, sc_poly[3];
+  float scale_log2, sc_pre, sc_unit, sc_poly[3];  // scale log2 e; scale / softcap, and its inverse
   int use_softcap, keep_kv;  // keep_kv: other CTAs read the same K and V
   ErrCtx ec;
 };
@@ -393,47 +393,58 @@ __global__ void __launch_bounds__(PaCfg<D, NQT>::THREADS, PaCfg<D, NQT>::MIN_BLO
     // keys [0, vis) are visible to this row (a row past the segment's last token is computed like the last)
     const int vis = CAUSAL ? past + tok0 + t * p.TQ + min(tl, t_toks - 1) + 1 : limit;
     const int vis_min = CAUSAL ? past + tok0 + t * p.TQ + 1 : limit;
-    // S with a softcap applied and columns from `hi` on at -inf, written back;
-    // returns the factor that takes it to base-2 units
+    constexpr bool AHEAD = D > 64;  // 32 columns are on their way while 32 are worked on
+    uint32_t sc[AHEAD ? 64 : 32];   // (D = 64: other CTAs fill the wait, and registers are few)
+    // First pass where scores change: softcapped, -inf from column `hi` on, written
+    // back to TMEM; returns their maximum.  A softcap becomes y with tanh(k s) = k y,
+    // k = scale / softcap, so that scores keep one factor: by the polynomial where
+    // every argument of the warp's 32 columns is within 1/2.
     auto rewrite = [&](int hi) -> float {
-      bool small = true;
-      if (p.use_softcap) {
-        // tanh by its polynomial where every argument of the warp is within 1/2
-        float top = 0.f;
-#pragma unroll 1
-        for (int c = 0; c < BN; c += 32) {
-          uint32_t s[32];
-          tmem_ld32(tS + c, s);
-          tmem_ld_wait32(s);
-#pragma unroll
-          for (int e = 0; e < 32; ++e) top = c + e < hi ? fmaxf(top, fabsf(__uint_as_float(s[e]))) : top;
-        }
-        small = __all_sync(0xffffffffu, top * p.sc_pre <= 0.5f);
-      }
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
       for (int c = 0; c < BN; c += 32) {
         uint32_t s[32];
         tmem_ld32(tS + c, s);
         tmem_ld_wait32(s);
-        if (p.use_softcap && small) {
+        if (p.use_softcap) {
+          float lo[4] = {0.f, 0.f, 0.f, 0.f};
+          if (c + 32 <= hi) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const float2 y = softcap_small2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), p.sc_poly[0],
-                                            p.sc_poly[1], p.sc_poly[2]);
-            s[e] = __float_as_uint(y.x);
-            s[e + 1] = __float_as_uint(y.y);
+            for (int e = 0; e < 32; e += 8)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                lo[i] = fmax3(lo[i], fabsf(__uint_as_float(s[e + i])), fabsf(__uint_as_float(s[e + i + 4])));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) lo[e % 4] = c + e < hi ? fmaxf(lo[e % 4], fabsf(__uint_as_float(s[e]))) : lo[e % 4];
           }
-        } else if (p.use_softcap) {
+          if (__all_sync(0xffffffffu, fmaxf(fmaxf(lo[0], lo[1]), fmaxf(lo[2], lo[3])) * p.sc_pre <= 0.5f)) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(tanh_acc(__uint_as_float(s[e]) * p.sc_pre));
+            for (int e = 0; e < 32; e += 2) {
+              const float2 y = softcap_small2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])),
+                                              p.sc_poly[0], p.sc_poly[1], p.sc_poly[2]);
+              s[e] = __float_as_uint(y.x);
+              s[e + 1] = __float_as_uint(y.y);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              s[e] = __float_as_uint(tanh_acc(__uint_as_float(s[e]) * p.sc_pre) * p.sc_unit);
+          }
         }
+        if (!__all_sync(0xffffffffu, c + 32 <= hi)) {
 #pragma unroll
-        for (int e = 0; e < 32; ++e)
-          if (c + e >= hi) s[e] = __float_as_uint(-INFINITY);
+          for (int e = 0; e < 32; ++e)
+            if (c + e >= hi) s[e] = __float_as_uint(-INFINITY);
+        }
         tmem_st32(tS + c, s);
+#pragma unroll
+        for (int e = 0; e < 32; e += 8)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mx[i] = fmax3(mx[i], __uint_as_float(s[e + i]), __uint_as_float(s[e + i + 4]));
       }
       tmem_st_wait();
-      return p.use_softcap && !small ? p.sc_post : p.scale_log2;
+      return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
     };
     float m = -INFINITY, l = 0.f;
     bool ok = true;
@@ -465,28 +476,30 @@ __global__ void __launch_bounds__(PaCfg<D, NQT>::THREADS, PaCfg<D, NQT>::MIN_BLO
         }
         continue;
       }
-      // Tiles with masked keys, and softcaps: a pass of its own that writes the
-      // scores back to TMEM, so that the two passes below stay free of both.
-      // Scores are then in base-2 units as s * mul.
-      float mul = p.scale_log2;
-      if (p.use_softcap || c0 + BN > vis_min) mul = rewrite(vis - c0);
-      // first pass: the row's maximum (scale is positive)
-      constexpr bool AHEAD = D > 64;  // the next 32 columns are on their way while these are worked on
-      uint32_t sc[AHEAD ? 64 : 32];   // (D = 64: other CTAs fill the wait, and registers are few)
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      if (AHEAD) tmem_ld32(tS, sc);
+      // First pass: the row's maximum, in base-2 units (scale is positive).  Softcaps
+      // and masks are written back to TMEM in a pass of its own, so that the second
+      // pass knows neither.
+      float top;
+      if (p.use_softcap || c0 + BN > vis_min) {
+        top = rewrite(vis - c0);
+        if (AHEAD) tmem_ld32(tS, sc);
+      } else {
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        if (AHEAD) tmem_ld32(tS, sc);
 #pragma unroll
-      for (int c = 0; c < BN; c += 32) {
-        uint32_t* s = sc + (AHEAD ? c % 64 : 0);
-        if (!AHEAD) tmem_ld32(tS + c, s);
-        tmem_ld_wait32(s);
-        if (AHEAD) tmem_ld32(tS + (c + 32) % BN, sc + (c + 32) % 64);  // (the last one: the second pass's first)
+        for (int c = 0; c < BN; c += 32) {
+          uint32_t* s = sc + (AHEAD ? c % 64 : 0);
+          if (!AHEAD) tmem_ld32(tS + c, s);
+          tmem_ld_wait32(s);
+          if (AHEAD) tmem_ld32(tS + (c + 32) % BN, sc + (c + 32) % 64);  // (the last one: the second pass's first)
 #pragma unroll
-        for (int e = 0; e < 32; e += 8)
+          for (int e = 0; e < 32; e += 8)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) mx[i] = fmax3(mx[i], __uint_as_float(s[e + i]), __uint_as_float(s[e + i + 4]));
+            for (int i = 0; i < 4; ++i) mx[i] = fmax3(mx[i], __uint_as_float(s[e + i]), __uint_as_float(s[e + i + 4]));
+        }
+        top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
       }
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * mul;
+      top *= p.scale_log2;
       const float m_new = fmaxf(m, top);
       if (__any_sync(0xffffffffu, m_new > m + 8.f)) {
         // lazy rescale: exact, numerator and denominator share the stale maximum
@@ -515,7 +528,7 @@ __global__ void __launch_bounds__(PaCfg<D, NQT>::THREADS, PaCfg<D, NQT>::MIN_BLO
       }
       // second pass: P over S, handed over in two halves of 64 keys
       const float mu = m == -INFINITY ? 0.f : m;
-      const float2 mul2 = f2(mul), nmu2 = f2(-mu);
+      const float2 mul2 = f2(p.scale_log2), nmu2 = f2(-mu);
       float2 acc[2] = {f2(0.f), f2(0.f)};
 #pragma unroll
       for (int c = 0; c < BN; c += 32) {
@@ -746,7 +759,7 @@ int page_attn(const PaCall& c, const PaShape& shape, void* stream) {
   p.scale_log2 = c.scale * 1.4426950408889634f;
   p.use_softcap = c.softcap > 0.f;
   p.sc_pre = p.use_softcap ? c.scale / c.softcap : 0.f;
-  p.sc_post = p.use_softcap ? c.softcap * 1.4426950408889634f : 0.f;
+  p.sc_unit = p.use_softcap ? c.softcap / c.scale : 0.f;
   softcap_poly_coeffs(p.sc_pre, p.sc_poly);
   const int64_t per = (int64_t)p.TQ * shape.nqt;
   const int64_t items = c.N + c.T / per;  // the sum of ceil(n / per) over segments of c.T tokens is at most this

@@ -73,9 +73,13 @@ def assign_slots(block_table: torch.Tensor, ctx_lens: torch.Tensor, new_lens: to
     new_lens = _lib.int32(new_lens)
     # one allocation: slots and positions (each at a multiple of 16 bytes), starts, and the lengths and state where
     # they are not written over
-    sizes = [max_tokens, -max_tokens % 4, max_tokens, -max_tokens % 4, R + 1] + ([] if advance else [R, 2])
-    slots, _, positions, _, starts, *rest = ctx_lens.new_empty(sum(sizes)).split_with_sizes(sizes)
-    lens_out, state_out = rest or (ctx_lens, free_state)
+    pad = -max_tokens % 4
+    sizes = [max_tokens, pad, max_tokens, pad, R + 1, R, 2] if pad else [max_tokens, max_tokens, R + 1, R, 2]
+    if advance:
+        sizes = sizes[:-2]
+    parts = ctx_lens.new_empty(sum(sizes)).split_with_sizes(sizes)
+    slots, positions, starts = (parts[0], parts[2], parts[4]) if pad else parts[:3]
+    lens_out, state_out = (ctx_lens, free_state) if advance else parts[-2:]
     with _lib.device_of(ctx_lens):
         st = _lib.direct().ffa_assign_slots(
             block_table.data_ptr(), width, ctx_lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr(),
