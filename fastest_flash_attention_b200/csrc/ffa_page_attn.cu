@@ -111,9 +111,28 @@ enum : uint32_t {
 // its segment, the segment's first token, tokens and keys, and the block within
 // it.  CTAs that run long start early: of a segment the block with the most keys
 // comes first and, where contexts are not cut into shares of one length, so do of
-// every 32 segments those with the most keys (nine ragged prompts 196 -> 172 us).
+// every 32 segments those with the most keys (nine ragged prompts 161 -> 151 us).
+// Of more segments than a warp's lanes the last blocks come first, segment by
+// segment, so that of many with one block each none is searched for.
 __device__ __forceinline__ bool pa_find(const PaParams& p, int per, int item, int lane, int& seg, int& first, int& n,
                                         int& kv, int& block) {
+  const bool many = p.N > 32;
+  auto bad = [&](int lo, int hi) -> bool {
+    if (lo >= 0 && hi >= lo && hi <= p.T) return false;
+    if (p.ec.err) atomicCAS(p.ec.err, 0u, SITE_PA_BAD_STARTS);
+    return true;
+  };
+  if (many && item < p.N) {
+    seg = item;
+    first = p.starts[seg];
+    const int end = p.starts[seg + 1];
+    kv = p.kv_lens[seg];
+    if (bad(first, end)) return false;
+    n = end - first;
+    block = (n + per - 1) / per - 1;
+    return n > 0;
+  }
+  if (many) item -= p.N;
   int base = 0;
   for (int i0 = 0; i0 < p.N; i0 += 32) {
     const int i = i0 + lane;
@@ -122,12 +141,9 @@ __device__ __forceinline__ bool pa_find(const PaParams& p, int per, int item, in
       lo = p.starts[i];
       hi = p.starts[i + 1];
       keys = p.kv_lens[i];
-      if (lo < 0 || hi < lo || hi > p.T) {
-        if (p.ec.err) atomicCAS(p.ec.err, 0u, SITE_PA_BAD_STARTS);
-        lo = hi = 0;
-      }
+      if (bad(lo, hi)) lo = hi = 0;
     }
-    const int blocks = (hi - lo + per - 1) / per;
+    const int blocks = max((hi - lo + per - 1) / per - (many ? 1 : 0), 0);
     int before = base, all = 0;  // blocks of the segments that come before this lane's; of the 32
     if (p.shares == 1) {
       for (int k = 0; k < min(32, p.N - i0); ++k) {
@@ -665,15 +681,9 @@ __global__ void ffa_page_attn_merge_kernel(const PaParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (w >= (int64_t)p.T * p.Hq) return;
   const int tok = (int)(w / p.Hq), head = (int)(w % p.Hq);
-  // the request: the last one that starts at or before the token
-  int seg = -1;
-  for (int i0 = 0; i0 < p.N; i0 += 32) {
-    const uint32_t has = __ballot_sync(0xffffffffu, i0 + lane < p.N && p.starts[i0 + lane] <= tok);
-    if (has) seg = i0 + 31 - __clz(has);
-  }
-  if (seg < 0) return;
+  const int seg = warp_search(p.starts, p.N, tok, lane);  // the request
   const int first = p.starts[seg], end = p.starts[seg + 1], kv = p.kv_lens[seg], n = end - first;
-  if (first < 0 || tok >= end || end > p.T || kv < n || kv > p.max_ctx || kv <= p.chunk) return;
+  if (first < 0 || tok < first || tok >= end || end > p.T || kv < n || kv > p.max_ctx || kv <= p.chunk) return;
   const int vis = kv - n + tok - first + 1;
   const int parts = min(p.shares, (vis + p.chunk - 1) / p.chunk);
   const int64_t step = (int64_t)p.T * p.Hq;
@@ -714,16 +724,20 @@ PaShape pa_shape(int64_t tokens, int64_t segments, int64_t kv, int Hkv, int G, i
   const int64_t per = (int64_t)tq * s.nqt, slots = s.nqt == 2 ? 148 : D > 64 ? 296 : 592;
   const int64_t base = segments * ((mean + per - 1) / per) * Hkv;
   const int64_t tiles = (kv + PA_BN - 1) / PA_BN;
-  // time of a CTA: 4 us of start and end, and a key tile at a time; a partial
-  // result costs its writing and reading
+  // time of a CTA: 5 us of start and end, and its key tiles (us a tile, alone on an
+  // SM and with its slots full; the latter at the memory's rate where nobody else
+  // reads the same keys); a partial result costs its writing and reading
+  const double alone = 1.9, shared = s.nqt == 2 ? 2.05 : D > 64 ? 2.1 : 3.7;
+  const double fresh = PA_BN * D * 4.0 * slots / 6.5e6, full = mean > per || fresh < shared ? shared : fresh;
   double least = 0;
   int64_t best = 1;
   for (int64_t n = 1; n <= tiles && n <= PA_MAX_SHARES; ++n) {
     const int64_t each = (tiles + n - 1) / n, used = (tiles + each - 1) / each;
     if (used != n) continue;
-    const int64_t waves = (base * n + slots - 1) / slots;
-    double t = waves * (4.0 + each * (s.nqt == 1 ? 2.0 : 2.2));
-    if (n > 1) t += 2.0 + (double)n * tokens * Hkv * G * 1024 / 4.0e6;
+    const int64_t ctas = base * n, waves = (ctas + slots - 1) / slots;
+    const double load = ctas < slots ? (double)ctas / slots : 1.0;
+    double t = waves * (5.0 + each * (alone + (full > alone ? full - alone : 0.0) * load));
+    if (n > 1) t += 2.0 + (double)n * tokens * Hkv * G * D * 8 / 6.0e6;
     if (n == 1 || t < least) least = t, best = n;
   }
   const int64_t each = (tiles + best - 1) / best;

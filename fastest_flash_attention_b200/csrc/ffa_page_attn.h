@@ -12,6 +12,22 @@ enum : uint32_t { SITE_PA_BAD_STARTS = 0x3E6 };
 
 constexpr int PA_MAX_SHARES = 64;
 
+#ifdef __CUDACC__
+// Last i in [0, n) with a[i] <= x in ascending a (0 if there is none), by one warp:
+// 32 places at a time.
+__device__ __forceinline__ int warp_search(const int* a, int n, int x, int lane) {
+  int lo = 0;
+  for (int len = n; len > 1;) {
+    const int step = (len + 31) / 32, at = lo + lane * step;
+    const uint32_t below = __ballot_sync(0xffffffffu, lane * step < len && a[at < n ? at : n - 1] <= x);
+    const int skip = (below ? 31 - __clz(below) : 0) * step;
+    lo += skip;
+    len = step < len - skip ? step : len - skip;
+  }
+  return lo;
+}
+#endif
+
 struct PaCall {
   const void *q, *k_pages, *v_pages;
   const int* block_table;

@@ -147,21 +147,19 @@ __device__ __forceinline__ __nv_bfloat16 wd_round<__nv_bfloat16>(float x) { retu
 template <>
 __device__ __forceinline__ __half wd_round<__half>(float x) { return __float2half_rn(x); }
 
-// Tokens of request r that its group's partial results cover: the group's
-// prefix, unless the request is shorter (it then shares nothing).  One warp.
-__device__ __forceinline__ int wd_prefix(const WdParams& p, int r, int ctx, int lane) {
+// Prefix length of request r's group (0: in none), found by one warp.  A request
+// shorter than it shares nothing.
+__device__ __forceinline__ int wd_prefix(const WdParams& p, int r, int lane) {
   if (p.groups == 0) return 0;
-  int before = 0, len = 0;  // groups that start at or before r; this lane's prefix length
-  for (int i0 = 0; i0 <= p.groups; i0 += 32) {
-    const int i = i0 + lane;
-    const bool le = i <= p.groups && p.starts[i] <= r;
-    if (p.groups < 32 && i < p.groups) len = p.prefix_lens[i];  // (asked for with the starts, not after them)
-    before += __popc(__ballot_sync(0xffffffffu, le));
+  if (p.groups >= 32) {
+    const int g = warp_search(p.starts, p.groups + 1, r, lane);
+    return g < p.groups && p.starts[g] <= r ? p.prefix_lens[g] : 0;
   }
-  const int g = before - 1;
-  if (g < 0 || g >= p.groups) return 0;
-  len = p.groups < 32 ? __shfl_sync(0xffffffffu, len, g) : p.prefix_lens[g];
-  return len > 0 && len <= ctx ? len : 0;
+  // few groups: their lengths asked for with the starts, not after them
+  const bool le = lane <= p.groups && p.starts[lane] <= r;
+  const int len = lane < p.groups ? p.prefix_lens[lane] : 0;
+  const int g = __popc(__ballot_sync(0xffffffffu, le)) - 1;
+  return g < 0 || g >= p.groups ? 0 : __shfl_sync(0xffffffffu, len, g);
 }
 
 template <typename T, int DP, int WARPS, bool PREFIX>
@@ -180,11 +178,12 @@ __global__ void __launch_bounds__(WARPS * 32) ffa_window_decode_kernel(const WdP
   const int g0 = hb * 16, G = min(16, p.G - g0);  // query heads h * p.G + g0 + [0, G)
 
   int ctx = p.ctx_lens[r];
+  const int prefix = PREFIX ? wd_prefix(p, r, lane) : 0;  // (its loads travel with the length's)
   if (ctx < 0 || ctx > p.max_ctx) {
     if (threadIdx.x == 0 && p.err) atomicCAS(p.err, 0u, SITE_DEC_BAD_CTX);
     ctx = 0;
   }
-  const int shared = PREFIX ? wd_prefix(p, r, ctx, lane) : 0;
+  const int shared = prefix > 0 && prefix <= ctx ? prefix : 0;
   const int w0 = PREFIX ? shared : max(ctx - p.window, 0);
   WdRows rows;
   rows.table = p.block_table + (int64_t)r * p.bt_stride;

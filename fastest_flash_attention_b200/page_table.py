@@ -168,9 +168,9 @@ class DevicePageTable:
             raise ValueError(f"{tokens} tokens are past a row's {self.block_table.shape[1]} pages")
         if not 0 <= owner < R or any(not 0 <= r < R or r == owner for r in rows) or len(set(rows)) < len(rows):
             raise ValueError(f"rows must be distinct, in [0, {R}) and not the owner's")
-        idx = torch.tensor(list(rows), dtype=torch.int64).to(self.block_table.device, non_blocking=True)
-        self.block_table[idx, :n] = self.block_table[owner, :n]
-        self.ctx_lens[idx] = tokens
+        for r in rows:
+            self.block_table[r, :n].copy_(self.block_table[owner, :n])
+            self.ctx_lens[r] = tokens
 
     @property
     def num_free_pages(self) -> int:

@@ -79,6 +79,10 @@ CASES = [
     ([400, 20], [9, 20], 40, 128, 1, 8, None, torch.float16),                # group of 128, head dim 8, page 40
     ([33] * 70, [1] * 70, 16, 16, 8, 128, 50.0, torch.bfloat16),             # more requests than a warp's lanes
     ([6000], [1500], 16, 4, 1, 64, None, torch.bfloat16),
+    # more requests than lanes, of no token, one block and several
+    ([(37 * i) % 300 + i % 3 for i in range(45)], [((37 * i) % 300 + i % 3) // (1 + i % 4) for i in range(45)], 16, 12, 3,
+     64, None, torch.float16),
+    ([900 + i for i in range(40)], [(i * 29) % 90 for i in range(40)], 64, 8, 2, 128, None, torch.bfloat16),
 ]
 
 
