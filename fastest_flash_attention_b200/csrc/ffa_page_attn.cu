@@ -284,6 +284,7 @@ __global__ void __launch_bounds__(PaCfg<D, NQT>::THREADS, PaCfg<D, NQT>::MIN_BLO
   tc_fence_after();
   const uint32_t tmem = bars->tmem_base;
 
+  int issued = 0;  // (producer) slots armed so far
   if (warp == WARP_LOAD) {
     // ------------------------------- producer -------------------------------
     const uint64_t pol = p.keep_kv ? policy_evict_last() : policy_evict_first();
@@ -310,7 +311,6 @@ __global__ void __launch_bounds__(PaCfg<D, NQT>::THREADS, PaCfg<D, NQT>::MIN_BLO
       return (page * p.Hkv + h) * p.page_size + tok - i * p.page_size;
     };
     int at = box_row(0);
-    int issued = 0;
     bool ok = true;
     for (int j = 0; j < n_tiles && ok; ++j) {
       const int next = j + 1 < n_tiles ? box_row(j + 1) : -1;
@@ -332,13 +332,6 @@ __global__ void __launch_bounds__(PaCfg<D, NQT>::THREADS, PaCfg<D, NQT>::MIN_BLO
       }
       at = next;
     }
-    if (*abort_flag && lane == 0) {
-      // let copies still in flight land before the CTA gives up its smem
-      mbar_wait(&bars->q_full, 0, p.ec, abort_flag, SITE_PA_DRAIN, true);
-      for (int s = max(0, issued - Cfg::NBUF); s < issued; ++s)
-        mbar_wait(&bars->kv_full[s % Cfg::NBUF], (s / Cfg::NBUF) & 1, p.ec, abort_flag, SITE_PA_DRAIN, true);
-    }
-    __syncwarp();
   } else if (warp == WARP_MMA) {
     // ------------------------------ MMA issuer ------------------------------
     {
@@ -669,6 +662,12 @@ __global__ void __launch_bounds__(PaCfg<D, NQT>::THREADS, PaCfg<D, NQT>::MIN_BLO
   if (warp == WARP_MMA) {
     tc_fence_after();
     tmem_dealloc(tmem, Cfg::TMEM_COLS);
+  }
+  if (*abort_flag && warp == WARP_LOAD && lane == 0) {
+    // a wait gave up somewhere: copies still in flight land before the CTA's smem is another's
+    mbar_wait(&bars->q_full, 0, p.ec, abort_flag, SITE_PA_DRAIN, true);
+    for (int s = max(0, issued - Cfg::NBUF); s < issued; ++s)
+      mbar_wait(&bars->kv_full[s % Cfg::NBUF], (s / Cfg::NBUF) & 1, p.ec, abort_flag, SITE_PA_DRAIN, true);
   }
 }
 
