@@ -64,11 +64,14 @@ struct PaParams {
   ErrCtx ec;
 };
 
-template <int D, int NQT>
+template <int D, int NQT, bool FEW>
 struct PaCfg {
   // D = 128, NQT = 1: 6 warps, two CTAs per SM (each half the TMEM; the two
   // interleave on the tensor core).  NQT = 2: 10 warps, one CTA, K and V read once
   // for both tiles.  At most 168 registers a thread either way.
+  // FEW (D = 128, at most 32 rows, NQT = 1): Q takes 8 KB, which leaves room for a
+  // third slot of the ring: bound by memory, whose latency two slots do not cover.
+  // (The products read 128 rows there all the same, whatever lies behind Q's.)
   // D = 64, where the exponentials outweigh the products: key tiles of 64, a quarter
   // of the TMEM, four CTAs per SM, so that some softmax always has its scores.
   static constexpr int BN = D == 64 ? 64 : 128;  // keys of a tile
@@ -76,9 +79,10 @@ struct PaCfg {
   static constexpr int MIN_BLOCKS = NQT == 2 ? 1 : D == 64 ? 4 : 2;
   static constexpr int TMEM_COLS = 512 / MIN_BLOCKS;
   static constexpr int O_COL = NQT * BN;      // TMEM: S_t / P_t at [128 t, ...), O_t at O_COL + 128 t
-  static constexpr int TILE = PA_BM * D * 2;  // a tile of Q
+  static constexpr int Q_ROWS = FEW ? 32 : PA_BM;
+  static constexpr int TILE = Q_ROWS * D * 2;  // a tile of Q
   static constexpr int KV_TILE = BN * D * 2;  // a tile of K or V
-  static constexpr int NBUF = NQT == 1 && D == 128 ? 2 : 4;
+  static constexpr int NBUF = FEW ? 3 : NQT == 1 && D == 128 ? 2 : 4;
   static constexpr int KV_OFF = NQT * TILE;
   static constexpr int BAR_OFF = KV_OFF + NBUF * KV_TILE;
   static constexpr int SMEM = BAR_OFF + 512 + 1024;
@@ -192,14 +196,14 @@ __device__ __forceinline__ float2 exp2_fma2(float2 x) {
                      x.y < -125.f ? 0.f : __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
 }
 
-template <typename T, int D, int NQT, bool CAUSAL>
-__global__ void __launch_bounds__(PaCfg<D, NQT>::THREADS, PaCfg<D, NQT>::MIN_BLOCKS)
+template <typename T, int D, int NQT, bool FEW, bool CAUSAL>
+__global__ void __launch_bounds__(PaCfg<D, NQT, FEW>::THREADS, PaCfg<D, NQT, FEW>::MIN_BLOCKS)
     ffa_page_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                          const __grid_constant__ CUtensorMap tmV, const PaParams p) {
-  using Cfg = PaCfg<D, NQT>;
+  using Cfg = PaCfg<D, NQT, FEW>;
   constexpr int WARP_MMA = 0, WARP_LOAD = 1;  // then four softmax warps for each query tile
   constexpr int O_COL = Cfg::O_COL, BN = Cfg::BN;
-  constexpr int HALVES = D / 64, HALF = 128 * 128;  // 64-column halves of a tile (two only where BN = 128)
+  constexpr int HALVES = D / 64, HALF = 128 * 128, Q_HALF = Cfg::Q_ROWS * 128;  // 64-column halves of a tile
   static_assert(HALVES == 1 || BN == 128, "a half's bytes");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -293,7 +297,7 @@ __global__ void __launch_bounds__(PaCfg<D, NQT>::THREADS, PaCfg<D, NQT>::MIN_BLO
       mbar_arrive_expect_tx(&bars->q_full, tiles_q * HALVES * q_rows * 128);
       for (int t = 0; t < tiles_q; ++t)
         for (int c = 0; c < HALVES; ++c)
-          tma_load_4d(&tmQ, &bars->q_full, sQ + t * Cfg::TILE + c * HALF, c * 64, 0, first + tok0 + t * p.TQ, h, pol);
+          tma_load_4d(&tmQ, &bars->q_full, sQ + t * Cfg::TILE + c * Q_HALF, c * 64, 0, first + tok0 + t * p.TQ, h, pol);
     }
     __syncwarp();
     const int* table = p.table + (int64_t)row * p.bt_stride;
@@ -350,9 +354,8 @@ __global__ void __launch_bounds__(PaCfg<D, NQT>::THREADS, PaCfg<D, NQT>::MIN_BLO
         constexpr int t = decltype(tile)::value;
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
-          const int off = (ks / 4) * HALF + (ks % 4) * 32;
-          mma_ss_warp(tmem + t * 128, q_base + (uint64_t)((t * Cfg::TILE + off) >> 4), kb + (uint64_t)(off >> 4),
-                      idesc_qk, ks > 0);
+          const int qo = t * Cfg::TILE + (ks / 4) * Q_HALF + (ks % 4) * 32, ko = (ks / 4) * HALF + (ks % 4) * 32;
+          mma_ss_warp(tmem + t * 128, q_base + (uint64_t)(qo >> 4), kb + (uint64_t)(ko >> 4), idesc_qk, ks > 0);
         }
         mma_commit_warp(&bars->s_full[t]);
       };
@@ -717,8 +720,9 @@ __global__ void ffa_page_attn_merge_kernel(const PaParams p) {
 // 202).
 PaShape pa_shape(int64_t tokens, int64_t segments, int64_t kv, int Hkv, int G, int D) {
   PaShape s;
-  const int tq = 128 / G;
   const int64_t mean = (tokens + segments - 1) / segments;  // tokens of a segment
+  s.rows = D > 64 && mean * G <= 32 ? 32 : 128;
+  const int tq = s.rows / G;
   s.nqt = D > 64 && mean > tq ? 2 : 1;
   const int64_t per = (int64_t)tq * s.nqt, slots = s.nqt == 2 ? 148 : D > 64 ? 296 : 592;
   const int64_t base = segments * ((mean + per - 1) / per) * Hkv;
@@ -745,11 +749,11 @@ PaShape pa_shape(int64_t tokens, int64_t segments, int64_t kv, int Hkv, int G, i
   return s;
 }
 
-template <typename T, int D, int NQT, bool CAUSAL>
+template <typename T, int D, int NQT, bool FEW, bool CAUSAL>
 static int launch_page_attn(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const PaParams& p,
                             int64_t grid, cudaStream_t st) {
-  using Cfg = PaCfg<D, NQT>;
-  auto kern = ffa_page_attn_kernel<T, D, NQT, CAUSAL>;
+  using Cfg = PaCfg<D, NQT, FEW>;
+  auto kern = ffa_page_attn_kernel<T, D, NQT, FEW, CAUSAL>;
   static std::atomic<uint64_t> done{0};
   if (int s = smem_attr_once(kern, Cfg::SMEM, done)) return s;
   kern<<<(unsigned)grid, Cfg::THREADS, Cfg::SMEM, st>>>(mq, mk, mv, p);
@@ -775,7 +779,7 @@ int page_attn(const PaCall& c, const PaShape& shape, void* stream) {
   p.Hq = c.Hq;
   p.Hkv = c.Hkv;
   p.G = c.Hq / c.Hkv;
-  p.TQ = 128 / p.G;
+  p.TQ = shape.rows / p.G;
   p.D = c.D;
   p.num_pages = c.num_pages;
   p.page_size = c.page_size;
@@ -815,9 +819,10 @@ int page_attn(const PaCall& c, const PaShape& shape, void* stream) {
     auto shaped = [&](auto causal) -> int {
       constexpr bool C = decltype(causal)::value;
       if (c.D <= 64)
-        return launch_page_attn<T, 64, 1, C>(mq, mk, mv, p, grid, s);
-      return shape.nqt == 1 ? launch_page_attn<T, 128, 1, C>(mq, mk, mv, p, grid, s)
-                            : launch_page_attn<T, 128, 2, C>(mq, mk, mv, p, grid, s);
+        return launch_page_attn<T, 64, 1, false, C>(mq, mk, mv, p, grid, s);
+      if (shape.rows == 32) return launch_page_attn<T, 128, 1, true, C>(mq, mk, mv, p, grid, s);
+      return shape.nqt == 1 ? launch_page_attn<T, 128, 1, false, C>(mq, mk, mv, p, grid, s)
+                            : launch_page_attn<T, 128, 2, false, C>(mq, mk, mv, p, grid, s);
     };
     if (!c.causal) return shaped(std::false_type{});
     int status = shaped(std::true_type{});

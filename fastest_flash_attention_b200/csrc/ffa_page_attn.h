@@ -44,10 +44,11 @@ struct PaCall {
   uint32_t* dev_err;
 };
 
-// Query tiles per CTA, and the shares that a context is cut into: share s takes
-// tokens [s * chunk, (s + 1) * chunk), the last one all that follow.
+// Query tiles per CTA and rows in use of each (128, or 32), and the shares that a
+// context is cut into: share s takes tokens [s * chunk, (s + 1) * chunk), the last
+// one all that follow.
 struct PaShape {
-  int nqt, shares, chunk;
+  int nqt, rows, shares, chunk;
 };
 
 PaShape pa_shape(int64_t tokens, int64_t segments, int64_t kv, int Hkv, int G, int D);
