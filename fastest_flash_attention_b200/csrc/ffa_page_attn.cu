@@ -716,12 +716,14 @@ __global__ void ffa_page_attn_merge_kernel(const PaParams p) {
 // Shares of the context and query tiles per CTA.  Two tiles where a segment's rows
 // fill more than one and the head dim is above 64 (chunk of 2048 tokens, D 128: 965
 // us against 1007 with one; at D 64, whose K and V are half the bytes and whose CTAs
-// are half as long, one tile and two CTAs an SM: nine ragged prompts 180 us against
-// 202).
+// are half as long, one tile: nine ragged prompts 180 us against 202).  The form for
+// 32 rows where segments have at most 16 on average, so that twice as many still
+// fit (64 requests of 16 rows 363 us against 378 in the form for 128; 17 requests of
+// 2 to 58 rows, which take two blocks then, 165 against 94).
 PaShape pa_shape(int64_t tokens, int64_t segments, int64_t kv, int Hkv, int G, int D) {
   PaShape s;
   const int64_t mean = (tokens + segments - 1) / segments;  // tokens of a segment
-  s.rows = D > 64 && mean * G <= 32 ? 32 : 128;
+  s.rows = D > 64 && mean * G <= 16 ? 32 : 128;
   const int tq = s.rows / G;
   s.nqt = D > 64 && mean > tq ? 2 : 1;
   const int64_t per = (int64_t)tq * s.nqt, slots = s.nqt == 2 ? 148 : D > 64 ? 296 : 592;
