@@ -12,16 +12,15 @@
 // 128 rows for each byte of the prefix instead of G.
 //
 // One CTA owns NQT tiles of 128 rows of one (segment, kv head), a segment being
-// a request or a group, and walks key tiles of 128 tokens of one share of the
-// context:
+// a request or a group, and walks key tiles of 128 tokens (64 at D = 64) of one
+// share of the context:
 //   warp LOAD  TMA producer: Q once (one box of G x floor(128 / G) rows for
 //              each 64 columns), then K_j and V_j into a ring of slots, in boxes
 //              of `box` rows, the largest power of two that divides the page
 //              size (a box never leaves its page); a lane each looks its box's
 //              page up one tile ahead
 //   warp MMA   S_t = Q_t K_j^T into TMEM, O_t += P_t V_j with P_t from TMEM; the
-//              whole warp in step, one lane issuing (2048 tokens behind 30 720, 32/8
-//              heads of 128: 1061 us issued by a single thread's code, 959 so)
+//              whole warp in step, one lane issuing (mma_ss_warp)
 //   4 warps for each query tile: thread = row = TMEM lane.  Two passes over S
 //              in TMEM (maximum, then 2^(s - m) written back as 16-bit P), so
 //              that a row never lives in registers whole.
@@ -35,6 +34,20 @@
 // merge kernel (prefill) or the decode kernel (prefix) joins them.
 // P is rounded to the data's type once, as the tensor core's operand; the row
 // sums add the unrounded values; statistics, O and the join are fp32.
+//
+// What bounds it, by the rows that share K and V:
+//   many (2048 tokens behind 30 720, 32/8 heads of 128: 945-980 us, 1090-1130
+//     TFLOP/s, 0.65-0.67 of a measured GEMM): the chain S - softmax - P V of the
+//     two query tiles, about 3500 cycles for a key tile of both against 2048 of
+//     products and as many of exponentials.  On that case, us: issued by a single
+//     thread's code 1061, by the warp 959; two threads a row 1096; S in two
+//     buffers of 64 keys 1031; an issuing warp for each tile 1234; scores kept in
+//     registers 1396 against 1313; the tiles taking turns at the exponentials no
+//     faster.
+//   few (64 requests of 4 tokens at 512 to 16 388: 360 us, 6.2 TB/s, 0.94 of a
+//     measured copy): memory.
+//   D = 64 (nine ragged prompts, 20 heads: 150-165 us): latencies and the
+//     exponentials, 512 of the 825 cycles that a step of 64 keys takes an SM.
 #include "ffa_common.cuh"
 #include "ffa_host.h"
 #include "ffa_page_attn.h"

@@ -15,6 +15,9 @@
 // written over the inputs, and an invalid call changes nothing), then the CTAs
 // share tokens and pages, each of which finds its row by bisection.
 // Bound by latencies in sequence: launch, lengths, scan, meeting, table entry.
+// Device time: 64 requests of one token 6.0 us, 131 072 prompt tokens of 1024
+// requests 12.9 (35.5 by bisection alone with 8 CTAs of 512 threads), 33 000 pages
+// of 64 requests given back 6.3 (12.4).
 #include <cooperative_groups.h>
 
 #include "ffa_common.cuh"
