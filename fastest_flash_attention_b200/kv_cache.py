@@ -496,12 +496,14 @@ class PagedKVCache:
             from .prefix import prefix_decode
 
             starts, prefixes = self.prefix_groups(seq_ids)
-            own = max(self.sequences[s]["len"] - n for b, e, n in zip(starts, starts[1:], prefixes)
+            if not any(prefixes):  # nothing is shared: no group
+                starts, prefixes = [0], []
+            own = 0 if not prefixes else max(self.sequences[s]["len"] - n for b, e, n in zip(starts, starts[1:], prefixes)
                       for s in seq_ids[b:e])
             meta = torch.tensor(starts + prefixes, dtype=torch.int32).to(q.device)
             return prefix_decode(q, self.k_pages, self.v_pages, bt, lens, meta[:len(starts)], meta[len(starts):],
-                                 scale=scale, softcap=softcap, return_lse=return_lse, max_prefix=max(prefixes),
-                                 max_own=own)
+                                 scale=scale, softcap=softcap, return_lse=return_lse,
+                                 max_prefix=max(prefixes, default=0), max_own=own or max_ctx)
         return paged_decode(q, self.k_pages, self.v_pages, bt, lens, scale=scale, softcap=softcap,
                             return_lse=return_lse, max_ctx=max_ctx, sliding_window=sliding_window,
                             sink_tokens=sink_tokens)

@@ -162,7 +162,8 @@ def test_host_cache_prefill_and_shared_decode():
     ids = [0, 1, 2, 3, 9]
     assert c.prefix_groups(ids) == ([0, 4, 5], [496, 0])
     q = rand(5, H)
-    for softcap in (None, 30.0):
+    for softcap, ids in ((None, ids), (30.0, ids), (None, [1, 9, 2, 9, 3])):
+        # (the last: neighbours that share nothing)
         o, lse = c.decode(q, ids, share_prefix=True, return_lse=True, softcap=softcap)
         o2, lse2 = c.decode(q, ids, return_lse=True, softcap=softcap)
         V = float(c.v_pages.abs().max())
