@@ -734,7 +734,7 @@ __global__ void ffa_page_attn_merge_kernel(const PaParams p) {
 // fit (64 requests of 16 rows 363 us against 378 in the form for 128; 17 requests of
 // 2 to 58 rows, which take two blocks then, 165 against 94).
 PaShape pa_shape(int64_t tokens, int64_t segments, int64_t kv, int Hkv, int G, int D) {
-  PaShape s;
+  PaShape s{};
   const int64_t mean = (tokens + segments - 1) / segments;  // tokens of a segment
   s.rows = D > 64 && mean * G <= 16 ? 32 : 128;
   const int tq = s.rows / G;
@@ -747,6 +747,8 @@ PaShape pa_shape(int64_t tokens, int64_t segments, int64_t kv, int Hkv, int G, i
   // reads the same keys); a partial result costs its writing and reading
   const double alone = 1.9, shared = s.nqt == 2 ? 2.05 : D > 64 ? 2.1 : 3.7;
   const double fresh = PA_BN * D * 4.0 * slots / 6.5e6, full = mean > per || fresh < shared ? shared : fresh;
+  // (a CTA of one query tile where others have two is done in about half the time)
+  const double busy = 0.5 + 0.5 * (double)((mean + tq - 1) / tq) / (double)((mean + per - 1) / per * s.nqt);
   double least = 0;
   int64_t best = 1;
   for (int64_t n = 1; n <= tiles && n <= PA_MAX_SHARES; ++n) {
@@ -756,7 +758,11 @@ PaShape pa_shape(int64_t tokens, int64_t segments, int64_t kv, int Hkv, int G, i
     const double load = ctas < slots ? (double)ctas / slots : 1.0;
     double t = waves * (5.0 + each * (alone + (full > alone ? full - alone : 0.0) * load));
     if (n > 1) t += 2.0 + (double)n * tokens * Hkv * G * D * 8 / 6.0e6;
-    if (n == 1 || t < least) least = t, best = n;
+    if (n == 1 || t < least) {
+      least = t, best = n;
+      s.time = (float)t;
+      s.idle = (float)(1.0 - (double)ctas / (double)(waves * slots) * busy);
+    }
   }
   const int64_t each = (tiles + best - 1) / best;
   s.shares = (int)best;

@@ -46,9 +46,11 @@ struct PaCall {
 
 // Query tiles per CTA and rows in use of each (128, or 32), and the shares that a
 // context is cut into: share s takes tokens [s * chunk, (s + 1) * chunk), the last
-// one all that follow.
+// one all that follow.  `time`: estimated (us); `idle`: the part of its CTAs'
+// slots that is empty meanwhile.
 struct PaShape {
   int nqt, rows, shares, chunk;
+  float time, idle;
 };
 
 PaShape pa_shape(int64_t tokens, int64_t segments, int64_t kv, int Hkv, int G, int D);

@@ -31,7 +31,9 @@
 // shared prefix: a request that shares attends its own tokens alone, those
 // behind the prefix, and joins the partial results that ffa_page_attn.cu left
 // for its rows.  It starts while that kernel still runs (programmatic launch:
-// its loads need nothing of it) and waits for it only before the join.
+// its loads need nothing of it) and waits for it only before the join.  Where
+// the prefix leaves SMs idle for long, it leaves a partial result of its own
+// tokens instead, and a third launch joins them, so that nothing waits.
 #include <cooperative_groups.h>
 #include <math.h>
 
@@ -78,6 +80,9 @@ struct WdParams {
   const int *starts, *prefix_lens;
   int groups, shares, chunk;
   const float *o_part, *lse_part;
+  // own tokens' partial results [R, Hq, D] and [R, Hq] (base 2) of requests that
+  // share, for ffa_prefix_join_kernel to join with those; or nullptr
+  float *o_own, *lse_own;
 };
 
 // WARPS per CTA, each with STAGES chunks in flight.  Two shapes:
@@ -177,6 +182,8 @@ __global__ void __launch_bounds__(WARPS * 32) ffa_window_decode_kernel(const WdP
   const int h = pair % p.Hkv, r = pair / p.Hkv;
   const int g0 = hb * 16, G = min(16, p.G - g0);  // query heads h * p.G + g0 + [0, G)
 
+  const bool apart = PREFIX && p.o_own;  // the joining kernel may start, and wait
+  if (apart) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   int ctx = p.ctx_lens[r];
   const int prefix = PREFIX ? wd_prefix(p, r, lane) : 0;  // (its loads travel with the length's)
   if (ctx < 0 || ctx > p.max_ctx) {
@@ -386,9 +393,12 @@ __global__ void __launch_bounds__(WARPS * 32) ffa_window_decode_kernel(const WdP
     *reinterpret_cast<float2*>(wm + g * P2 + d) = make_float2(o[nt][0], o[nt][1]);
     *reinterpret_cast<float2*>(wm + (g + 8) * P2 + d) = make_float2(o[nt][2], o[nt][3]);
   }
-  // PREFIX: the prefix's shares, which the cluster's CTAs divide, are one more state
-  constexpr int STATES = WARPS + (PREFIX ? 1 : 0);
-  if constexpr (PREFIX) {
+  // PREFIX: the prefix's shares, which the cluster's CTAs divide, are one more state,
+  // or a launch of their own joins them.  That one waits for this kernel only, so
+  // one CTA here waits for the one before.
+  const int states = WARPS + (PREFIX && !apart ? 1 : 0);
+  if (apart && blockIdx.x + 1 == gridDim.x) asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (PREFIX && !apart) {
     const int parts = shared ? min(p.shares, (shared + p.chunk - 1) / p.chunk) : 0;
     const int64_t step = (int64_t)p.R * p.Hq;
     float* fold = reinterpret_cast<float*>(smem) + WARPS * Cfg::STATE;
@@ -449,6 +459,12 @@ __global__ void __launch_bounds__(WARPS * 32) ffa_window_decode_kernel(const WdP
   auto store = [&](int row, int d, float M, float L, float2 acc) {
     const int head = h * p.G + g0 + row;
     const float inv = L > 0.f ? 1.f / L : 0.f;
+    if (apart && shared) {
+      const int64_t at = (int64_t)r * p.Hq + head;
+      *reinterpret_cast<float2*>(p.o_own + at * p.D + d) = make_float2(acc.x * inv, acc.y * inv);
+      if (d == 0) p.lse_own[at] = L > 0.f ? M + lg2(L) : -INFINITY;
+      return;
+    }
     T* dst = reinterpret_cast<T*>(p.out) + (int64_t)r * p.o_sr + (int64_t)head * p.o_sh + d;
     dst[0] = wd_round<T>(acc.x * inv);
     dst[1] = wd_round<T>(acc.y * inv);
@@ -461,7 +477,7 @@ __global__ void __launch_bounds__(WARPS * 32) ffa_window_decode_kernel(const WdP
     const int row = it / (p.D / 2), d = it % (p.D / 2) * 2;
     float M, L;
     float2 acc;
-    join(STATES, [&](int s) { return warps + s * Cfg::STATE; }, row, d, M, L, acc);
+    join(states, [&](int s) { return warps + s * Cfg::STATE; }, row, d, M, L, acc);
     if (p.splits == 1) {
       store(row, d, M, L, acc);
     } else {
@@ -484,6 +500,65 @@ __global__ void __launch_bounds__(WARPS * 32) ffa_window_decode_kernel(const WdP
     store(row, d, M, L, acc);
   }
   cluster.sync();  // no CTA leaves while another reads its shared memory
+}
+
+// Joins the prefix's shares and the own tokens of each request that shares: one
+// warp for each (request, query head), FOLD partial results in flight.
+template <typename T>
+__global__ void __launch_bounds__(256) ffa_prefix_join_kernel(const WdParams p) {
+  const int64_t at = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / 32;
+  const int lane = threadIdx.x % 32;
+  int r = 0, head = 0, prefix = 0, ctx = 0;
+  if (at < (int64_t)p.R * p.Hq) {
+    r = (int)(at / p.Hq);
+    head = (int)(at % p.Hq);
+    ctx = p.ctx_lens[r];
+    prefix = wd_prefix(p, r, lane);
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // (every warp: what follows this launch may count on both before)
+  if (prefix <= 0 || prefix > ctx || ctx > p.max_ctx) return;
+  const int parts = min(p.shares, (prefix + p.chunk - 1) / p.chunk);
+  const int64_t step = (int64_t)p.R * p.Hq;
+  const bool live = lane * 4 < p.D;
+  auto load = [&](const float* o) {  // (from L2: nothing of it may be in an L1 from before the wait)
+    return live ? __ldcg(reinterpret_cast<const float4*>(o + lane * 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
+  };
+  float M = __ldcg(p.lse_own + at), L = M == -INFINITY ? 0.f : 1.f;
+  float4 acc = load(p.o_own + at * p.D);
+  for (int s0 = 0; s0 < parts; s0 += FOLD) {
+    float x[FOLD], top = M;
+    float4 v[FOLD];
+#pragma unroll
+    for (int k = 0; k < FOLD; ++k) {
+      const int s = min(s0 + k, parts - 1);
+      x[k] = s0 + k < parts ? __ldcg(p.lse_part + at + s * step) : -INFINITY;
+      v[k] = load(p.o_part + (at + s * step) * p.D);
+    }
+#pragma unroll
+    for (int k = 0; k < FOLD; ++k) top = fmaxf(top, x[k]);
+    const float keep = M == -INFINITY ? 0.f : ex2(M - top);
+    L *= keep;
+    acc = make_float4(acc.x * keep, acc.y * keep, acc.z * keep, acc.w * keep);
+#pragma unroll
+    for (int k = 0; k < FOLD; ++k) {
+      const float f = x[k] == -INFINITY ? 0.f : ex2(x[k] - top);
+      L += f;
+      acc.x += v[k].x * f;
+      acc.y += v[k].y * f;
+      acc.z += v[k].z * f;
+      acc.w += v[k].w * f;
+    }
+    M = top;
+  }
+  const float inv = L > 0.f ? 1.f / L : 0.f;
+  if (live) {
+    T* dst = reinterpret_cast<T*>(p.out) + (int64_t)r * p.o_sr + (int64_t)head * p.o_sh + lane * 4;
+    dst[0] = wd_round<T>(acc.x * inv);
+    dst[1] = wd_round<T>(acc.y * inv);
+    dst[2] = wd_round<T>(acc.z * inv);
+    dst[3] = wd_round<T>(acc.w * inv);
+  }
+  if (lane == 0 && p.lse) p.lse[at] = L > 0.f ? (M + lg2(L)) * 0.6931471805599453f : -INFINITY;
 }
 
 // Estimated time (us) of `pairs` clusters of s CTAs over `visible` tokens each.
@@ -558,12 +633,26 @@ static int launch_window_decode(const WdParams& p, int64_t grid, cudaStream_t st
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = PREFIX && p.groups ? 2 : 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, kern, p));
+  if (int s = cuda_status(cudaLaunchKernelEx(&cfg, kern, p))) return s;
+  if (!PREFIX || !p.o_own) return FFA_OK;
+  cudaLaunchConfig_t join{};
+  join.gridDim = dim3((unsigned)(((int64_t)p.R * p.Hq + 7) / 8));
+  join.blockDim = dim3(256);
+  join.stream = st;
+  join.attrs = attr + 1;
+  join.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&join, ffa_prefix_join_kernel<T>, p));
 }
 
-// The launch for either form; `visible`: the most tokens a request sees here.
+// The launch for either form; `visible`: the most tokens a request sees here;
+// `before` (PREFIX): the launch of the prefix.  What it leaves idle works off own
+// tokens while it runs, if their CTAs do not wait for its partial results, which
+// costs the joining launch 4 us (256 requests of 1 to 512 tokens behind 32768, 32/8
+// heads, D 128, where 128 CTAs take the prefix: 187 us to 174; 64 requests of 1 to
+// 1024 behind 8192, where 144 do: 54 to 57).  Nothing is gained where all of them
+// find room beside the prefix (four requests behind 200 tokens: 12.3 us to 13.7).
 template <bool PREFIX>
-static int window_decode(WdParams& p, int dtype, int64_t visible, cudaStream_t st) {
+static int window_decode(WdParams& p, int dtype, int64_t visible, const PaShape& before, cudaStream_t st) {
   int k = 0;
   while ((1ll << k) < p.page_size) ++k;
   p.ps_shift = 31 + k;
@@ -575,6 +664,8 @@ static int window_decode(WdParams& p, int dtype, int64_t visible, cudaStream_t s
   wd_shape(PREFIX, pairs, visible, p.D, p.splits, warps);
   const int64_t grid = pairs * p.splits;
   if (grid > 0x7fffffffLL) return FFA_ERR_UNSUPPORTED;
+  if (PREFIX && (before.idle * before.time <= 6.f || grid <= before.idle * 148 * (warps == 2 ? 4 : 3)))
+    p.o_own = nullptr;
   auto typed = [&](auto t) -> int {
     using T = decltype(t);
     if (p.D <= 64) return launch_window_decode<T, 64, 4, PREFIX>(p, grid, st);
@@ -636,7 +727,7 @@ extern "C" int ffa_window_decode(const void* q, const void* k_pages, const void*
   // the most tokens a request can see
   int64_t visible = max_ctx > 0 && max_ctx < p.max_ctx ? max_ctx : p.max_ctx;
   if (visible > (int64_t)window + sinks) visible = (int64_t)window + sinks;
-  return window_decode<false>(p, dtype, visible, static_cast<cudaStream_t>(stream));
+  return window_decode<false>(p, dtype, visible, PaShape{}, static_cast<cudaStream_t>(stream));
 }
 
 // The shares of a prefix: ffa_page_attn.cu's shape, with a workspace for every one.
@@ -648,7 +739,7 @@ extern "C" size_t ffa_prefix_decode_workspace_size(int R, int groups, int Hq, in
   if (R <= 0 || groups <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || Hq / Hkv > 128 || D <= 0 || D > 128 ||
       max_prefix < 0)
     return 0;
-  return (size_t)R * Hq * prefix_shape(R, groups, Hq, Hkv, D, max_prefix).shares * (D + 1) * 4;
+  return (size_t)R * Hq * (prefix_shape(R, groups, Hq, Hkv, D, max_prefix).shares + 1) * (D + 1) * 4;
 }
 
 extern "C" int ffa_prefix_decode(const void* q, const void* k_pages, const void* v_pages, const int* block_table,
@@ -684,18 +775,25 @@ extern "C" int ffa_prefix_decode(const void* q, const void* k_pages, const void*
   if (int s = pa_check(c)) return s;
   if (!ctx_lens || !out || !o_strides || groups < 0 || max_prefix < 0 || max_own < 0) return FFA_ERR_INVALID_ARG;
   WdParams p{};
+  PaShape shape{};
   if (groups) {
-    const PaShape shape = prefix_shape(R, groups, Hq, Hkv, D, max_prefix);
+    shape = prefix_shape(R, groups, Hq, Hkv, D, max_prefix);
     const size_t need = ffa_prefix_decode_workspace_size(R, groups, Hq, Hkv, D, max_prefix);
     if (!workspace || workspace_bytes < need || !aligned16(workspace)) return FFA_ERR_WORKSPACE;
+    // [own tokens' O][shares' O][shares' lse][own tokens' lse]
+    const int64_t rows = (int64_t)R * Hq;
+    float* ws = static_cast<float*>(workspace);
+    c.workspace = ws + rows * D;
     if (int s = page_attn(c, shape, stream)) return s;
     p.starts = group_starts;
     p.prefix_lens = prefix_lens;
     p.groups = groups;
     p.shares = shape.shares;
     p.chunk = shape.chunk;
-    p.o_part = static_cast<float*>(workspace);
-    p.lse_part = p.o_part + (int64_t)R * Hq * shape.shares * D;
+    p.o_part = ws + rows * D;
+    p.lse_part = p.o_part + rows * shape.shares * D;
+    p.o_own = ws;
+    p.lse_own = ws + rows * (D + (int64_t)shape.shares * (D + 1));
   }
   p.q = q;
   p.q_sr = q_strides[0];
@@ -722,5 +820,5 @@ extern "C" int ffa_prefix_decode(const void* q, const void* k_pages, const void*
   p.sc_post = p.use_softcap ? softcap * 1.4426950408889634f : 0.f;
   p.err = dev_err;
   const int64_t visible = max_own > 0 && max_own < p.max_ctx ? max_own : p.max_ctx;
-  return window_decode<true>(p, dtype, visible, static_cast<cudaStream_t>(stream));
+  return window_decode<true>(p, dtype, visible, shape, static_cast<cudaStream_t>(stream));
 }

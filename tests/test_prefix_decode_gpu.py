@@ -217,3 +217,36 @@ def test_calls_in_a_row_wait_for_each_other(monkeypatch):
         chain.append(prefix_decode(chain[-1], kp, vp, bt, ln, st, pf))
     for a, b in zip(chain[::7], chain[1::7]):
         check(a, kp, vp, bt, ln, b, None)
+
+
+@pytest.mark.parametrize("groups,alone,page,Hq,Hkv,D,softcap,dtype", [
+    ([(20000, [3, 0, 40] * 13)], [0, 30], 16, 8, 4, 64, None, torch.float16),
+    ([(12000, [1, 17] * 80)], [5] * 9, 40, 2, 1, 96, 20.0, torch.bfloat16),
+    ([(9000, [i % 50 for i in range(150)]), (0, [4, 4]), (4001, [0])], [], 64, 8, 2, 128, None, torch.bfloat16),
+])
+def test_own_tokens_beside_a_long_prefix(groups, alone, page, Hq, Hkv, D, softcap, dtype):
+    """Shapes whose own tokens are partial results too, joined by a third launch; eager, in a graph, on unshared rows."""
+    from fastest_flash_attention_b200 import prefix_decode
+    kp, vp, bt, ln, st, pf, g = make(groups, alone, page, Hkv, D, dtype, 11)
+    R = ln.shape[0]
+    q = torch.randn(R, Hq, D, generator=g, device="cuda").to(dtype)
+    top = int(pf.max())
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        a = prefix_decode(q, kp, vp, bt, ln, st, pf, softcap=softcap, return_lse=True, max_prefix=top, max_own=50)
+    torch.cuda.current_stream().wait_stream(s)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr, stream=s):
+        b = prefix_decode(q, kp, vp, bt, ln, st, pf, softcap=softcap, return_lse=True, max_prefix=top, max_own=50)
+        c = b[0] + 0  # what follows the call in a graph sees all of it
+    for t in b:
+        t.fill_(math.nan)
+    gr.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) and torch.equal(a[0], c)
+    check(q, kp, vp, bt, ln, a[0], a[1], softcap)
+    top = bt.shape[1] * page  # nobody is as long: each request by itself
+    assert top > int(ln.max())
+    o = prefix_decode(q, kp, vp, bt, ln, st, pf * 0 + top, softcap=softcap, max_prefix=top, max_own=top)
+    check(q, kp, vp, bt, ln, o, None, softcap, rows=range(0, R, 7))
