@@ -584,8 +584,9 @@ __global__ void __launch_bounds__(PaCfg<D, NQT, FEW>::THREADS, PaCfg<D, NQT, FEW
         for (int e = 0; e < 16; ++e) {
           const float2 a = ffma2(make_float2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), mul2, nmu2);
           // three pairs of sixteen leave the special-function unit (D 128: 256 requests
-          // behind 32 768 tokens 193 -> 184 us, two pairs 188; 64 of 4 drafted tokens 386 -> 382)
-          const float2 pv = D > 64 && e % 5 == 3 ? exp2_fma2(a) : make_float2(ex2(a.x), ex2(a.y));
+          // behind 32 768 tokens 193 -> 184 us, two pairs 188; D 64: 2048 tokens behind
+          // 30 720 876 -> 818, two pairs 834, four 834, five 855)
+          const float2 pv = e % 5 == 3 ? exp2_fma2(a) : make_float2(ex2(a.x), ex2(a.y));
           acc[e & 1] = fadd2(acc[e & 1], pv);
           pk[e] = pack2<T>(pv.x, pv.y);
         }
@@ -688,38 +689,57 @@ __global__ void __launch_bounds__(PaCfg<D, NQT, FEW>::THREADS, PaCfg<D, NQT, FEW
 }
 
 // Joins the shares of a prefill: one warp for each (token, query head) of the
-// requests longer than a share.
+// requests longer than a share, the loads of four shares in flight (one share at a
+// time: 50 us behind the last CTA of a chunk of 2048 tokens, D 128, against 33).
 template <typename T>
-__global__ void ffa_page_attn_merge_kernel(const PaParams p) {
+__global__ void __launch_bounds__(256, 6) ffa_page_attn_merge_kernel(const PaParams p) {
+  constexpr int FOLD = 4;
   const int64_t w = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / 32;
   const int lane = threadIdx.x % 32;
+  int tok = 0, head = 0, parts = 0;
+  if (w < (int64_t)p.T * p.Hq) {  // (lengths and boundaries are nothing that the launch before writes)
+    tok = (int)(w / p.Hq);
+    head = (int)(w % p.Hq);
+    const int seg = warp_search(p.starts, p.N, tok, lane);  // the request
+    const int first = p.starts[seg], end = p.starts[seg + 1], kv = p.kv_lens[seg], n = end - first;
+    if (first >= 0 && tok >= first && tok < end && end <= p.T && kv >= n && kv <= p.max_ctx && kv > p.chunk)
+      parts = min(p.shares, (kv - n + tok - first + p.chunk) / p.chunk);
+  }
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (w >= (int64_t)p.T * p.Hq) return;
-  const int tok = (int)(w / p.Hq), head = (int)(w % p.Hq);
-  const int seg = warp_search(p.starts, p.N, tok, lane);  // the request
-  const int first = p.starts[seg], end = p.starts[seg + 1], kv = p.kv_lens[seg], n = end - first;
-  if (first < 0 || tok < first || tok >= end || end > p.T || kv < n || kv > p.max_ctx || kv <= p.chunk) return;
-  const int vis = kv - n + tok - first + 1;
-  const int parts = min(p.shares, (vis + p.chunk - 1) / p.chunk);
+  if (parts == 0) return;
   const int64_t step = (int64_t)p.T * p.Hq;
-  float M = -INFINITY;
-  for (int s = 0; s < parts; ++s) M = fmaxf(M, p.lse_part[w + s * step]);
-  float L = 0.f;
+  const bool live = lane * 4 < p.D;
+  float M = -INFINITY, L = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s = 0; s < parts; ++s) {
-    const float x = p.lse_part[w + s * step];
-    const float f = x == -INFINITY ? 0.f : ex2(x - M);
-    L += f;
-    if (lane * 4 < p.D) {
-      const float4 v = *reinterpret_cast<const float4*>(p.o_part + (w + s * step) * p.D + lane * 4);
-      acc.x += f * v.x;
-      acc.y += f * v.y;
-      acc.z += f * v.z;
-      acc.w += f * v.w;
+  for (int s0 = 0; s0 < parts; s0 += FOLD) {
+    float x[FOLD], top = M;
+    float4 v[FOLD];
+#pragma unroll
+    for (int k = 0; k < FOLD; ++k) {
+      const int64_t at = w + (s0 + k) * step;
+      const bool has = s0 + k < parts;
+      x[k] = has ? __ldcg(p.lse_part + at) : -INFINITY;
+      v[k] = has && live ? __ldcg(reinterpret_cast<const float4*>(p.o_part + at * p.D + lane * 4))
+                         : make_float4(0.f, 0.f, 0.f, 0.f);
     }
+#pragma unroll
+    for (int k = 0; k < FOLD; ++k) top = fmaxf(top, x[k]);
+    const float keep = M == -INFINITY ? 0.f : ex2(M - top);
+    L *= keep;
+    acc = make_float4(acc.x * keep, acc.y * keep, acc.z * keep, acc.w * keep);
+#pragma unroll
+    for (int k = 0; k < FOLD; ++k) {
+      const float f = x[k] == -INFINITY ? 0.f : ex2(x[k] - top);
+      L += f;
+      acc.x += f * v[k].x;
+      acc.y += f * v[k].y;
+      acc.z += f * v[k].z;
+      acc.w += f * v[k].w;
+    }
+    M = top;
   }
   const float inv = L > 0.f ? 1.f / L : 0.f;
-  if (lane * 4 < p.D) {
+  if (live) {
     T* dst = reinterpret_cast<T*>(p.out) + tok * p.o_st + head * p.o_sh + lane * 4;
     *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
   }
@@ -745,7 +765,7 @@ PaShape pa_shape(int64_t tokens, int64_t segments, int64_t kv, int Hkv, int G, i
   // time of a CTA: 5 us of start and end, and its key tiles (us a tile, alone on an
   // SM and with its slots full; the latter at the memory's rate where nobody else
   // reads the same keys); a partial result costs its writing and reading
-  const double alone = 1.9, shared = s.nqt == 2 ? 2.05 : D > 64 ? 2.1 : 3.7;
+  const double alone = 1.9, shared = s.nqt == 2 ? 2.05 : D > 64 ? 2.1 : 3.5;
   const double fresh = PA_BN * D * 4.0 * slots / 6.5e6, full = mean > per || fresh < shared ? shared : fresh;
   // (a CTA of one query tile where others have two is done in about half the time)
   const double busy = 0.5 + 0.5 * (double)((mean + tq - 1) / tq) / (double)((mean + per - 1) / per * s.nqt);
