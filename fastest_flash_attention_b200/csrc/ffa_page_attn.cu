@@ -433,6 +433,9 @@ __global__ void __launch_bounds__(PaCfg<D, NQT, FEW>::THREADS, PaCfg<D, NQT, FEW
     const int t_toks = min(p.TQ, toks - t * p.TQ);   // tokens of this tile
     const bool live = (warp % 4) * 32 < t_toks * p.G;  // any row of this warp
     const int tl = r / p.G, g = r - tl * p.G;        // this row's token in the tile, and head
+    // Rows that are not stored (another segment's, or whatever shared memory held) have
+    // no vote on what their warp does, so that a result does not depend on them.
+    const bool votes = tl < t_toks;
     // keys [0, vis) are visible to this row (a row past the segment's last token is computed like the last)
     const int vis = CAUSAL ? past + tok0 + t * p.TQ + min(tl, t_toks - 1) + 1 : limit;
     const int vis_min = CAUSAL ? past + tok0 + t * p.TQ + 1 : limit;
@@ -461,7 +464,8 @@ __global__ void __launch_bounds__(PaCfg<D, NQT, FEW>::THREADS, PaCfg<D, NQT, FEW
 #pragma unroll
             for (int e = 0; e < 32; ++e) lo[e % 4] = c + e < hi ? fmaxf(lo[e % 4], fabsf(__uint_as_float(s[e]))) : lo[e % 4];
           }
-          if (__all_sync(0xffffffffu, fmaxf(fmaxf(lo[0], lo[1]), fmaxf(lo[2], lo[3])) * p.sc_pre <= 0.5f)) {
+          if (__all_sync(0xffffffffu,
+                         !votes || fmaxf(fmaxf(lo[0], lo[1]), fmaxf(lo[2], lo[3])) * p.sc_pre <= 0.5f)) {
 #pragma unroll
             for (int e = 0; e < 32; e += 2) {
               const float2 y = softcap_small2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])),
@@ -544,7 +548,7 @@ __global__ void __launch_bounds__(PaCfg<D, NQT, FEW>::THREADS, PaCfg<D, NQT, FEW
       }
       top *= p.scale_log2;
       const float m_new = fmaxf(m, top);
-      if (__any_sync(0xffffffffu, m_new > m + 8.f)) {
+      if (__any_sync(0xffffffffu, votes && m_new > m + 8.f)) {
         // lazy rescale: exact, numerator and denominator share the stale maximum
         const float alpha = m_new == -INFINITY ? 1.f : ex2(m - m_new);
         l *= alpha;
@@ -608,11 +612,10 @@ __global__ void __launch_bounds__(PaCfg<D, NQT, FEW>::THREADS, PaCfg<D, NQT, FEW
       if (ok) {
         tc_fence_after();
         const float inv = l > 0.f ? 1.f / l : 0.f;
-        const bool store = tl < t_toks;
         const int64_t tok = first + tok0 + t * p.TQ + tl;
         const int head = h * p.G + g;
         const int64_t part = ((int64_t)share * p.T + tok) * p.Hq + head;
-        if (store) {
+        if (votes) {
           const float lse = l > 0.f ? m + lg2(l) : -INFINITY;
           if (!(CAUSAL && direct)) p.lse_part[part] = lse;
           else if (p.lse) p.lse[tok * p.Hq + head] = lse * 0.6931471805599453f;
@@ -652,7 +655,7 @@ __global__ void __launch_bounds__(PaCfg<D, NQT, FEW>::THREADS, PaCfg<D, NQT, FEW
               *reinterpret_cast<uint4*>(mine + (((c / 8 + e) ^ (lane % W)) << 4)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
             }
           }
-          leave(reinterpret_cast<T*>(p.out), store ? tok * p.o_st + head * p.o_sh : -1, 8, 0);
+          leave(reinterpret_cast<T*>(p.out), votes ? tok * p.o_st + head * p.o_sh : -1, 8, 0);
         } else {
 #pragma unroll
           for (int c0 = 0; c0 < D; c0 += D / 2) {
@@ -667,7 +670,7 @@ __global__ void __launch_bounds__(PaCfg<D, NQT, FEW>::THREADS, PaCfg<D, NQT, FEW
                     make_float4(__uint_as_float(ov[4 * e]) * inv, __uint_as_float(ov[4 * e + 1]) * inv,
                                 __uint_as_float(ov[4 * e + 2]) * inv, __uint_as_float(ov[4 * e + 3]) * inv);
             }
-            leave(p.o_part, store ? part * p.D : -1, 4, c0);
+            leave(p.o_part, votes ? part * p.D : -1, 4, c0);
           }
         }
       }

@@ -214,3 +214,26 @@ def test_nothing_to_do():
     assert bool((paged_prefill(out.clone(), kp, vp, bt, ln, starts_of([0]), out=out) == 2).all())
     none = torch.zeros(0, dtype=torch.int32, device="cuda")
     assert bool((paged_prefill(out.clone(), kp, vp, none.view(0, 1), none, starts_of([])[:1], out=out) == 2).all())
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,softcap,dtype", [
+    (28, 4, 128, 30.0, torch.float16),   # seven heads a group: two rows of a tile are nobody's
+    (8, 2, 64, None, torch.bfloat16),
+    (6, 2, 96, 5.0, torch.bfloat16),
+])
+def test_a_request_does_not_depend_on_what_shares_its_tile(Hq, Hkv, D, softcap, dtype):
+    """The same bits whatever the next request's queries are, and whatever ran before."""
+    from fastest_flash_attention_b200 import paged_prefill
+    lens, new = [700, 900], [5, 60]
+    kp, vp, bt, ln, g = make(lens, 16, Hkv, D, dtype, 31)
+    st = starts_of(new)
+    q = torch.randn(sum(new), Hq, D, generator=g, device="cuda").to(dtype)
+    first = None
+    for factor in (1.0, 40.0, 0.0, -300.0, math.nan, 1.0):
+        other = q.clone()
+        other[new[0]:] *= factor
+        o, lse = paged_prefill(other, kp, vp, bt, ln, st, softcap=softcap, return_lse=True)
+        if first is None:
+            first = o[:new[0]].clone(), lse[:new[0]].clone()
+            check(q, kp, vp, bt, lens, new, o, lse, softcap)
+        assert torch.equal(o[:new[0]], first[0]) and torch.equal(lse[:new[0]], first[1]), factor
