@@ -33,7 +33,9 @@
 // for its rows.  It starts while that kernel still runs (programmatic launch:
 // its loads need nothing of it) and waits for it only before the join.  Where
 // the prefix leaves SMs idle for long, it leaves a partial result of its own
-// tokens instead, and a third launch joins them, so that nothing waits.
+// tokens instead, and a third launch joins them, so that nothing waits.  Where
+// little is shared, it is the only launch, and every request attends all of its
+// tokens, those of the prefix through the table row that lends them.
 #include <cooperative_groups.h>
 #include <math.h>
 
@@ -83,6 +85,7 @@ struct WdParams {
   // own tokens' partial results [R, Hq, D] and [R, Hq] (base 2) of requests that
   // share, for ffa_prefix_join_kernel to join with those; or nullptr
   float *o_own, *lse_own;
+  int whole;  // or no launch before: each request attends its prefix too, through its group's row
 };
 
 // WARPS per CTA, each with STAGES chunks in flight.  Two shapes:
@@ -117,8 +120,10 @@ __device__ __forceinline__ void cp_wait() {
 }
 
 // What one lane needs to turn a virtual index into a pool row.
+template <bool PREFIX>
 struct WdRows {
   const int* table;
+  const int* lead;  // PREFIX: the table row of virtual indexes below ns
   int h, Hkv, page_size, num_pages, ns, skip, nv;  // skip: added to v >= ns
   uint32_t ps_mul;
   int ps_shift;
@@ -132,7 +137,7 @@ struct WdRows {
     const uint32_t tok = v < ns ? v : v + skip;
     const uint32_t i = (uint32_t)(((uint64_t)tok * ps_mul) >> ps_shift);
     off = (int)(tok - i * page_size);
-    return table[i];
+    return (PREFIX && v < ns ? lead : table)[i];
   }
   // pool row, or -1: past the end, or a page id outside the pool (recorded)
   __device__ __forceinline__ int row(int v, int page, int off) const {
@@ -152,19 +157,35 @@ __device__ __forceinline__ __nv_bfloat16 wd_round<__nv_bfloat16>(float x) { retu
 template <>
 __device__ __forceinline__ __half wd_round<__half>(float x) { return __float2half_rn(x); }
 
-// Prefix length of request r's group (0: in none), found by one warp.  A request
-// shorter than it shares nothing.
-__device__ __forceinline__ int wd_prefix(const WdParams& p, int r, int lane) {
+// Prefix length of request r's group (0: in none) and the group's first request,
+// found by one warp.  A request shorter than it shares nothing.
+__device__ __forceinline__ int wd_prefix(const WdParams& p, int r, int lane, int& first) {
+  first = r;
   if (p.groups == 0) return 0;
   if (p.groups >= 32) {
     const int g = warp_search(p.starts, p.groups + 1, r, lane);
-    return g < p.groups && p.starts[g] <= r ? p.prefix_lens[g] : 0;
+    if (g >= p.groups || p.starts[g] > r) return 0;
+    first = p.starts[g];
+    return p.prefix_lens[g];
   }
   // few groups: their lengths asked for with the starts, not after them
-  const bool le = lane <= p.groups && p.starts[lane] <= r;
+  const int start = lane <= p.groups ? p.starts[lane] : 0x7fffffff;
   const int len = lane < p.groups ? p.prefix_lens[lane] : 0;
-  const int g = __popc(__ballot_sync(0xffffffffu, le)) - 1;
-  return g < 0 || g >= p.groups ? 0 : __shfl_sync(0xffffffffu, len, g);
+  const int g = __popc(__ballot_sync(0xffffffffu, start <= r)) - 1;
+  if (g < 0 || g >= p.groups) return 0;
+  first = __shfl_sync(0xffffffffu, start, g);
+  return __shfl_sync(0xffffffffu, len, g);
+}
+
+// The first request of [first, r] that is as long as the prefix (its table row is
+// the group's), or -1, found by one warp.
+__device__ __forceinline__ int wd_lead(const WdParams& p, int first, int r, int prefix, int lane) {
+  for (int i0 = max(first, 0); i0 <= r; i0 += 32) {
+    const int len = i0 + lane <= r ? p.ctx_lens[i0 + lane] : -1;
+    const uint32_t has = __ballot_sync(0xffffffffu, len >= prefix && len <= p.max_ctx);
+    if (has) return i0 + __ffs(has) - 1;
+  }
+  return -1;
 }
 
 template <typename T, int DP, int WARPS, bool PREFIX>
@@ -185,20 +206,34 @@ __global__ void __launch_bounds__(WARPS * 32) ffa_window_decode_kernel(const WdP
   const bool apart = PREFIX && p.o_own;  // the joining kernel may start, and wait
   if (apart) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   int ctx = p.ctx_lens[r];
-  const int prefix = PREFIX ? wd_prefix(p, r, lane) : 0;  // (its loads travel with the length's)
+  int first = r;
+  const int prefix = PREFIX ? wd_prefix(p, r, lane, first) : 0;  // (its loads travel with the length's)
   if (ctx < 0 || ctx > p.max_ctx) {
     if (threadIdx.x == 0 && p.err) atomicCAS(p.err, 0u, SITE_DEC_BAD_CTX);
     ctx = 0;
   }
-  const int shared = prefix > 0 && prefix <= ctx ? prefix : 0;
+  int shared = prefix > 0 && prefix <= ctx ? prefix : 0;
+  const bool whole = PREFIX && p.whole;
+  int lead = r;
+  if (whole) {
+    if (shared) lead = wd_lead(p, first, r, prefix, lane);
+    if (lead < 0) shared = 0, lead = r;  // (boundaries that decrease)
+    if (blockIdx.x == 0 && p.err)
+      for (int g = threadIdx.x; g < p.groups; g += WD_THREADS) {
+        const int lo = p.starts[g], hi = p.starts[g + 1], len = p.prefix_lens[g];
+        if (lo < 0 || hi < lo || hi > p.R || (hi > lo && (len < 0 || len > p.max_ctx)))
+          atomicCAS(p.err, 0u, SITE_PA_BAD_STARTS);
+      }
+  }
   const int w0 = PREFIX ? shared : max(ctx - p.window, 0);
-  WdRows rows;
+  WdRows<PREFIX> rows;
   rows.table = p.block_table + (int64_t)r * p.bt_stride;
+  rows.lead = whole ? p.block_table + (int64_t)lead * p.bt_stride : rows.table;
   rows.h = h;
   rows.Hkv = p.Hkv;
   rows.page_size = p.page_size;
   rows.num_pages = p.num_pages;
-  rows.ns = PREFIX ? 0 : min(p.sinks, w0);
+  rows.ns = whole ? shared : PREFIX ? 0 : min(p.sinks, w0);
   rows.skip = w0 - rows.ns;
   rows.nv = rows.ns + ctx - w0;
   rows.ps_mul = p.ps_mul;
@@ -396,9 +431,9 @@ __global__ void __launch_bounds__(WARPS * 32) ffa_window_decode_kernel(const WdP
   // PREFIX: the prefix's shares, which the cluster's CTAs divide, are one more state,
   // or a launch of their own joins them.  That one waits for this kernel only, so
   // one CTA here waits for the one before.
-  const int states = WARPS + (PREFIX && !apart ? 1 : 0);
+  const int states = WARPS + (PREFIX && !apart && !whole ? 1 : 0);
   if (apart && blockIdx.x + 1 == gridDim.x) asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (PREFIX && !apart) {
+  if (PREFIX && !apart && !whole) {
     const int parts = shared ? min(p.shares, (shared + p.chunk - 1) / p.chunk) : 0;
     const int64_t step = (int64_t)p.R * p.Hq;
     float* fold = reinterpret_cast<float*>(smem) + WARPS * Cfg::STATE;
@@ -513,7 +548,8 @@ __global__ void __launch_bounds__(256) ffa_prefix_join_kernel(const WdParams p) 
     r = (int)(at / p.Hq);
     head = (int)(at % p.Hq);
     ctx = p.ctx_lens[r];
-    prefix = wd_prefix(p, r, lane);
+    int first;
+    prefix = wd_prefix(p, r, lane, first);
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");  // (every warp: what follows this launch may count on both before)
   if (prefix <= 0 || prefix > ctx || ctx > p.max_ctx) return;
@@ -632,7 +668,7 @@ static int launch_window_decode(const WdParams& p, int64_t grid, cudaStream_t st
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = PREFIX && p.groups ? 2 : 1;
+  cfg.numAttrs = PREFIX && p.groups && !p.whole ? 2 : 1;
   if (int s = cuda_status(cudaLaunchKernelEx(&cfg, kern, p))) return s;
   if (!PREFIX || !p.o_own) return FFA_OK;
   cudaLaunchConfig_t join{};
@@ -661,7 +697,7 @@ static int window_decode(WdParams& p, int dtype, int64_t visible, const PaShape&
   p.head_blocks = (p.G + 15) / 16;
   const int64_t pairs = (int64_t)p.R * p.Hkv * p.head_blocks;
   int warps = 4;
-  wd_shape(PREFIX, pairs, visible, p.D, p.splits, warps);
+  wd_shape(PREFIX && !p.whole, pairs, visible, p.D, p.splits, warps);
   const int64_t grid = pairs * p.splits;
   if (grid > 0x7fffffffLL) return FFA_ERR_UNSUPPORTED;
   if (PREFIX && (before.idle * before.time <= 6.f || grid <= before.idle * 148 * (warps == 2 ? 4 : 3)))
@@ -731,15 +767,29 @@ extern "C" int ffa_window_decode(const void* q, const void* k_pages, const void*
 }
 
 // The shares of a prefix: ffa_page_attn.cu's shape, with a workspace for every one.
+// No share where each request reads the prefix itself (from the group's pages), in
+// one launch: where that takes 5 us at most, the bytes of all of them at the
+// memory's rate, or a CTA's part of the tokens at its own speed.  Shared against
+// whole, us on the device with own tokens of 1 to 100, 32/8 heads of 128: 16
+// requests behind 100 tokens (estimate 1) 11.9, 8.8; behind 400 (4) 12.1, 11.2;
+// behind 1000 (10) 12.4, 16.6; 64 behind 100 (4) 17.4, 13.6; behind 400 (16) 18.6,
+// 24; 8/2 heads of 64: 4 behind 8000 (5) 14.8, 12.2; 16 behind 4000 (5) 12.1, 12.0;
+// 64 behind 1000 (5) 10.9, 12.7 (but one launch and its tensor maps less to call).
 static ffa::PaShape prefix_shape(int R, int groups, int Hq, int Hkv, int D, int max_prefix) {
-  return ffa::pa_shape(R, groups, max_prefix, Hkv, Hq / Hkv, D);
+  ffa::PaShape s = ffa::pa_shape(R, groups, max_prefix, Hkv, Hq / Hkv, D);
+  const double pairs = (double)R * Hkv * ((Hq / Hkv + 15) / 16);
+  const double parts = pairs < 27 ? 16.0 : pairs < 444 ? 444.0 / pairs : 1.0;
+  const double read = fmax(pairs * max_prefix * D * 4.0 / 6.5e6, max_prefix / parts * (D > 64 ? 0.0136 : 0.010));
+  if (read <= 5.0) s.shares = 0;
+  return s;
 }
 
 extern "C" size_t ffa_prefix_decode_workspace_size(int R, int groups, int Hq, int Hkv, int D, int max_prefix) {
   if (R <= 0 || groups <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || Hq / Hkv > 128 || D <= 0 || D > 128 ||
       max_prefix < 0)
     return 0;
-  return (size_t)R * Hq * (prefix_shape(R, groups, Hq, Hkv, D, max_prefix).shares + 1) * (D + 1) * 4;
+  const int shares = prefix_shape(R, groups, Hq, Hkv, D, max_prefix).shares;
+  return shares ? (size_t)R * Hq * (shares + 1) * (D + 1) * 4 : 0;
 }
 
 extern "C" int ffa_prefix_decode(const void* q, const void* k_pages, const void* v_pages, const int* block_table,
@@ -778,6 +828,12 @@ extern "C" int ffa_prefix_decode(const void* q, const void* k_pages, const void*
   PaShape shape{};
   if (groups) {
     shape = prefix_shape(R, groups, Hq, Hkv, D, max_prefix);
+    p.starts = group_starts;
+    p.prefix_lens = prefix_lens;
+    p.groups = groups;
+    p.whole = shape.shares == 0;
+  }
+  if (groups && !p.whole) {
     const size_t need = ffa_prefix_decode_workspace_size(R, groups, Hq, Hkv, D, max_prefix);
     if (!workspace || workspace_bytes < need || !aligned16(workspace)) return FFA_ERR_WORKSPACE;
     // [own tokens' O][shares' O][shares' lse][own tokens' lse]
@@ -785,9 +841,6 @@ extern "C" int ffa_prefix_decode(const void* q, const void* k_pages, const void*
     float* ws = static_cast<float*>(workspace);
     c.workspace = ws + rows * D;
     if (int s = page_attn(c, shape, stream)) return s;
-    p.starts = group_starts;
-    p.prefix_lens = prefix_lens;
-    p.groups = groups;
     p.shares = shape.shares;
     p.chunk = shape.chunk;
     p.o_part = ws + rows * D;
@@ -819,6 +872,8 @@ extern "C" int ffa_prefix_decode(const void* q, const void* k_pages, const void*
   p.sc_pre = p.use_softcap ? scale / softcap : 0.f;
   p.sc_post = p.use_softcap ? softcap * 1.4426950408889634f : 0.f;
   p.err = dev_err;
-  const int64_t visible = max_own > 0 && max_own < p.max_ctx ? max_own : p.max_ctx;
+  int64_t visible = max_own > 0 ? max_own : p.max_ctx;
+  if (p.whole) visible += max_prefix;
+  if (visible > p.max_ctx) visible = p.max_ctx;
   return window_decode<true>(p, dtype, visible, shape, static_cast<cudaStream_t>(stream));
 }

@@ -5,7 +5,8 @@ counterpart in the reference).
 ``paged_decode`` reads a shared page once for every request.  ``prefix_decode``
 reads it once for the group: one launch attends the prefix with the query heads
 of all its requests as the rows of tensor-core products, a second, overlapping
-one attends each request's own tokens and joins the two by their LSE.
+one attends each request's own tokens and joins the two by their LSE.  Where there
+is little to share, one launch attends each request's tokens instead.
 """
 from __future__ import annotations
 

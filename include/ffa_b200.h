@@ -242,8 +242,8 @@ int ffa_window_decode(const void* q, const void* k_pages, const void* v_pages, c
  * max_own (0: not known) bound the prefixes and the tokens behind them for the
  * choice of the split (larger ones are no error); max_prefix sets the
  * workspace.  Boundaries that decrease or pass R, and a prefix length outside
- * [0, max_pages_per_req * page_size], record 0x3E6 in *dev_err.  Two
- * launches, the second overlapping the first, or three.
+ * [0, max_pages_per_req * page_size], record 0x3E6 in *dev_err.  One
+ * to three overlapping launches, by the sizes.
  * ------------------------------------------------------------------------- */
 size_t ffa_prefix_decode_workspace_size(int R, int groups, int Hq, int Hkv, int D, int max_prefix);
 

@@ -225,7 +225,7 @@ def test_calls_in_a_row_wait_for_each_other(monkeypatch):
     ([(9000, [i % 50 for i in range(150)]), (0, [4, 4]), (4001, [0])], [], 64, 8, 2, 128, None, torch.bfloat16),
 ])
 def test_own_tokens_beside_a_long_prefix(groups, alone, page, Hq, Hkv, D, softcap, dtype):
-    """Shapes whose own tokens are partial results too, joined by a third launch; eager, in a graph, on unshared rows."""
+    """Shapes whose own tokens are partial results too, joined by a third launch; eager, captured, on unshared rows."""
     from fastest_flash_attention_b200 import prefix_decode
     kp, vp, bt, ln, st, pf, g = make(groups, alone, page, Hkv, D, dtype, 11)
     R = ln.shape[0]
@@ -250,3 +250,62 @@ def test_own_tokens_beside_a_long_prefix(groups, alone, page, Hq, Hkv, D, softca
     assert top > int(ln.max())
     o = prefix_decode(q, kp, vp, bt, ln, st, pf * 0 + top, softcap=softcap, max_prefix=top, max_own=top)
     check(q, kp, vp, bt, ln, o, None, softcap, rows=range(0, R, 7))
+
+
+def padded(bt, tokens, page):
+    """bt with columns for `tokens` tokens, which lets max_prefix say anything."""
+    wide = torch.full((bt.shape[0], tokens // page), -1, dtype=torch.int32, device="cuda")
+    wide[:, :bt.shape[1]] = bt
+    return wide
+
+
+@pytest.mark.parametrize("groups,alone,page,Hq,Hkv,D,softcap,dtype", CASES + [
+    ([(128, [1, 0] * 50), (129, [3] * 60), (40, [2] * 40)], [5], 16, 32, 8, 128, None, torch.bfloat16),
+    ([(77, [i % 9 for i in range(90)]), (256, [0] * 70)], [1, 0], 8, 40, 8, 96, 5.0, torch.float16),
+])
+def test_prefix_for_the_group_or_for_each_request(groups, alone, page, Hq, Hkv, D, softcap, dtype):
+    """Either way that the sizes may choose, eager and in a graph; the prefix is read through the group's first row."""
+    from fastest_flash_attention_b200 import prefix_decode
+    kp, vp, bt, ln, st, pf, g = make(groups, alone, page, Hkv, D, dtype, 5)
+    q = torch.randn(ln.shape[0], Hq, D, generator=g, device="cuda").to(dtype)
+    lent = padded(bt, 65536, page)
+    for i, (n, own) in enumerate(groups):
+        lent[sum(len(x) for _, x in groups[:i]) + 1:sum(len(x) for _, x in groups[:i + 1]), :n // page] = -1
+    for hint in (1, 65536):
+        args = (q, kp, vp, lent, ln, st, pf)
+        kw = dict(softcap=softcap, return_lse=True, max_prefix=hint, max_own=50)
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            a = prefix_decode(*args, **kw)
+        torch.cuda.current_stream().wait_stream(s)
+        check(q, kp, vp, bt, ln, a[0], a[1], softcap)
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, stream=s):
+            b = prefix_decode(*args, **kw)
+        for _ in range(2):
+            for t in b:
+                t.fill_(math.nan)
+            gr.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("hint", [1, 65536])
+def test_data_that_means_nothing_is_reported_either_way(hint):
+    from fastest_flash_attention_b200 import prefix_decode
+    kp, vp, bt, ln, st, pf, g = make([(64, [3, 5]), (32, [1])], [7], 16, 2, 64, torch.float16, 4)
+    q = torch.randn(4, 8, 64, generator=g, device="cuda").half()
+    bt = padded(bt, 65536, 16)
+
+    def ints(*x):
+        return torch.tensor(x, dtype=torch.int32, device="cuda")
+    for kw, word in ((dict(st=ints(0, 2, 5)), "boundaries"), (dict(st=ints(0, 3, 1)), "boundaries"),
+                     (dict(st=ints(-2 ** 31, 2, 3)), "boundaries"), (dict(pf=ints(64, -1)), "prefix"),
+                     (dict(pf=ints(2 ** 31 - 1, 32)), "prefix"), (dict(ln=ints(67, 65537, 33, 7)), "context length"),
+                     (dict(ln=ints(67, 69, -1, 7)), "context length"), (dict(bt=bt * 0 + 99), "block-table entry")):
+        a = dict(dict(bt=bt, ln=ln, st=st, pf=pf), **kw)
+        with pytest.raises(RuntimeError, match=word):
+            prefix_decode(q, kp, vp, a["bt"], a["ln"], a["st"], a["pf"], max_prefix=hint)
+    o, lse = prefix_decode(q, kp, vp, bt, ln, st, pf, return_lse=True, max_prefix=hint)
+    check(q, kp, vp, bt, ln, o, lse)
