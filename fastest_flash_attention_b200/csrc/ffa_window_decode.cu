@@ -686,7 +686,8 @@ static int launch_window_decode(const WdParams& p, int64_t grid, cudaStream_t st
 // costs the joining launch 4 us (256 requests of 1 to 512 tokens behind 32768, 32/8
 // heads, D 128, where 128 CTAs take the prefix: 187 us to 174; 64 requests of 1 to
 // 1024 behind 8192, where 144 do: 54 to 57).  Nothing is gained where all of them
-// find room beside the prefix (four requests behind 200 tokens: 12.3 us to 13.7).
+// find room beside the prefix (four requests behind 200 tokens, if the prefix is
+// done for the group: 12.3 us to 13.7).
 template <bool PREFIX>
 static int window_decode(WdParams& p, int dtype, int64_t visible, const PaShape& before, cudaStream_t st) {
   int k = 0;

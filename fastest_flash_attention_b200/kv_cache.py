@@ -498,8 +498,8 @@ class PagedKVCache:
             starts, prefixes = self.prefix_groups(seq_ids)
             if not any(prefixes):  # nothing is shared: no group
                 starts, prefixes = [0], []
-            own = 0 if not prefixes else max(self.sequences[s]["len"] - n for b, e, n in zip(starts, starts[1:], prefixes)
-                      for s in seq_ids[b:e])
+            own = max((self.sequences[s]["len"] - n for b, e, n in zip(starts, starts[1:], prefixes)
+                       for s in seq_ids[b:e]), default=0)
             meta = torch.tensor(starts + prefixes, dtype=torch.int32).to(q.device)
             return prefix_decode(q, self.k_pages, self.v_pages, bt, lens, meta[:len(starts)], meta[len(starts):],
                                  scale=scale, softcap=softcap, return_lse=return_lse,

@@ -99,8 +99,9 @@ def paged_prefill(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 or (out.stride(0) | out.stride(1)) % 8 \
-            or out.data_ptr() % 16:
-        raise ValueError("out must be like q, with contiguous heads and other strides and the base multiples of 16 bytes")
+            or out.data_ptr() % 16 or (T > 1 and out.stride(0) < D) or (Hq > 1 and out.stride(1) < D):
+        raise ValueError("out must be like q, with heads apart and contiguous, other strides and the base multiples of "
+                         "16 bytes")
     lse = q.new_empty((T, Hq), dtype=torch.float32) if return_lse else None
     if T == 0 or R == 0:
         return (out, lse) if return_lse else out

@@ -61,3 +61,15 @@ def test_arguments_are_refused(monkeypatch):
                dict(out=torch.zeros(4, 64, 8).half().transpose(1, 2))):
         with pytest.raises(ValueError):
             ffa.paged_prefill(q, pool, pool, bt, ln, st, **kw)
+
+
+def test_an_output_that_overlaps_itself_is_refused(monkeypatch):
+    from fastest_flash_attention_b200 import _lib
+    q, pool = torch.zeros(4, 8, 64).half(), torch.zeros(3, 2, 16, 64).half()
+    bt, ln, st = torch.zeros(2, 3).int(), torch.zeros(2).int(), torch.zeros(3).int()
+    monkeypatch.setattr(_lib, "require_cuda", lambda *a: None)
+    monkeypatch.setattr(_lib, "direct", lambda: pytest.fail("the call was not refused"))
+    for out in (torch.zeros(1, 8, 64).half().expand(4, 8, 64), torch.zeros(4, 1, 64).half().expand(4, 8, 64),
+                torch.zeros(4096).half().as_strided((4, 8, 64), (512, 32, 1))):
+        with pytest.raises(ValueError):
+            ffa.paged_prefill(q, pool, pool, bt, ln, st, out=out)

@@ -27,8 +27,11 @@ def test_entry_point_refuses_sizes_that_mean_nothing():
                dict(q=p + 2), dict(vp=p + 2), dict(qs=_lib.i64arr(512, 60)), dict(qs=None), dict(os=None)):
         assert call(**kw) in bad, kw
     assert call(R=0) == _lib.FFA_OK
-    assert call(ws=None) == call(bytes=100) == call(ws=p + 8) == _lib.FFA_ERR_WORKSPACE
-    assert lib.ffa_prefix_decode_workspace_size(2, 1, 8, 2, 64, 32) > 0
+    # a prefix long enough to be read once for the group needs its workspace; a short one needs none
+    for kw in (dict(ws=None), dict(bytes=100), dict(ws=p + 8)):
+        assert call(mp=50000, **kw) == _lib.FFA_ERR_WORKSPACE
+    assert lib.ffa_prefix_decode_workspace_size(2, 1, 8, 2, 64, 50000) > 0
+    assert lib.ffa_prefix_decode_workspace_size(2, 1, 8, 2, 64, 32) == 0
     for sizes in ((0, 1, 8, 2, 64, 9), (2, 0, 8, 2, 64, 9), (2, 1, 7, 2, 64, 9), (2, 1, 8, 0, 64, 9),
                   (2, 1, 8, 2, 0, 9), (2, 1, 8, 2, 64, -1), (2, 1, 258, 2, 64, 9)):
         assert lib.ffa_prefix_decode_workspace_size(*sizes) == 0
