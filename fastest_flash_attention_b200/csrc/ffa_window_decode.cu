@@ -74,6 +74,7 @@ struct WdParams {
   int splits;       // CTAs per cluster
   int head_blocks;  // blocks of 16 query heads in a group
   float scale_log2, sc_pre, sc_post;
+  float sc_poly[3];  // PREFIX: softcap_small2's
   int use_softcap;
   uint32_t* err;
   // PREFIX: requests [starts[g], starts[g + 1]) share their first prefix_lens[g]
@@ -328,7 +329,30 @@ __global__ void __launch_bounds__(WARPS * 32) ffa_window_decode_kernel(const WdP
     }
     const int left = rows.nv - (c0 + warp + i * WD_WARPS) * WD_CHUNK;  // tokens of this chunk
     float mul = p.scale_log2;
-    if (p.use_softcap) {
+    // PREFIX: the polynomial where every argument is within 1/2, as the prefix's kernel
+    // has it (the tanh's absolute error counts among few tokens of small scores: an
+    // LSE of two was 1.1e-6 off, relatively)
+    bool tanhs = p.use_softcap;
+    if (PREFIX && p.use_softcap) {
+      float top = 0.f;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(x[nt][e]));
+      tanhs = !__all_sync(0xffffffffu, top * p.sc_pre <= 0.5f);
+      if (!tanhs) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; e += 2) {
+            const float2 y =
+                softcap_small2(make_float2(x[nt][e], x[nt][e + 1]), p.sc_poly[0], p.sc_poly[1], p.sc_poly[2]);
+            x[nt][e] = y.x;
+            x[nt][e + 1] = y.y;
+          }
+      }
+    }
+    if (tanhs) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -872,6 +896,7 @@ extern "C" int ffa_prefix_decode(const void* q, const void* k_pages, const void*
   p.use_softcap = softcap > 0.f;
   p.sc_pre = p.use_softcap ? scale / softcap : 0.f;
   p.sc_post = p.use_softcap ? softcap * 1.4426950408889634f : 0.f;
+  softcap_poly_coeffs(p.sc_pre, p.sc_poly);
   p.err = dev_err;
   int64_t visible = max_own > 0 ? max_own : p.max_ctx;
   if (p.whole) visible += max_prefix;

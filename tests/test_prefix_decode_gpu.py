@@ -309,3 +309,19 @@ def test_data_that_means_nothing_is_reported_either_way(hint):
             prefix_decode(q, kp, vp, a["bt"], a["ln"], a["st"], a["pf"], max_prefix=hint)
     o, lse = prefix_decode(q, kp, vp, bt, ln, st, pf, return_lse=True, max_prefix=hint)
     check(q, kp, vp, bt, ln, o, lse)
+
+
+@pytest.mark.parametrize("own", [0, 1])
+def test_softcap_of_few_small_scores(own):
+    """LSEs of one and two tokens to 16 fp32 roundings of the larger of 1 and the score (the product, the scale, the
+    cap, the logarithm's parts), and not to an absolute error that grows with the cap."""
+    from fastest_flash_attention_b200 import prefix_decode
+    kp, vp, bt, ln, st, pf, g = make([(1, [own] * 9)], [], 16, 1, 64, torch.float16, 8)
+    q = (torch.randn(9, 4, 64, generator=g, device="cuda") / 4).half()
+    for cap in (30.0, 300.0):
+        _, lse = prefix_decode(q, kp, vp, bt, ln, st, pf, softcap=cap, return_lse=True)
+        tok = torch.arange(1 + own, device="cuda")
+        k = kp[bt[:, tok // 16].long(), 0, tok % 16].double()
+        s = cap * torch.tanh((q.double() @ k.transpose(1, 2)) / 8 / cap)
+        bound = 16 * 2.0 ** -24 * s.abs().amax(-1).clamp(min=1.0)
+        assert bool(((lse.double() - torch.logsumexp(s, -1)).abs() <= bound).all())
