@@ -36,7 +36,7 @@
 // sums add the unrounded values; statistics, O and the join are fp32.
 //
 // What bounds it, by the rows that share K and V:
-//   many (2048 tokens behind 30 720, 32/8 heads of 128: 945-980 us, 1090-1130
+//   many (2048 tokens behind 30 720, 32/8 heads of 128: 949-965 us, 1100-1120
 //     TFLOP/s, 0.65-0.67 of a measured GEMM): the chain S - softmax - P V of the
 //     two query tiles, about 3500 cycles for a key tile of both against 2048 of
 //     products and as many of exponentials.  On that case, us: issued by a single
@@ -44,10 +44,11 @@
 //     buffers of 64 keys 1031; an issuing warp for each tile 1234; scores kept in
 //     registers 1396 against 1313; the tiles taking turns at the exponentials no
 //     faster.
-//   few (64 requests of 4 tokens at 512 to 16 388: 360 us, 6.2 TB/s, 0.94 of a
+//   few (64 requests of 4 tokens at 512 to 16 388: 357-372 us, 6.0-6.2 TB/s, 0.91-0.94 of a
 //     measured copy): memory.
-//   D = 64 (nine ragged prompts, 20 heads: 150-165 us): latencies and the
-//     exponentials, 512 of the 825 cycles that a step of 64 keys takes an SM.
+//   D = 64 (nine ragged prompts, 20 heads: 152-190 us by their order): latencies and
+//     the exponentials, 416 (512 before 3 of 16 left the special-function unit) of
+//     the 850 cycles that a step of 64 keys takes an SM.
 #include "ffa_common.cuh"
 #include "ffa_host.h"
 #include "ffa_page_attn.h"
