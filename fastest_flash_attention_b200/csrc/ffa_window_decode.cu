@@ -455,9 +455,9 @@ __global__ void __launch_bounds__(WARPS * 32) ffa_window_decode_kernel(const WdP
   // PREFIX: the prefix's shares, which the cluster's CTAs divide, are one more state,
   // or a launch of their own joins them.  That one waits for this kernel only, so
   // one CTA here waits for the one before.
-  const int states = WARPS + (PREFIX && !apart && !whole ? 1 : 0);
+  const bool folds = PREFIX && !apart && !whole;
   if (apart && blockIdx.x + 1 == gridDim.x) asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (PREFIX && !apart && !whole) {
+  if (folds) {
     const int parts = shared ? min(p.shares, (shared + p.chunk - 1) / p.chunk) : 0;
     const int64_t step = (int64_t)p.R * p.Hq;
     float* fold = reinterpret_cast<float*>(smem) + WARPS * Cfg::STATE;
@@ -536,7 +536,10 @@ __global__ void __launch_bounds__(WARPS * 32) ffa_window_decode_kernel(const WdP
     const int row = it / (p.D / 2), d = it % (p.D / 2) * 2;
     float M, L;
     float2 acc;
-    join(states, [&](int s) { return warps + s * Cfg::STATE; }, row, d, M, L, acc);
+    const auto state = [&](int s) { return warps + s * Cfg::STATE; };
+    // (a constant count each way, so that the loops unroll: 37 requests' groups 20.7 -> 20.0 us)
+    if (folds) join(WARPS + 1, state, row, d, M, L, acc);
+    else join(WARPS, state, row, d, M, L, acc);
     if (p.splits == 1) {
       store(row, d, M, L, acc);
     } else {
