@@ -194,10 +194,23 @@ __device__ __forceinline__ bool pa_find(const PaParams& p, int per, int item, in
   return false;
 }
 
+// Maxima that are NaN where a score is, at the price of the others.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // 2^x for two lanes on the FMA and integer pipes: x = n + f with n whole and f in
 // [-1/2, 1/2] (adding 1.5 2^23 rounds, and leaves n in the low bits), 2^f by a
 // quartic fitted to it (least squares on Chebyshev nodes, reweighted towards
-// minimax: relative error 2.7e-6 in fp32), n added to the exponent.
+// minimax: relative error 2.7e-6 in fp32), n added to the exponent.  NaN becomes
+// some number: a row whose scores have one is NaN by its maximum.
 __device__ __forceinline__ float2 exp2_fma2(float2 x) {
   const float2 t = fadd2(x, f2(12582912.f));
   const float2 f = ffma2(fadd2(t, f2(-12582912.f)), f2(-1.f), x);
@@ -489,10 +502,10 @@ __global__ void __launch_bounds__(PaCfg<D, NQT, FEW>::THREADS, PaCfg<D, NQT, FEW
 #pragma unroll
         for (int e = 0; e < 32; e += 8)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) mx[i] = fmax3(mx[i], __uint_as_float(s[e + i]), __uint_as_float(s[e + i + 4]));
+          for (int i = 0; i < 4; ++i) mx[i] = max3_nan(mx[i], __uint_as_float(s[e + i]), __uint_as_float(s[e + i + 4]));
       }
       tmem_st_wait();
-      return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      return max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3]));
     };
     float m = -INFINITY, l = 0.f;
     bool ok = true;
@@ -543,14 +556,18 @@ __global__ void __launch_bounds__(PaCfg<D, NQT, FEW>::THREADS, PaCfg<D, NQT, FEW
 #pragma unroll
           for (int e = 0; e < 32; e += 8)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) mx[i] = fmax3(mx[i], __uint_as_float(s[e + i]), __uint_as_float(s[e + i + 4]));
+            for (int i = 0; i < 4; ++i)
+              mx[i] = max3_nan(mx[i], __uint_as_float(s[e + i]), __uint_as_float(s[e + i + 4]));
         }
-        top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        top = max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3]));
       }
       top *= p.scale_log2;
-      const float m_new = fmaxf(m, top);
-      if (__any_sync(0xffffffffu, votes && m_new > m + 8.f)) {
+      // A row that sees a NaN, or a score of +inf (inf - inf), is NaN from here on: its
+      // maximum, so its sum, O and LSE, whatever exp2_fma2 makes of one score.
+      float m_new = max_nan(m, top);
+      if (__any_sync(0xffffffffu, votes && !(m_new <= m + 8.f))) {
         // lazy rescale: exact, numerator and denominator share the stale maximum
+        if (m_new == INFINITY) m_new = NAN;
         const float alpha = m_new == -INFINITY ? 1.f : ex2(m - m_new);
         l *= alpha;
         m = m_new;
@@ -612,12 +629,13 @@ __global__ void __launch_bounds__(PaCfg<D, NQT, FEW>::THREADS, PaCfg<D, NQT, FEW
                       mbar_wait(&bars->o_done[t], (n_tiles - 1) & 1, p.ec, abort_flag, SITE_PA_O_DONE));
       if (ok) {
         tc_fence_after();
-        const float inv = l > 0.f ? 1.f / l : 0.f;
+        // (a sum of NaN is no empty row: O and LSE say NaN, and so do the joins')
+        const float inv = l == 0.f ? 0.f : 1.f / l;
         const int64_t tok = first + tok0 + t * p.TQ + tl;
         const int head = h * p.G + g;
         const int64_t part = ((int64_t)share * p.T + tok) * p.Hq + head;
         if (votes) {
-          const float lse = l > 0.f ? m + lg2(l) : -INFINITY;
+          const float lse = l == 0.f ? -INFINITY : m + lg2(l);
           if (!(CAUSAL && direct)) p.lse_part[part] = lse;
           else if (p.lse) p.lse[tok * p.Hq + head] = lse * 0.6931471805599453f;
         }
@@ -742,12 +760,12 @@ __global__ void __launch_bounds__(256, 6) ffa_page_attn_merge_kernel(const PaPar
     }
     M = top;
   }
-  const float inv = L > 0.f ? 1.f / L : 0.f;
+  const float inv = L == 0.f ? 0.f : 1.f / L;
   if (live) {
     T* dst = reinterpret_cast<T*>(p.out) + tok * p.o_st + head * p.o_sh + lane * 4;
     *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
   }
-  if (lane == 0 && p.lse) p.lse[w] = L > 0.f ? (M + lg2(L)) * 0.6931471805599453f : -INFINITY;
+  if (lane == 0 && p.lse) p.lse[w] = L == 0.f ? -INFINITY : (M + lg2(L)) * 0.6931471805599453f;
 }
 
 // Shares of the context and query tiles per CTA.  Two tiles where a segment's rows

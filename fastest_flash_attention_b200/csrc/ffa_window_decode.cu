@@ -517,17 +517,18 @@ __global__ void __launch_bounds__(WARPS * 32) ffa_window_decode_kernel(const WdP
   };
   auto store = [&](int row, int d, float M, float L, float2 acc) {
     const int head = h * p.G + g0 + row;
-    const float inv = L > 0.f ? 1.f / L : 0.f;
+    const bool none = PREFIX ? L == 0.f : !(L > 0.f);  // (PREFIX: a sum of NaN is no empty row, its LSE is NaN too)
+    const float inv = none ? 0.f : 1.f / L;
     if (apart && shared) {
       const int64_t at = (int64_t)r * p.Hq + head;
       *reinterpret_cast<float2*>(p.o_own + at * p.D + d) = make_float2(acc.x * inv, acc.y * inv);
-      if (d == 0) p.lse_own[at] = L > 0.f ? M + lg2(L) : -INFINITY;
+      if (d == 0) p.lse_own[at] = none ? -INFINITY : M + lg2(L);
       return;
     }
     T* dst = reinterpret_cast<T*>(p.out) + (int64_t)r * p.o_sr + (int64_t)head * p.o_sh + d;
     dst[0] = wd_round<T>(acc.x * inv);
     dst[1] = wd_round<T>(acc.y * inv);
-    if (d == 0 && p.lse) p.lse[(int64_t)r * p.Hq + head] = L > 0.f ? (M + lg2(L)) * 0.6931471805599453f : -INFINITY;
+    if (d == 0 && p.lse) p.lse[(int64_t)r * p.Hq + head] = none ? -INFINITY : (M + lg2(L)) * 0.6931471805599453f;
   };
   const int items = G * (p.D / 2);
   const float* warps = reinterpret_cast<const float*>(smem);
@@ -613,7 +614,7 @@ __global__ void __launch_bounds__(256) ffa_prefix_join_kernel(const WdParams p) 
     }
     M = top;
   }
-  const float inv = L > 0.f ? 1.f / L : 0.f;
+  const float inv = L == 0.f ? 0.f : 1.f / L;
   if (live) {
     T* dst = reinterpret_cast<T*>(p.out) + (int64_t)r * p.o_sr + (int64_t)head * p.o_sh + lane * 4;
     dst[0] = wd_round<T>(acc.x * inv);
@@ -621,7 +622,7 @@ __global__ void __launch_bounds__(256) ffa_prefix_join_kernel(const WdParams p) 
     dst[2] = wd_round<T>(acc.z * inv);
     dst[3] = wd_round<T>(acc.w * inv);
   }
-  if (lane == 0 && p.lse) p.lse[at] = L > 0.f ? (M + lg2(L)) * 0.6931471805599453f : -INFINITY;
+  if (lane == 0 && p.lse) p.lse[at] = L == 0.f ? -INFINITY : (M + lg2(L)) * 0.6931471805599453f;
 }
 
 // Estimated time (us) of `pairs` clusters of s CTAs over `visible` tokens each.
