@@ -60,6 +60,17 @@ def tma_rows(t: torch.Tensor) -> torch.Tensor:
     return t
 
 
+def heads_apart(t: torch.Tensor) -> bool:
+    """Whether no two heads of t [tokens, heads, D], D contiguous, share memory."""
+    (T, H, D), (st, sh) = t.shape, t.stride()[:2]
+    if (T > 1 and st < D) or (H > 1 and sh < D):
+        return False
+    if T < 2 or H < 2 or st >= (H - 1) * sh + D or sh >= (T - 1) * st + D:
+        return True
+    # neither axis lies within the other: head h of a token against head 0 of those whose heads begin next to it
+    return all(n >= T or abs(h * sh - n * st) >= D for h in range(1, H) for n in (h * sh // st, h * sh // st + 1))
+
+
 @functools.lru_cache(maxsize=1024)
 def _workspace(*sizes: int) -> int:
     return _lib.load().ffa_paged_prefill_workspace_size(*sizes)
@@ -99,7 +110,7 @@ def paged_prefill(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 or (out.stride(0) | out.stride(1)) % 8 \
-            or out.data_ptr() % 16 or (T > 1 and out.stride(0) < D) or (Hq > 1 and out.stride(1) < D):
+            or out.data_ptr() % 16 or not heads_apart(out):
         raise ValueError("out must be like q, with heads apart and contiguous, other strides and the base multiples of "
                          "16 bytes")
     lse = q.new_empty((T, Hq), dtype=torch.float32) if return_lse else None
