@@ -183,6 +183,10 @@ SIGNATURES: dict[str, tuple] = {
         _c_void_p, _c_void_p, _c_void_p, _c_void_p,  # ring state lens_out state_out
         _c_int, _c_int, _c_int, _c_u32p, _c_void_p,  # R num_pages page_size err stream
     ]),
+    "ffa_share_pages": (_c_int, [
+        _c_void_p, _c_int, _c_void_p, _c_int, ctypes.POINTER(_c_int), _c_int,  # block_table width lens owner rows n
+        _c_int, _c_int, _c_int, _c_int, _c_u32p, _c_void_p,  # R num_pages page_size tokens err stream
+    ]),
     "ffa_rotary": (_c_int, [
         _c_void_p, _c_i64p, _c_void_p, _c_i64p, _c_void_p, _c_i64p, _c_void_p, _c_i64p,  # q s qo s k s ko s
         _c_void_p, _c_void_p, ctypes.c_int64, _c_void_p, _c_int, ctypes.c_int64,  # cos sin len pos pos64 pos_sb
@@ -330,6 +334,7 @@ _DATA_ERRORS = {
     0x3E3: "rotary: a position is outside the cos / sin tables",
     0x3E6: "request boundaries decrease or pass the batch, or a shared prefix's length is out of range",
     0x3E4: "assign_slots: too few free pages, too many tokens, or a length, page id or free list out of range",
+    0x3E7: "share: the owner holds fewer tokens, a row is not empty, or a page id is outside the pool",
     0x3E5: "release_pages: more pages than places, or a length, page id or free list out of range",
 }
 

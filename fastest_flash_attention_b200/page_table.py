@@ -12,6 +12,7 @@ in a CUDA graph.  ``DevicePageTable`` keeps the tensors of one pool together.
 """
 from __future__ import annotations
 
+import ctypes
 from typing import NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
@@ -49,8 +50,8 @@ def assign_slots(block_table: torch.Tensor, ctx_lens: torch.Tensor, new_lens: to
                  free_state: torch.Tensor, *, page_size: int, max_tokens: int, advance: bool = False) -> SlotPlan:
     """Pages and slots for new_lens[r] more tokens of each request, in one launch.
 
-    block_table int32 [R, max_pages]: the entries of a request's new pages are
-    written, the others left as they are.  ctx_lens int32 [R]: tokens cached so
+    block_table int32 [R, max_pages], R at most 16384: the entries of a
+    request's new pages are written, the others left as they are.  ctx_lens int32 [R]: tokens cached so
     far.  new_lens int32 / int64 [R]; zero for a request without new tokens.
     free_pages int32 [num_pages] is a ring, one place for every page of the
     pool: with free_state = (head, count), the free pages are
@@ -130,8 +131,8 @@ def release_pages(block_table: torch.Tensor, ctx_lens: torch.Tensor, done: torch
 
 class DevicePageTable:
     """The device tensors of one page pool: a table row and a length for each of
-    ``max_requests`` requests, and the ring of free pages.  Every method but
-    ``num_free_pages`` is one or a few launches without a synchronisation.
+    ``max_requests`` requests (at most 16384), and the ring of free pages.  Every method but
+    ``num_free_pages`` is one launch without a synchronisation.
 
     Rows are the places of a serving batch: a row of length 0 is empty.  Pass
     ``block_table`` and ``ctx_lens`` to ``paged_prefill``, ``paged_decode`` and
@@ -159,18 +160,29 @@ class DevicePageTable:
                       page_size=self.page_size, keep=keep, advance=True)
 
     def share(self, owner: int, rows: Sequence[int], tokens: int) -> None:
-        """Rows (empty so far) begin with the first ``tokens`` of row ``owner``: whole pages, which stay the
-        owner's.  Release these rows with keep = tokens, and the owner after them."""
+        """Rows begin with the first ``tokens`` of row ``owner``: whole pages, which stay the owner's.  Release these
+        rows with keep = tokens, and the owner after them.
+
+        The owner has to hold that many tokens and the rows none: where they do not (a row that was released keeps
+        its old entries), the device error word is set and nothing changes."""
+        owner, rows, tokens = int(owner), [int(r) for r in rows], int(tokens)
+        R, width, P = _check(self.block_table, self.ctx_lens, self.free_pages, self.free_state, self.ctx_lens,
+                             "ctx_lens", self.page_size)
         if tokens <= 0 or tokens % self.page_size:
             raise ValueError(f"a shared prefix is whole pages of {self.page_size} tokens, got {tokens}")
-        n, R = tokens // self.page_size, self.block_table.shape[0]
-        if n > self.block_table.shape[1]:
-            raise ValueError(f"{tokens} tokens are past a row's {self.block_table.shape[1]} pages")
+        if tokens > width * self.page_size:
+            raise ValueError(f"{tokens} tokens are past a row's {width} pages")
         if not 0 <= owner < R or any(not 0 <= r < R or r == owner for r in rows) or len(set(rows)) < len(rows):
             raise ValueError(f"rows must be distinct, in [0, {R}) and not the owner's")
-        for r in rows:
-            self.block_table[r, :n].copy_(self.block_table[owner, :n])
-            self.ctx_lens[r] = tokens
+        _lib.require_cuda(self.block_table, self.ctx_lens)
+        with _lib.device_of(self.ctx_lens):
+            st = _lib.load().ffa_share_pages(
+                self.block_table.data_ptr(), width, self.ctx_lens.data_ptr(), owner, (ctypes.c_int * len(rows))(*rows),
+                len(rows), R, P, self.page_size, tokens, _lib.err_ptr(self.ctx_lens),
+                _lib.stream_of(self.ctx_lens))
+        _lib.check(st, "ffa_share_pages")
+        if _lib.sync_check_enabled():
+            _lib.check_device_errors(self.ctx_lens.device)
 
     @property
     def num_free_pages(self) -> int:

@@ -58,7 +58,8 @@ const char* ffa_last_error(void);
  * [0, max_pages_per_req * page_size], 0x3E1 a block-table page id outside
  * [0, num_pages), 0x3E2 a page id or slot of a copy outside the pool, 0x3E3 a
  * rotary position outside the tables, 0x3E4 / 0x3E5 a page assignment /
- * release that cannot be done, 0x3E6 request boundaries or a prefix that mean nothing, 0x1FF a block mask keeping more key tiles than the forward's
+ * release that cannot be done, 0x3E6 request boundaries or a prefix that mean nothing, 0x3E7 a prefix that cannot
+ * be shared, 0x1FF a block mask keeping more key tiles than the forward's
  * tile list holds (the offending loads are skipped; treat the call as failed).
  * ffa_read_error copies it to *out (synchronising `stream`). */
 int ffa_read_error(const uint32_t* dev_err, uint32_t* out, void* stream);
@@ -374,6 +375,11 @@ int ffa_token_move(void* k_pages, void* v_pages, const int* src_slots, const int
  *   ffa_release_pages  the pages of the rows with done[r] != 0, but those that
  *     hold the first keep[r] tokens (keep NULL: none), go behind the ring's
  *     last; ctx_lens_out of those rows is 0.
+ *   ffa_share_pages    rows (a host array of num_rows distinct row numbers, read
+ *     before the call returns; not the owner's), empty so far, begin with the
+ *     owner's first `tokens` tokens, whole pages: its table entries copied,
+ *     their lengths set.  An owner of fewer tokens, a row that is not empty or
+ *     an id outside the pool records 0x3E7 and changes nothing.
  * What cannot be done (too few pages or places, more than max_tokens tokens, a
  * length outside [0, width * page_size], an id outside the pool) records 0x3E4
  * / 0x3E5 in *dev_err and changes nothing (slots -1, starts 0).
@@ -386,6 +392,9 @@ int ffa_assign_slots(int* block_table, int width, const int* ctx_lens, const int
 int ffa_release_pages(const int* block_table, int width, const int* ctx_lens, const uint8_t* done, const int* keep,
                       int* free_pages, const int* free_state, int* ctx_lens_out, int* free_state_out, int R,
                       int num_pages, int page_size, uint32_t* dev_err, void* stream);
+
+int ffa_share_pages(int* block_table, int width, int* ctx_lens, int owner, const int* rows, int num_rows, int R,
+                    int num_pages, int page_size, int tokens, uint32_t* dev_err, void* stream);
 
 /* ----------------------------------------------------------------------------
  * Rotary positions.  The reference's rotary (modules/flash_mla.py:29-52) is a
