@@ -725,7 +725,7 @@ __global__ void __launch_bounds__(256, 6) ffa_page_attn_merge_kernel(const PaPar
     const int seg = warp_search(p.starts, p.N, tok, lane);  // the request
     const int first = p.starts[seg], end = p.starts[seg + 1], kv = p.kv_lens[seg], n = end - first;
     if (first >= 0 && tok >= first && tok < end && end <= p.T && kv >= n && kv <= p.max_ctx && kv > p.chunk)
-      parts = min(p.shares, (kv - n + tok - first + p.chunk) / p.chunk);
+      parts = share_count(kv - n + tok - first + 1, p.chunk, p.shares);
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (parts == 0) return;

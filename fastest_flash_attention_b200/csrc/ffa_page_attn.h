@@ -26,6 +26,11 @@ __device__ __forceinline__ int warp_search(const int* a, int n, int x, int lane)
   }
   return lo;
 }
+
+// Shares that hold `keys` tokens (one or more; no sum that could pass 2^31).
+__device__ __forceinline__ int share_count(int keys, int chunk, int shares) {
+  return min(shares, (keys - 1) / chunk + 1);
+}
 #endif
 
 struct PaCall {

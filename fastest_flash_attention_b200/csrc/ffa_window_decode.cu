@@ -458,7 +458,7 @@ __global__ void __launch_bounds__(WARPS * 32) ffa_window_decode_kernel(const WdP
   const bool folds = PREFIX && !apart && !whole;
   if (apart && blockIdx.x + 1 == gridDim.x) asm volatile("griddepcontrol.wait;" ::: "memory");
   if (folds) {
-    const int parts = shared ? min(p.shares, (shared + p.chunk - 1) / p.chunk) : 0;
+    const int parts = shared ? share_count(shared, p.chunk, p.shares) : 0;
     const int64_t step = (int64_t)p.R * p.Hq;
     float* fold = reinterpret_cast<float*>(smem) + WARPS * Cfg::STATE;
     asm volatile("griddepcontrol.wait;" ::: "memory");  // they are complete
@@ -581,7 +581,7 @@ __global__ void __launch_bounds__(256) ffa_prefix_join_kernel(const WdParams p) 
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");  // (every warp: what follows this launch may count on both before)
   if (prefix <= 0 || prefix > ctx || ctx > p.max_ctx) return;
-  const int parts = min(p.shares, (prefix + p.chunk - 1) / p.chunk);
+  const int parts = share_count(prefix, p.chunk, p.shares);
   const int64_t step = (int64_t)p.R * p.Hq;
   const bool live = lane * 4 < p.D;
   auto load = [&](const float* o) {  // (from L2: nothing of it may be in an L1 from before the wait)
