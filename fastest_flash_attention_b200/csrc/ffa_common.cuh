@@ -100,8 +100,18 @@ __device__ __forceinline__ bool mbar_poll(uint64_t* bar, uint32_t parity) {
 // user limit can never let a CTA free shared memory or TMEM under a copy or
 // an MMA that is still running.
 constexpr unsigned long long kDrainFloorNs = 4000000000ull;
+//
+// A probe suspends its thread for as long as most waits take, so that a limit of a
+// few ns runs out only where a wait is longer than that.  AT_ONCE: with a limit of 1
+// ns a wait that is not complete when it begins has run out, without a probe.
+template <bool AT_ONCE = false>
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, const ErrCtx& ec,
                                           volatile int* abort, uint32_t site, bool drain = false) {
+  if (AT_ONCE && !drain && ec.limit_ns == 1 && !mbar_poll(bar, parity)) {
+    if (!*abort && ec.err) atomicCAS(ec.err, 0u, site);
+    *abort = 1;
+    return false;
+  }
   if (mbar_test(bar, parity)) return true;
   if (!drain && *abort) return false;
   // The limit is counted in SM clock cycles (cheap to read); 2 cycles per ns

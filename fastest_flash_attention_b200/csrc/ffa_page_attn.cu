@@ -403,7 +403,12 @@ __global__ void __launch_bounds__(PaCfg<D, NQT, FEW>::THREADS, PaCfg<D, NQT, FEW
       };
       using H0 = std::integral_constant<int, 0>;
       using H1 = std::integral_constant<int, 1>;
-      bool ok = wait(&bars->q_full, 0, SITE_PA_Q) && wait(&bars->kv_full[0], 0, SITE_PA_KV_FULL);
+      // A limit of 1 ns ends one wait of a CTA at once, so that giving up can be tested:
+      // this one, with copies in flight, or that for the last O, with products in flight.
+      // (In the loops' waits it costs up to 4 %: a chunk 968 -> 1004 us.)
+      const bool early = 2 * n_tiles <= Cfg::NBUF || blockIdx.x % 2;
+      bool ok = !early || __all_sync(0xffffffffu, mbar_wait<true>(&bars->q_full, 0, p.ec, abort_flag, SITE_PA_Q));
+      ok = ok && wait(&bars->q_full, 0, SITE_PA_Q) && wait(&bars->kv_full[0], 0, SITE_PA_KV_FULL);
       if (ok) {
         tc_fence_after();
         tiles([&](auto t) { issue_qk(t, k_base); });
@@ -623,10 +628,12 @@ __global__ void __launch_bounds__(PaCfg<D, NQT, FEW>::THREADS, PaCfg<D, NQT, FEW
       const float2 a = fadd2(acc[0], acc[1]);
       l += a.x + a.y;
     }
+    // (a wait gave up: a read of S ahead of its use may be on its way, and TMEM is given back below)
+    if (AHEAD && !ok) tmem_ld_wait();
     // -------------------------------- epilogue --------------------------------
     if (ok && live) {
       ok = __all_sync(0xffffffffu,
-                      mbar_wait(&bars->o_done[t], (n_tiles - 1) & 1, p.ec, abort_flag, SITE_PA_O_DONE));
+                      mbar_wait<true>(&bars->o_done[t], (n_tiles - 1) & 1, p.ec, abort_flag, SITE_PA_O_DONE));
       if (ok) {
         tc_fence_after();
         // (a sum of NaN is no empty row: O and LSE say NaN, and so do the joins')
