@@ -14,6 +14,7 @@ import math
 from typing import Optional
 
 import torch
+from torch.autograd import Function, forward_ad
 
 from . import _lib
 
@@ -71,6 +72,28 @@ def heads_apart(t: torch.Tensor) -> bool:
     return all(n >= T or abs(h * sh - n * st) >= D for h in range(1, H) for n in (h * sh // st, h * sh // st + 1))
 
 
+class _NoGradient(Function):
+    """The results of a call that has no backward pass; a gradient that reaches them is refused, not left out."""
+
+    @staticmethod
+    def forward(ctx, what, results, *inputs):
+        ctx.what = what
+        return results  # (no inputs of this function, so not views of them)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"{ctx.what} has no backward pass")
+
+
+def without_gradient(what: str, o: torch.Tensor, lse: Optional[torch.Tensor], *inputs: torch.Tensor,
+                     given: bool = False) -> tuple:
+    """(o, lse), which refuse a gradient (or a tangent) where an input is part of a graph.  given: o is the caller's
+    own tensor, which does not become part of one."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in inputs) or forward_ad._current_level >= 0:
+        return _NoGradient.apply(what, (o.detach() if given else o, lse), *inputs)
+    return o, lse
+
+
 @functools.lru_cache(maxsize=1024)
 def _workspace(*sizes: int) -> int:
     return _lib.load().ffa_paged_prefill_workspace_size(*sizes)
@@ -91,7 +114,8 @@ def paged_prefill(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     three).  max_ctx: the longest context, if known (it only chooses how
     contexts are split).  Returns o [T, Hq, D] and, if requested, lse [T, Hq]
     fp32 (natural log); ``out`` takes o in a given tensor.  Rows that belong to
-    no request are not written.
+    no request are not written.  There is no backward pass: a gradient that
+    reaches the results raises.
 
     query_starts that decrease or pass T, a request with more queries than
     tokens, a length past the table and a page id outside the pool set the
@@ -107,7 +131,8 @@ def paged_prefill(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
         raise ValueError(f"max_ctx must not be negative, got {max_ctx}")
     scale, softcap = check_scale(scale, softcap, D)
     R, width = table
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 or (out.stride(0) | out.stride(1)) % 8 \
             or out.data_ptr() % 16 or not heads_apart(out):
@@ -131,4 +156,5 @@ def paged_prefill(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     _lib.check(st, "ffa_paged_prefill")
     if _lib.sync_check_enabled():
         _lib.check_device_errors(q.device)
+    out, lse = without_gradient("paged_prefill", out, lse, q, k_pages, v_pages, given=given)
     return (out, lse) if return_lse else out

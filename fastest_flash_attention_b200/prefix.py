@@ -16,7 +16,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .prefill import check_pools, check_scale, tma_rows
+from .prefill import check_pools, check_scale, tma_rows, without_gradient
 
 
 @functools.lru_cache(maxsize=1024)
@@ -41,6 +41,7 @@ def prefix_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     the most tokens of a request behind it, if known (they only choose how the
     work is split).  Returns o [R, Hq, D] (q's dtype) and, if requested, lse
     [R, Hq] fp32 (natural log; a request without tokens gets 0 and -inf).
+    There is no backward pass: a gradient that reaches the results raises.
 
     Boundaries that decrease or pass R, a length past the table and a page id
     outside the pool set the device error word.
@@ -78,4 +79,5 @@ def prefix_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     _lib.check(st, "ffa_prefix_decode")
     if _lib.sync_check_enabled():
         _lib.check_device_errors(q.device)
+    out, lse = without_gradient("prefix_decode", out, lse, q, k_pages, v_pages)
     return (out, lse) if return_lse else out
