@@ -175,6 +175,8 @@ __global__ void __launch_bounds__(PT_THREADS) ffa_page_table_kernel(const PtPara
   const int pages = pages64 <= p.P ? (int)pages64 : 0, toks = (int)toks64;
   bad |= pages64 > p.P;
   const int step = ctas * threads, i0 = cta * threads + tid;
+  // (places of pages and tokens are counted unsigned: up to 2^31, a step past it)
+  auto least = [](unsigned a, int b) { return (int)min(a, (unsigned)b); };
   const bool sums_ok = __syncthreads_or(bad) == 0;
   // the page ids concerned, each checked by one thread of the cluster; `ids`
   // (release): the first PT_ILP of this thread
@@ -185,16 +187,16 @@ __global__ void __launch_bounds__(PT_THREADS) ffa_page_table_kernel(const PtPara
     return p.ring + (at >= p.P ? at - p.P : at);
   };
   // (a warp's PT_ILP pieces of 32 items follow one another)
-  const int w0 = (cta * threads / 32 + warp) * 32 * PT_ILP;
-  auto items = [&](int j0, int n, int* j) {  // this lane's of the warp's items from j0 on, all below n
+  const unsigned w0 = (cta * threads / 32 + warp) * 32 * PT_ILP;
+  auto items = [&](unsigned j0, int n, int* j) {  // this lane's of the warp's items from j0 on, all below n
 #pragma unroll
-    for (int k = 0; k < PT_ILP; ++k) j[k] = min(j0 + 32 * k + lane, n - 1);
+    for (int k = 0; k < PT_ILP; ++k) j[k] = least(j0 + 32 * k + lane, n - 1);
   };
   if (sums_ok) {
-    for (int j0 = w0; j0 < pages; j0 += PT_ILP * step) {
+    for (unsigned j0 = w0; j0 < (unsigned)pages; j0 += PT_ILP * step) {
       int j[PT_ILP], row[PT_ILP], id[PT_ILP];
       items(j0, pages, j);
-      if (!ASSIGN) pt_rows<PT_ILP>(page0, p.R, j0, min(j0 + 32 * PT_ILP, pages) - 1, j, row, lane);
+      if (!ASSIGN) pt_rows<PT_ILP>(page0, p.R, (int)j0, least(j0 + 32 * PT_ILP, pages) - 1, j, row, lane);
 #pragma unroll
       for (int k = 0; k < PT_ILP; ++k) id[k] = ASSIGN ? *place(j[k]) : *entry(j[k], row[k]);
 #pragma unroll
@@ -233,14 +235,14 @@ __global__ void __launch_bounds__(PT_THREADS) ffa_page_table_kernel(const PtPara
     if (!ok && p.err) atomicCAS(p.err, 0u, ASSIGN ? SITE_ASSIGN : SITE_RELEASE);
   }
   if (ok) {
-    for (int j0 = w0; j0 < pages; j0 += PT_ILP * step) {
+    for (unsigned j0 = w0; j0 < (unsigned)pages; j0 += PT_ILP * step) {
       int j[PT_ILP], row[PT_ILP];
       items(j0, pages, j);
-      if (ASSIGN || j0 > w0) pt_rows<PT_ILP>(page0, p.R, j0, min(j0 + 32 * PT_ILP, pages) - 1, j, row, lane);
+      if (ASSIGN || j0 > w0) pt_rows<PT_ILP>(page0, p.R, (int)j0, least(j0 + 32 * PT_ILP, pages) - 1, j, row, lane);
 #pragma unroll
       for (int k = 0; k < PT_ILP; ++k) {
         if (j0 > w0) ids[k] = ASSIGN ? *place(j[k]) : *entry(j[k], row[k]);
-        if (j0 + 32 * k + lane >= pages) continue;
+        if (j0 + 32 * k + lane >= (unsigned)pages) continue;
         if (ASSIGN) *entry(j[k], row[k]) = ids[k];
         else *place(j[k]) = ids[k];
       }
@@ -248,37 +250,37 @@ __global__ void __launch_bounds__(PT_THREADS) ffa_page_table_kernel(const PtPara
   }
   if (ASSIGN) {
     // PT_ILP tokens in a row for each thread: one store
-    for (int tw = w0; tw < p.max_tokens; tw += PT_ILP * step) {
-      const int t0 = tw + PT_ILP * lane;
+    for (unsigned tw = w0; tw < (unsigned)p.max_tokens; tw += PT_ILP * step) {
+      const unsigned t0 = tw + PT_ILP * lane;
       int pos[PT_ILP], slot[PT_ILP];
 #pragma unroll
       for (int k = 0; k < PT_ILP; ++k) {
         pos[k] = 0;
         slot[k] = -1;
       }
-      if (ok && tw < toks) {
+      if (ok && tw < (unsigned)toks) {
         int t[PT_ILP], row[PT_ILP];
 #pragma unroll
-        for (int k = 0; k < PT_ILP; ++k) t[k] = min(t0 + k, toks - 1);
-        pt_rows<PT_ILP>(tok0, p.R, tw, min(tw + 32 * PT_ILP, toks) - 1, t, row, lane);
+        for (int k = 0; k < PT_ILP; ++k) t[k] = least(t0 + k, toks - 1);
+        pt_rows<PT_ILP>(tok0, p.R, (int)tw, least(tw + 32 * PT_ILP, toks) - 1, t, row, lane);
 #pragma unroll
         for (int k = 0; k < PT_ILP; ++k) {
           const int r = row[k], x = own[r] + t[k] - tok0[r];
           const int i = div_ps(x), n = i - base(r);
           const int page = *(n >= 0 ? place(page0[r] + n) : p.table + (int64_t)r * p.width + i);
-          if (t0 + k < toks) {
+          if (t0 + k < (unsigned)toks) {
             pos[k] = x;
             slot[k] = page * p.page_size + x - i * p.page_size;
           }
         }
       }
-      if (p.vec && t0 + PT_ILP <= p.max_tokens) {
+      if (p.vec && t0 + PT_ILP <= (unsigned)p.max_tokens) {
         *reinterpret_cast<int4*>(p.slots + t0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
         *reinterpret_cast<int4*>(p.positions + t0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
       } else {
 #pragma unroll
         for (int k = 0; k < PT_ILP; ++k)
-          if (t0 + k < p.max_tokens) {
+          if (t0 + k < (unsigned)p.max_tokens) {
             p.slots[t0 + k] = slot[k];
             p.positions[t0 + k] = pos[k];
           }
