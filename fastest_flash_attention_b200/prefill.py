@@ -85,12 +85,13 @@ class _NoGradient(Function):
         raise RuntimeError(f"{ctx.what} has no backward pass")
 
 
-def without_gradient(what: str, o: torch.Tensor, lse: Optional[torch.Tensor], *inputs: torch.Tensor,
-                     given: bool = False) -> tuple:
+def without_gradient(what: str, o: torch.Tensor, lse: Optional[torch.Tensor], q: torch.Tensor, k_pages: torch.Tensor,
+                     v_pages: torch.Tensor, given: bool = False) -> tuple:
     """(o, lse), which refuse a gradient (or a tangent) where an input is part of a graph.  given: o is the caller's
     own tensor, which does not become part of one."""
-    if torch.is_grad_enabled() and any(t.requires_grad for t in inputs) or forward_ad._current_level >= 0:
-        return _NoGradient.apply(what, (o.detach() if given else o, lse), *inputs)
+    if (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad) and torch.is_grad_enabled() \
+            or forward_ad._current_level >= 0:
+        return _NoGradient.apply(what, (o.detach() if given else o, lse), q, k_pages, v_pages)
     return o, lse
 
 
