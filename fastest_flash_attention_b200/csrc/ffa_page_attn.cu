@@ -36,15 +36,15 @@
 // sums add the unrounded values; statistics, O and the join are fp32.
 //
 // What bounds it, by the rows that share K and V:
-//   many (2048 tokens behind 30 720, 32/8 heads of 128: 949-965 us, 1100-1120
-//     TFLOP/s, 0.65-0.67 of a measured GEMM): the chain S - softmax - P V of the
-//     two query tiles, about 3500 cycles for a key tile of both against 2048 of
-//     products and as many of exponentials.  On that case, us: issued by a single
+//   many (2048 tokens behind 30 720, 32/8 heads of 128: 938-968 us by the box,
+//     1100-1135 TFLOP/s, 0.66-0.68 of a measured GEMM): the chain S - softmax - P V
+//     of the two query tiles, about 3500 cycles for a key tile of both against 2048
+//     of products and 1664 of exponentials.  On that case, us: issued by a single
 //     thread's code 1061, by the warp 959; two threads a row 1096; S in two
 //     buffers of 64 keys 1031; an issuing warp for each tile 1234; scores kept in
 //     registers 1396 against 1313; the tiles taking turns at the exponentials no
 //     faster.
-//   few (64 requests of 4 tokens at 512 to 16 388: 357-372 us, 6.0-6.2 TB/s, 0.91-0.94 of a
+//   few (64 requests of 4 tokens at 512 to 16 388: 357-373 us, 6.0-6.2 TB/s, 0.91-0.94 of a
 //     measured copy): memory.
 //   D = 64 (nine ragged prompts, 20 heads: 152-190 us by their order): latencies and
 //     the exponentials, 416 (512 before 3 of 16 left the special-function unit) of
@@ -596,7 +596,7 @@ __global__ void __launch_bounds__(PaCfg<D, NQT, FEW>::THREADS, PaCfg<D, NQT, FEW
           }
         }
       }
-      // second pass: P over S, handed over in two halves of 64 keys
+      // second pass: P over S, handed over in two halves of the tile
       const float mu = m == -INFINITY ? 0.f : m;
       const float2 mul2 = f2(p.scale_log2), nmu2 = f2(-mu);
       float2 acc[2] = {f2(0.f), f2(0.f)};

@@ -485,7 +485,11 @@ class PagedKVCache:
         """One-token attention of q [R, Hq, D] over each sequence's cached K/V
         (with a window: over its last tokens and the first sink_tokens).
         share_prefix: pages that neighbouring sequences share (``prefix_groups``)
-        are read once for all of them; not with a window."""
+        are read once for all of them; not with a window.  Three of 16 of the
+        prefix's exponentials are good to 2.7e-6 there, without the flag all to 2e-7.
+        The groups are found on the host in every call, page by page: 1.0 ms for 64
+        sequences of 512 shared pages, 4.0 for 256, beside the tables' 1.9 and 7.4;
+        a caller with tables on the device calls ``prefix_decode``."""
         from .decode import paged_decode
 
         if share_prefix and sliding_window:

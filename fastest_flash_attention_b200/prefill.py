@@ -113,7 +113,10 @@ def paged_prefill(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     contiguous, page_size a multiple of 8; block_table [R, max_pages],
     ctx_lens [R], query_starts [R + 1] int32 / int64 (``assign_slots`` gives all
     three).  max_ctx: the longest context, if known (it only chooses how
-    contexts are split).  Returns o [T, Hq, D] and, if requested, lse [T, Hq]
+    contexts are split, and with that the last bits; without it they are split
+    as if they filled the table).  A value that is NaN or infinite reaches the
+    queries that share a tile with one that sees it, as in the dense forward; a
+    key only those that see it.  Returns o [T, Hq, D] and, if requested, lse [T, Hq]
     fp32 (natural log); ``out`` takes o in a given tensor.  Rows that belong to
     no request are not written.  There is no backward pass: a gradient that
     reaches the results raises.

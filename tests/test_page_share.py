@@ -14,11 +14,11 @@ def test_entry_point_refuses_what_means_nothing():
 
     def call(table=p, width=4, lens=p, owner=0, rows=(1, 2), R=4, P=8, page=16, tokens=32, n=None):
         ids = (ctypes.c_int * len(rows))(*rows) if rows is not None else None
-        return lib.ffa_share_pages(table, width, lens, owner, ids, len(rows) if n is None else n, R, P, page, tokens, None,
-                                   None)
+        return lib.ffa_share_pages(table, width, lens, owner, ids, len(rows) if n is None else n, R, P, page, tokens,
+                                   None, None)
     for kw in (dict(table=None), dict(lens=None), dict(width=0), dict(owner=-1), dict(owner=4), dict(rows=(1, 1)),
-               dict(rows=(0,)), dict(rows=(4,)), dict(rows=(-1,)), dict(rows=None, n=1), dict(n=-1), dict(R=0), dict(R=-1),
-               dict(R=16385), dict(P=0), dict(P=2 ** 30), dict(page=0), dict(tokens=0), dict(tokens=-16),
+               dict(rows=(0,)), dict(rows=(4,)), dict(rows=(-1,)), dict(rows=None, n=1), dict(n=-1), dict(R=0),
+               dict(R=-1), dict(R=16385), dict(P=0), dict(P=2 ** 30), dict(page=0), dict(tokens=0), dict(tokens=-16),
                dict(tokens=17), dict(tokens=80), dict(width=2 ** 30)):
         assert call(**kw) in bad, kw
     assert call(rows=()) == _lib.FFA_OK

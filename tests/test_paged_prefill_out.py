@@ -36,7 +36,8 @@ def test_heads_that_overlap_are_refused_and_no_others(monkeypatch):
         bad = _overlaps(T, H, D, st, sh)
         seen.add(bad)
         with pytest.raises(ValueError if bad else Reached):
-            ffa.paged_prefill(q, pool, pool, torch.zeros(1, 3).int(), torch.zeros(1).int(), torch.zeros(2).int(), out=out)
+            ffa.paged_prefill(q, pool, pool, torch.zeros(1, 3).int(), torch.zeros(1).int(), torch.zeros(2).int(),
+                              out=out)
     assert seen == {True, False}
 
 

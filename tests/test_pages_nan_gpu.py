@@ -109,8 +109,8 @@ def test_every_column_of_a_shared_prefix(page, Hq, Hkv, D, dtype, hint, what):
     for keep in (False, True):  # and a second time where only every other group has one
         some = rows[1::2] if keep else rows
         bad = plant(kp, bt, 2 * some, some, page, what)
-        o, lse = prefix_decode(q, bad, vp, bt, ints([n + 3] * (2 * G)), ints(list(range(0, 2 * G + 1, 2))), ints([n] * G),
-                               return_lse=True, max_prefix=hint, max_own=page)
+        o, lse = prefix_decode(q, bad, vp, bt, ints([n + 3] * (2 * G)), ints(list(range(0, 2 * G + 1, 2))),
+                               ints([n] * G), return_lse=True, max_prefix=hint, max_own=page)
         hit = torch.zeros(G, dtype=torch.bool, device="cuda")
         hit[some] = True
         hit = hit.repeat_interleave(2)
