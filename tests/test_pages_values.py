@@ -119,6 +119,10 @@ PREFILL = [
     ([900 + i for i in range(40)], [(i * 29) % 90 for i in range(40)], 64, 8, 2, 128, None, torch.bfloat16),
     ([127, 1, 0, 333], [127, 1, 0, 64], 8, 4, 4, 72, None, torch.float16),
     ([400, 20], [9, 20], 40, 128, 1, 8, None, torch.float16),
+    # lopsided: one long context among short ones, a chunk beside single tokens
+    ([40000] + [900] * 70, [4] * 71, 64, 8, 2, 128, None, torch.bfloat16),
+    ([1] * 40 + [8512] + [1000] * 30, [1] * 40 + [512] + [1] * 30, 16, 4, 1, 128, None, torch.float16),
+    ([20, 30000, 17], [20, 1, 3], 24, 5, 5, 64, None, torch.bfloat16),
 ]
 
 
@@ -150,6 +154,10 @@ PREFIX = [
     ([(12000, [1, 17] * 80)], [5] * 9, 40, 2, 1, 96, 20.0, torch.bfloat16),
     ([(9000, [i % 50 for i in range(150)]), (4001, [0])], [], 64, 8, 2, 128, None, torch.bfloat16),
     ([(8192, [1 + 97 * i % 1024 for i in range(24)])], [], 16, 8, 2, 128, None, torch.bfloat16),
+    # lopsided: a long request that shares nothing, one long among a group's own tokens, groups of 1 and 60
+    ([(960, [40] * 40)], [30000], 64, 8, 2, 128, None, torch.bfloat16),
+    ([(128, [3] * 9 + [20000] + [0] * 20)], [], 16, 4, 4, 64, None, torch.float16),
+    ([(9000, [5]), (40, [i % 7 for i in range(60)])], [1], 8, 16, 2, 96, None, torch.bfloat16),
 ]
 
 
