@@ -36,7 +36,7 @@
 // sums add the unrounded values; statistics, O and the join are fp32.
 //
 // What bounds it, by the rows that share K and V:
-//   many (2048 tokens behind 30 720, 32/8 heads of 128: 938-968 us by the box,
+//   many (2048 tokens behind 30 720, 32/8 heads of 128: 938-968 us from run to run,
 //     1100-1135 TFLOP/s, 0.66-0.68 of a measured GEMM): the chain S - softmax - P V
 //     of the two query tiles, about 3500 cycles for a key tile of both against 2048
 //     of products and 1664 of exponentials.  On that case, us: issued by a single

@@ -65,7 +65,9 @@ const char* ffa_last_error(void);
 int ffa_read_error(const uint32_t* dev_err, uint32_t* out, void* stream);
 
 /* Wall-clock limit (nanoseconds) applied to every in-kernel wait of later
- * launches on this host thread; default 2e9 (2 s). */
+ * launches on this host thread; default 2e9 (2 s).  A wait's first probe takes
+ * its own time, whatever the limit; a limit of 1 ns also ends a wait that
+ * ffa_paged_prefill and ffa_prefix_decode begin with or end in, for tests. */
 void ffa_set_wait_limit_ns(unsigned long long ns);
 
 /* ----------------------------------------------------------------------------
